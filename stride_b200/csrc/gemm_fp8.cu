@@ -1,0 +1,684 @@
+// Linear layers with 8-bit weights, out = x . W^T: W in e4m3 with one float32 scale per block of 128 rows and 128 columns, x quantised on the
+// way in, one scale per token and block of 128 columns.
+//
+// `quantize_kernel`: with a = max |x_j| of a token's block, s = 2^e, e = max(ceil(log2(a / 448)), -100) (448 is the largest e4m3 value) and
+// q_j = e4m3(x_j / s), to nearest even. A power of two, because then x / s and q s are exact: what is lost is the one rounding to e4m3, the
+// same however it is computed (a scale a / 448 uses up to one more bit of the largest elements' range, but rounds the quotient twice). A block
+// with an infinity or a NaN gets the scale NaN, so the token's whole result is NaN.
+//
+// `gemm_fp8_kernel`: y[t, m] = sum over blocks b of columns of s[t, b] w_s[m / 128, b] (sum of q w over the block). The inner sum runs on the
+// tensor cores (tcgen05.mma kind::f8f6f4, float32 accumulators, 128 weight rows by BN tokens): every block of 128 columns, one row of the
+// 128-byte swizzle, is a fresh accumulator in tensor memory, of which there is a ring; the epilogue's warps take it from there and add it,
+// times its two scales, to the tile's sum in registers, one fused multiply-add an element, in 32 bits. The scales' products s w_s come
+// from two warps of their own through shared memory.
+//
+// K is cut into ranges, a function of the weight's shape alone (`fp8_ranges`): few weight tiles leave SMs without work. The sum of a range
+// starts from zero, the ranges are added in ascending order. With few tokens the ranges are the CTAs of a cluster, which add up through
+// distributed shared memory; with many one CTA walks them all. So a token's bits depend neither on the step it is part of nor on the tile.
+#include <algorithm>
+
+#include "gemm_tc_tile.cuh"
+#include "step_ops.h"
+
+SB_DEFINE_LAST_ERROR()
+
+namespace {
+
+using namespace sb::tc5;
+using sb::gemm_tile::bf16;
+using sb::gemm_tile::Gate;
+using sb::gemm_tile::gated_product;
+
+constexpr int kBlock = 128;            // columns (and weight rows) of a scale
+constexpr int kStageA = kBlock * 128;  // bytes of a weight tile's block
+constexpr int kMaxStages = 8;
+constexpr int kMaxRanges = 8;
+constexpr int kSmemBudget = 200 * 1024;
+
+enum Epilogue { kStore = 0, kAdd = 1, kGated = 2 };
+
+// ------------------------------------------------------------------ quantisation
+// The scale's exponent: amax = 1.m 2^E -> E - 8 if 1.m <= 1.75 (448 = 1.75 2^8), else E - 7; never below -100.
+__device__ __forceinline__ int scale_exponent(uint32_t amax_bits) {
+  return max(static_cast<int>((amax_bits + 0x1FFFFFu) >> 23) - 127 - 8, -100);
+}
+__device__ __forceinline__ float power_of_two(int e) { return __uint_as_float(static_cast<uint32_t>(e + 127) << 23); }   // -126 <= e <= 127
+__device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {
+  uint16_t r;
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %2, %1;" : "=h"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+
+// x [n][ldx], q [rows][ldq] bytes, scales [ceil(K / 128)][lds]. order (or null): row i of the result is token order[i] % n. used (or null): how
+// many of the rows there are.
+// A warp takes a block of 128 columns of a row, four columns a lane.
+template <class T, bool VEC>
+__global__ void __launch_bounds__(256) quantize_kernel(const T* __restrict__ x, int64_t ldx, const int32_t* __restrict__ order,
+                                                       const int32_t* __restrict__ used, int n, int rows, int K, int blocks, uint8_t* __restrict__ q, int64_t ldq, float* __restrict__ scales, int64_t lds) {
+  sb::grid_launch_dependents();
+  sb::grid_dependency_wait();
+  const int64_t item = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
+  if (item >= static_cast<int64_t>(rows) * blocks) return;
+  const int row = static_cast<int>(item / blocks), b = static_cast<int>(item % blocks), lane = threadIdx.x & 31;
+  if (used != nullptr && row >= *used) return;
+  const int k = b * kBlock + lane * 4;
+  const int src = order != nullptr ? order[row] % n : row;
+  const T* from = x + static_cast<int64_t>(src) * ldx + k;
+  float v[4];
+  if (VEC && k < K) {
+    if (sizeof(T) == 2) {
+      const uint2 raw = *reinterpret_cast<const uint2*>(from);
+      v[0] = __uint_as_float(raw.x << 16), v[1] = __uint_as_float(raw.x & 0xFFFF0000u);
+      v[2] = __uint_as_float(raw.y << 16), v[3] = __uint_as_float(raw.y & 0xFFFF0000u);
+    } else {
+      const float4 raw = *reinterpret_cast<const float4*>(from);
+      v[0] = raw.x, v[1] = raw.y, v[2] = raw.z, v[3] = raw.w;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = k + i < K ? sb::widen(from[i]) : 0.0f;
+  }
+  uint32_t amax = 0;               // (the bit patterns of |x| are ordered as the values are, infinity and NaN above them)
+#pragma unroll
+  for (int i = 0; i < 4; ++i) amax = max(amax, __float_as_uint(v[i]) & 0x7FFFFFFFu);
+  amax = __reduce_max_sync(0xffffffffu, amax);
+  const bool finite = amax < 0x7F800000u;
+  const int e = finite ? scale_exponent(amax) : 0;
+  const float inverse = power_of_two(-e);
+  const uint32_t packed = e4m3x2(v[0] * inverse, v[1] * inverse) | (e4m3x2(v[2] * inverse, v[3] * inverse) << 16);
+  uint8_t* to = q + static_cast<int64_t>(row) * ldq + k;
+  if (k + 4 <= K) {
+    *reinterpret_cast<uint32_t*>(to) = packed;         // (rows of q start 16-byte aligned)
+  } else {
+    for (int i = 0; k + i < K; ++i) to[i] = static_cast<uint8_t>(packed >> (8 * i));
+  }
+  if (lane == 0) scales[static_cast<int64_t>(b) * lds + row] = finite ? power_of_two(e) : __uint_as_float(0x7FC00000u);
+}
+
+// ------------------------------------------------------------------ the product
+struct Fp8Params {
+  void* out;                 // kStore: [n][ldo] of OUT; kAdd: float32 [n][ldo]; kGated: OUT [n][ldo]
+  int64_t ldo;
+  const float* x_scales;     // [blocks][ldxs]
+  int64_t ldxs;
+  const float* w_scales;     // [blocks of rows][blocks]
+  int n, M, K, blocks;       // M: rows of the weight (of one expert); kGated: gate rows, then up rows
+  int half_rows;
+  int scale_rows;            // blocks of rows of one expert's scales
+  int ranges, range_blocks;  // K ranges and blocks of columns in each
+  int stages;
+  const int32_t* tiles;      // experts: the list of `expert_order_kernel`; else null
+  const int32_t* order;      // experts: row -> pair k n + token
+  const float* pair_weight;  // experts: a factor on every pair's result, by pair, or null
+  Gate gate;
+  int* status;
+};
+
+__device__ __forceinline__ uint32_t instr_desc_e4m3(int n) {      // D float32, A and B e4m3, both K-major, M = 128
+  return (1u << 4) | (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(kBlock >> 4) << 24);
+}
+__device__ __forceinline__ void umma_e4m3(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem_d),
+      "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ float cluster_load_float(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+  return v;
+}
+
+template <int BN>
+struct Shape {
+  static constexpr int kEpilogueWarps = BN >= 64 ? 8 : 4;
+  static constexpr int kColumns = BN * 4 / kEpilogueWarps;             // columns of a thread's row of the tile
+  static constexpr int kThreads = 128 + 32 * kEpilogueWarps;
+  static constexpr int kSlots = BN <= 32 ? 8 : 4;                      // accumulators under way
+  static constexpr int kStage = kStageA + BN * 128;
+  static constexpr int kTmem = kSlots * BN < 32 ? 32 : kSlots * BN;    // (a power of two)
+};
+
+// blockIdx = (weight tile, token tile, K range: the rank in the cluster when SPLIT). Warp 0 loads, warp 1 issues the products, warps 2 and 3
+// multiply the scales, the others are the epilogue: four of them see all 128 rows, with eight each half takes half of the columns.
+template <int EPI, int BN, class OUT, bool GROUPED, bool SPLIT>
+__global__ void __launch_bounds__(Shape<BN>::kThreads, 1)
+gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const Fp8Params p) {
+  using S = Shape<BN>;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  __shared__ __align__(8) uint64_t full_bar[kMaxStages], empty_bar[kMaxStages];
+  __shared__ __align__(8) uint64_t accum_full[S::kSlots], scale_full[S::kSlots], slot_empty[S::kSlots];
+  __shared__ __align__(16) float factor[S::kSlots][2][BN];
+  __shared__ uint32_t tmem_base_s;
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  sb::grid_launch_dependents();
+  int expert = 0, n0 = blockIdx.y * BN, end = p.n;
+  if (GROUPED) {
+    sb::grid_dependency_wait();        // whose rows this tile holds is an earlier kernel's result
+    if (static_cast<int>(blockIdx.y) >= p.tiles[0]) return;
+    expert = p.tiles[2 + 3 * blockIdx.y], n0 = p.tiles[3 + 3 * blockIdx.y], end = p.tiles[4 + 3 * blockIdx.y];
+  }
+  const uint32_t smem0 = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  uint8_t* smem0_p = smem_raw + (smem0 - smem_u32(smem_raw));
+  const int tile_m = blockIdx.x;
+  const int b0 = SPLIT ? blockIdx.z * p.range_blocks : 0;
+  const int iters = (SPLIT ? min(p.blocks, b0 + p.range_blocks) : p.blocks) - b0;
+
+  if (threadIdx.x == 0) {
+    prefetch_tensormap(&map_w);
+    prefetch_tensormap(&map_x);
+    for (int s = 0; s < p.stages; ++s) mbar_init(smem_u32(&full_bar[s]), 1), mbar_init(smem_u32(&empty_bar[s]), 1);
+    for (int s = 0; s < S::kSlots; ++s) {
+      mbar_init(smem_u32(&accum_full[s]), 1);
+      mbar_init(smem_u32(&scale_full[s]), 64);
+      mbar_init(smem_u32(&slot_empty[s]), S::kEpilogueWarps);
+    }
+    mbar_init_fence();
+  }
+  if (warp == 1) tmem_alloc(smem_u32(&tmem_base_s), S::kTmem);
+  fence_before_sync();
+  __syncthreads();
+  fence_after_sync();
+  const uint32_t tmem_base = tmem_base_s;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      const int row_w = expert * p.M + tile_m * (EPI == kGated ? 64 : kBlock);
+      auto load_w = [&](int i, int st) {
+        const uint32_t bar = smem_u32(&full_bar[st]), a = smem0 + st * S::kStage;
+        mbar_expect_tx(bar, S::kStage);
+        tma_load_2d(a, &map_w, bar, (b0 + i) * kBlock, row_w);
+        if (EPI == kGated) tma_load_2d(a + kStageA / 2, &map_w, bar, (b0 + i) * kBlock, row_w + p.half_rows);
+      };
+      auto load_x = [&](int i, int st) { tma_load_2d(smem0 + st * S::kStage + kStageA, &map_x, smem_u32(&full_bar[st]), (b0 + i) * kBlock, n0); };
+      // (the weights are nobody's result: the first ring of them is under way before the kernels in front have ended)
+      const int ahead = min(iters, p.stages);
+      for (int i = 0; i < ahead; ++i) load_w(i, i);
+      if (!GROUPED) sb::grid_dependency_wait();
+      for (int i = 0; i < ahead; ++i) load_x(i, i);
+      int st = ahead == p.stages ? 0 : ahead;
+      uint32_t par = 0;
+      for (int i = ahead; i < iters; ++i) {
+        mbar_wait(smem_u32(&empty_bar[st]), par, p.status, 41);
+        load_w(i, st);
+        load_x(i, st);
+        if (++st == p.stages) st = 0, par ^= 1;
+      }
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    if (lane == 0) {
+      const uint32_t idesc = instr_desc_e4m3(BN);
+      const uint64_t desc_fixed = smem_desc_sw128(0);
+      int st = 0, slot = 0;
+      uint32_t par = 0, slot_par = 1;
+      for (int i = 0; i < iters; ++i) {
+        mbar_wait(smem_u32(&slot_empty[slot]), slot_par, p.status, 42);
+        mbar_wait(smem_u32(&full_bar[st]), par, p.status, 43);
+        fence_after_sync();
+        const uint64_t da = desc_fixed | (((smem0 + st * S::kStage) & 0x3FFFF) >> 4), db = da + (kStageA >> 4);
+        const uint32_t d = tmem_base + slot * BN;
+        umma_e4m3(d, da, db, idesc, 0u);              // 32 columns = 32 bytes a step
+        umma_e4m3(d, da + 2, db + 2, idesc, 1u);
+        umma_e4m3(d, da + 4, db + 4, idesc, 1u);
+        umma_e4m3(d, da + 6, db + 6, idesc, 1u);
+        umma_commit(smem_u32(&empty_bar[st]));
+        umma_commit(smem_u32(&accum_full[slot]));
+        if (++st == p.stages) st = 0, par ^= 1;
+        if (++slot == S::kSlots) slot = 0, slot_par ^= 1;
+      }
+    }
+    __syncwarp();
+  } else if (warp < 4) {
+    // the scales' products, two columns a thread; four blocks are read ahead of their turn
+    constexpr int kAhead = 4, kPer = (BN + 63) / 64;
+    const int t = threadIdx.x - 64;
+    const float* ws0 = p.w_scales + static_cast<int64_t>(expert * p.scale_rows + (EPI == kGated ? tile_m / 2 : tile_m)) * p.blocks + b0;
+    const float* ws1 = EPI == kGated ? ws0 + static_cast<int64_t>(p.scale_rows / 2) * p.blocks : ws0;
+    if (!GROUPED) sb::grid_dependency_wait();
+    float xs[kAhead][kPer], w0[kAhead], w1[kAhead];
+    auto fetch = [&](int i, int a) {
+      if (i >= iters) return;
+      w0[a] = __ldg(ws0 + i), w1[a] = EPI == kGated ? __ldg(ws1 + i) : 0.0f;
+#pragma unroll
+      for (int k = 0; k < kPer; ++k) {
+        const int c = t + 64 * k;
+        xs[a][k] = c < BN && n0 + c < end ? p.x_scales[static_cast<int64_t>(b0 + i) * p.ldxs + n0 + c] : 0.0f;
+      }
+    };
+#pragma unroll
+    for (int a = 0; a < kAhead; ++a) fetch(a, a);
+    int slot = 0;
+    uint32_t slot_par = 1;
+    for (int i0 = 0; i0 < iters; i0 += kAhead) {
+#pragma unroll
+      for (int a = 0; a < kAhead; ++a) {
+        const int i = i0 + a;
+        if (i >= iters) break;
+        mbar_wait(smem_u32(&slot_empty[slot]), slot_par, p.status, 44);
+#pragma unroll
+        for (int k = 0; k < kPer; ++k) {
+          const int c = t + 64 * k;
+          if (c < BN) {
+            factor[slot][0][c] = xs[a][k] * w0[a];
+            if (EPI == kGated) factor[slot][1][c] = xs[a][k] * w1[a];
+          }
+        }
+        mbar_arrive(smem_u32(&scale_full[slot]));
+        fetch(i + kAhead, a);
+        if (++slot == S::kSlots) slot = 0, slot_par ^= 1;
+      }
+    }
+  } else {
+    const int quarter = warp & 3, half = (warp - 4) >> 2, row = quarter * 32 + lane;
+    constexpr int C = S::kColumns, kChunk = C < 32 ? C : 32;
+    float acc[C], total[SPLIT ? 1 : C];
+#pragma unroll
+    for (int c = 0; c < C; ++c) acc[c] = 0.0f;
+    if (!SPLIT) {
+#pragma unroll
+      for (int c = 0; c < C; ++c) total[c] = -0.0f;          // (the first range is added to nothing: -0 + v = v, signs of zeros too)
+    }
+    bool ok = true;
+    int slot = 0, left = p.range_blocks;
+    uint32_t slot_par = 0;
+    for (int i = 0; i < iters; ++i) {
+      ok = mbar_wait(smem_u32(&accum_full[slot]), slot_par, p.status, 45) && ok;
+      ok = mbar_wait(smem_u32(&scale_full[slot]), slot_par, p.status, 46) && ok;
+      fence_after_sync();
+      const uint32_t from = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + slot * BN + half * C;
+      const float* f = factor[slot][EPI == kGated && quarter >= 2 ? 1 : 0] + half * C;
+#pragma unroll
+      for (int c0 = 0; c0 < C; c0 += kChunk) {
+        uint32_t v[kChunk];
+        if (kChunk == 32) tmem_load32_nowait(from + c0, v);
+        else tmem_load16_nowait(from + c0, v);
+        tmem_load_wait();
+#pragma unroll
+        for (int c = 0; c < kChunk; c += 4) {
+          const float4 s = *reinterpret_cast<const float4*>(f + c0 + c);
+          acc[c0 + c] = fmaf(__uint_as_float(v[c]), s.x, acc[c0 + c]);
+          acc[c0 + c + 1] = fmaf(__uint_as_float(v[c + 1]), s.y, acc[c0 + c + 1]);
+          acc[c0 + c + 2] = fmaf(__uint_as_float(v[c + 2]), s.z, acc[c0 + c + 2]);
+          acc[c0 + c + 3] = fmaf(__uint_as_float(v[c + 3]), s.w, acc[c0 + c + 3]);
+        }
+      }
+      fence_before_sync();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&slot_empty[slot]));
+      if (++slot == S::kSlots) slot = 0, slot_par ^= 1;
+      if (!SPLIT && (--left == 0 || i + 1 == iters)) {
+        left = p.range_blocks;
+#pragma unroll
+        for (int c = 0; c < C; ++c) total[c] += acc[c], acc[c] = 0.0f;
+      }
+    }
+    // the tile's sums to shared memory, [token][row]: every load has arrived and every product that reads the ring is done
+    float* tile = reinterpret_cast<float*>(smem0_p);
+    if (ok) {
+#pragma unroll
+      for (int c = 0; c < C; ++c) tile[(half * C + c) * kBlock + row] = SPLIT ? acc[c] : total[c];
+    }
+    if (!ok) tile = nullptr;
+    asm volatile("bar.sync 1, %0;" ::"r"(32 * S::kEpilogueWarps) : "memory");
+    if (!GROUPED) sb::grid_dependency_wait();
+    if (!SPLIT) {
+      const int thread = threadIdx.x - 128;
+      constexpr int kFeatures = EPI == kGated ? 64 : kBlock, kStride = 32 * S::kEpilogueWarps / kFeatures;
+      const int j = thread % kFeatures, m = tile_m * kFeatures + j;
+      if (tile != nullptr && m < (EPI == kGated ? p.half_rows : p.M)) {
+        for (int c = thread / kFeatures; c < BN && n0 + c < end; c += kStride) {
+          float v = tile[c * kBlock + j];
+          int64_t to = n0 + c;
+          if (EPI == kGated) v = gated_product(v, tile[c * kBlock + 64 + j], p.gate);
+          if (GROUPED && EPI != kGated) {
+            to = p.order[n0 + c];
+            if (p.pair_weight != nullptr) v *= p.pair_weight[to];
+          }
+          OUT* o = static_cast<OUT*>(p.out) + to * p.ldo + m;
+          if (EPI == kAdd) v += sb::widen(*o);
+          *o = sb::narrow<OUT>(v);
+        }
+      }
+    }
+  }
+  if (SPLIT) {
+    sb::cluster_sync();
+    if (warp >= 4) {
+      const int thread = threadIdx.x - 128, rank = static_cast<int>(sb::cluster_rank());
+      constexpr int kFeatures = EPI == kGated ? 64 : kBlock, kStride = 32 * S::kEpilogueWarps / kFeatures;
+      const int j = thread % kFeatures, m = tile_m * kFeatures + j;
+      const bool ok = *reinterpret_cast<volatile int*>(p.status) == 0;       // (a range that lost a signal has left no sums)
+      if (ok && m < (EPI == kGated ? p.half_rows : p.M)) {
+        const uint32_t here = smem0 + 4 * j;
+        for (int c = rank + p.ranges * (thread / kFeatures); c < BN && n0 + c < end; c += p.ranges * kStride) {
+          float v = 0.0f, u = 0.0f;
+          for (int r = 0; r < p.ranges; ++r) {
+            uint32_t peer;
+            asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(peer) : "r"(here + c * kBlock * 4), "r"(r));
+            const float a = cluster_load_float(peer);
+            v = r == 0 ? a : v + a;
+            if (EPI == kGated) {
+              const float b = cluster_load_float(peer + 64 * 4);
+              u = r == 0 ? b : u + b;
+            }
+          }
+          if (EPI == kGated) v = gated_product(v, u, p.gate);
+          OUT* o = static_cast<OUT*>(p.out) + static_cast<int64_t>(n0 + c) * p.ldo + m;
+          if (EPI == kAdd) v += sb::widen(*o);
+          *o = sb::narrow<OUT>(v);
+        }
+      }
+    }
+    sb::cluster_sync();                // (nobody leaves while another reads its sums)
+  }
+  fence_before_sync();
+  __syncthreads();
+  if (warp == 1) {
+    fence_after_sync();
+    tmem_dealloc(tmem_base, S::kTmem);
+  }
+}
+
+// ------------------------------------------------------------------ experts
+// choice [n][top] -> the pairs p = k n + token in expert order, and the row tiles of the products. An id outside [0, E) is no expert: its pair
+// is left out. list: [0] tiles, [1] rows, then (expert, first row, end row) of every tile. (Which of an expert's pairs comes first does not
+// matter: every row is computed on its own.)
+constexpr int kMaxExperts = 1024;
+constexpr int kOrderThreads = 1024;
+__global__ void __launch_bounds__(kOrderThreads) expert_order_kernel(const int32_t* __restrict__ choice, int n, int top, int E, int tile,
+                                                                     int32_t* __restrict__ order, int32_t* __restrict__ list) {
+  __shared__ int count[kMaxExperts], place[kMaxExperts], tile_at[kMaxExperts];
+  sb::grid_launch_dependents();
+  for (int e = threadIdx.x; e < E; e += blockDim.x) count[e] = 0;
+  __syncthreads();
+  sb::grid_dependency_wait();
+  const int pairs = n * top;
+  auto expert_of = [&](int p) { return static_cast<uint32_t>(choice[static_cast<int64_t>(p % n) * top + p / n]); };
+  for (int p = threadIdx.x; p < pairs; p += blockDim.x) {
+    const uint32_t e = expert_of(p);
+    if (e < static_cast<uint32_t>(E)) atomicAdd(&count[e], 1);
+  }
+  __syncthreads();
+  if (threadIdx.x < 32) {
+    const int lane = threadIdx.x;
+    int rows_before = 0, tiles_before = 0;
+    for (int e0 = 0; e0 < E; e0 += 32) {
+      const int e = e0 + lane, c = e < E ? count[e] : 0, t = (c + tile - 1) / tile;
+      int cs = c, ts = t;
+      for (int o = 1; o < 32; o <<= 1) {
+        const int a = __shfl_up_sync(0xffffffffu, cs, o), b = __shfl_up_sync(0xffffffffu, ts, o);
+        if (lane >= o) cs += a, ts += b;
+      }
+      if (e < E) place[e] = rows_before + cs - c, tile_at[e] = tiles_before + ts - t;
+      rows_before += __shfl_sync(0xffffffffu, cs, 31), tiles_before += __shfl_sync(0xffffffffu, ts, 31);
+    }
+    if (lane == 0) list[0] = tiles_before, list[1] = rows_before;
+  }
+  __syncthreads();
+  for (int e = threadIdx.x; e < E; e += blockDim.x) {
+    const int first = place[e], end = first + count[e];
+    int32_t* to = list + 2 + 3 * static_cast<int64_t>(tile_at[e]);
+    for (int r = first; r < end; r += tile, to += 3) to[0] = e, to[1] = r, to[2] = end;
+  }
+  __syncthreads();
+  for (int p = threadIdx.x; p < pairs; p += blockDim.x) {
+    const uint32_t e = expert_of(p);
+    if (e < static_cast<uint32_t>(E)) order[atomicAdd(&place[e], 1)] = p;
+  }
+}
+
+// out[t] = the token's weighted results in the order of its choices; a choice that is no expert has none.
+template <class OUT>
+__global__ void __launch_bounds__(256) expert_combine_kernel(const float* __restrict__ parts, const int32_t* __restrict__ choice, int n, int top, int E,
+                                                             int W, OUT* __restrict__ out, int64_t ldo) {
+  sb::grid_launch_dependents();
+  sb::grid_dependency_wait();
+  const int t = blockIdx.x;
+  const int32_t* mine = choice + static_cast<int64_t>(t) * top;
+  for (int m = blockIdx.y * blockDim.x + threadIdx.x; m < W; m += gridDim.y * blockDim.x) {
+    float sum = 0.0f;
+    for (int k = 0; k < top; ++k)
+      if (static_cast<uint32_t>(mine[k]) < static_cast<uint32_t>(E)) sum += parts[(static_cast<int64_t>(k) * n + t) * W + m];
+    out[static_cast<int64_t>(t) * ldo + m] = sb::narrow<OUT>(sum);
+  }
+}
+
+// ------------------------------------------------------------------ host side
+// Tensor map of bytes [rows][K] (row stride ld, a multiple of 16) in boxes of 128 columns by `box_rows`, 128-byte swizzle, zeros beyond.
+bool byte_map(const void* base, int64_t rows, int64_t K, int64_t ld, int box_rows, CUtensorMap* out) {
+  EncodeTiledFn fn = encode_fn();
+  if (!fn) return false;
+  const cuuint64_t dims[2] = {static_cast<cuuint64_t>(K), static_cast<cuuint64_t>(rows)}, strides[1] = {static_cast<cuuint64_t>(ld)};
+  const cuuint32_t box[2] = {128, static_cast<cuuint32_t>(box_rows)}, one[2] = {1, 1};
+  return fn(out, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// K ranges of a weight of `tiles` tiles of 128 rows and `blocks` blocks of columns.
+int fp8_ranges(int tiles, int blocks) {
+  int s = 1;
+  while (s < kMaxRanges && tiles * s * 2 <= 148 && blocks >= s * 4) s *= 2;
+  return (blocks + (blocks + s - 1) / s - 1) / ((blocks + s - 1) / s);        // (no empty range)
+}
+
+// Up to this many tokens the ranges run on CTAs of their own.
+constexpr int kSplitTokens = 128;
+
+template <int EPI, int BN, class OUT, bool GROUPED>
+int launch_tile(const void* w, int64_t rows_w, int64_t ldw, const void* q, int64_t rows_q, int64_t ldq, Fp8Params p, int tiles_m, int tiles_n,
+                cudaStream_t st) {
+  using S = Shape<BN>;
+  CUtensorMap map_w, map_x;
+  if (!byte_map(w, rows_w, p.K, ldw, EPI == kGated ? 64 : kBlock, &map_w) || !byte_map(q, rows_q, p.K, ldq, BN, &map_x))
+    return sb::fail("gemm_fp8: no tensor map for a weight of %lld x %d (stride %lld)", (long long)rows_w, p.K, (long long)ldw);
+  p.stages = std::min(kMaxStages, kSmemBudget / S::kStage);
+  const size_t smem = std::max<size_t>(static_cast<size_t>(p.stages) * S::kStage, BN * kBlock * 4) + 1024;
+  const bool split = !GROUPED && p.ranges > 1 && p.n <= kSplitTokens;
+  const dim3 grid(tiles_m, tiles_n, split ? p.ranges : 1);
+  if (split) {
+    auto kernel = gemm_fp8_kernel<EPI, BN, OUT, false, true>;
+    static sb::DeviceOnce once;
+    if (once.needed()) {
+      if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024 - 8192) != cudaSuccess) return sb::check_launch("gemm_fp8");
+      once.done();
+    }
+    sb::launch_pdl_cluster(kernel, grid, dim3(S::kThreads), smem, st, dim3(1, 1, p.ranges), map_w, map_x, p);
+  } else {
+    auto kernel = gemm_fp8_kernel<EPI, BN, OUT, GROUPED, false>;
+    static sb::DeviceOnce once;
+    if (once.needed()) {
+      if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024 - 8192) != cudaSuccess) return sb::check_launch("gemm_fp8");
+      once.done();
+    }
+    sb::launch_pdl(kernel, grid, dim3(S::kThreads), smem, st, map_w, map_x, p);
+  }
+  return sb::check_launch("gemm_fp8");
+}
+
+template <int EPI, class OUT, bool GROUPED>
+int launch_product(const void* w, int64_t rows_w, int64_t ldw, const void* q, int64_t rows_q, int64_t ldq, const Fp8Params& p, int tile_n, int tiles_n,
+                   cudaStream_t st) {
+  const int tiles_m = EPI == kGated ? (p.half_rows + 63) / 64 : (p.M + kBlock - 1) / kBlock;
+  switch (tile_n) {
+    case 16: return launch_tile<EPI, 16, OUT, GROUPED>(w, rows_w, ldw, q, rows_q, ldq, p, tiles_m, tiles_n, st);
+    case 32: return launch_tile<EPI, 32, OUT, GROUPED>(w, rows_w, ldw, q, rows_q, ldq, p, tiles_m, tiles_n, st);
+    case 64: return launch_tile<EPI, 64, OUT, GROUPED>(w, rows_w, ldw, q, rows_q, ldq, p, tiles_m, tiles_n, st);
+    default: return launch_tile<EPI, 128, OUT, GROUPED>(w, rows_w, ldw, q, rows_q, ldq, p, tiles_m, tiles_n, st);
+  }
+}
+
+int launch_quantize(const void* x, int xdtype, int64_t ldx, const int32_t* order, const int32_t* used, int n, int rows, int K, void* q, int64_t ldq, float* scales, int64_t lds,
+                    cudaStream_t st) {
+  const int blocks = (K + kBlock - 1) / kBlock;
+  const int64_t items = static_cast<int64_t>(rows) * blocks;
+  if ((items + 7) / 8 > 0x7FFFFFFF) return sb::fail("quantize_fp8: %d rows of %d columns are too many", rows, K);
+  const dim3 grid(static_cast<unsigned>((items + 7) / 8)), block(256);
+  const int size = xdtype == 0 ? 4 : 2;
+  const bool vec = K % 4 == 0 && ldx % 4 == 0 && (reinterpret_cast<uintptr_t>(x) & (4 * size - 1)) == 0;
+  uint8_t* to = static_cast<uint8_t*>(q);
+  if (xdtype == 0) {
+    const float* f = static_cast<const float*>(x);
+    if (vec) sb::launch_pdl(quantize_kernel<float, true>, grid, block, 0, st, f, ldx, order, used, n, rows, K, blocks, to, ldq, scales, lds);
+    else sb::launch_pdl(quantize_kernel<float, false>, grid, block, 0, st, f, ldx, order, used, n, rows, K, blocks, to, ldq, scales, lds);
+  } else {
+    const bf16* h = static_cast<const bf16*>(x);
+    if (vec) sb::launch_pdl(quantize_kernel<bf16, true>, grid, block, 0, st, h, ldx, order, used, n, rows, K, blocks, to, ldq, scales, lds);
+    else sb::launch_pdl(quantize_kernel<bf16, false>, grid, block, 0, st, h, ldx, order, used, n, rows, K, blocks, to, ldq, scales, lds);
+  }
+  return sb::check_launch("quantize_fp8");
+}
+
+// One product; `half_rows` > 0: gated. out_dtype 0 float32, 1 bfloat16.
+int launch_gemm(const void* q, int64_t ldq, const float* xs, int64_t ldxs, const void* w, int64_t ldw, const float* ws, void* out, int out_dtype,
+                int64_t ldo, int n, int M, int K, int epilogue, int half_rows, const Gate& gate, cudaStream_t st) {
+  Fp8Params p = {};
+  p.out = out, p.ldo = ldo, p.x_scales = xs, p.ldxs = ldxs, p.w_scales = ws;
+  p.n = n, p.M = M, p.K = K, p.blocks = (K + kBlock - 1) / kBlock, p.half_rows = half_rows;
+  p.scale_rows = epilogue == kGated ? 2 * ((half_rows + kBlock - 1) / kBlock) : (M + kBlock - 1) / kBlock;
+  p.ranges = fp8_ranges((M + kBlock - 1) / kBlock, p.blocks);
+  p.range_blocks = (p.blocks + p.ranges - 1) / p.ranges;
+  p.gate = gate;
+  p.status = status_word();
+  if (p.status == nullptr) return sb::fail("gemm_fp8: no status word on this device");
+  const int tile = n <= 16 ? 16 : n <= 32 ? 32 : n <= 64 ? 64 : 128, tiles_n = (n + tile - 1) / tile;
+  if (tiles_n > 65535) return sb::fail("gemm_fp8: %d tokens are too many", n);
+  if (epilogue == kAdd) return launch_product<kAdd, float, false>(w, M, ldw, q, n, ldq, p, tile, tiles_n, st);
+  if (epilogue == kStore)
+    return out_dtype == 0 ? launch_product<kStore, float, false>(w, M, ldw, q, n, ldq, p, tile, tiles_n, st)
+                          : launch_product<kStore, bf16, false>(w, M, ldw, q, n, ldq, p, tile, tiles_n, st);
+  return out_dtype == 0 ? launch_product<kGated, float, false>(w, M, ldw, q, n, ldq, p, tile, tiles_n, st)
+                        : launch_product<kGated, bf16, false>(w, M, ldw, q, n, ldq, p, tile, tiles_n, st);
+}
+int check_quantized(const char* who, const void* q, int64_t ldq, int64_t ldxs, int n, int K) {
+  if (n < 0 || K <= 0) return sb::fail("%s: %d rows of %d columns", who, n, K);
+  if (ldq < K || ldq % 16 || (reinterpret_cast<uintptr_t>(q) & 15)) return sb::fail("%s: rows of 8-bit values are 16-byte aligned (stride %lld, %d columns)", who, (long long)ldq, K);
+  if (ldxs < n) return sb::fail("%s: %lld scales for %d rows", who, (long long)ldxs, n);
+  return 0;
+}
+int check_product(const char* who, const void* w, int64_t ldw, int out_dtype, int64_t ldo, int M, int K, int epilogue, int half_rows) {
+  if (M <= 0 || epilogue < kStore || epilogue > kGated) return sb::fail("%s: %d weight rows, epilogue %d", who, M, epilogue);
+  if (ldw < K || ldw % 16 || (reinterpret_cast<uintptr_t>(w) & 15)) return sb::fail("%s: weight rows are 16-byte aligned (stride %lld, %d columns)", who, (long long)ldw, K);
+  if (epilogue == kGated && (half_rows <= 0 || 2 * half_rows != M)) return sb::fail("%s: a gated product has as many gate rows as up rows (%d of %d)", who, half_rows, M);
+  if (out_dtype < 0 || out_dtype > 1 || (epilogue == kAdd && out_dtype != 0)) return sb::fail("%s: results are float32 or bfloat16, sums float32", who);
+  if (ldo < (epilogue == kGated ? half_rows : M)) return sb::fail("%s: rows of %lld results for %d weight rows", who, (long long)ldo, M);
+  return 0;
+}
+
+// Rows of a tile of the experts' products: near the rows an expert gets on average (a row's result does not depend on it).
+int expert_tile(int pairs, int E) {
+  const int mean = (pairs + E - 1) / E;
+  return mean <= 16 ? 16 : mean <= 32 ? 32 : mean <= 64 ? 64 : 128;
+}
+int most_tiles(int pairs, int E, int tile) { return std::min(pairs, pairs / tile + std::min(pairs, E)); }
+
+// Where an expert call's intermediate results lie in its scratch buffer, every one 256-byte aligned.
+struct ExpertScratch {
+  int64_t order, list, xq, xs, z, zq, zs, parts, bytes, ldx, ldz;
+};
+ExpertScratch expert_scratch(int64_t n, int64_t top, int64_t E, int64_t W, int64_t F) {
+  ExpertScratch s;
+  const int64_t pairs = n * top;
+  int64_t at = 0;
+  auto take = [&](int64_t bytes) {
+    const int64_t here = at;
+    at += (bytes + 255) / 256 * 256;
+    return here;
+  };
+  s.ldx = (W + 15) / 16 * 16, s.ldz = (F + 15) / 16 * 16;
+  s.order = take(4 * pairs), s.list = take(4 * (2 + 3 * pairs));
+  s.xq = take(pairs * s.ldx), s.xs = take(4 * pairs * ((W + kBlock - 1) / kBlock));
+  s.z = take(4 * pairs * F), s.zq = take(pairs * s.ldz), s.zs = take(4 * pairs * ((F + kBlock - 1) / kBlock));
+  s.parts = take(4 * pairs * W);
+  s.bytes = at;
+  return s;
+}
+
+}  // namespace
+
+SB_EXPORT void sb_gemm_fp8_use_status_word(int* device_word) { status_word_given() = device_word; }
+
+// x [n][ldx] float32 (0) or bfloat16 (1) -> q [n][ldq] e4m3, scales [ceil(K / 128)][lds] float32.
+SB_EXPORT int sb_quantize_fp8(const void* x, int xdtype, int64_t ldx, void* q, int64_t ldq, float* scales, int64_t lds, int n, int K, void* stream) {
+  if (int rc = check_quantized("quantize_fp8", q, ldq, lds, n, K)) return rc;
+  if (xdtype < 0 || xdtype > 1 || ldx < K) return sb::fail("quantize_fp8: rows of %lld elements, %d columns", (long long)ldx, K);
+  if (n == 0) return 0;
+  return launch_quantize(x, xdtype, ldx, nullptr, nullptr, n, n, K, q, ldq, scales, lds, static_cast<cudaStream_t>(stream));
+}
+
+// out = x . w^T of quantised x; epilogue 0 store, 1 add, 2 gated (w: half_rows gate rows, then as many up rows; act, limit, slope: the gate).
+SB_EXPORT int sb_gemm_fp8(const void* q, int64_t ldq, const float* xs, int64_t ldxs, const void* w, int64_t ldw, const float* ws, void* out, int out_dtype,
+                          int64_t ldo, int n, int M, int K, int epilogue, int half_rows, int act, float limit, float slope, void* stream) {
+  if (int rc = check_quantized("gemm_fp8", q, ldq, ldxs, n, K)) return rc;
+  if (int rc = check_product("gemm_fp8", w, ldw, out_dtype, ldo, M, K, epilogue, half_rows)) return rc;
+  if (n == 0) return 0;
+  Gate gate;
+  gate.act = act, gate.limit = limit, gate.slope = slope;
+  return launch_gemm(q, ldq, xs, ldxs, w, ldw, ws, out, out_dtype, ldo, n, M, K, epilogue, half_rows, gate, static_cast<cudaStream_t>(stream));
+}
+
+// Both: x is quantised into the buffers q and xs first.
+SB_EXPORT int sb_linear_fp8(const void* x, int xdtype, int64_t ldx, void* q, int64_t ldq, float* xs, int64_t ldxs, const void* w, int64_t ldw, const float* ws,
+                            void* out, int out_dtype, int64_t ldo, int n, int M, int K, int epilogue, int half_rows, int act, float limit, float slope,
+                            void* stream) {
+  if (int rc = check_quantized("linear_fp8", q, ldq, ldxs, n, K)) return rc;
+  if (int rc = check_product("linear_fp8", w, ldw, out_dtype, ldo, M, K, epilogue, half_rows)) return rc;
+  if (xdtype < 0 || xdtype > 1 || ldx < K) return sb::fail("linear_fp8: rows of %lld elements, %d columns", (long long)ldx, K);
+  if (n == 0) return 0;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (int rc = launch_quantize(x, xdtype, ldx, nullptr, nullptr, n, n, K, q, ldq, xs, ldxs, st)) return rc;
+  Gate gate;
+  gate.act = act, gate.limit = limit, gate.slope = slope;
+  return launch_gemm(q, ldq, xs, ldxs, w, ldw, ws, out, out_dtype, ldo, n, M, K, epilogue, half_rows, gate, st);
+}
+
+// Bytes of scratch that `sb_experts_fp8` needs for n tokens.
+SB_EXPORT int64_t sb_experts_fp8_scratch(int n, int top, int E, int W, int F) { return expert_scratch(n, top, E, W, F).bytes; }
+
+// out[t] = sum over k of weights[k][t] D_e (silu(G_e x_t) * (U_e x_t)), e = choice[t][k] (no expert: no term). gate_up [E 2F][ldg] e4m3 (an
+// expert's gate rows, then its up rows) with scales [E 2 ceil(F / 128)][ceil(W / 128)], down [E W][ldd] with [E ceil(W / 128)][ceil(F / 128)].
+// The gated products stay in 32-bit until they are quantised.
+SB_EXPORT int sb_experts_fp8(const void* x, int xdtype, int64_t ldx, const int32_t* choice, const float* weights, const void* gate_up, int64_t ldg,
+                             const float* gate_up_scales, const void* down, int64_t ldd, const float* down_scales, void* out, int out_dtype, int64_t ldo,
+                             int n, int top, int E, int W, int F, void* scratch, int64_t scratch_bytes, void* stream) {
+  const char* who = "experts_fp8";
+  if (n < 0 || top < 1 || E < 1 || E > kMaxExperts || W < 1 || F < 1) return sb::fail("%s: %d of %d experts (at most %d), %d tokens, sizes %d and %d", who, top, E, kMaxExperts, n, W, F);
+  if (static_cast<int64_t>(n) * top > (1 << 24) || static_cast<int64_t>(E) * std::max(2 * F, W) > 0x7FFFFFFF)
+    return sb::fail("%s: %d tokens with %d choices, %d experts of %d x %d: too many rows", who, n, top, E, F, W);
+  if (xdtype < 0 || xdtype > 1 || ldx < W || out_dtype < 0 || out_dtype > 1 || ldo < W) return sb::fail("%s: rows of %lld and %lld elements for a width of %d", who, (long long)ldx, (long long)ldo, W);
+  if (int rc = check_product(who, gate_up, ldg, 0, F, 2 * F, W, kGated, F)) return rc;
+  if (int rc = check_product(who, down, ldd, 0, W, W, F, kStore, 0)) return rc;
+  const ExpertScratch s = expert_scratch(n, top, E, W, F);
+  if (scratch_bytes < s.bytes || (reinterpret_cast<uintptr_t>(scratch) & 15)) return sb::fail("%s: %lld bytes of scratch where %lld are needed", who, (long long)scratch_bytes, (long long)s.bytes);
+  if (n == 0) return 0;
+  int* status = status_word();
+  if (status == nullptr) return sb::fail("%s: no status word on this device", who);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  uint8_t* base = static_cast<uint8_t*>(scratch);
+  int32_t *order = reinterpret_cast<int32_t*>(base + s.order), *list = reinterpret_cast<int32_t*>(base + s.list);
+  float *xs = reinterpret_cast<float*>(base + s.xs), *z = reinterpret_cast<float*>(base + s.z), *zs = reinterpret_cast<float*>(base + s.zs);
+  float* parts = reinterpret_cast<float*>(base + s.parts);
+  const int pairs = n * top, tile = expert_tile(pairs, E), tiles = most_tiles(pairs, E, tile);
+  if (tiles > 65535) return sb::fail("%s: %d tiles of rows are too many", who, tiles);
+  sb::launch_pdl(expert_order_kernel, dim3(1), dim3(kOrderThreads), 0, st, choice, n, top, E, tile, order, list);
+  if (int rc = sb::check_launch(who)) return rc;
+  if (int rc = launch_quantize(x, xdtype, ldx, order, list + 1, n, pairs, W, base + s.xq, s.ldx, xs, pairs, st)) return rc;
+  Fp8Params p = {};
+  p.tiles = list, p.order = order, p.status = status, p.n = n, p.ranges = 1;
+  p.out = z, p.ldo = F, p.x_scales = xs, p.ldxs = pairs, p.w_scales = gate_up_scales, p.M = 2 * F, p.K = W, p.half_rows = F;
+  p.blocks = p.range_blocks = (W + kBlock - 1) / kBlock, p.scale_rows = 2 * ((F + kBlock - 1) / kBlock);
+  if (int rc = launch_product<kGated, float, true>(gate_up, static_cast<int64_t>(E) * 2 * F, ldg, base + s.xq, pairs, s.ldx, p, tile, tiles, st)) return rc;
+  if (int rc = launch_quantize(z, 0, F, nullptr, list + 1, pairs, pairs, F, base + s.zq, s.ldz, zs, pairs, st)) return rc;
+  p.out = parts, p.ldo = W, p.x_scales = zs, p.w_scales = down_scales, p.M = W, p.K = F, p.half_rows = 0, p.pair_weight = weights;
+  p.blocks = p.range_blocks = (F + kBlock - 1) / kBlock, p.scale_rows = (W + kBlock - 1) / kBlock;
+  if (int rc = launch_product<kStore, float, true>(down, static_cast<int64_t>(E) * W, ldd, base + s.zq, pairs, s.ldz, p, tile, tiles, st)) return rc;
+  const dim3 grid(n, n >= 296 ? 1 : std::min((W + 255) / 256, (296 + n - 1) / n));
+  if (out_dtype == 0)
+    sb::launch_pdl(expert_combine_kernel<float>, grid, dim3(256), 0, st, static_cast<const float*>(parts), choice, n, top, E, W, static_cast<float*>(out), ldo);
+  else
+    sb::launch_pdl(expert_combine_kernel<bf16>, grid, dim3(256), 0, st, static_cast<const float*>(parts), choice, n, top, E, W, static_cast<bf16*>(out), ldo);
+  return sb::check_launch(who);
+}

@@ -53,6 +53,8 @@ SOURCES = {
     "streams": "streams.cu",
     "grouped_gemm": "grouped_gemm.cu",
     "short_conv": "short_conv.cu",
+    "gemm_fp8": "gemm_fp8.cu",
+    "router": "router.cu",
     "runtime": "runtime.cpp",        # host code only: the cache manager's books and the scheduler's decisions
 }
 HOST_FLAGS = ["-O2", "-std=c++17", "-g1", "-shared", "-fPIC", "-fvisibility=hidden"]

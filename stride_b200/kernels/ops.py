@@ -306,7 +306,7 @@ def gemm_tc_status() -> int:
 _status_word = None
 _status_users = {"gemm_tc": "sb_gemm_tc_use_status_word", "attention_tc5": "sb_attention_tc5_use_status_word",
                  "decode_chain": "sb_decode_chain_use_status_word", "grouped_gemm": "sb_grouped_gemm_use_status_word",
-                 "masked_attention": "sb_masked_attention_use_status_word",
+                 "masked_attention": "sb_masked_attention_use_status_word", "gemm_fp8": "sb_gemm_fp8_use_status_word",
                  "sampling": "sb_sampling_use_status_word"}   # the sampling kernels only read it
 _status_registered: set = set()
 
@@ -719,3 +719,136 @@ def head_linear(x: torch.Tensor, weight: torch.Tensor, out: torch.Tensor, tail: 
                                                          c_int, c_int, c_int, c_void_p])
     _check(lib, fn(_ptr(x), x.stride(0), x.stride(1), _ptr(weight), _ptr(out), out.stride(0), out.stride(1), dtype_code(x.dtype), x.shape[0], H, K, N,
                    tail, _stream()))
+
+
+# ---------------------------------------------------------------------------------------------------------------------------------
+# 8-bit weights with a scale per block of 128 x 128, routing to experts, the experts' products (csrc/gemm_fp8.cu, csrc/router.cu)
+
+FP8_BLOCK = 128
+_EPILOGUES_FP8 = {STORE: 0, ADD: 1, SWIGLU: 2, GEGLU_TANH: 2, CLAMPED_GLU: 2}
+
+
+def _check_fp8_rows(what: str, q: torch.Tensor, scales: torch.Tensor, n: int, K: int) -> None:
+    if q.dtype != torch.float8_e4m3fn or scales.dtype != torch.float32:
+        raise TypeError(f"{what}: quantised rows are float8_e4m3fn with float32 scales")
+    if q.dim() != 2 or q.shape[0] != n or q.shape[1] < K or (q.shape[1] > 1 and q.stride(1) != 1):
+        raise ValueError(f"{what}: {n} rows of {K} columns in a buffer of shape {tuple(q.shape)}")
+    if scales.dim() != 2 or scales.shape[0] != -(-K // FP8_BLOCK) or scales.shape[1] < n or (scales.shape[1] > 1 and scales.stride(1) != 1):
+        raise ValueError(f"{what}: scales are [ceil({K} / {FP8_BLOCK}), {n}], not {tuple(scales.shape)}")
+
+
+def _row_stride(t: torch.Tensor) -> int:
+    """Elements from a row to the next (of a single row: its length, whatever its stride says)."""
+    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1])
+
+
+def quantize_fp8(x: torch.Tensor, q: torch.Tensor, scales: torch.Tensor) -> None:
+    """q[i, j] = e4m3(x[i, j] / s), s = scales[j // 128, i] = 2^e the smallest power of two (e >= -100) with max |x| of the row's block of 128
+    columns / s <= 448. x [n, K] float32 or bfloat16; q [n, K or more columns] float8_e4m3fn with rows 16-byte aligned; scales float32
+    [ceil(K / 128), n or more]. A block that holds an infinity or a NaN gets the scale NaN."""
+    _cuda(x, q, scales)
+    n, K = x.shape
+    _check_fp8_rows("quantize_fp8", q, scales, n, K)
+    if x.stride(1) != 1 and K > 1:
+        raise ValueError("quantize_fp8 takes rows of consecutive elements")
+    lib, fn = _fn("gemm_fp8", "sb_quantize_fp8", [c_void_p, c_int, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_int, c_int, c_void_p])
+    _check(lib, fn(_ptr(x), dtype_code(x.dtype), _row_stride(x), _ptr(q), _row_stride(q), _ptr(scales), _row_stride(scales), n, K, _stream()))
+
+
+def _fp8_product(weight, out: torch.Tensor, epilogue: int, n: int):
+    """(weight's address, stride, scales, out's address, dtype, stride, M, epilogue code, half rows, gate) of a product, checked."""
+    M = weight.shape[0]
+    code = _EPILOGUES_FP8[epilogue]
+    half = M // 2 if code == 2 else 0
+    if code == 2 and weight.halves != 2:
+        raise ValueError("a gated product takes a weight stacked from a gate and an up matrix of one shape")
+    if code != 2 and not weight.in_blocks:
+        raise ValueError("a stacked weight whose matrices are no whole number of 128 rows only has the gated product")
+    if out.dim() != 2 or out.shape[0] != n or out.shape[1] != (half or M) or (out.shape[1] > 1 and out.stride(1) != 1):
+        raise ValueError(f"gemm_fp8 writes [{n}, {half or M}], not {tuple(out.shape)}")
+    return M, code, half
+
+
+def gemm_fp8(q: torch.Tensor, scales: torch.Tensor, weight, out: torch.Tensor, epilogue: int = STORE, constants=(0.0, 0.0)) -> None:
+    """out = x . weight^T of rows that `quantize_fp8` made, weight an `Fp8Weight`: sums of blocks of 128 columns times both scales, added in 32-bit.
+
+    STORE: out float32 or bfloat16 [n, M]. ADD: out float32 += result. SWIGLU, GEGLU_TANH, CLAMPED_GLU: weight stacked from gate and up rows,
+    out float32 or bfloat16 [n, M / 2] (`gemm_tc`)."""
+    _cuda(q, scales, weight.q, out)
+    n, K = q.shape[0], weight.shape[1]
+    _check_fp8_rows("gemm_fp8", q, scales, n, K)
+    M, code, half = _fp8_product(weight, out, epilogue, n)
+    lib, fn = _fn("gemm_fp8", "sb_gemm_fp8", [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_int, c_int64, c_int, c_int,
+                                              c_int, c_int, c_int, c_int, c_float, c_float, c_void_p])
+    _check(lib, fn(_ptr(q), _row_stride(q), _ptr(scales), _row_stride(scales), _ptr(weight.q), weight.stride, _ptr(weight.scales), _ptr(out),
+                   dtype_code(out.dtype), _row_stride(out), n, M, K, code, half, max(epilogue - SWIGLU, 0), *constants, _stream()))
+
+
+def linear_fp8(x: torch.Tensor, q: torch.Tensor, scales: torch.Tensor, weight, out: torch.Tensor, epilogue: int = STORE, constants=(0.0, 0.0)) -> None:
+    """`quantize_fp8` of x into the buffers q and scales, then `gemm_fp8`, in one call."""
+    _cuda(x, q, scales, weight.q, out)
+    n, K = x.shape
+    if K != weight.shape[1] or (K > 1 and x.stride(1) != 1):
+        raise ValueError(f"linear_fp8 shapes: x {tuple(x.shape)}, weight {tuple(weight.shape)}")
+    _check_fp8_rows("linear_fp8", q, scales, n, K)
+    M, code, half = _fp8_product(weight, out, epilogue, n)
+    lib, fn = _fn("gemm_fp8", "sb_linear_fp8", [c_void_p, c_int, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p,
+                                                c_int, c_int64, c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_float, c_void_p])
+    _check(lib, fn(_ptr(x), dtype_code(x.dtype), _row_stride(x), _ptr(q), _row_stride(q), _ptr(scales), _row_stride(scales), _ptr(weight.q), weight.stride,
+                   _ptr(weight.scales), _ptr(out), dtype_code(out.dtype), _row_stride(out), n, M, K, code, half, max(epilogue - SWIGLU, 0), *constants,
+                   _stream()))
+
+
+ROUTER_SCORES = {"sigmoid": 0, "softmax": 1}
+
+
+def route_experts(logits: torch.Tensor, choice: torch.Tensor, weights: torch.Tensor, score: str = "sigmoid", bias=None, groups: int = 1,
+                  top_groups: int = 1, group_best: int = 2, renormalise: bool = True, scale: float = 1.0) -> None:
+    """Every token's experts and their weights from a router's logits [n, experts] float32 (csrc/router.cu): s = softmax or sigmoid of the logits, the
+    `top` experts with the largest s + bias of the `top_groups` groups with the largest sums of their `group_best` largest s + bias, by descending
+    s + bias; weight s (divided by (the chosen s' sum + 1e-20) if `renormalise`) times `scale`.
+    choice [n, top] int32, weights [top, n] float32. An expert with a logit or a bias of -infinity or NaN is never chosen; a place that nothing is
+    left for gets -1 and weight 0."""
+    _cuda(logits, bias, choice, weights)
+    if score not in ROUTER_SCORES:
+        raise ValueError(f"route_experts: unknown score '{score}' (known: {', '.join(ROUTER_SCORES)})")
+    n, E = logits.shape
+    top = choice.shape[1]
+    if logits.dtype != torch.float32 or weights.dtype != torch.float32 or choice.dtype != torch.int32 or (bias is not None and bias.dtype != torch.float32):
+        raise TypeError("route_experts takes float32 logits, bias and weights and an int32 choice")
+    if tuple(choice.shape) != (n, top) or not choice.is_contiguous() or tuple(weights.shape) != (top, n) or (n > 1 and weights.stride(1) != 1) \
+            or (E > 1 and logits.stride(1) != 1) or (bias is not None and (tuple(bias.shape) != (E,) or not bias.is_contiguous())):
+        raise ValueError(f"route_experts shapes: logits {tuple(logits.shape)}, choice {tuple(choice.shape)}, weights {tuple(weights.shape)}"
+                         + (f", bias {tuple(bias.shape)}" if bias is not None else ""))
+    lib, fn = _fn("router", "sb_route_experts", [c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_int64, c_int, c_int, c_int, c_int, c_int, c_int, c_int,
+                                                 c_int, c_float, c_void_p])
+    _check(lib, fn(_ptr(logits), _row_stride(logits), _ptr(bias), _ptr(choice), _ptr(weights), _row_stride(weights), n, E, top, ROUTER_SCORES[score], groups,
+                   top_groups, group_best, int(renormalise), scale, _stream()))
+
+
+def experts_fp8_scratch(n: int, top: int, experts: int, width: int, inner: int) -> int:
+    """Bytes of scratch `experts_fp8` needs for n tokens."""
+    lib = library("gemm_fp8")
+    lib.sb_experts_fp8_scratch.argtypes, lib.sb_experts_fp8_scratch.restype = [c_int] * 5, c_int64
+    return lib.sb_experts_fp8_scratch(n, top, experts, width, inner)
+
+
+def experts_fp8(x: torch.Tensor, choice: torch.Tensor, weights: torch.Tensor, experts, out: torch.Tensor, scratch: torch.Tensor) -> None:
+    """out[t] = sum over k of weights[k, t] * down_e (silu(gate_e x_t) * (up_e x_t)), e = choice[t, k], in the order of the choices; an id that is no
+    expert's has no term. x [n, width] float32 or bfloat16, choice [n, top] int32, weights [top, n] float32, `experts` an `Fp8Experts`, out float32 or
+    bfloat16 [n, width], scratch uint8 of `experts_fp8_scratch` bytes. Inputs of both projections are quantised as `quantize_fp8` does."""
+    _cuda(x, choice, weights, experts.gate_up, out, scratch)
+    n, W = x.shape
+    top = choice.shape[1]
+    if choice.dtype != torch.int32 or weights.dtype != torch.float32 or scratch.dtype != torch.uint8:
+        raise TypeError("experts_fp8 takes an int32 choice, float32 weights and uint8 scratch")
+    if W != experts.width or tuple(out.shape) != (n, W) or tuple(choice.shape) != (n, top) or tuple(weights.shape) != (top, n) \
+            or not choice.is_contiguous() or not weights.is_contiguous() or not scratch.is_contiguous() \
+            or (W > 1 and (x.stride(1) != 1 or out.stride(1) != 1)):
+        raise ValueError(f"experts_fp8 shapes: x {tuple(x.shape)}, choice {tuple(choice.shape)}, weights {tuple(weights.shape)}, out {tuple(out.shape)}, "
+                         f"experts of width {experts.width}")
+    lib, fn = _fn("gemm_fp8", "sb_experts_fp8", [c_void_p, c_int, c_int64, c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_void_p,
+                                                 c_void_p, c_int, c_int64, c_int, c_int, c_int, c_int, c_int, c_void_p, c_int64, c_void_p])
+    _check(lib, fn(_ptr(x), dtype_code(x.dtype), _row_stride(x), _ptr(choice), _ptr(weights), _ptr(experts.gate_up), experts.gate_up.stride(0),
+                   _ptr(experts.gate_up_scales), _ptr(experts.down), experts.down.stride(0), _ptr(experts.down_scales), _ptr(out), dtype_code(out.dtype),
+                   _row_stride(out), n, top, experts.experts, W, experts.inner, _ptr(scratch), scratch.numel(), _stream()))

@@ -1,0 +1,344 @@
+"""Linear layers with 8-bit weights, routing to experts and the experts' products, against their formulas in 64 bits (plain_fp8.py)."""
+from __future__ import annotations
+
+import pytest
+import torch
+
+import plain_fp8 as plain
+
+pytestmark = pytest.mark.gpu
+
+BF, F32, F64 = torch.bfloat16, torch.float32, torch.float64
+HALF_STEP = {BF: 2.0 ** -8, F32: 2.0 ** -24}
+
+
+def _rand(seed, *shape, dtype=F32, std=1.0):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    return (std * torch.randn(*shape, generator=g, device="cuda")).to(dtype)
+
+
+def _weight(seed, M, K):
+    from stride_b200.kernels.linear import Fp8Weight
+    return Fp8Weight.quantize(_rand(seed, M, K, std=K ** -0.5))
+
+
+def _values(w):
+    """What a plain (not stacked) weight stands for, in 64 bits."""
+    return plain.weight_values(w.q[:, :w.shape[1]].to(F32), w.scales)
+
+
+def _workspace(n):
+    from stride_b200.parts.context import Workspace
+    return Workspace(torch.device("cuda"), n)
+
+
+def _quantize(x):
+    from stride_b200.kernels import ops
+    n, K = x.shape
+    q = torch.zeros(n, -(-K // 16) * 16, dtype=torch.uint8, device="cuda").view(torch.float8_e4m3fn)
+    s = torch.zeros(-(-K // 128), n, device="cuda")
+    ops.quantize_fp8(x, q, s)
+    return q, s
+
+
+@pytest.mark.parametrize("n,K", [(1, 1), (1, 128), (3, 127), (5, 129), (17, 200), (2, 1000), (333, 2056), (64, 4096), (700, 260)])
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_quantised_rows(n, K, dtype):
+    """Scales and values are exact: equal to the formula's, blocks of zeros, of tiny and of huge values and borders of the grid among them."""
+    x = _rand(n * K, n, K, dtype=dtype)
+    x[0, : K // 2] = 0
+    x[-1] *= 2.0 ** 40
+    if n > 2:
+        x[1] *= 2.0 ** -120
+        x[2] = 448.0
+        x[2, ::3] = 26.0         # between two values: 448 has the scale 1, 26 is one of the grid's
+        x[2, 1::3] = 25.0        # half way between 24 and 26: to even
+    q, s = _quantize(x)
+    want, scales = plain.quantised(x.to(F64))
+    assert torch.equal(s.t().to(F64), scales)
+    assert torch.equal(q[:, :K].to(F64), want)
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), float("-inf")])
+def test_a_block_that_is_not_finite_poisons_its_token_only(bad):
+    from stride_b200.kernels.linear import Linear
+    x = _rand(1, 5, 300, dtype=BF)
+    clean, out = torch.empty(5, 70, device="cuda"), torch.empty(5, 70, device="cuda")
+    layer = Linear(_weight(2, 70, 300), BF)
+    layer.forward(x, clean, workspace=_workspace(5))
+    x[3, 170] = bad
+    layer.forward(x, out, workspace=_workspace(5))
+    assert torch.isnan(out[3]).all()
+    assert torch.equal(out[[0, 1, 2, 4]], clean[[0, 1, 2, 4]])
+
+
+SIZES = [(1, 1, 1), (1, 128, 128), (2, 130, 100), (16, 2048, 2048), (17, 500, 1000), (40, 128, 4096), (64, 1000, 900), (65, 300, 2056), (129, 256, 640),
+         (333, 2500, 2056), (1000, 640, 384)]
+
+
+@pytest.mark.parametrize("n,M,K", SIZES)
+@pytest.mark.parametrize("x_dtype,out_dtype", [(BF, F32), (F32, BF), (BF, BF), (F32, F32)])
+def test_product(n, M, K, x_dtype, out_dtype):
+    from stride_b200.kernels.linear import Linear
+    x, w = _rand(n + M, n, K, dtype=x_dtype), _weight(K, M, K)
+    out = torch.full((n, M), float("nan"), dtype=out_dtype, device="cuda")
+    Linear(w, BF).forward(x, out, workspace=_workspace(n))
+    xv, wv = plain.quantised_values(x.to(F64)), _values(w)
+    want, bound = xv @ wv.t(), plain.product_bound(xv, wv)
+    assert ((out.to(F64) - want).abs() <= bound + HALF_STEP[out_dtype] * (want.abs() + bound)).all()
+
+
+@pytest.mark.parametrize("n,I,K", [(1, 1, 16), (1, 64, 128), (3, 100, 300), (8, 8192, 2048), (31, 65, 2048), (64, 1000, 520), (200, 200, 700), (333, 1408, 2056)])
+@pytest.mark.parametrize("out_dtype", [BF, F32])
+def test_gated_product(n, I, K, out_dtype):
+    """Gate and up matrices of any height, also where the up rows' scales do not begin at a multiple of 128."""
+    from stride_b200.kernels.linear import Fp8Weight, Linear
+    x, gate, up = _rand(n + I, n, K, dtype=BF), _weight(K, I, K), _weight(K + 1, I, K)
+    out = torch.full((n, I), float("nan"), dtype=out_dtype, device="cuda")
+    Linear(Fp8Weight.stack([gate, up]), BF).forward_swiglu(x, out, None, workspace=_workspace(n))
+    want, bound = plain.gated(plain.quantised_values(x.to(F64)), _values(gate), _values(up))
+    assert ((out.to(F64) - want).abs() <= bound + HALF_STEP[out_dtype] * (want.abs() + bound)).all()
+
+
+@pytest.mark.parametrize("n", [1, 20, 300])
+@pytest.mark.parametrize("activation,constants", [("gelu_tanh", ()), ("clamped", (1.5, 1.7))])
+def test_other_gates(n, activation, constants):
+    from stride_b200.kernels import ops
+    from stride_b200.kernels.linear import Fp8Weight, Linear
+    x, gate, up = _rand(n, n, 256, dtype=BF), _weight(5, 192, 256), _weight(6, 192, 256)
+    out, ws = torch.empty(n, 192, dtype=BF, device="cuda"), _workspace(n)
+    Linear(Fp8Weight.stack([gate, up]), BF).forward_swiglu(x, out, None, activation, constants, workspace=ws)
+    g, u = torch.empty(n, 192, device="cuda"), torch.empty(n, 192, device="cuda")
+    Linear(gate, BF).forward(x, g, workspace=ws)
+    Linear(up, BF).forward(x, u, workspace=ws)
+    g, u = g.to(F64), u.to(F64)
+    if activation == "gelu_tanh":
+        want = 0.5 * g * (1.0 + torch.tanh((2.0 / torch.pi) ** 0.5 * (g + 0.044715 * g ** 3))) * u
+    else:
+        want = g.clamp(max=1.5) * torch.sigmoid(1.7 * g.clamp(max=1.5)) * (u.clamp(-1.5, 1.5) + 1.0)
+    assert ((out.to(F64) - want).abs() <= 2.0 ** -8 * want.abs() + 2.0 ** -18 * (1.0 + u.abs())).all()
+
+
+@pytest.mark.parametrize("n", [1, 30, 200])
+def test_added_to_the_residual(n):
+    from stride_b200.kernels import ops
+    x, w, h = _rand(n, n, 512, dtype=BF), _weight(9, 384, 512), _rand(8, n, 384)
+    q, s = _quantize(x)
+    alone, out = torch.empty(n, 384, device="cuda"), h.clone()
+    ops.gemm_fp8(q, s, w, alone)
+    ops.gemm_fp8(q, s, w, out, ops.ADD)
+    assert torch.equal(out, alone + h)
+
+
+@pytest.mark.parametrize("M,K", [(128, 8192), (2048, 2048), (1500, 4104), (640, 260), (20000, 256)])
+def test_a_tokens_bits_do_not_depend_on_the_step(M, K):
+    """Alone, in a few, in tiles of every size, the ranges of K on CTAs of their own and walked by one: the same bits."""
+    from stride_b200.kernels.linear import Linear
+    x, layer = _rand(M, 300, K, dtype=BF), Linear(_weight(K, M, K), BF)
+    whole = torch.empty(300, M, device="cuda")
+    layer.forward(x, whole, workspace=_workspace(300))
+    for first, n in [(0, 1), (7, 16), (30, 17), (60, 33), (100, 65), (100, 128), (170, 129)]:
+        part = torch.full((n, M), float("nan"), device="cuda")
+        layer.forward(x[first:first + n], part, workspace=_workspace(300))
+        assert torch.equal(part, whole[first:first + n]), (first, n)
+
+
+def test_rows_of_larger_tensors_and_what_lies_around_them():
+    """Input and result as column ranges of wider buffers, a narrow slice that starts off a 16-byte border; what is around the result stays."""
+    from stride_b200.kernels.linear import Linear
+    wide, layer = _rand(3, 50, 1003, dtype=BF), Linear(_weight(4, 200, 257), BF)
+    x = wide[:, 5:262]
+    want = torch.empty(50, 200, device="cuda")
+    layer.forward(x.contiguous(), want, workspace=_workspace(64))
+    held = torch.full((52, 333), 7.0, device="cuda")
+    layer.forward(x, held[1:51, 100:300], workspace=_workspace(64))
+    assert torch.equal(held[1:51, 100:300], want)
+    held[1:51, 100:300] = 7.0
+    assert (held == 7.0).all()
+
+
+def test_product_in_a_graph_and_on_another_stream():
+    from stride_b200.kernels.linear import Linear
+    x, layer, ws = _rand(3, 9, 640, dtype=BF), Linear(_weight(4, 512, 640), BF), _workspace(9)
+    out, want = torch.empty(9, 512, device="cuda"), torch.empty(9, 512, device="cuda")
+    layer.forward(x, want, workspace=ws)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        layer.forward(x, out, workspace=ws)
+    side.synchronize()
+    assert torch.equal(out, want)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        layer.forward(x, out, workspace=ws)
+    x.copy_(_rand(5, 9, 640, dtype=BF))
+    layer.forward(x, want, workspace=ws)
+    out.zero_()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, want)
+
+
+# ------------------------------------------------------------------ routing
+ROUTES = [(1, 8, 2, {}), (5, 1, 1, {}), (33, 90, 6, {"score": "softmax", "renormalise": False}), (200, 256, 8, {"groups": 8, "top_groups": 4, "scale": 2.5}),
+          (64, 160, 6, {"score": "softmax", "groups": 8, "top_groups": 3, "group_best": 1, "renormalise": False, "scale": 16.0}),
+          (40, 1024, 32, {"groups": 32, "top_groups": 5}), (17, 33, 33 - 1, {}), (9, 12, 3, {"groups": 4, "top_groups": 1}), (100, 511, 9, {"score": "softmax"}),
+          (7, 6, 2, {"groups": 6, "top_groups": 2})]
+
+
+def _route(z, top, bias=None, **kw):
+    from stride_b200.kernels import ops
+    n = z.shape[0]
+    choice = torch.full((n, top), -7, dtype=torch.int32, device="cuda")
+    weights = torch.full((top, n), float("nan"), device="cuda")
+    ops.route_experts(z, choice, weights, bias=bias, **kw)
+    return choice.cpu(), weights.cpu()
+
+
+def _close(weights, want):
+    return ((weights.to(F64) - want).abs() <= 2.0 ** -20 * want.abs() + 1e-37).all()
+
+
+@pytest.mark.parametrize("n,E,top,kw", ROUTES)
+@pytest.mark.parametrize("biased", [False, True])
+def test_routes(n, E, top, kw, biased):
+    z = _rand(E, n, E, std=1.5)
+    bias = _rand(E + 1, E, std=0.1) if biased else None
+    choice, weights = _route(z, top, bias, **kw)
+    want, want_weights = plain.route(z.cpu(), top, kw.get("score", "sigmoid"), None if bias is None else bias.cpu(), **{k: v for k, v in kw.items() if k != "score"})
+    assert torch.equal(choice, want)
+    assert _close(weights, want_weights)
+
+
+@pytest.mark.parametrize("score", ["sigmoid", "softmax"])
+@pytest.mark.parametrize("kw", [{}, {"groups": 4, "top_groups": 2}])
+def test_routes_with_ties_masks_and_odd_logits(score, kw):
+    """Equal logits, experts switched off by their logit or their bias, rows with fewer experts than places or none, infinities, NaN, the largest and
+    the smallest floats."""
+    z = _rand(3, 12, 32)
+    z[0] = 0.25
+    z[1] = torch.arange(32, device="cuda") // 5
+    z[2] = float("-inf")
+    z[3, 3:] = float("-inf")
+    z[4] = float("nan")
+    z[5, ::2] = float("nan")
+    z[6, 7] = float("inf")
+    z[7, 7], z[7, 20] = float("inf"), float("inf")
+    z[8] = -3.0e38
+    z[9] = 3.0e38
+    z[10] = torch.linspace(30, 45, 32, device="cuda")
+    z[11, 1:] = float("-inf")
+    bias = _rand(4, 32, std=0.1)
+    bias[5], bias[9] = float("-inf"), float("nan")
+    for b in (None, bias):
+        choice, weights = _route(z, 6, b, score=score, **kw)
+        want, want_weights = plain.route(z.cpu(), 6, score, None if b is None else b.cpu(), **kw)
+        assert torch.equal(choice, want)
+        assert _close(weights, want_weights)
+
+
+def test_routes_that_only_64_bits_tell_apart():
+    """Scores plus bias that differ by less than half a 32-bit step of their size: the larger wins, whatever its place."""
+    z = torch.zeros(64, 40, device="cuda")
+    z += torch.arange(40, device="cuda") * 2.0 ** -26 * (1 - 2 * (torch.arange(64, device="cuda") % 2))[:, None]
+    bias = torch.full((40,), 4.0, device="cuda")
+    for kw in ({}, {"score": "softmax"}, {"groups": 4, "top_groups": 2}):
+        choice, _ = _route(z, 7, bias, **kw)
+        want, _ = plain.route(z.cpu(), 7, kw.get("score", "sigmoid"), bias.cpu(), **{k: v for k, v in kw.items() if k != "score"})
+        assert torch.equal(choice, want), kw
+
+
+def test_routes_of_rows_of_a_wider_tensor():
+    from stride_b200.kernels import ops
+    wide = _rand(6, 21, 77)
+    z = wide[:, 3:51]
+    choice, weights = torch.empty(21, 4, dtype=torch.int32, device="cuda"), torch.full((4, 30), 7.0, device="cuda")
+    ops.route_experts(z, choice, weights[:, 2:23])
+    want, want_weights = plain.route(z.cpu(), 4, "sigmoid")
+    assert torch.equal(choice.cpu(), want)
+    assert _close(weights[:, 2:23].cpu(), want_weights)
+    weights[:, 2:23] = 7.0
+    assert (weights == 7.0).all()
+
+
+# ------------------------------------------------------------------ experts
+def _experts(E, W, F, seed=0):
+    from stride_b200.kernels.linear import Fp8Experts
+    gate, up, down = ([_weight(seed + 1000 * k + e, *shape) for e in range(E)] for k, shape in ((1, (F, W)), (2, (F, W)), (3, (W, F))))
+    layer = Fp8Experts([w for pair in zip(gate, up) for w in pair], down)
+    return layer, [[_values(w) for w in ws] for ws in (gate, up, down)]
+
+
+def _choices(seed, n, E, top, missing=0.0):
+    g = torch.Generator().manual_seed(seed)
+    choice = torch.rand(n, E, generator=g).add(torch.linspace(0, 0.5, E)).argsort(dim=1, descending=True)[:, :top].to(torch.int32)
+    choice[torch.rand(n, top, generator=g) < missing] = -1
+    return choice.contiguous().cuda(), torch.rand(top, n, generator=g).cuda()
+
+
+EXPERTS = [(1, 4, 2, 128, 128, 0.0), (1, 64, 6, 256, 200, 0.0), (3, 8, 3, 300, 100, 0.3), (32, 8, 2, 512, 384, 0.0), (64, 3, 3, 200, 70, 0.2),
+           (257, 16, 4, 256, 520, 0.1), (1000, 4, 1, 384, 256, 0.5), (500, 40, 6, 640, 260, 0.0)]
+
+
+@pytest.mark.parametrize("n,E,top,W,F,missing", EXPERTS)
+@pytest.mark.parametrize("x_dtype,out_dtype", [(BF, BF), (F32, F32)])
+def test_experts(n, E, top, W, F, missing, x_dtype, out_dtype):
+    """Ids that are no expert's have no term; a token without any gets zeros."""
+    layer, (gate, up, down) = _experts(E, W, F)
+    x = _rand(n, n, W, dtype=x_dtype)
+    choice, weights = _choices(n, n, E, top, missing)
+    if n > 2:
+        choice[1], choice[2, 0] = -1, E
+    out = torch.full((n, W), float("nan"), dtype=out_dtype, device="cuda")
+    layer.forward(x, choice, weights, out, layer.scratch(n, top))
+    want, bound = plain.experts(x.to(F64), choice, weights, gate, up, down)
+    assert ((out.to(F64) - want).abs() <= bound + HALF_STEP[out_dtype] * (want.abs() + bound)).all()
+    if n > 2:
+        assert (out[1] == 0).all()
+
+
+def test_experts_of_a_token_do_not_depend_on_the_step():
+    """Alone, in a few and in many, whoever else chose the same experts; the same twice over the same scratch."""
+    layer, _ = _experts(8, 384, 264)
+    x = _rand(1, 400, 384, dtype=BF)
+    choice, weights = _choices(2, 400, 8, 3)
+    whole, again = torch.empty(400, 384, device="cuda"), torch.empty(400, 384, device="cuda")
+    scratch = layer.scratch(400, 3)
+    layer.forward(x, choice, weights, whole, scratch)
+    layer.forward(x, choice, weights, again, scratch)
+    assert torch.equal(whole, again)
+    for first, n in [(0, 1), (9, 5), (100, 40), (200, 150)]:
+        part = torch.full((n, 384), float("nan"), device="cuda")
+        rows = slice(first, first + n)
+        layer.forward(x[rows], choice[rows].contiguous(), weights[:, rows].contiguous(), part, scratch)
+        assert torch.equal(part, whole[rows]), (first, n)
+
+
+def test_router_and_experts_together():
+    """As a feed-forward runs them: logits, choice and weights, the experts' products; in a captured graph, replayed with other inputs."""
+    from stride_b200.kernels import ops
+    E, W, F, n, top = 16, 256, 192, 37, 4
+    layer, (gate, up, down) = _experts(E, W, F)
+    router, bias = _rand(3, E, W, std=W ** -0.5), _rand(4, E, std=0.05)
+    x = _rand(5, n, W, dtype=BF)
+    logits, choice = torch.empty(n, E, device="cuda"), torch.empty(n, top, dtype=torch.int32, device="cuda")
+    weights, out, scratch = torch.empty(top, n, device="cuda"), torch.empty(n, W, dtype=BF, device="cuda"), layer.scratch(n, top)
+
+    def run():
+        ops.gemm_f32(x, router, logits)
+        ops.route_experts(logits, choice, weights, bias=bias, groups=4, top_groups=2, scale=2.0)
+        layer.forward(x, choice, weights, out, scratch)
+
+    run()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        run()
+    for seed in (6, 7):
+        x.copy_(_rand(seed, n, W, dtype=BF))
+        graph.replay()
+        torch.cuda.synchronize()
+        want_choice, want_weights = plain.route(logits.cpu(), top, "sigmoid", bias.cpu(), 4, 2, 2, True, 2.0)
+        assert torch.equal(choice.cpu(), want_choice)
+        want, bound = plain.experts(x.to(F64), choice, want_weights.cuda(), gate, up, down)
+        bound = bound + 2.0 ** -20 * want.abs().amax()
+        assert ((out.to(F64) - want).abs() <= bound + 2.0 ** -8 * (want.abs() + bound)).all()
