@@ -101,12 +101,16 @@ struct Fp8Params {
   int64_t ldo;
   const float* x_scales;     // [blocks][ldxs]
   int64_t ldxs;
+  const void* x;             // for the forms that quantise it themselves: float32 (x_f32) or bfloat16 [n][ldx], rows 16-byte aligned
+  int64_t ldx;
+  int x_f32, x_gathered;     // x_gathered: row i is token order[i] % n
   const float* w_scales;     // [blocks of rows][blocks]
   int n, M, K, blocks;       // M: rows of the weight (of one expert); kGated: gate rows, then up rows
   int half_rows;
   int scale_rows;            // blocks of rows of one expert's scales
   int ranges, range_blocks;  // K ranges and blocks of columns in each
   int stages;
+  int tiles_m, tiles_n, vec_out;      // (the kernel on pairs; vec_out: the result takes 16-byte stores)
   const int32_t* tiles;      // experts: the list of `expert_order_kernel`; else null
   const int32_t* order;      // experts: row -> pair k n + token
   const float* pair_weight;  // experts: a factor on every pair's result, by pair, or null
@@ -125,6 +129,44 @@ __device__ __forceinline__ void umma_e4m3(uint32_t tmem_d, uint64_t desc_a, uint
       "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate)
       : "memory");
 }
+// Waits for this warp's loads from tensor memory; what they brought passes through, so that no use of it can be moved in front of the wait.
+__device__ __forceinline__ void tmem_arrived16(uint32_t* r) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]),
+                 "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
+               :
+               : "memory");
+}
+__device__ __forceinline__ void tmem_arrived32(uint32_t* r) {
+  tmem_arrived16(r);
+  tmem_arrived16(r + 16);            // (nothing is left to wait for)
+}
+// sum[c] += v[c] * f[c], N sums of a thread.
+template <int N>
+__device__ __forceinline__ void add_scaled(float* sum, const uint32_t* v, const float* f) {
+#pragma unroll
+  for (int c = 0; c < N; c += 4) {
+    const float4 s = *reinterpret_cast<const float4*>(f + c);
+    sum[c] = fmaf(__uint_as_float(v[c]), s.x, sum[c]);
+    sum[c + 1] = fmaf(__uint_as_float(v[c + 1]), s.y, sum[c + 1]);
+    sum[c + 2] = fmaf(__uint_as_float(v[c + 2]), s.z, sum[c + 2]);
+    sum[c + 3] = fmaf(__uint_as_float(v[c + 3]), s.w, sum[c + 3]);
+  }
+}
+template <int N>
+__device__ __forceinline__ void add_scaled(float* sum, const uint32_t* v, float f) {
+#pragma unroll
+  for (int c = 0; c < N; ++c) sum[c] = fmaf(__uint_as_float(v[c]), f, sum[c]);
+}
+// Sixteen bytes from global to shared memory on their own, the last 16 - `bytes` as zeros.
+__device__ __forceinline__ void copy16_async(uint32_t to, const void* from, int bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int LEFT>
+__device__ __forceinline__ void copies_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory");
+}
 __device__ __forceinline__ float cluster_load_float(uint32_t addr) {
   float v;
   asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
@@ -135,26 +177,33 @@ template <int BN>
 struct Shape {
   static constexpr int kEpilogueWarps = BN >= 64 ? 8 : 4;
   static constexpr int kColumns = BN * 4 / kEpilogueWarps;             // columns of a thread's row of the tile
-  static constexpr int kThreads = 128 + 32 * kEpilogueWarps;
+  static constexpr int threads(bool quant) { return 128 + 32 * kEpilogueWarps + (quant ? 64 : 0); }
   static constexpr int kSlots = BN <= 32 ? 8 : 4;                      // accumulators under way
   static constexpr int kStage = kStageA + BN * 128;
-  static constexpr int kTmem = kSlots * BN < 32 ? 32 : kSlots * BN;    // (a power of two)
+  static constexpr int kTmem = kSlots * BN;                            // (a power of two)
+  static constexpr int kCtas = BN <= 32 ? 2 : 1;                       // of an SM: with few tokens one fills its ring while the other drains
+  static constexpr int kSmem = kCtas == 2 ? 100 * 1024 : kSmemBudget;
 };
 
 // blockIdx = (weight tile, token tile, K range: the rank in the cluster when SPLIT). Warp 0 loads, warp 1 issues the products, warps 2 and 3
-// multiply the scales, the others are the epilogue: four of them see all 128 rows, with eight each half takes half of the columns.
-template <int EPI, int BN, class OUT, bool GROUPED, bool SPLIT>
-__global__ void __launch_bounds__(Shape<BN>::kThreads, 1)
+// multiply the scales, the others are the epilogue: four of them see all 128 rows, with eight each half takes half of the columns. QUANT (few
+// tokens): the input comes as it is, and four warps quantise it, the same arithmetic as `quantize_kernel`, straight into the ring's stages. They
+// copy it ahead of its turn (kCopies blocks are under way, each thread's columns by the thread itself): without, a block took its trip to L2.
+constexpr int kCopies = 4;
+template <int EPI, int BN, class OUT, bool GROUPED, bool SPLIT, bool QUANT>
+__global__ void __launch_bounds__(Shape<BN>::threads(QUANT), Shape<BN>::kCtas)
 gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const Fp8Params p) {
   using S = Shape<BN>;
+  constexpr int kScaleWarps = QUANT ? 4 : 2, kFirst = 2 + kScaleWarps;        // the epilogue's first warp
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   __shared__ __align__(8) uint64_t full_bar[kMaxStages], empty_bar[kMaxStages];
   __shared__ __align__(8) uint64_t accum_full[S::kSlots], scale_full[S::kSlots], slot_empty[S::kSlots];
   __shared__ __align__(16) float factor[S::kSlots][2][BN];
+  __shared__ int pair_s[GROUPED ? BN : 1];           // the tile's rows' pairs and the factors on their results
+  __shared__ float weight_s[GROUPED ? BN : 1];
   __shared__ uint32_t tmem_base_s;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  sb::grid_launch_dependents();
   int expert = 0, n0 = blockIdx.y * BN, end = p.n;
   if (GROUPED) {
     sb::grid_dependency_wait();        // whose rows this tile holds is an earlier kernel's result
@@ -170,34 +219,41 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
   if (threadIdx.x == 0) {
     prefetch_tensormap(&map_w);
     prefetch_tensormap(&map_x);
-    for (int s = 0; s < p.stages; ++s) mbar_init(smem_u32(&full_bar[s]), 1), mbar_init(smem_u32(&empty_bar[s]), 1);
+    for (int s = 0; s < p.stages; ++s) mbar_init(smem_u32(&full_bar[s]), QUANT ? 1 + kScaleWarps : 1), mbar_init(smem_u32(&empty_bar[s]), 1);
     for (int s = 0; s < S::kSlots; ++s) {
       mbar_init(smem_u32(&accum_full[s]), 1);
-      mbar_init(smem_u32(&scale_full[s]), 64);
+      mbar_init(smem_u32(&scale_full[s]), 32 * kScaleWarps);
       mbar_init(smem_u32(&slot_empty[s]), S::kEpilogueWarps);
     }
     mbar_init_fence();
+  }
+  if (GROUPED && threadIdx.x >= 128 && threadIdx.x < 128 + BN) {
+    const int c = threadIdx.x - 128, pair = n0 + c < end ? p.order[n0 + c] : 0;
+    pair_s[c] = pair, weight_s[c] = p.pair_weight != nullptr ? p.pair_weight[pair] : 1.0f;
   }
   if (warp == 1) tmem_alloc(smem_u32(&tmem_base_s), S::kTmem);
   fence_before_sync();
   __syncthreads();
   fence_after_sync();
   const uint32_t tmem_base = tmem_base_s;
+  sb::grid_launch_dependents();        // (behind the allocation: a kernel let in before it could take the columns and wait for this one)
 
   if (warp == 0) {
     if (lane == 0) {
       const int row_w = expert * p.M + tile_m * (EPI == kGated ? 64 : kBlock);
       auto load_w = [&](int i, int st) {
         const uint32_t bar = smem_u32(&full_bar[st]), a = smem0 + st * S::kStage;
-        mbar_expect_tx(bar, S::kStage);
+        mbar_expect_tx(bar, QUANT ? kStageA : S::kStage);
         tma_load_2d(a, &map_w, bar, (b0 + i) * kBlock, row_w);
         if (EPI == kGated) tma_load_2d(a + kStageA / 2, &map_w, bar, (b0 + i) * kBlock, row_w + p.half_rows);
       };
-      auto load_x = [&](int i, int st) { tma_load_2d(smem0 + st * S::kStage + kStageA, &map_x, smem_u32(&full_bar[st]), (b0 + i) * kBlock, n0); };
+      auto load_x = [&](int i, int st) {
+        if (!QUANT) tma_load_2d(smem0 + st * S::kStage + kStageA, &map_x, smem_u32(&full_bar[st]), (b0 + i) * kBlock, n0);
+      };
       // (the weights are nobody's result: the first ring of them is under way before the kernels in front have ended)
       const int ahead = min(iters, p.stages);
       for (int i = 0; i < ahead; ++i) load_w(i, i);
-      if (!GROUPED) sb::grid_dependency_wait();
+      if (!GROUPED && !QUANT) sb::grid_dependency_wait();
       for (int i = 0; i < ahead; ++i) load_x(i, i);
       int st = ahead == p.stages ? 0 : ahead;
       uint32_t par = 0;
@@ -232,13 +288,84 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
       }
     }
     __syncwarp();
-  } else if (warp < 4) {
+  } else if (warp < kFirst) {
     // the scales' products, two columns a thread; four blocks are read ahead of their turn
     constexpr int kAhead = 4, kPer = (BN + 63) / 64;
     const int t = threadIdx.x - 64;
     const float* ws0 = p.w_scales + static_cast<int64_t>(expert * p.scale_rows + (EPI == kGated ? tile_m / 2 : tile_m)) * p.blocks + b0;
     const float* ws1 = EPI == kGated ? ws0 + static_cast<int64_t>(p.scale_rows / 2) * p.blocks : ws0;
     if (!GROUPED) sb::grid_dependency_wait();
+    if constexpr (QUANT) {
+      constexpr int kPerRow = 128 / BN, kColumns = 128 / kPerRow;           // threads of a row of the tile, columns of a thread
+      const int r = t / kPerRow, part = t % kPerRow, size = p.x_f32 ? 4 : 2, pieces = kColumns * size / 16;
+      const bool live = n0 + r < end;
+      const int64_t row = !live ? 0 : GROUPED && p.x_gathered ? pair_s[GROUPED ? r : 0] % p.n : n0 + r;
+      const uint8_t* from = static_cast<const uint8_t*>(p.x) + (row * p.ldx + b0 * kBlock + part * kColumns) * size;
+      const int columns = live ? p.K - b0 * kBlock - part * kColumns : 0;        // what the row has from there on
+      const uint32_t raw = smem0 + p.stages * S::kStage + t * 16;               // this thread's pieces, 128 x 16 bytes from one to the next
+      auto copy = [&](int i) {
+        if (i < iters) {
+          for (int j = 0; j < pieces; ++j) {
+            const int there = (columns - i * kBlock) * size - 16 * j;
+            copy16_async(raw + ((i % kCopies) * pieces + j) * 2048, there > 0 ? from + i * kBlock * size + 16 * j : static_cast<const uint8_t*>(p.x),
+                         min(max(there, 0), 16));
+          }
+        }
+        copies_commit();
+      };
+#pragma unroll
+      for (int i = 0; i < kCopies; ++i) copy(i);
+      float w0 = __ldg(ws0), w1 = EPI == kGated ? __ldg(ws1) : 0.0f;
+      int st = 0, slot = 0;
+      uint32_t par = 1, slot_par = 1;
+      for (int i = 0; i < iters; ++i) {
+        copies_wait<kCopies - 1>();
+        float v[kColumns];
+        const uint8_t* mine = smem0_p + p.stages * S::kStage + t * 16 + (i % kCopies) * pieces * 2048;
+        if (p.x_f32) {
+#pragma unroll
+          for (int j = 0; j < kColumns / 4; ++j) *reinterpret_cast<float4*>(v + 4 * j) = *reinterpret_cast<const float4*>(mine + j * 2048);
+        } else {
+#pragma unroll
+          for (int j = 0; j < kColumns / 8; ++j) {
+            const uint4 a = *reinterpret_cast<const uint4*>(mine + j * 2048);
+            const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+            for (int k = 0; k < 4; ++k) v[8 * j + 2 * k] = __uint_as_float(w[k] << 16), v[8 * j + 2 * k + 1] = __uint_as_float(w[k] & 0xFFFF0000u);
+          }
+        }
+        copy(i + kCopies);
+        uint32_t amax = 0;
+#pragma unroll
+        for (int j = 0; j < kColumns; ++j) amax = max(amax, __float_as_uint(v[j]) & 0x7FFFFFFFu);
+#pragma unroll
+        for (int o = 1; o < kPerRow; o <<= 1) amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+        const bool finite = amax < 0x7F800000u;
+        const int e = finite ? scale_exponent(amax) : 0;
+        const float inverse = power_of_two(-e), scale = finite ? power_of_two(e) : __uint_as_float(0x7FC00000u);
+        uint32_t q[kColumns / 4];
+#pragma unroll
+        for (int j = 0; j < kColumns / 4; ++j)
+          q[j] = e4m3x2(v[4 * j] * inverse, v[4 * j + 1] * inverse) | (e4m3x2(v[4 * j + 2] * inverse, v[4 * j + 3] * inverse) << 16);
+        mbar_wait(smem_u32(&empty_bar[st]), par, p.status, 47);
+        uint8_t* to = smem0_p + st * S::kStage + kStageA + r * 128;
+#pragma unroll
+        for (int h = 0; h < kColumns / 16; ++h)          // (16-byte pieces of a row change places as the 128-byte swizzle has them)
+          *reinterpret_cast<uint4*>(to + (((part * (kColumns / 16) + h) ^ (r & 7)) << 4)) = make_uint4(q[4 * h], q[4 * h + 1], q[4 * h + 2], q[4 * h + 3]);
+        fence_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&full_bar[st]));
+        mbar_wait(smem_u32(&slot_empty[slot]), slot_par, p.status, 44);
+        if (part == 0) {
+          factor[slot][0][r] = scale * w0;
+          if (EPI == kGated) factor[slot][1][r] = scale * w1;
+        }
+        mbar_arrive(smem_u32(&scale_full[slot]));
+        if (i + 1 < iters) w0 = __ldg(ws0 + i + 1), w1 = EPI == kGated ? __ldg(ws1 + i + 1) : 0.0f;
+        if (++st == p.stages) st = 0, par ^= 1;
+        if (++slot == S::kSlots) slot = 0, slot_par ^= 1;
+      }
+    } else {
     float xs[kAhead][kPer], w0[kAhead], w1[kAhead];
     auto fetch = [&](int i, int a) {
       if (i >= iters) return;
@@ -272,8 +399,9 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
         if (++slot == S::kSlots) slot = 0, slot_par ^= 1;
       }
     }
+    }
   } else {
-    const int quarter = warp & 3, half = (warp - 4) >> 2, row = quarter * 32 + lane;
+    const int quarter = warp & 3, half = (warp - kFirst) >> 2, row = quarter * 32 + lane;
     constexpr int C = S::kColumns, kChunk = C < 32 ? C : 32;
     float acc[C], total[SPLIT ? 1 : C];
 #pragma unroll
@@ -294,17 +422,9 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
 #pragma unroll
       for (int c0 = 0; c0 < C; c0 += kChunk) {
         uint32_t v[kChunk];
-        if (kChunk == 32) tmem_load32_nowait(from + c0, v);
-        else tmem_load16_nowait(from + c0, v);
-        tmem_load_wait();
-#pragma unroll
-        for (int c = 0; c < kChunk; c += 4) {
-          const float4 s = *reinterpret_cast<const float4*>(f + c0 + c);
-          acc[c0 + c] = fmaf(__uint_as_float(v[c]), s.x, acc[c0 + c]);
-          acc[c0 + c + 1] = fmaf(__uint_as_float(v[c + 1]), s.y, acc[c0 + c + 1]);
-          acc[c0 + c + 2] = fmaf(__uint_as_float(v[c + 2]), s.z, acc[c0 + c + 2]);
-          acc[c0 + c + 3] = fmaf(__uint_as_float(v[c + 3]), s.w, acc[c0 + c + 3]);
-        }
+        if (kChunk == 32) tmem_load32_nowait(from + c0, v), tmem_arrived32(v);
+        else tmem_load16_nowait(from + c0, v), tmem_arrived16(v);
+        add_scaled<kChunk>(acc + c0, v, f + c0);
       }
       fence_before_sync();
       __syncwarp();
@@ -326,7 +446,7 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
     asm volatile("bar.sync 1, %0;" ::"r"(32 * S::kEpilogueWarps) : "memory");
     if (!GROUPED) sb::grid_dependency_wait();
     if (!SPLIT) {
-      const int thread = threadIdx.x - 128;
+      const int thread = threadIdx.x - 32 * kFirst;
       constexpr int kFeatures = EPI == kGated ? 64 : kBlock, kStride = 32 * S::kEpilogueWarps / kFeatures;
       const int j = thread % kFeatures, m = tile_m * kFeatures + j;
       if (tile != nullptr && m < (EPI == kGated ? p.half_rows : p.M)) {
@@ -334,10 +454,7 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
           float v = tile[c * kBlock + j];
           int64_t to = n0 + c;
           if (EPI == kGated) v = gated_product(v, tile[c * kBlock + 64 + j], p.gate);
-          if (GROUPED && EPI != kGated) {
-            to = p.order[n0 + c];
-            if (p.pair_weight != nullptr) v *= p.pair_weight[to];
-          }
+          if (GROUPED && EPI != kGated) to = pair_s[GROUPED ? c : 0], v *= weight_s[GROUPED ? c : 0];
           OUT* o = static_cast<OUT*>(p.out) + to * p.ldo + m;
           if (EPI == kAdd) v += sb::widen(*o);
           *o = sb::narrow<OUT>(v);
@@ -347,8 +464,8 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
   }
   if (SPLIT) {
     sb::cluster_sync();
-    if (warp >= 4) {
-      const int thread = threadIdx.x - 128, rank = static_cast<int>(sb::cluster_rank());
+    if (warp >= kFirst) {
+      const int thread = threadIdx.x - 32 * kFirst, rank = static_cast<int>(sb::cluster_rank());
       constexpr int kFeatures = EPI == kGated ? 64 : kBlock, kStride = 32 * S::kEpilogueWarps / kFeatures;
       const int j = thread % kFeatures, m = tile_m * kFeatures + j;
       const bool ok = *reinterpret_cast<volatile int*>(p.status) == 0;       // (a range that lost a signal has left no sums)
@@ -380,6 +497,270 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
   if (warp == 1) {
     fence_after_sync();
     tmem_dealloc(tmem_base, S::kTmem);
+  }
+}
+
+// The same for many tokens, on pairs of CTAs (a cluster of two, cta_group::2) that walk tiles, with the operands' places changed: the 256 rows
+// of a product are tokens, 128 a CTA, its columns are weight rows. A thread of the epilogue then holds one token's sums, and the scales of a
+// block are one factor a thread and 128 weight rows instead of one a sum. (With weight rows as the product's rows, a factor from shared memory
+// for every four sums, the gated product of 4,096 tokens, 2 x 14,336 rows of 4,096, took 870 us.) WIDE: 256 weight rows a tile, or 128 gate rows
+// and their 128 up rows: each CTA loads 128 of them and 128 tokens, 32 KB a block for 512 cycles of the tensor cores. A weight with several K
+// ranges needs its totals beside the sums in registers and has 128 rows a tile.
+constexpr int kPairTokens = 256;
+constexpr int kPairThreads = 384;
+template <bool WIDE>
+struct PairShape {
+  static constexpr int kRows = WIDE ? 256 : 128;             // weight rows of a tile
+  static constexpr int kStage = kStageA + kRows / 2 * 128;
+  static constexpr int kSlots = WIDE ? 2 : 4;                // accumulators under way: all of tensor memory
+  static constexpr int kStages = WIDE ? 6 : 8;
+};
+__device__ __forceinline__ void umma_pair_e4m3(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem_d),
+      "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+// The tiles of a launch in the order in which the pairs walk them. Dense: the tiles of tokens first, so that the pairs of a round share few weight
+// rows and every tile of tokens (which stay in L2); experts: the weight tiles of a tile of rows first.
+struct PairTile {
+  int tile_m, expert, n0, end;
+  __device__ __forceinline__ PairTile(const Fp8Params& p, bool grouped, int tile) {
+    if (grouped) {
+      const int t = tile / p.tiles_m;
+      tile_m = tile - t * p.tiles_m;
+      expert = p.tiles[2 + 3 * t], n0 = p.tiles[3 + 3 * t], end = p.tiles[4 + 3 * t];
+    } else {
+      tile_m = tile / p.tiles_n;
+      expert = 0, n0 = (tile - tile_m * p.tiles_n) * kPairTokens, end = p.n;
+    }
+  }
+};
+
+// 64 results of a token, features m .. m + 63 of `rows`, to `to` (the address of the first).
+template <int EPI, class OUT>
+__device__ __forceinline__ void store_token(OUT* to, const float* v, int m, int rows, bool vec) {
+  constexpr int kPer = 16 / sizeof(OUT);
+  if (vec && m + 64 <= rows) {
+#pragma unroll
+    for (int c = 0; c < 64; c += kPer) {
+      float r[kPer];
+      uint4 raw = EPI == kAdd ? *reinterpret_cast<const uint4*>(to + c) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) r[i] = v[c + i] + (EPI == kAdd ? sb::widen(reinterpret_cast<const OUT*>(&raw)[i]) : 0.0f);
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) reinterpret_cast<OUT*>(&raw)[i] = sb::narrow<OUT>(EPI == kAdd ? r[i] : v[c + i]);
+      *reinterpret_cast<uint4*>(to + c) = raw;
+    }
+  } else {
+#pragma unroll
+    for (int c = 0; c < 64; ++c)
+      if (m + c < rows) to[c] = sb::narrow<OUT>(EPI == kAdd ? v[c] + sb::widen(to[c]) : v[c]);
+  }
+}
+
+template <int EPI, bool WIDE, class OUT, bool GROUPED>
+__global__ void __launch_bounds__(kPairThreads, 1)
+gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const Fp8Params p) {
+  using S = PairShape<WIDE>;
+  constexpr int kFactors = WIDE ? 2 : 1;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  __shared__ __align__(8) uint64_t full_bar[S::kStages];      // used in the leader: both CTAs' tiles have landed
+  __shared__ __align__(8) uint64_t empty_bar[S::kStages];     // in each CTA: the products that read its stage are done
+  __shared__ __align__(8) uint64_t accum_full[S::kSlots];     // in each CTA
+  __shared__ __align__(8) uint64_t accum_empty[S::kSlots];    // used in the leader: both CTAs have taken an accumulator's sums
+  __shared__ __align__(8) uint64_t factor_full[S::kSlots], factor_empty[S::kSlots];      // in each CTA, its own
+  __shared__ float factor[S::kSlots][kFactors][kBlock];       // by token
+  __shared__ uint32_t tmem_base_s;
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = static_cast<int>(sb::cluster_rank());
+  const uint32_t smem0 = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+  if (threadIdx.x == 0) {
+    prefetch_tensormap(&map_w);
+    prefetch_tensormap(&map_x);
+    for (int s = 0; s < S::kStages; ++s) mbar_init(smem_u32(&full_bar[s]), 1), mbar_init(smem_u32(&empty_bar[s]), 1);
+    for (int s = 0; s < S::kSlots; ++s) {
+      mbar_init(smem_u32(&accum_full[s]), 1);
+      mbar_init(smem_u32(&accum_empty[s]), 16);
+      mbar_init(smem_u32(&factor_full[s]), 64);
+      mbar_init(smem_u32(&factor_empty[s]), 8);
+    }
+    mbar_init_fence();
+  }
+  if (warp == 1) tmem_alloc_pair(smem_u32(&tmem_base_s), 512);
+  fence_before_sync();
+  __syncthreads();
+  sb::cluster_sync();          // the peer's barriers exist before anything signals them
+  fence_after_sync();
+  const uint32_t tmem_base = tmem_base_s;
+  sb::grid_launch_dependents();
+  sb::grid_dependency_wait();
+  const int total = p.tiles_m * (GROUPED ? p.tiles[0] : p.tiles_n);
+
+  if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");      // 384 x 168 registers at launch: 128 x 80 + 256 x 208 and a rest
+    if (warp == 0) {
+      if (lane == 0) {
+        int st = 0;
+        uint32_t par = 1;
+        for (int tile = pair; tile < total; tile += pairs) {
+          const PairTile t(p, GROUPED, tile);
+          const int row = t.expert * p.M + (EPI == kGated ? t.tile_m * kBlock + rank * p.half_rows : t.tile_m * S::kRows + rank * (S::kRows / 2));
+          const int token = t.n0 + rank * kBlock;
+          for (int i = 0; i < p.blocks; ++i) {
+            mbar_wait(smem_u32(&empty_bar[st]), par, p.status, 51);
+            const uint32_t bar = smem_u32(&full_bar[st]), a = smem0 + st * S::kStage;
+            if (rank == 0) mbar_expect_tx(bar, 2 * S::kStage);
+            tma_load_2d_pair(a, &map_x, bar, i * kBlock, token);
+            tma_load_2d_pair(a + kStageA, &map_w, bar, i * kBlock, row);
+            if (++st == S::kStages) st = 0, par ^= 1;
+          }
+        }
+      }
+      __syncwarp();
+    } else if (warp == 1) {
+      if (lane == 0 && rank == 0) {
+        const uint64_t desc_fixed = smem_desc_sw128(0);
+        const uint32_t idesc = (1u << 4) | (static_cast<uint32_t>(S::kRows >> 3) << 17) | (static_cast<uint32_t>(256 >> 4) << 24);
+        int st = 0, slot = 0;
+        uint32_t par = 0, slot_par = 1;
+        for (int tile = pair; tile < total; tile += pairs) {
+          for (int i = 0; i < p.blocks; ++i) {
+            mbar_wait(smem_u32(&accum_empty[slot]), slot_par, p.status, 52);
+            mbar_wait(smem_u32(&full_bar[st]), par, p.status, 53);
+            fence_after_sync();
+            const uint64_t da = desc_fixed | (((smem0 + st * S::kStage) & 0x3FFFF) >> 4), db = da + (kStageA >> 4);
+            const uint32_t d = tmem_base + slot * S::kRows;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) umma_pair_e4m3(d, da + 2 * k, db + 2 * k, idesc, k > 0);
+            umma_pair_commit(smem_u32(&empty_bar[st]));
+            umma_pair_commit(smem_u32(&accum_full[slot]));
+            if (++st == S::kStages) st = 0, par ^= 1;
+            if (++slot == S::kSlots) slot = 0, slot_par ^= 1;
+          }
+        }
+      }
+      __syncwarp();
+    } else {
+      // the scales' products, two tokens a thread; four blocks are read ahead of their turn
+      constexpr int kAhead = 4;
+      const int c = threadIdx.x - 64;
+      int slot = 0;
+      uint32_t slot_par = 1;
+      for (int tile = pair; tile < total; tile += pairs) {
+        const PairTile t(p, GROUPED, tile);
+        const int last = (EPI == kGated ? p.scale_rows / 2 : p.scale_rows) - 1;      // (rows beyond the weight: their sums are nobody's)
+        const float* base = p.w_scales + static_cast<int64_t>(t.expert) * p.scale_rows * p.blocks;
+        const float* ws0 = base + static_cast<int64_t>(min(EPI == kGated || !WIDE ? t.tile_m : 2 * t.tile_m, last)) * p.blocks;
+        const float* ws1 = EPI == kGated ? ws0 + static_cast<int64_t>(p.scale_rows / 2) * p.blocks : base + static_cast<int64_t>(min(2 * t.tile_m + 1, last)) * p.blocks;
+        const int token = t.n0 + rank * kBlock + c;
+        const bool in0 = token < t.end, in1 = token + 64 < t.end;
+        const float* xs = p.x_scales + token;
+        float x0[kAhead], x1[kAhead], w0[kAhead], w1[kAhead];
+        auto fetch = [&](int i, int a) {
+          if (i >= p.blocks) return;
+          w0[a] = __ldg(ws0 + i), w1[a] = WIDE ? __ldg(ws1 + i) : 0.0f;
+          x0[a] = in0 ? xs[i * p.ldxs] : 0.0f, x1[a] = in1 ? xs[i * p.ldxs + 64] : 0.0f;
+        };
+#pragma unroll
+        for (int a = 0; a < kAhead; ++a) fetch(a, a);
+        for (int i0 = 0; i0 < p.blocks; i0 += kAhead) {
+#pragma unroll
+          for (int a = 0; a < kAhead; ++a) {
+            if (i0 + a >= p.blocks) break;
+            mbar_wait(smem_u32(&factor_empty[slot]), slot_par, p.status, 54);
+            factor[slot][0][c] = x0[a] * w0[a], factor[slot][0][c + 64] = x1[a] * w0[a];
+            if (WIDE) factor[slot][kFactors - 1][c] = x0[a] * w1[a], factor[slot][kFactors - 1][c + 64] = x1[a] * w1[a];
+            mbar_arrive(smem_u32(&factor_full[slot]));
+            fetch(i0 + a + kAhead, a);
+            if (++slot == S::kSlots) slot = 0, slot_par ^= 1;
+          }
+        }
+      }
+    }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+    // a token a thread; of the tile's weight rows this warp has 64 of every 128
+    const int quarter = warp & 3, half = (warp - 4) >> 2, mine = quarter * 32 + lane;
+    float acc[64], other[64];            // the sums; WIDE: of the second 128 rows, else: the ranges' totals
+    int slot = 0;
+    uint32_t slot_par = 0;
+    for (int tile = pair; tile < total; tile += pairs) {
+      const PairTile t(p, GROUPED, tile);
+#pragma unroll
+      for (int c = 0; c < 64; ++c) acc[c] = 0.0f, other[c] = WIDE ? 0.0f : -0.0f;
+      bool ok = true;
+      int left = p.range_blocks;
+      for (int i = 0; i < p.blocks; ++i) {
+        ok = mbar_wait(smem_u32(&factor_full[slot]), slot_par, p.status, 56) && ok;
+        const float f0 = factor[slot][0][mine], f1 = factor[slot][kFactors - 1][mine];
+        ok = mbar_wait(smem_u32(&accum_full[slot]), slot_par, p.status, 55) && ok;
+        fence_after_sync();
+        const uint32_t from = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + slot * S::kRows + half * 64;
+        uint32_t v[2][32];               // (one set is added while the next is on its way)
+        tmem_load32_nowait(from, v[0]);
+        tmem_arrived32(v[0]);
+        tmem_load32_nowait(from + 32, v[1]);
+        add_scaled<32>(acc, v[0], f0);
+        tmem_arrived32(v[1]);
+        if (WIDE) tmem_load32_nowait(from + 128, v[0]);
+        add_scaled<32>(acc + 32, v[1], f0);
+        if (WIDE) {
+          tmem_arrived32(v[0]);
+          tmem_load32_nowait(from + 160, v[1]);
+          add_scaled<32>(other, v[0], f1);
+          tmem_arrived32(v[1]);
+        }
+        fence_before_sync();
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive_leader(smem_u32(&accum_empty[slot]));
+          mbar_arrive(smem_u32(&factor_empty[slot]));
+        }
+        if (WIDE) add_scaled<32>(other + 32, v[1], f1);
+        if (++slot == S::kSlots) slot = 0, slot_par ^= 1;
+        if (!WIDE && (--left == 0 || i + 1 == p.blocks)) {
+          left = p.range_blocks;
+#pragma unroll
+          for (int c = 0; c < 64; ++c) other[c] += acc[c], acc[c] = 0.0f;
+        }
+      }
+      const int token = t.n0 + rank * kBlock + mine;
+      if (ok && token < t.end) {
+        OUT* out = static_cast<OUT*>(p.out);
+        if (EPI == kGated) {
+          const int m = t.tile_m * kBlock + half * 64;
+#pragma unroll
+          for (int c = 0; c < 64; ++c) acc[c] = gated_product(acc[c], other[c], p.gate);
+          store_token<kStore>(out + static_cast<int64_t>(token) * p.ldo + m, acc, m, p.half_rows, p.vec_out);
+        } else {
+          int64_t row = token;
+          if (GROUPED) {
+            row = p.order[token];
+            const float by = p.pair_weight[row];
+#pragma unroll
+            for (int c = 0; c < 64; ++c) acc[c] *= by, other[c] *= by;
+          }
+          const int m = t.tile_m * S::kRows + half * 64;
+          OUT* o = out + row * p.ldo + m;
+          store_token<EPI>(o, WIDE ? acc : other, m, p.M, p.vec_out);
+          if (WIDE) store_token<EPI>(o + kBlock, other, m + kBlock, p.M, p.vec_out);
+        }
+      }
+      __syncwarp();
+    }
+  }
+  fence_before_sync();
+  __syncthreads();
+  sb::cluster_sync();          // neither CTA frees the pair's tensor memory, or leaves, while the other still works
+  if (warp == 1) {
+    fence_after_sync();
+    tmem_dealloc_pair(tmem_base, 512);
   }
 }
 
@@ -467,35 +848,68 @@ int fp8_ranges(int tiles, int blocks) {
 
 // Up to this many tokens the ranges run on CTAs of their own.
 constexpr int kSplitTokens = 128;
+// Up to this many rows of a tile the product quantises its input itself.
+constexpr int kQuantRows = 32;
 
 template <int EPI, int BN, class OUT, bool GROUPED>
 int launch_tile(const void* w, int64_t rows_w, int64_t ldw, const void* q, int64_t rows_q, int64_t ldq, Fp8Params p, int tiles_m, int tiles_n,
                 cudaStream_t st) {
   using S = Shape<BN>;
+  const bool quant = BN <= kQuantRows && p.x != nullptr;
   CUtensorMap map_w, map_x;
-  if (!byte_map(w, rows_w, p.K, ldw, EPI == kGated ? 64 : kBlock, &map_w) || !byte_map(q, rows_q, p.K, ldq, BN, &map_x))
+  if (!byte_map(w, rows_w, p.K, ldw, EPI == kGated ? 64 : kBlock, &map_w) || (!quant && !byte_map(q, rows_q, p.K, ldq, BN, &map_x)))
     return sb::fail("gemm_fp8: no tensor map for a weight of %lld x %d (stride %lld)", (long long)rows_w, p.K, (long long)ldw);
-  p.stages = std::min(kMaxStages, kSmemBudget / S::kStage);
-  const size_t smem = std::max<size_t>(static_cast<size_t>(p.stages) * S::kStage, BN * kBlock * 4) + 1024;
+  if (quant) map_x = map_w;                  // (not read)
+  p.stages = std::min(kMaxStages, (S::kSmem - (quant && p.x_f32 ? kCopies * BN * kBlock * 4 : quant ? kCopies * BN * kBlock * 2 : 0)) / S::kStage);
+  const int copies = quant ? kCopies * BN * kBlock * (p.x_f32 ? 4 : 2) : 0;
+  const size_t smem = static_cast<size_t>(p.stages) * S::kStage + copies + 1024;
   const bool split = !GROUPED && p.ranges > 1 && p.n <= kSplitTokens;
   const dim3 grid(tiles_m, tiles_n, split ? p.ranges : 1);
-  if (split) {
-    auto kernel = gemm_fp8_kernel<EPI, BN, OUT, false, true>;
-    static sb::DeviceOnce once;
+  auto run = [&](auto kernel, sb::DeviceOnce& once) {
     if (once.needed()) {
-      if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024 - 8192) != cudaSuccess) return sb::check_launch("gemm_fp8");
+      const int most = std::min(kMaxStages, S::kSmem / S::kStage) * S::kStage + kCopies * (BN <= kQuantRows ? BN : 0) * kBlock * 4 + 1024;
+      if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most) != cudaSuccess) return sb::check_launch("gemm_fp8");
       once.done();
     }
-    sb::launch_pdl_cluster(kernel, grid, dim3(S::kThreads), smem, st, dim3(1, 1, p.ranges), map_w, map_x, p);
-  } else {
-    auto kernel = gemm_fp8_kernel<EPI, BN, OUT, GROUPED, false>;
-    static sb::DeviceOnce once;
-    if (once.needed()) {
-      if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024 - 8192) != cudaSuccess) return sb::check_launch("gemm_fp8");
-      once.done();
+    if (split) sb::launch_pdl_cluster(kernel, grid, dim3(S::threads(quant)), smem, st, dim3(1, 1, p.ranges), map_w, map_x, p);
+    else sb::launch_pdl(kernel, grid, dim3(S::threads(quant)), smem, st, map_w, map_x, p);
+    return sb::check_launch("gemm_fp8");
+  };
+  static sb::DeviceOnce once[4];
+  if constexpr (BN <= kQuantRows) {
+    if (quant) {
+      if constexpr (!GROUPED) {
+        if (split) return run(gemm_fp8_kernel<EPI, BN, OUT, GROUPED, true, true>, once[0]);
+      }
+      return run(gemm_fp8_kernel<EPI, BN, OUT, GROUPED, false, true>, once[1]);
     }
-    sb::launch_pdl(kernel, grid, dim3(S::kThreads), smem, st, map_w, map_x, p);
   }
+  if constexpr (!GROUPED) {
+    if (split) return run(gemm_fp8_kernel<EPI, BN, OUT, GROUPED, true, false>, once[2]);
+  }
+  return run(gemm_fp8_kernel<EPI, BN, OUT, GROUPED, false, false>, once[3]);
+}
+
+template <int EPI, bool WIDE, class OUT, bool GROUPED>
+int launch_pair(const void* w, int64_t rows_w, int64_t ldw, const void* q, int64_t rows_q, int64_t ldq, Fp8Params p, int tiles_n, cudaStream_t st) {
+  using S = PairShape<WIDE>;
+  CUtensorMap map_w, map_x;
+  if (!byte_map(w, rows_w, p.K, ldw, S::kRows / 2, &map_w) || !byte_map(q, rows_q, p.K, ldq, kBlock, &map_x))
+    return sb::fail("gemm_fp8: no tensor map for a weight of %lld x %d (stride %lld)", (long long)rows_w, p.K, (long long)ldw);
+  p.tiles_m = EPI == kGated ? (p.half_rows + kBlock - 1) / kBlock : (p.M + S::kRows - 1) / S::kRows;
+  p.tiles_n = tiles_n;
+  p.vec_out = p.ldo * sizeof(OUT) % 16 == 0 && (reinterpret_cast<uintptr_t>(p.out) & 15) == 0;
+  const long long tiles = static_cast<long long>(p.tiles_m) * tiles_n;
+  if (tiles > (1ll << 30)) return sb::fail("gemm_fp8: too many tiles");
+  auto kernel = gemm_fp8_pair_kernel<EPI, WIDE, OUT, GROUPED>;
+  const size_t smem = static_cast<size_t>(S::kStages) * S::kStage + 1024;
+  static sb::DeviceOnce once;
+  if (once.needed()) {
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)) != cudaSuccess) return sb::check_launch("gemm_fp8");
+    once.done();
+  }
+  const int pairs = static_cast<int>(std::min<long long>(tiles, sb::sm_count() / 2));
+  sb::launch_pdl_cluster(kernel, dim3(2 * pairs), dim3(kPairThreads), smem, st, dim3(2, 1, 1), map_w, map_x, p);
   return sb::check_launch("gemm_fp8");
 }
 
@@ -503,6 +917,10 @@ template <int EPI, class OUT, bool GROUPED>
 int launch_product(const void* w, int64_t rows_w, int64_t ldw, const void* q, int64_t rows_q, int64_t ldq, const Fp8Params& p, int tile_n, int tiles_n,
                    cudaStream_t st) {
   const int tiles_m = EPI == kGated ? (p.half_rows + 63) / 64 : (p.M + kBlock - 1) / kBlock;
+  if (tile_n == kPairTokens) {
+    if (p.ranges == 1) return launch_pair<EPI, true, OUT, GROUPED>(w, rows_w, ldw, q, rows_q, ldq, p, tiles_n, st);
+    if constexpr (EPI != kGated && !GROUPED) return launch_pair<EPI, false, OUT, GROUPED>(w, rows_w, ldw, q, rows_q, ldq, p, tiles_n, st);
+  }
   switch (tile_n) {
     case 16: return launch_tile<EPI, 16, OUT, GROUPED>(w, rows_w, ldw, q, rows_q, ldq, p, tiles_m, tiles_n, st);
     case 32: return launch_tile<EPI, 32, OUT, GROUPED>(w, rows_w, ldw, q, rows_q, ldq, p, tiles_m, tiles_n, st);
@@ -532,8 +950,20 @@ int launch_quantize(const void* x, int xdtype, int64_t ldx, const int32_t* order
   return sb::check_launch("quantize_fp8");
 }
 
-// One product; `half_rows` > 0: gated. out_dtype 0 float32, 1 bfloat16.
-int launch_gemm(const void* q, int64_t ldq, const float* xs, int64_t ldxs, const void* w, int64_t ldw, const float* ws, void* out, int out_dtype,
+// Tokens of a tile of the product.
+int token_tile(const Fp8Params& p, int epilogue) {
+  if (p.n <= 64) return p.n <= 16 ? 16 : p.n <= 32 ? 32 : 64;
+  return p.n <= kSplitTokens || (epilogue == kGated && p.ranges > 1) ? 128 : kPairTokens;
+}
+
+// The input as it is, for the forms that quantise it themselves: they copy 16 bytes at a time.
+bool copied_input(const void* x, int xdtype, int64_t ldx) { return ldx % (xdtype == 0 ? 4 : 8) == 0 && (reinterpret_cast<uintptr_t>(x) & 15) == 0; }
+void set_input(Fp8Params& p, const void* x, int xdtype, int64_t ldx) {
+  p.x = x, p.ldx = ldx, p.x_f32 = xdtype == 0;
+}
+
+// One product; x (or null): the input that q and xs are to hold, where the form does not quantise it itself. out_dtype 0 float32, 1 bfloat16.
+int launch_gemm(const void* x, int xdtype, int64_t ldx, const void* q, int64_t ldq, const float* xs, int64_t ldxs, const void* w, int64_t ldw, const float* ws, void* out, int out_dtype,
                 int64_t ldo, int n, int M, int K, int epilogue, int half_rows, const Gate& gate, cudaStream_t st) {
   Fp8Params p = {};
   p.out = out, p.ldo = ldo, p.x_scales = xs, p.ldxs = ldxs, p.w_scales = ws;
@@ -542,9 +972,10 @@ int launch_gemm(const void* q, int64_t ldq, const float* xs, int64_t ldxs, const
   p.ranges = fp8_ranges((M + kBlock - 1) / kBlock, p.blocks);
   p.range_blocks = (p.blocks + p.ranges - 1) / p.ranges;
   p.gate = gate;
+  if (x != nullptr && copied_input(x, xdtype, ldx)) set_input(p, x, xdtype, ldx);
   p.status = status_word();
   if (p.status == nullptr) return sb::fail("gemm_fp8: no status word on this device");
-  const int tile = n <= 16 ? 16 : n <= 32 ? 32 : n <= 64 ? 64 : 128, tiles_n = (n + tile - 1) / tile;
+  const int tile = token_tile(p, epilogue), tiles_n = (n + tile - 1) / tile;
   if (tiles_n > 65535) return sb::fail("gemm_fp8: %d tokens are too many", n);
   if (epilogue == kAdd) return launch_product<kAdd, float, false>(w, M, ldw, q, n, ldq, p, tile, tiles_n, st);
   if (epilogue == kStore)
@@ -571,7 +1002,7 @@ int check_product(const char* who, const void* w, int64_t ldw, int out_dtype, in
 // Rows of a tile of the experts' products: near the rows an expert gets on average (a row's result does not depend on it).
 int expert_tile(int pairs, int E) {
   const int mean = (pairs + E - 1) / E;
-  return mean <= 16 ? 16 : mean <= 32 ? 32 : mean <= 64 ? 64 : 128;
+  return mean <= 16 ? 16 : mean <= 32 ? 32 : mean <= 64 ? 64 : mean <= 128 ? 128 : kPairTokens;
 }
 int most_tiles(int pairs, int E, int tile) { return std::min(pairs, pairs / tile + std::min(pairs, E)); }
 
@@ -591,7 +1022,7 @@ ExpertScratch expert_scratch(int64_t n, int64_t top, int64_t E, int64_t W, int64
   s.ldx = (W + 15) / 16 * 16, s.ldz = (F + 15) / 16 * 16;
   s.order = take(4 * pairs), s.list = take(4 * (2 + 3 * pairs));
   s.xq = take(pairs * s.ldx), s.xs = take(4 * pairs * ((W + kBlock - 1) / kBlock));
-  s.z = take(4 * pairs * F), s.zq = take(pairs * s.ldz), s.zs = take(4 * pairs * ((F + kBlock - 1) / kBlock));
+  s.z = take(4 * pairs * s.ldz), s.zq = take(pairs * s.ldz), s.zs = take(4 * pairs * ((F + kBlock - 1) / kBlock));
   s.parts = take(4 * pairs * W);
   s.bytes = at;
   return s;
@@ -617,10 +1048,10 @@ SB_EXPORT int sb_gemm_fp8(const void* q, int64_t ldq, const float* xs, int64_t l
   if (n == 0) return 0;
   Gate gate;
   gate.act = act, gate.limit = limit, gate.slope = slope;
-  return launch_gemm(q, ldq, xs, ldxs, w, ldw, ws, out, out_dtype, ldo, n, M, K, epilogue, half_rows, gate, static_cast<cudaStream_t>(stream));
+  return launch_gemm(nullptr, 0, 0, q, ldq, xs, ldxs, w, ldw, ws, out, out_dtype, ldo, n, M, K, epilogue, half_rows, gate, static_cast<cudaStream_t>(stream));
 }
 
-// Both: x is quantised into the buffers q and xs first.
+// Both: x is quantised into the buffers q and xs first (of few tokens on the way into the product, which leaves the buffers alone).
 SB_EXPORT int sb_linear_fp8(const void* x, int xdtype, int64_t ldx, void* q, int64_t ldq, float* xs, int64_t ldxs, const void* w, int64_t ldw, const float* ws,
                             void* out, int out_dtype, int64_t ldo, int n, int M, int K, int epilogue, int half_rows, int act, float limit, float slope,
                             void* stream) {
@@ -629,10 +1060,12 @@ SB_EXPORT int sb_linear_fp8(const void* x, int xdtype, int64_t ldx, void* q, int
   if (xdtype < 0 || xdtype > 1 || ldx < K) return sb::fail("linear_fp8: rows of %lld elements, %d columns", (long long)ldx, K);
   if (n == 0) return 0;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (int rc = launch_quantize(x, xdtype, ldx, nullptr, nullptr, n, n, K, q, ldq, xs, ldxs, st)) return rc;
+  if (n > kQuantRows || !copied_input(x, xdtype, ldx)) {
+    if (int rc = launch_quantize(x, xdtype, ldx, nullptr, nullptr, n, n, K, q, ldq, xs, ldxs, st)) return rc;
+  }
   Gate gate;
   gate.act = act, gate.limit = limit, gate.slope = slope;
-  return launch_gemm(q, ldq, xs, ldxs, w, ldw, ws, out, out_dtype, ldo, n, M, K, epilogue, half_rows, gate, st);
+  return launch_gemm(x, xdtype, ldx, q, ldq, xs, ldxs, w, ldw, ws, out, out_dtype, ldo, n, M, K, epilogue, half_rows, gate, st);
 }
 
 // Bytes of scratch that `sb_experts_fp8` needs for n tokens.
@@ -665,13 +1098,18 @@ SB_EXPORT int sb_experts_fp8(const void* x, int xdtype, int64_t ldx, const int32
   if (tiles > 65535) return sb::fail("%s: %d tiles of rows are too many", who, tiles);
   sb::launch_pdl(expert_order_kernel, dim3(1), dim3(kOrderThreads), 0, st, choice, n, top, E, tile, order, list);
   if (int rc = sb::check_launch(who)) return rc;
-  if (int rc = launch_quantize(x, xdtype, ldx, order, list + 1, n, pairs, W, base + s.xq, s.ldx, xs, pairs, st)) return rc;
+  const bool quant = tile <= kQuantRows, quant_x = quant && copied_input(x, xdtype, ldx);
+  if (!quant_x) {
+    if (int rc = launch_quantize(x, xdtype, ldx, order, list + 1, n, pairs, W, base + s.xq, s.ldx, xs, pairs, st)) return rc;
+  }
   Fp8Params p = {};
+  if (quant_x) set_input(p, x, xdtype, ldx), p.x_gathered = 1;
   p.tiles = list, p.order = order, p.status = status, p.n = n, p.ranges = 1;
-  p.out = z, p.ldo = F, p.x_scales = xs, p.ldxs = pairs, p.w_scales = gate_up_scales, p.M = 2 * F, p.K = W, p.half_rows = F;
+  p.out = z, p.ldo = s.ldz, p.x_scales = xs, p.ldxs = pairs, p.w_scales = gate_up_scales, p.M = 2 * F, p.K = W, p.half_rows = F;
   p.blocks = p.range_blocks = (W + kBlock - 1) / kBlock, p.scale_rows = 2 * ((F + kBlock - 1) / kBlock);
   if (int rc = launch_product<kGated, float, true>(gate_up, static_cast<int64_t>(E) * 2 * F, ldg, base + s.xq, pairs, s.ldx, p, tile, tiles, st)) return rc;
-  if (int rc = launch_quantize(z, 0, F, nullptr, list + 1, pairs, pairs, F, base + s.zq, s.ldz, zs, pairs, st)) return rc;
+  if (quant) set_input(p, z, 0, s.ldz), p.x_gathered = 0;
+  else if (int rc = launch_quantize(z, 0, s.ldz, nullptr, list + 1, pairs, pairs, F, base + s.zq, s.ldz, zs, pairs, st)) return rc;
   p.out = parts, p.ldo = W, p.x_scales = zs, p.w_scales = down_scales, p.M = W, p.K = F, p.half_rows = 0, p.pair_weight = weights;
   p.blocks = p.range_blocks = (F + kBlock - 1) / kBlock, p.scale_rows = (W + kBlock - 1) / kBlock;
   if (int rc = launch_product<kStore, float, true>(down, static_cast<int64_t>(E) * W, ldd, base + s.zq, pairs, s.ldz, p, tile, tiles, st)) return rc;
