@@ -121,13 +121,39 @@ struct Fp8Params {
 __device__ __forceinline__ uint32_t instr_desc_e4m3(int n) {      // D float32, A and B e4m3, both K-major, M = 128
   return (1u << 4) | (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(kBlock >> 4) << 24);
 }
-__device__ __forceinline__ void umma_e4m3(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem_d),
-      "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate)
-      : "memory");
+// One block of 128 columns: four products of 32 columns (32 bytes of both operands' rows each) into a fresh accumulator, then the signals that the
+// stage has been read and the accumulator is complete, by one thread of a warp that is here as a whole. Descriptors and addresses are then
+// values of the warp, not of a thread: issued from a branch of one thread, a block took 850 cycles of moving them instead of 250 (a pair's
+// tensor cores need 512 for 256 columns).
+template <bool PAIR>
+__device__ __forceinline__ void issue_block(uint32_t tmem_d, uint64_t da, uint64_t db, uint32_t idesc, uint32_t stage_read, uint32_t complete) {
+#define SB_PRODUCT(GROUP, STEP, ACCUMULATE)                                                                                                  \
+  asm volatile("{\n\t.reg .pred e, p;\n\telect.sync _|e, 0xffffffff;\n\tsetp.ne.b32 p, %4, 0;\n\t"                                             \
+               "@e tcgen05.mma.cta_group::" GROUP ".kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem_d), "l"(da + 2 * STEP), "l"(db + 2 * STEP), \
+               "r"(idesc), "n"(ACCUMULATE)                                                                                                   \
+               : "memory")
+  if (PAIR) {
+    SB_PRODUCT("2", 0, 0);
+    SB_PRODUCT("2", 1, 1);
+    SB_PRODUCT("2", 2, 1);
+    SB_PRODUCT("2", 3, 1);
+    asm volatile("{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\t"
+                 "@e tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %2;\n\t"
+                 "@e tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%1], %2;\n\t}" ::"r"(stage_read),
+                 "r"(complete), "h"(static_cast<unsigned short>(3))
+                 : "memory");
+  } else {
+    SB_PRODUCT("1", 0, 0);
+    SB_PRODUCT("1", 1, 1);
+    SB_PRODUCT("1", 2, 1);
+    SB_PRODUCT("1", 3, 1);
+    asm volatile("{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\t"
+                 "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t"
+                 "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%1];\n\t}" ::"r"(stage_read),
+                 "r"(complete)
+                 : "memory");
+  }
+#undef SB_PRODUCT
 }
 // Waits for this warp's loads from tensor memory; what they brought passes through, so that no use of it can be moved in front of the wait.
 __device__ __forceinline__ void tmem_arrived16(uint32_t* r) {
@@ -156,7 +182,13 @@ __device__ __forceinline__ void add_scaled(float* sum, const uint32_t* v, const 
 template <int N>
 __device__ __forceinline__ void add_scaled(float* sum, const uint32_t* v, float f) {
 #pragma unroll
-  for (int c = 0; c < N; ++c) sum[c] = fmaf(__uint_as_float(v[c]), f, sum[c]);
+  for (int c = 0; c < N; c += 2)           // (two of them an instruction)
+    asm("{\n\t.reg .b64 s, v, f;\n\t"
+        "mov.b64 s, {%0, %1};\n\tmov.b64 v, {%2, %3};\n\tmov.b64 f, {%4, %4};\n\t"
+        "fma.rn.f32x2 s, v, f, s;\n\t"
+        "mov.b64 {%0, %1}, s;\n\t}"
+        : "+f"(sum[c]), "+f"(sum[c + 1])
+        : "f"(__uint_as_float(v[c])), "f"(__uint_as_float(v[c + 1])), "f"(f));
 }
 // Sixteen bytes from global to shared memory on their own, the last 16 - `bytes` as zeros.
 __device__ __forceinline__ void copy16_async(uint32_t to, const void* from, int bytes) {
@@ -266,28 +298,20 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
     }
     __syncwarp();
   } else if (warp == 1) {
-    if (lane == 0) {
-      const uint32_t idesc = instr_desc_e4m3(BN);
-      const uint64_t desc_fixed = smem_desc_sw128(0);
-      int st = 0, slot = 0;
-      uint32_t par = 0, slot_par = 1;
-      for (int i = 0; i < iters; ++i) {
-        mbar_wait(smem_u32(&slot_empty[slot]), slot_par, p.status, 42);
-        mbar_wait(smem_u32(&full_bar[st]), par, p.status, 43);
-        fence_after_sync();
-        const uint64_t da = desc_fixed | (((smem0 + st * S::kStage) & 0x3FFFF) >> 4), db = da + (kStageA >> 4);
-        const uint32_t d = tmem_base + slot * BN;
-        umma_e4m3(d, da, db, idesc, 0u);              // 32 columns = 32 bytes a step
-        umma_e4m3(d, da + 2, db + 2, idesc, 1u);
-        umma_e4m3(d, da + 4, db + 4, idesc, 1u);
-        umma_e4m3(d, da + 6, db + 6, idesc, 1u);
-        umma_commit(smem_u32(&empty_bar[st]));
-        umma_commit(smem_u32(&accum_full[slot]));
-        if (++st == p.stages) st = 0, par ^= 1;
-        if (++slot == S::kSlots) slot = 0, slot_par ^= 1;
-      }
+    const uint32_t idesc = instr_desc_e4m3(BN);
+    const uint64_t first = smem_desc_sw128(smem0);
+    int st = 0, slot = 0;
+    uint32_t par = 0, slot_par = 1;
+    for (int i = 0; i < iters; ++i) {
+      mbar_wait(smem_u32(&slot_empty[slot]), slot_par, p.status, 42);
+      mbar_wait(smem_u32(&full_bar[st]), par, p.status, 43);
+      __syncwarp();
+      fence_after_sync();
+      const uint64_t da = first + static_cast<uint64_t>(st * (S::kStage >> 4));
+      issue_block<false>(tmem_base + slot * BN, da, da + (kStageA >> 4), idesc, smem_u32(&empty_bar[st]), smem_u32(&accum_full[slot]));
+      if (++st == p.stages) st = 0, par ^= 1;
+      if (++slot == S::kSlots) slot = 0, slot_par ^= 1;
     }
-    __syncwarp();
   } else if (warp < kFirst) {
     // the scales' products, two columns a thread; four blocks are read ahead of their turn
     constexpr int kAhead = 4, kPer = (BN + 63) / 64;
@@ -507,7 +531,8 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
 // and their 128 up rows: each CTA loads 128 of them and 128 tokens, 32 KB a block for 512 cycles of the tensor cores. A weight with several K
 // ranges needs its totals beside the sums in registers and has 128 rows a tile.
 constexpr int kPairTokens = 256;
-constexpr int kPairThreads = 384;
+constexpr int kPairThreads = 640;                // a warp that loads, one that issues the products, two for the scales, sixteen of the epilogue
+constexpr int kBatch = 4, kBatches = 3;          // blocks whose factors are handed over together; batches under way
 template <bool WIDE>
 struct PairShape {
   static constexpr int kRows = WIDE ? 256 : 128;             // weight rows of a tile
@@ -515,15 +540,6 @@ struct PairShape {
   static constexpr int kSlots = WIDE ? 2 : 4;                // accumulators under way: all of tensor memory
   static constexpr int kStages = WIDE ? 6 : 8;
 };
-__device__ __forceinline__ void umma_pair_e4m3(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem_d),
-      "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate)
-      : "memory");
-}
-
 // The tiles of a launch in the order in which the pairs walk them. Dense: the tiles of tokens first, so that the pairs of a round share few weight
 // rows and every tile of tokens (which stay in L2); experts: the weight tiles of a tile of rows first.
 struct PairTile {
@@ -540,13 +556,13 @@ struct PairTile {
   }
 };
 
-// 64 results of a token, features m .. m + 63 of `rows`, to `to` (the address of the first).
+// 32 results of a token, features m .. m + 31 of `rows`, to `to` (the address of the first).
 template <int EPI, class OUT>
 __device__ __forceinline__ void store_token(OUT* to, const float* v, int m, int rows, bool vec) {
   constexpr int kPer = 16 / sizeof(OUT);
-  if (vec && m + 64 <= rows) {
+  if (vec && m + 32 <= rows) {
 #pragma unroll
-    for (int c = 0; c < 64; c += kPer) {
+    for (int c = 0; c < 32; c += kPer) {
       float r[kPer];
       uint4 raw = EPI == kAdd ? *reinterpret_cast<const uint4*>(to + c) : make_uint4(0, 0, 0, 0);
 #pragma unroll
@@ -557,7 +573,7 @@ __device__ __forceinline__ void store_token(OUT* to, const float* v, int m, int 
     }
   } else {
 #pragma unroll
-    for (int c = 0; c < 64; ++c)
+    for (int c = 0; c < 32; ++c)
       if (m + c < rows) to[c] = sb::narrow<OUT>(EPI == kAdd ? v[c] + sb::widen(to[c]) : v[c]);
   }
 }
@@ -566,14 +582,13 @@ template <int EPI, bool WIDE, class OUT, bool GROUPED>
 __global__ void __launch_bounds__(kPairThreads, 1)
 gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const Fp8Params p) {
   using S = PairShape<WIDE>;
-  constexpr int kFactors = WIDE ? 2 : 1;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   __shared__ __align__(8) uint64_t full_bar[S::kStages];      // used in the leader: both CTAs' tiles have landed
   __shared__ __align__(8) uint64_t empty_bar[S::kStages];     // in each CTA: the products that read its stage are done
   __shared__ __align__(8) uint64_t accum_full[S::kSlots];     // in each CTA
   __shared__ __align__(8) uint64_t accum_empty[S::kSlots];    // used in the leader: both CTAs have taken an accumulator's sums
-  __shared__ __align__(8) uint64_t factor_full[S::kSlots], factor_empty[S::kSlots];      // in each CTA, its own
-  __shared__ float factor[S::kSlots][kFactors][kBlock];       // by token
+  __shared__ __align__(8) uint64_t factor_full[kBatches], factor_empty[kBatches];      // in each CTA, its own
+  __shared__ float factor[kBatches][kBatch][WIDE ? 2 : 1][kBlock];                     // by token
   __shared__ uint32_t tmem_base_s;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -586,10 +601,9 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
     for (int s = 0; s < S::kStages; ++s) mbar_init(smem_u32(&full_bar[s]), 1), mbar_init(smem_u32(&empty_bar[s]), 1);
     for (int s = 0; s < S::kSlots; ++s) {
       mbar_init(smem_u32(&accum_full[s]), 1);
-      mbar_init(smem_u32(&accum_empty[s]), 16);
-      mbar_init(smem_u32(&factor_full[s]), 64);
-      mbar_init(smem_u32(&factor_empty[s]), 8);
+      mbar_init(smem_u32(&accum_empty[s]), 2 * 16);      // one arrival a warp of either CTA's epilogue
     }
+    for (int s = 0; s < kBatches; ++s) mbar_init(smem_u32(&factor_full[s]), 64), mbar_init(smem_u32(&factor_empty[s]), 16);
     mbar_init_fence();
   }
   if (warp == 1) tmem_alloc_pair(smem_u32(&tmem_base_s), 512);
@@ -602,141 +616,132 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
   sb::grid_dependency_wait();
   const int total = p.tiles_m * (GROUPED ? p.tiles[0] : p.tiles_n);
 
-  if (warp < 4) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");      // 384 x 168 registers at launch: 128 x 80 + 256 x 208 and a rest
-    if (warp == 0) {
-      if (lane == 0) {
-        int st = 0;
-        uint32_t par = 1;
-        for (int tile = pair; tile < total; tile += pairs) {
-          const PairTile t(p, GROUPED, tile);
-          const int row = t.expert * p.M + (EPI == kGated ? t.tile_m * kBlock + rank * p.half_rows : t.tile_m * S::kRows + rank * (S::kRows / 2));
-          const int token = t.n0 + rank * kBlock;
-          for (int i = 0; i < p.blocks; ++i) {
-            mbar_wait(smem_u32(&empty_bar[st]), par, p.status, 51);
-            const uint32_t bar = smem_u32(&full_bar[st]), a = smem0 + st * S::kStage;
-            if (rank == 0) mbar_expect_tx(bar, 2 * S::kStage);
-            tma_load_2d_pair(a, &map_x, bar, i * kBlock, token);
-            tma_load_2d_pair(a + kStageA, &map_w, bar, i * kBlock, row);
-            if (++st == S::kStages) st = 0, par ^= 1;
-          }
-        }
-      }
-      __syncwarp();
-    } else if (warp == 1) {
-      if (lane == 0 && rank == 0) {
-        const uint64_t desc_fixed = smem_desc_sw128(0);
-        const uint32_t idesc = (1u << 4) | (static_cast<uint32_t>(S::kRows >> 3) << 17) | (static_cast<uint32_t>(256 >> 4) << 24);
-        int st = 0, slot = 0;
-        uint32_t par = 0, slot_par = 1;
-        for (int tile = pair; tile < total; tile += pairs) {
-          for (int i = 0; i < p.blocks; ++i) {
-            mbar_wait(smem_u32(&accum_empty[slot]), slot_par, p.status, 52);
-            mbar_wait(smem_u32(&full_bar[st]), par, p.status, 53);
-            fence_after_sync();
-            const uint64_t da = desc_fixed | (((smem0 + st * S::kStage) & 0x3FFFF) >> 4), db = da + (kStageA >> 4);
-            const uint32_t d = tmem_base + slot * S::kRows;
-#pragma unroll
-            for (int k = 0; k < 4; ++k) umma_pair_e4m3(d, da + 2 * k, db + 2 * k, idesc, k > 0);
-            umma_pair_commit(smem_u32(&empty_bar[st]));
-            umma_pair_commit(smem_u32(&accum_full[slot]));
-            if (++st == S::kStages) st = 0, par ^= 1;
-            if (++slot == S::kSlots) slot = 0, slot_par ^= 1;
-          }
-        }
-      }
-      __syncwarp();
-    } else {
-      // the scales' products, two tokens a thread; four blocks are read ahead of their turn
-      constexpr int kAhead = 4;
-      const int c = threadIdx.x - 64;
-      int slot = 0;
-      uint32_t slot_par = 1;
+  if (warp == 0) {
+    if (lane == 0) {
+      int st = 0;
+      uint32_t par = 1;
       for (int tile = pair; tile < total; tile += pairs) {
         const PairTile t(p, GROUPED, tile);
-        const int last = (EPI == kGated ? p.scale_rows / 2 : p.scale_rows) - 1;      // (rows beyond the weight: their sums are nobody's)
-        const float* base = p.w_scales + static_cast<int64_t>(t.expert) * p.scale_rows * p.blocks;
-        const float* ws0 = base + static_cast<int64_t>(min(EPI == kGated || !WIDE ? t.tile_m : 2 * t.tile_m, last)) * p.blocks;
-        const float* ws1 = EPI == kGated ? ws0 + static_cast<int64_t>(p.scale_rows / 2) * p.blocks : base + static_cast<int64_t>(min(2 * t.tile_m + 1, last)) * p.blocks;
-        const int token = t.n0 + rank * kBlock + c;
-        const bool in0 = token < t.end, in1 = token + 64 < t.end;
-        const float* xs = p.x_scales + token;
-        float x0[kAhead], x1[kAhead], w0[kAhead], w1[kAhead];
-        auto fetch = [&](int i, int a) {
-          if (i >= p.blocks) return;
-          w0[a] = __ldg(ws0 + i), w1[a] = WIDE ? __ldg(ws1 + i) : 0.0f;
-          x0[a] = in0 ? xs[i * p.ldxs] : 0.0f, x1[a] = in1 ? xs[i * p.ldxs + 64] : 0.0f;
-        };
-#pragma unroll
-        for (int a = 0; a < kAhead; ++a) fetch(a, a);
-        for (int i0 = 0; i0 < p.blocks; i0 += kAhead) {
-#pragma unroll
-          for (int a = 0; a < kAhead; ++a) {
-            if (i0 + a >= p.blocks) break;
-            mbar_wait(smem_u32(&factor_empty[slot]), slot_par, p.status, 54);
-            factor[slot][0][c] = x0[a] * w0[a], factor[slot][0][c + 64] = x1[a] * w0[a];
-            if (WIDE) factor[slot][kFactors - 1][c] = x0[a] * w1[a], factor[slot][kFactors - 1][c + 64] = x1[a] * w1[a];
-            mbar_arrive(smem_u32(&factor_full[slot]));
-            fetch(i0 + a + kAhead, a);
-            if (++slot == S::kSlots) slot = 0, slot_par ^= 1;
-          }
+        const int row = t.expert * p.M + (EPI == kGated ? t.tile_m * kBlock + rank * p.half_rows : t.tile_m * S::kRows + rank * (S::kRows / 2));
+        const int token = t.n0 + rank * kBlock;
+        for (int i = 0; i < p.blocks; ++i) {
+          mbar_wait(smem_u32(&empty_bar[st]), par, p.status, 51);
+          const uint32_t bar = smem_u32(&full_bar[st]), a = smem0 + st * S::kStage;
+          if (rank == 0) mbar_expect_tx(bar, 2 * S::kStage);
+          tma_load_2d_pair(a, &map_x, bar, i * kBlock, token);
+          tma_load_2d_pair(a + kStageA, &map_w, bar, i * kBlock, row);
+          if (++st == S::kStages) st = 0, par ^= 1;
         }
       }
     }
-  } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
-    // a token a thread; of the tile's weight rows this warp has 64 of every 128
-    const int quarter = warp & 3, half = (warp - 4) >> 2, mine = quarter * 32 + lane;
-    float acc[64], other[64];            // the sums; WIDE: of the second 128 rows, else: the ranges' totals
-    int slot = 0;
-    uint32_t slot_par = 0;
-    for (int tile = pair; tile < total; tile += pairs) {
-      const PairTile t(p, GROUPED, tile);
-#pragma unroll
-      for (int c = 0; c < 64; ++c) acc[c] = 0.0f, other[c] = WIDE ? 0.0f : -0.0f;
-      bool ok = true;
-      int left = p.range_blocks;
-      for (int i = 0; i < p.blocks; ++i) {
-        ok = mbar_wait(smem_u32(&factor_full[slot]), slot_par, p.status, 56) && ok;
-        const float f0 = factor[slot][0][mine], f1 = factor[slot][kFactors - 1][mine];
-        ok = mbar_wait(smem_u32(&accum_full[slot]), slot_par, p.status, 55) && ok;
-        fence_after_sync();
-        const uint32_t from = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + slot * S::kRows + half * 64;
-        uint32_t v[2][32];               // (one set is added while the next is on its way)
-        tmem_load32_nowait(from, v[0]);
-        tmem_arrived32(v[0]);
-        tmem_load32_nowait(from + 32, v[1]);
-        add_scaled<32>(acc, v[0], f0);
-        tmem_arrived32(v[1]);
-        if (WIDE) tmem_load32_nowait(from + 128, v[0]);
-        add_scaled<32>(acc + 32, v[1], f0);
-        if (WIDE) {
-          tmem_arrived32(v[0]);
-          tmem_load32_nowait(from + 160, v[1]);
-          add_scaled<32>(other, v[0], f1);
-          tmem_arrived32(v[1]);
-        }
-        fence_before_sync();
-        __syncwarp();
-        if (lane == 0) {
-          mbar_arrive_leader(smem_u32(&accum_empty[slot]));
-          mbar_arrive(smem_u32(&factor_empty[slot]));
-        }
-        if (WIDE) add_scaled<32>(other + 32, v[1], f1);
-        if (++slot == S::kSlots) slot = 0, slot_par ^= 1;
-        if (!WIDE && (--left == 0 || i + 1 == p.blocks)) {
-          left = p.range_blocks;
-#pragma unroll
-          for (int c = 0; c < 64; ++c) other[c] += acc[c], acc[c] = 0.0f;
+    __syncwarp();
+  } else if (warp == 1) {
+    if (rank == 0) {
+      const uint64_t first = smem_desc_sw128(smem0);
+      const uint32_t idesc = (1u << 4) | (static_cast<uint32_t>(S::kRows >> 3) << 17) | (static_cast<uint32_t>(256 >> 4) << 24);
+      int st = 0, slot = 0;
+      uint32_t par = 0, slot_par = 1;
+      for (int tile = pair; tile < total; tile += pairs) {
+        for (int i = 0; i < p.blocks; ++i) {
+          mbar_wait(smem_u32(&accum_empty[slot]), slot_par, p.status, 52);
+          mbar_wait(smem_u32(&full_bar[st]), par, p.status, 53);
+          __syncwarp();
+          fence_after_sync();
+          const uint64_t da = first + static_cast<uint64_t>(st * (S::kStage >> 4));
+          issue_block<true>(tmem_base + slot * S::kRows, da, da + (kStageA >> 4), idesc, smem_u32(&empty_bar[st]), smem_u32(&accum_full[slot]));
+          if (++st == S::kStages) st = 0, par ^= 1;
+          if (++slot == S::kSlots) slot = 0, slot_par ^= 1;
         }
       }
-      const int token = t.n0 + rank * kBlock + mine;
+    }
+  } else if (warp < 4) {
+    // the scales' products, two tokens a thread, a batch ahead of those that wait in shared memory (a trip to L2 takes longer than a block)
+    const int c = threadIdx.x - 64;
+    int slot = 0;
+    uint32_t slot_par = 1;
+    for (int tile = pair; tile < total; tile += pairs) {
+      const PairTile t(p, GROUPED, tile);
+      const int last = (EPI == kGated ? p.scale_rows / 2 : p.scale_rows) - 1;      // (rows beyond the weight: their sums are nobody's)
+      const float* base = p.w_scales + static_cast<int64_t>(t.expert) * p.scale_rows * p.blocks;
+      const float* ws0 = base + static_cast<int64_t>(min(EPI == kGated || !WIDE ? t.tile_m : 2 * t.tile_m, last)) * p.blocks;
+      const float* ws1 = EPI == kGated ? ws0 + static_cast<int64_t>(p.scale_rows / 2) * p.blocks : base + static_cast<int64_t>(min(2 * t.tile_m + 1, last)) * p.blocks;
+      const int token = t.n0 + rank * kBlock + c;
+      const bool in0 = token < t.end, in1 = token + 64 < t.end;
+      const float* xs = p.x_scales + token;
+      float x0[kBatch], x1[kBatch], w0[kBatch], w1[kBatch];
+      auto fetch = [&](int i0) {
+#pragma unroll
+        for (int a = 0; a < kBatch; ++a) {
+          const int i = i0 + a;
+          const bool there = i < p.blocks;
+          w0[a] = there ? __ldg(ws0 + i) : 0.0f, w1[a] = WIDE && there ? __ldg(ws1 + i) : 0.0f;
+          x0[a] = there && in0 ? xs[i * p.ldxs] : 0.0f, x1[a] = there && in1 ? xs[i * p.ldxs + 64] : 0.0f;
+        }
+      };
+      fetch(0);
+      for (int i0 = 0; i0 < p.blocks; i0 += kBatch) {
+        mbar_wait(smem_u32(&factor_empty[slot]), slot_par, p.status, 54);
+#pragma unroll
+        for (int a = 0; a < kBatch; ++a) {
+          factor[slot][a][0][c] = x0[a] * w0[a], factor[slot][a][0][c + 64] = x1[a] * w0[a];
+          if (WIDE) factor[slot][a][WIDE ? 1 : 0][c] = x0[a] * w1[a], factor[slot][a][WIDE ? 1 : 0][c + 64] = x1[a] * w1[a];
+        }
+        mbar_arrive(smem_u32(&factor_full[slot]));
+        fetch(i0 + kBatch);
+        if (++slot == kBatches) slot = 0, slot_par ^= 1;
+      }
+    }
+  } else {
+    // a token a thread; of every 128 of the tile's weight rows this warp has 32
+    const int quarter = warp & 3, group = (warp - 4) >> 2;
+    float acc[32], other[32];            // the sums; WIDE: of the second 128 rows, else: the ranges' totals
+    int slot = 0, batch = 0;
+    uint32_t slot_par = 0, batch_par = 0;
+    for (int tile = pair; tile < total; tile += pairs) {
+      const PairTile t(p, GROUPED, tile);
+      const int token = t.n0 + rank * kBlock + quarter * 32 + lane, blocks = p.blocks;
+#pragma unroll
+      for (int c = 0; c < 32; ++c) acc[c] = 0.0f, other[c] = WIDE ? 0.0f : -0.0f;
+      bool ok = true;
+      int left = p.range_blocks;
+#pragma unroll 1
+      for (int i = 0, in_batch = 0; i < blocks; ++i) {
+        if (in_batch == 0) ok = mbar_wait(smem_u32(&factor_full[batch]), batch_par, p.status, 56) && ok;
+        const float f0 = factor[batch][in_batch][0][quarter * 32 + lane], f1 = factor[batch][in_batch][WIDE ? 1 : 0][quarter * 32 + lane];
+        ok = mbar_wait(smem_u32(&accum_full[slot]), slot_par, p.status, 55) && ok;
+        fence_after_sync();
+        const uint32_t from = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + slot * S::kRows + group * 32;
+        uint32_t v[16];
+#pragma unroll
+        for (int c0 = 0; c0 < (WIDE ? 64 : 32); c0 += 16) {
+          tmem_load16_nowait(from + (c0 & 31) + (c0 & 32 ? 128 : 0), v);
+          tmem_arrived16(v);
+          if (c0 + 16 == (WIDE ? 64 : 32)) {         // (the last of them: the accumulator is free)
+            fence_before_sync();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_leader(smem_u32(&accum_empty[slot]));
+          }
+          add_scaled<16>((c0 & 32 ? other : acc) + (c0 & 31), v, c0 & 32 ? f1 : f0);
+        }
+        if (++slot == S::kSlots) slot = 0, slot_par ^= 1;
+        if (!WIDE && (--left == 0 || i + 1 == blocks)) {
+          left = p.range_blocks;
+#pragma unroll
+          for (int c = 0; c < 32; ++c) other[c] += acc[c], acc[c] = 0.0f;
+        }
+        if (++in_batch == kBatch || i + 1 == blocks) {
+          in_batch = 0;
+          __syncwarp();
+          if (lane == 0) mbar_arrive(smem_u32(&factor_empty[batch]));
+          if (++batch == kBatches) batch = 0, batch_par ^= 1;
+        }
+      }
       if (ok && token < t.end) {
         OUT* out = static_cast<OUT*>(p.out);
         if (EPI == kGated) {
-          const int m = t.tile_m * kBlock + half * 64;
+          const int m = t.tile_m * kBlock + group * 32;
 #pragma unroll
-          for (int c = 0; c < 64; ++c) acc[c] = gated_product(acc[c], other[c], p.gate);
+          for (int c = 0; c < 32; ++c) acc[c] = gated_product(acc[c], other[c], p.gate);
           store_token<kStore>(out + static_cast<int64_t>(token) * p.ldo + m, acc, m, p.half_rows, p.vec_out);
         } else {
           int64_t row = token;
@@ -744,9 +749,9 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
             row = p.order[token];
             const float by = p.pair_weight[row];
 #pragma unroll
-            for (int c = 0; c < 64; ++c) acc[c] *= by, other[c] *= by;
+            for (int c = 0; c < 32; ++c) acc[c] *= by, other[c] *= by;
           }
-          const int m = t.tile_m * S::kRows + half * 64;
+          const int m = t.tile_m * S::kRows + group * 32;
           OUT* o = out + row * p.ldo + m;
           store_token<EPI>(o, WIDE ? acc : other, m, p.M, p.vec_out);
           if (WIDE) store_token<EPI>(o + kBlock, other, m + kBlock, p.M, p.vec_out);
