@@ -121,12 +121,12 @@ struct Fp8Params {
 __device__ __forceinline__ uint32_t instr_desc_e4m3(int n) {      // D float32, A and B e4m3, both K-major, M = 128
   return (1u << 4) | (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(kBlock >> 4) << 24);
 }
-// One block of 128 columns: four products of 32 columns (32 bytes of both operands' rows each) into a fresh accumulator, then the signals that the
-// stage has been read and the accumulator is complete, by one thread of a warp that is here as a whole. Descriptors and addresses are then
+// One block of 128 columns: four products of 32 columns (32 bytes of both operands' rows each) into a fresh accumulator, by one thread of a warp
+// that is here as a whole, as it is for the signals behind them. Descriptors and addresses are then
 // values of the warp, not of a thread: issued from a branch of one thread, a block took 850 cycles of moving them instead of 250 (a pair's
 // tensor cores need 512 for 256 columns).
 template <bool PAIR>
-__device__ __forceinline__ void issue_block(uint32_t tmem_d, uint64_t da, uint64_t db, uint32_t idesc, uint32_t stage_read, uint32_t complete) {
+__device__ __forceinline__ void issue_products(uint32_t tmem_d, uint64_t da, uint64_t db, uint32_t idesc) {
 #define SB_PRODUCT(GROUP, STEP, ACCUMULATE)                                                                                                  \
   asm volatile("{\n\t.reg .pred e, p;\n\telect.sync _|e, 0xffffffff;\n\tsetp.ne.b32 p, %4, 0;\n\t"                                             \
                "@e tcgen05.mma.cta_group::" GROUP ".kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem_d), "l"(da + 2 * STEP), "l"(db + 2 * STEP), \
@@ -137,23 +137,26 @@ __device__ __forceinline__ void issue_block(uint32_t tmem_d, uint64_t da, uint64
     SB_PRODUCT("2", 1, 1);
     SB_PRODUCT("2", 2, 1);
     SB_PRODUCT("2", 3, 1);
-    asm volatile("{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\t"
-                 "@e tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %2;\n\t"
-                 "@e tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%1], %2;\n\t}" ::"r"(stage_read),
-                 "r"(complete), "h"(static_cast<unsigned short>(3))
-                 : "memory");
   } else {
     SB_PRODUCT("1", 0, 0);
     SB_PRODUCT("1", 1, 1);
     SB_PRODUCT("1", 2, 1);
     SB_PRODUCT("1", 3, 1);
-    asm volatile("{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\t"
-                 "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t"
-                 "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%1];\n\t}" ::"r"(stage_read),
-                 "r"(complete)
-                 : "memory");
   }
 #undef SB_PRODUCT
+}
+// Arrives on the barrier (of both CTAs of a pair) once the products issued so far are done.
+template <bool PAIR>
+__device__ __forceinline__ void issue_signal(uint32_t bar) {
+  if (PAIR)
+    asm volatile("{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\t"
+                 "@e tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n\t}" ::"r"(bar),
+                 "h"(static_cast<unsigned short>(3))
+                 : "memory");
+  else
+    asm volatile("{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\t"
+                 "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(bar)
+                 : "memory");
 }
 // Waits for this warp's loads from tensor memory; what they brought passes through, so that no use of it can be moved in front of the wait.
 __device__ __forceinline__ void tmem_arrived16(uint32_t* r) {
@@ -308,7 +311,9 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
       __syncwarp();
       fence_after_sync();
       const uint64_t da = first + static_cast<uint64_t>(st * (S::kStage >> 4));
-      issue_block<false>(tmem_base + slot * BN, da, da + (kStageA >> 4), idesc, smem_u32(&empty_bar[st]), smem_u32(&accum_full[slot]));
+      issue_products<false>(tmem_base + slot * BN, da, da + (kStageA >> 4), idesc);
+      issue_signal<false>(smem_u32(&empty_bar[st]));
+      issue_signal<false>(smem_u32(&accum_full[slot]));
       if (++st == p.stages) st = 0, par ^= 1;
       if (++slot == S::kSlots) slot = 0, slot_par ^= 1;
     }
@@ -531,15 +536,21 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
 // and their 128 up rows: each CTA loads 128 of them and 128 tokens, 32 KB a block for 512 cycles of the tensor cores. A weight with several K
 // ranges needs its totals beside the sums in registers and has 128 rows a tile.
 constexpr int kPairTokens = 256;
-constexpr int kPairThreads = 640;                // a warp that loads, one that issues the products, two for the scales, sixteen of the epilogue
+constexpr int kPairThreads = 640;                // a warp that loads, two that issue the products, one for the scales, sixteen of the epilogue
 constexpr int kBatch = 4, kBatches = 3;          // blocks whose factors are handed over together; batches under way
+//
+// A block's product is issued as two chains, each with half of both CTAs' weight rows (of a gated product: a feature's gate row and its up row
+// in the same chain) and accumulators of its own, and the epilogue's warps as two sets, one a chain: a set's way from one accumulator to the
+// next (signals, first loads) then falls into the other's additions. (All sixteen warps on one accumulator at a time: 526 us.)
 template <bool WIDE>
 struct PairShape {
   static constexpr int kRows = WIDE ? 256 : 128;             // weight rows of a tile
+  static constexpr int kColumns = kRows / 2;                 // of a chain
   static constexpr int kStage = kStageA + kRows / 2 * 128;
-  static constexpr int kSlots = WIDE ? 2 : 4;                // accumulators under way: all of tensor memory
+  static constexpr int kSlots = 512 / kColumns;              // accumulators under way, all of tensor memory; even ones are the first chain's
   static constexpr int kStages = WIDE ? 6 : 8;
 };
+
 // The tiles of a launch in the order in which the pairs walk them. Dense: the tiles of tokens first, so that the pairs of a round share few weight
 // rows and every tile of tokens (which stay in L2); experts: the weight tiles of a tile of rows first.
 struct PairTile {
@@ -598,12 +609,12 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
   if (threadIdx.x == 0) {
     prefetch_tensormap(&map_w);
     prefetch_tensormap(&map_x);
-    for (int s = 0; s < S::kStages; ++s) mbar_init(smem_u32(&full_bar[s]), 1), mbar_init(smem_u32(&empty_bar[s]), 1);
+    for (int s = 0; s < S::kStages; ++s) mbar_init(smem_u32(&full_bar[s]), 1), mbar_init(smem_u32(&empty_bar[s]), 2);      // (both chains')
     for (int s = 0; s < S::kSlots; ++s) {
       mbar_init(smem_u32(&accum_full[s]), 1);
-      mbar_init(smem_u32(&accum_empty[s]), 2 * 16);      // one arrival a warp of either CTA's epilogue
+      mbar_init(smem_u32(&accum_empty[s]), 2 * 8);       // one arrival a warp of either CTA's set
     }
-    for (int s = 0; s < kBatches; ++s) mbar_init(smem_u32(&factor_full[s]), 64), mbar_init(smem_u32(&factor_empty[s]), 16);
+    for (int s = 0; s < kBatches; ++s) mbar_init(smem_u32(&factor_full[s]), 32), mbar_init(smem_u32(&factor_empty[s]), 16);
     mbar_init_fence();
   }
   if (warp == 1) tmem_alloc_pair(smem_u32(&tmem_base_s), 512);
@@ -635,11 +646,12 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
       }
     }
     __syncwarp();
-  } else if (warp == 1) {
+  } else if (warp < 3) {
     if (rank == 0) {
+      const int chain = warp - 1;
       const uint64_t first = smem_desc_sw128(smem0);
-      const uint32_t idesc = (1u << 4) | (static_cast<uint32_t>(S::kRows >> 3) << 17) | (static_cast<uint32_t>(256 >> 4) << 24);
-      int st = 0, slot = 0;
+      const uint32_t idesc = (1u << 4) | (static_cast<uint32_t>(S::kColumns >> 3) << 17) | (static_cast<uint32_t>(256 >> 4) << 24);
+      int st = 0, slot = chain;
       uint32_t par = 0, slot_par = 1;
       for (int tile = pair; tile < total; tile += pairs) {
         for (int i = 0; i < p.blocks; ++i) {
@@ -648,15 +660,16 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
           __syncwarp();
           fence_after_sync();
           const uint64_t da = first + static_cast<uint64_t>(st * (S::kStage >> 4));
-          issue_block<true>(tmem_base + slot * S::kRows, da, da + (kStageA >> 4), idesc, smem_u32(&empty_bar[st]), smem_u32(&accum_full[slot]));
+          issue_products<true>(tmem_base + slot * S::kColumns, da, da + (kStageA >> 4) + chain * (S::kColumns / 2 * 128 >> 4), idesc);
+          issue_signal<true>(smem_u32(&empty_bar[st]));
+          issue_signal<true>(smem_u32(&accum_full[slot]));
           if (++st == S::kStages) st = 0, par ^= 1;
-          if (++slot == S::kSlots) slot = 0, slot_par ^= 1;
+          if ((slot += 2) >= S::kSlots) slot = chain, slot_par ^= 1;
         }
       }
     }
-  } else if (warp < 4) {
-    // the scales' products, two tokens a thread, a batch ahead of those that wait in shared memory (a trip to L2 takes longer than a block)
-    const int c = threadIdx.x - 64;
+  } else if (warp == 3) {
+    // the scales' products, four tokens a lane, a batch ahead of those that wait in shared memory (a trip to L2 takes longer than a block)
     int slot = 0;
     uint32_t slot_par = 1;
     for (int tile = pair; tile < total; tile += pairs) {
@@ -665,37 +678,39 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
       const float* base = p.w_scales + static_cast<int64_t>(t.expert) * p.scale_rows * p.blocks;
       const float* ws0 = base + static_cast<int64_t>(min(EPI == kGated || !WIDE ? t.tile_m : 2 * t.tile_m, last)) * p.blocks;
       const float* ws1 = EPI == kGated ? ws0 + static_cast<int64_t>(p.scale_rows / 2) * p.blocks : base + static_cast<int64_t>(min(2 * t.tile_m + 1, last)) * p.blocks;
-      const int token = t.n0 + rank * kBlock + c;
-      const bool in0 = token < t.end, in1 = token + 64 < t.end;
+      const int token = t.n0 + rank * kBlock + lane;
       const float* xs = p.x_scales + token;
-      float x0[kBatch], x1[kBatch], w0[kBatch], w1[kBatch];
+      float x[kBatch][4], w0[kBatch], w1[kBatch];
       auto fetch = [&](int i0) {
 #pragma unroll
         for (int a = 0; a < kBatch; ++a) {
           const int i = i0 + a;
           const bool there = i < p.blocks;
           w0[a] = there ? __ldg(ws0 + i) : 0.0f, w1[a] = WIDE && there ? __ldg(ws1 + i) : 0.0f;
-          x0[a] = there && in0 ? xs[i * p.ldxs] : 0.0f, x1[a] = there && in1 ? xs[i * p.ldxs + 64] : 0.0f;
+#pragma unroll
+          for (int c = 0; c < 4; ++c) x[a][c] = there && token + 32 * c < t.end ? xs[i * p.ldxs + 32 * c] : 0.0f;
         }
       };
       fetch(0);
       for (int i0 = 0; i0 < p.blocks; i0 += kBatch) {
         mbar_wait(smem_u32(&factor_empty[slot]), slot_par, p.status, 54);
 #pragma unroll
-        for (int a = 0; a < kBatch; ++a) {
-          factor[slot][a][0][c] = x0[a] * w0[a], factor[slot][a][0][c + 64] = x1[a] * w0[a];
-          if (WIDE) factor[slot][a][WIDE ? 1 : 0][c] = x0[a] * w1[a], factor[slot][a][WIDE ? 1 : 0][c + 64] = x1[a] * w1[a];
-        }
+        for (int a = 0; a < kBatch; ++a)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            factor[slot][a][0][lane + 32 * c] = x[a][c] * w0[a];
+            if (WIDE) factor[slot][a][WIDE ? 1 : 0][lane + 32 * c] = x[a][c] * w1[a];
+          }
         mbar_arrive(smem_u32(&factor_full[slot]));
         fetch(i0 + kBatch);
         if (++slot == kBatches) slot = 0, slot_par ^= 1;
       }
     }
   } else {
-    // a token a thread; of every 128 of the tile's weight rows this warp has 32
-    const int quarter = warp & 3, group = (warp - 4) >> 2;
+    // a token a thread; WIDE: 32 weight rows of each CTA, else 32 of the CTA `part`
+    const int quarter = warp & 3, set = (warp - 4) >> 3, part = ((warp - 4) >> 2) & 1;
     float acc[32], other[32];            // the sums; WIDE: of the second 128 rows, else: the ranges' totals
-    int slot = 0, batch = 0;
+    int slot = set, batch = 0;
     uint32_t slot_par = 0, batch_par = 0;
     for (int tile = pair; tile < total; tile += pairs) {
       const PairTile t(p, GROUPED, tile);
@@ -710,11 +725,11 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
         const float f0 = factor[batch][in_batch][0][quarter * 32 + lane], f1 = factor[batch][in_batch][WIDE ? 1 : 0][quarter * 32 + lane];
         ok = mbar_wait(smem_u32(&accum_full[slot]), slot_par, p.status, 55) && ok;
         fence_after_sync();
-        const uint32_t from = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + slot * S::kRows + group * 32;
+        const uint32_t from = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + slot * S::kColumns + part * 32;
         uint32_t v[16];
 #pragma unroll
         for (int c0 = 0; c0 < (WIDE ? 64 : 32); c0 += 16) {
-          tmem_load16_nowait(from + (c0 & 31) + (c0 & 32 ? 128 : 0), v);
+          tmem_load16_nowait(from + (c0 & 31) + (c0 & 32 ? 64 : 0), v);
           tmem_arrived16(v);
           if (c0 + 16 == (WIDE ? 64 : 32)) {         // (the last of them: the accumulator is free)
             fence_before_sync();
@@ -723,7 +738,7 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
           }
           add_scaled<16>((c0 & 32 ? other : acc) + (c0 & 31), v, c0 & 32 ? f1 : f0);
         }
-        if (++slot == S::kSlots) slot = 0, slot_par ^= 1;
+        if ((slot += 2) >= S::kSlots) slot = set, slot_par ^= 1;
         if (!WIDE && (--left == 0 || i + 1 == blocks)) {
           left = p.range_blocks;
 #pragma unroll
@@ -739,7 +754,7 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
       if (ok && token < t.end) {
         OUT* out = static_cast<OUT*>(p.out);
         if (EPI == kGated) {
-          const int m = t.tile_m * kBlock + group * 32;
+          const int m = t.tile_m * kBlock + set * 64 + part * 32;
 #pragma unroll
           for (int c = 0; c < 32; ++c) acc[c] = gated_product(acc[c], other[c], p.gate);
           store_token<kStore>(out + static_cast<int64_t>(token) * p.ldo + m, acc, m, p.half_rows, p.vec_out);
@@ -751,7 +766,7 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
 #pragma unroll
             for (int c = 0; c < 32; ++c) acc[c] *= by, other[c] *= by;
           }
-          const int m = t.tile_m * S::kRows + group * 32;
+          const int m = t.tile_m * S::kRows + (WIDE ? set * 64 + part * 32 : part * 64 + set * 32);
           OUT* o = out + row * p.ldo + m;
           store_token<EPI>(o, WIDE ? acc : other, m, p.M, p.vec_out);
           if (WIDE) store_token<EPI>(o + kBlock, other, m + kBlock, p.M, p.vec_out);
