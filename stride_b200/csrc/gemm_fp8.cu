@@ -16,6 +16,7 @@
 // starts from zero, the ranges are added in ascending order. With few tokens the ranges are the CTAs of a cluster, which add up through
 // distributed shared memory; with many one CTA walks them all. So a token's bits depend neither on the step it is part of nor on the tile.
 #include <algorithm>
+#include <type_traits>
 
 #include "gemm_tc_tile.cuh"
 #include "step_ops.h"
@@ -28,7 +29,11 @@ using namespace sb::tc5;
 using sb::gemm_tile::bf16;
 using sb::gemm_tile::Gate;
 using sb::gemm_tile::gated_product;
+using sb::gemm_tile::kGateSilu;
+using sb::gemm_tile::silu_fast;
 
+// (No kernel here promises that its inputs are read by it alone (__restrict__): the compiler may take loads of such an input in front of the wait
+// for the kernel that writes it.)
 constexpr int kBlock = 128;            // columns (and weight rows) of a scale
 constexpr int kStageA = kBlock * 128;  // bytes of a weight tile's block
 constexpr int kMaxStages = 8;
@@ -49,50 +54,60 @@ __device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {
   return r;
 }
 
-// x [n][ldx], q [rows][ldq] bytes, scales [ceil(K / 128)][lds]. order (or null): row i of the result is token order[i] % n. used (or null): how
-// many of the rows there are.
-// A warp takes a block of 128 columns of a row, four columns a lane.
+// Eight columns of a row, k .. k + 7 of K (zeros behind).
 template <class T, bool VEC>
-__global__ void __launch_bounds__(256) quantize_kernel(const T* __restrict__ x, int64_t ldx, const int32_t* __restrict__ order,
-                                                       const int32_t* __restrict__ used, int n, int rows, int K, int blocks, uint8_t* __restrict__ q, int64_t ldq, float* __restrict__ scales, int64_t lds) {
-  sb::grid_launch_dependents();
-  sb::grid_dependency_wait();
-  const int64_t item = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
-  if (item >= static_cast<int64_t>(rows) * blocks) return;
-  const int row = static_cast<int>(item / blocks), b = static_cast<int>(item % blocks), lane = threadIdx.x & 31;
-  if (used != nullptr && row >= *used) return;
-  const int k = b * kBlock + lane * 4;
-  const int src = order != nullptr ? order[row] % n : row;
-  const T* from = x + static_cast<int64_t>(src) * ldx + k;
-  float v[4];
-  if (VEC && k < K) {
+__device__ __forceinline__ void load8(const T* from, int k, int K, float* v) {
+  if (VEC && k + 8 <= K) {
     if (sizeof(T) == 2) {
-      const uint2 raw = *reinterpret_cast<const uint2*>(from);
-      v[0] = __uint_as_float(raw.x << 16), v[1] = __uint_as_float(raw.x & 0xFFFF0000u);
-      v[2] = __uint_as_float(raw.y << 16), v[3] = __uint_as_float(raw.y & 0xFFFF0000u);
+      const uint4 raw = *reinterpret_cast<const uint4*>(from);
+      const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[2 * i] = __uint_as_float(w[i] << 16), v[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
     } else {
-      const float4 raw = *reinterpret_cast<const float4*>(from);
-      v[0] = raw.x, v[1] = raw.y, v[2] = raw.z, v[3] = raw.w;
+      const float4 a = reinterpret_cast<const float4*>(from)[0], b = reinterpret_cast<const float4*>(from)[1];
+      v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
     }
   } else {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = k + i < K ? sb::widen(from[i]) : 0.0f;
+    for (int i = 0; i < 8; ++i) v[i] = k + i < K ? sb::widen(from[i]) : 0.0f;
   }
+}
+
+// x [n][ldx] -> q bytes [rows][ldq], scales [ceil(K / 128)][lds]. Sixteen lanes take a block of 128 columns of a row, a warp two blocks; the CTA's
+// warps take neighbouring rows, whose scales lie side by side. used (or null): how many of the n rows there are. place (or null): a row is
+// stored `copies` times, as rows place[row copies + i] (left out where that is negative).
+template <class T, bool VEC>
+__global__ void __launch_bounds__(256) quantize_kernel(const T* x, int64_t ldx, const int32_t* used, const int32_t* place,
+                                                       int copies, int n, int K, int blocks, uint8_t* q, int64_t ldq,
+                                                       float* scales, int64_t lds) {
+  sb::grid_launch_dependents();
+  sb::grid_dependency_wait();
+  const int row = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31, b = blockIdx.y * 2 + (lane >> 4), k = b * kBlock + (lane & 15) * 8;
+  if (row >= n || (used != nullptr && row >= *used)) return;
+  float v[8];
+  load8<T, VEC>(x + static_cast<int64_t>(row) * ldx + k, k, K, v);
   uint32_t amax = 0;               // (the bit patterns of |x| are ordered as the values are, infinity and NaN above them)
 #pragma unroll
-  for (int i = 0; i < 4; ++i) amax = max(amax, __float_as_uint(v[i]) & 0x7FFFFFFFu);
-  amax = __reduce_max_sync(0xffffffffu, amax);
+  for (int i = 0; i < 8; ++i) amax = max(amax, __float_as_uint(v[i]) & 0x7FFFFFFFu);
+#pragma unroll
+  for (int o = 1; o < 16; o <<= 1) amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, o));
   const bool finite = amax < 0x7F800000u;
   const int e = finite ? scale_exponent(amax) : 0;
-  const float inverse = power_of_two(-e);
-  const uint32_t packed = e4m3x2(v[0] * inverse, v[1] * inverse) | (e4m3x2(v[2] * inverse, v[3] * inverse) << 16);
-  uint8_t* to = q + static_cast<int64_t>(row) * ldq + k;
-  if (k + 4 <= K) {
-    *reinterpret_cast<uint32_t*>(to) = packed;         // (rows of q start 16-byte aligned)
-  } else {
-    for (int i = 0; k + i < K; ++i) to[i] = static_cast<uint8_t>(packed >> (8 * i));
+  const float inverse = power_of_two(-e), scale = finite ? power_of_two(e) : __uint_as_float(0x7FC00000u);
+  const uint32_t lo = e4m3x2(v[0] * inverse, v[1] * inverse) | (e4m3x2(v[2] * inverse, v[3] * inverse) << 16);
+  const uint32_t hi = e4m3x2(v[4] * inverse, v[5] * inverse) | (e4m3x2(v[6] * inverse, v[7] * inverse) << 16);
+  if (b >= blocks) return;
+  for (int i = 0; i < copies; ++i) {
+    const int at = place != nullptr ? place[static_cast<int64_t>(row) * copies + i] : row;
+    if (at < 0) continue;
+    uint8_t* to = q + static_cast<int64_t>(at) * ldq + k;
+    if (k + 8 <= K) {
+      *reinterpret_cast<uint2*>(to) = make_uint2(lo, hi);            // (rows of q start 16-byte aligned)
+    } else {
+      for (int j = 0; k + j < K; ++j) to[j] = static_cast<uint8_t>((j < 4 ? lo : hi) >> (8 * (j & 3)));
+    }
+    if ((lane & 15) == 0) scales[static_cast<int64_t>(b) * lds + at] = scale;
   }
-  if (lane == 0) scales[static_cast<int64_t>(b) * lds + row] = finite ? power_of_two(e) : __uint_as_float(0x7FC00000u);
 }
 
 // ------------------------------------------------------------------ the product
@@ -114,6 +129,7 @@ struct Fp8Params {
   const int32_t* tiles;      // experts: the list of `expert_order_kernel`; else null
   const int32_t* order;      // experts: row -> pair k n + token
   const float* pair_weight;  // experts: a factor on every pair's result, by pair, or null
+  float* z_scales;           // experts, gated products quantised by the epilogue: [blocks of features][ldxs]
   Gate gate;
   int* status;
 };
@@ -222,14 +238,19 @@ struct Shape {
 
 // blockIdx = (weight tile, token tile, K range: the rank in the cluster when SPLIT). Warp 0 loads, warp 1 issues the products, warps 2 and 3
 // multiply the scales, the others are the epilogue: four of them see all 128 rows, with eight each half takes half of the columns. QUANT (few
-// tokens): the input comes as it is, and four warps quantise it, the same arithmetic as `quantize_kernel`, straight into the ring's stages. They
-// copy it ahead of its turn (kCopies blocks are under way, each thread's columns by the thread itself): without, a block took its trip to L2.
-constexpr int kCopies = 4;
+// tokens): the input comes as it is, and four warps quantise it, the same arithmetic as `quantize_kernel`, straight into the ring's stages. A
+// block is one warp's, so that four are on their way at a time (all four warps on one block at a time took 1.2 us for it), and where there is
+// room the warp's next block is copied meanwhile; a lane copies the columns that it reads. The ring's stages are a multiple of the warps: every
+// stage (and every accumulator, of which there are eight) then belongs to one warp, which sees each of its barriers' phases; a warp that met a
+// barrier only now and then could take a phase for the one two further on.
+constexpr int kQuantWarps = 4;
+__host__ __device__ constexpr int quant_depth(int bn, bool f32) { return bn * (f32 ? 4 : 2) <= 32 ? 2 : 1; }
+__host__ __device__ constexpr int quant_bytes(int bn, bool f32) { return kQuantWarps * quant_depth(bn, f32) * bn * kBlock * (f32 ? 4 : 2); }
 template <int EPI, int BN, class OUT, bool GROUPED, bool SPLIT, bool QUANT>
 __global__ void __launch_bounds__(Shape<BN>::threads(QUANT), Shape<BN>::kCtas)
 gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const Fp8Params p) {
   using S = Shape<BN>;
-  constexpr int kScaleWarps = QUANT ? 4 : 2, kFirst = 2 + kScaleWarps;        // the epilogue's first warp
+  constexpr int kScaleWarps = QUANT ? kQuantWarps : 2, kFirst = 2 + kScaleWarps;        // the epilogue's first warp
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   __shared__ __align__(8) uint64_t full_bar[kMaxStages], empty_bar[kMaxStages];
   __shared__ __align__(8) uint64_t accum_full[S::kSlots], scale_full[S::kSlots], slot_empty[S::kSlots];
@@ -254,10 +275,10 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
   if (threadIdx.x == 0) {
     prefetch_tensormap(&map_w);
     prefetch_tensormap(&map_x);
-    for (int s = 0; s < p.stages; ++s) mbar_init(smem_u32(&full_bar[s]), QUANT ? 1 + kScaleWarps : 1), mbar_init(smem_u32(&empty_bar[s]), 1);
+    for (int s = 0; s < p.stages; ++s) mbar_init(smem_u32(&full_bar[s]), QUANT ? 2 : 1), mbar_init(smem_u32(&empty_bar[s]), 1);
     for (int s = 0; s < S::kSlots; ++s) {
       mbar_init(smem_u32(&accum_full[s]), 1);
-      mbar_init(smem_u32(&scale_full[s]), 32 * kScaleWarps);
+      mbar_init(smem_u32(&scale_full[s]), QUANT ? 1 : 64);
       mbar_init(smem_u32(&slot_empty[s]), S::kEpilogueWarps);
     }
     mbar_init_fence();
@@ -325,74 +346,86 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
     const float* ws1 = EPI == kGated ? ws0 + static_cast<int64_t>(p.scale_rows / 2) * p.blocks : ws0;
     if (!GROUPED) sb::grid_dependency_wait();
     if constexpr (QUANT) {
-      constexpr int kPerRow = 128 / BN, kColumns = 128 / kPerRow;           // threads of a row of the tile, columns of a thread
-      const int r = t / kPerRow, part = t % kPerRow, size = p.x_f32 ? 4 : 2, pieces = kColumns * size / 16;
-      const bool live = n0 + r < end;
+      constexpr int kPerRow = 32 / BN, kColumns = 128 / kPerRow;            // lanes of a row of the tile, columns of a lane
+      const int r = lane / kPerRow, part = lane % kPerRow, first = warp - 2, size = p.x_f32 ? 4 : 2, pieces = kColumns * size / 16;
+      const bool live = n0 + r < end, two = quant_depth(BN, p.x_f32) == 2;
       const int64_t row = !live ? 0 : GROUPED && p.x_gathered ? pair_s[GROUPED ? r : 0] % p.n : n0 + r;
       const uint8_t* from = static_cast<const uint8_t*>(p.x) + (row * p.ldx + b0 * kBlock + part * kColumns) * size;
       const int columns = live ? p.K - b0 * kBlock - part * kColumns : 0;        // what the row has from there on
-      const uint32_t raw = smem0 + p.stages * S::kStage + t * 16;               // this thread's pieces, 128 x 16 bytes from one to the next
-      auto copy = [&](int i) {
+      const int mine = p.stages * S::kStage + first * (two ? 2 : 1) * pieces * 512 + lane * 16;      // this lane's pieces, 32 x 16 bytes from one to the next
+      auto copy = [&](int i, int buffer) {
         if (i < iters) {
           for (int j = 0; j < pieces; ++j) {
             const int there = (columns - i * kBlock) * size - 16 * j;
-            copy16_async(raw + ((i % kCopies) * pieces + j) * 2048, there > 0 ? from + i * kBlock * size + 16 * j : static_cast<const uint8_t*>(p.x),
+            copy16_async(smem0 + mine + (buffer * pieces + j) * 512, there > 0 ? from + i * kBlock * size + 16 * j : static_cast<const uint8_t*>(p.x),
                          min(max(there, 0), 16));
           }
         }
         copies_commit();
       };
-#pragma unroll
-      for (int i = 0; i < kCopies; ++i) copy(i);
-      float w0 = __ldg(ws0), w1 = EPI == kGated ? __ldg(ws1) : 0.0f;
-      int st = 0, slot = 0;
-      uint32_t par = 1, slot_par = 1;
-      for (int i = 0; i < iters; ++i) {
-        copies_wait<kCopies - 1>();
-        float v[kColumns];
-        const uint8_t* mine = smem0_p + p.stages * S::kStage + t * 16 + (i % kCopies) * pieces * 2048;
+      copy(first, 0);
+      if (two) copy(first + kQuantWarps, 1);
+      int buffer = 0;
+      for (int i = first; i < iters; i += kQuantWarps) {
+        const float w0 = __ldg(ws0 + i), w1 = EPI == kGated ? __ldg(ws1 + i) : 0.0f;
+        if (two) copies_wait<1>();
+        else copies_wait<0>();
+        const uint8_t* piece = smem0_p + mine + buffer * pieces * 512;
+        uint32_t amax = 0;
         if (p.x_f32) {
-#pragma unroll
-          for (int j = 0; j < kColumns / 4; ++j) *reinterpret_cast<float4*>(v + 4 * j) = *reinterpret_cast<const float4*>(mine + j * 2048);
+#pragma unroll 8
+          for (int j = 0; j < kColumns / 4; ++j) {
+            const uint4 a = *reinterpret_cast<const uint4*>(piece + j * 512);
+            amax = max(max(amax, max(a.x & 0x7FFFFFFFu, a.y & 0x7FFFFFFFu)), max(a.z & 0x7FFFFFFFu, a.w & 0x7FFFFFFFu));
+          }
         } else {
-#pragma unroll
+#pragma unroll 4
           for (int j = 0; j < kColumns / 8; ++j) {
-            const uint4 a = *reinterpret_cast<const uint4*>(mine + j * 2048);
+            const uint4 a = *reinterpret_cast<const uint4*>(piece + j * 512);
             const uint32_t w[4] = {a.x, a.y, a.z, a.w};
 #pragma unroll
-            for (int k = 0; k < 4; ++k) v[8 * j + 2 * k] = __uint_as_float(w[k] << 16), v[8 * j + 2 * k + 1] = __uint_as_float(w[k] & 0xFFFF0000u);
+            for (int k = 0; k < 4; ++k) amax = max(amax, max((w[k] << 16) & 0x7FFFFFFFu, w[k] & 0x7FFF0000u));
           }
         }
-        copy(i + kCopies);
-        uint32_t amax = 0;
-#pragma unroll
-        for (int j = 0; j < kColumns; ++j) amax = max(amax, __float_as_uint(v[j]) & 0x7FFFFFFFu);
-#pragma unroll
-        for (int o = 1; o < kPerRow; o <<= 1) amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+        if (kPerRow == 2) amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
         const bool finite = amax < 0x7F800000u;
-        const int e = finite ? scale_exponent(amax) : 0;
+        const int e = finite ? scale_exponent(amax) : 0, st = i % p.stages, slot = i % S::kSlots;
         const float inverse = power_of_two(-e), scale = finite ? power_of_two(e) : __uint_as_float(0x7FC00000u);
-        uint32_t q[kColumns / 4];
-#pragma unroll
-        for (int j = 0; j < kColumns / 4; ++j)
-          q[j] = e4m3x2(v[4 * j] * inverse, v[4 * j + 1] * inverse) | (e4m3x2(v[4 * j + 2] * inverse, v[4 * j + 3] * inverse) << 16);
-        mbar_wait(smem_u32(&empty_bar[st]), par, p.status, 47);
+        mbar_wait(smem_u32(&empty_bar[st]), ((i / p.stages) & 1) ^ 1, p.status, 47);
         uint8_t* to = smem0_p + st * S::kStage + kStageA + r * 128;
+#pragma unroll 2
+        for (int h = 0; h < kColumns / 16; ++h) {
+          float v[16];
+          if (p.x_f32) {
 #pragma unroll
-        for (int h = 0; h < kColumns / 16; ++h)          // (16-byte pieces of a row change places as the 128-byte swizzle has them)
-          *reinterpret_cast<uint4*>(to + (((part * (kColumns / 16) + h) ^ (r & 7)) << 4)) = make_uint4(q[4 * h], q[4 * h + 1], q[4 * h + 2], q[4 * h + 3]);
+            for (int j = 0; j < 4; ++j) *reinterpret_cast<float4*>(v + 4 * j) = *reinterpret_cast<const float4*>(piece + (4 * h + j) * 512);
+          } else {
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              const uint4 a = *reinterpret_cast<const uint4*>(piece + (2 * h + j) * 512);
+              const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+              for (int k = 0; k < 4; ++k) v[8 * j + 2 * k] = __uint_as_float(w[k] << 16), v[8 * j + 2 * k + 1] = __uint_as_float(w[k] & 0xFFFF0000u);
+            }
+          }
+          uint32_t q[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            q[j] = e4m3x2(v[4 * j] * inverse, v[4 * j + 1] * inverse) | (e4m3x2(v[4 * j + 2] * inverse, v[4 * j + 3] * inverse) << 16);
+          *reinterpret_cast<uint4*>(to + (((part * (kColumns / 16) + h) ^ (r & 7)) << 4)) = make_uint4(q[0], q[1], q[2], q[3]);      // (the 128-byte swizzle)
+        }
         fence_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(smem_u32(&full_bar[st]));
-        mbar_wait(smem_u32(&slot_empty[slot]), slot_par, p.status, 44);
+        copy(i + (two ? 2 : 1) * kQuantWarps, buffer);
+        if (two) buffer ^= 1;
+        mbar_wait(smem_u32(&slot_empty[slot]), ((i / S::kSlots) & 1) ^ 1, p.status, 44);
         if (part == 0) {
           factor[slot][0][r] = scale * w0;
           if (EPI == kGated) factor[slot][1][r] = scale * w1;
         }
-        mbar_arrive(smem_u32(&scale_full[slot]));
-        if (i + 1 < iters) w0 = __ldg(ws0 + i + 1), w1 = EPI == kGated ? __ldg(ws1 + i + 1) : 0.0f;
-        if (++st == p.stages) st = 0, par ^= 1;
-        if (++slot == S::kSlots) slot = 0, slot_par ^= 1;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&scale_full[slot]));
       }
     } else {
     float xs[kAhead][kPer], w0[kAhead], w1[kAhead];
@@ -593,6 +626,7 @@ template <int EPI, bool WIDE, class OUT, bool GROUPED>
 __global__ void __launch_bounds__(kPairThreads, 1)
 gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const Fp8Params p) {
   using S = PairShape<WIDE>;
+  constexpr bool kQuantised = std::is_same<OUT, uint8_t>::value;       // the gated products leave as e4m3 with scales of their own
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   __shared__ __align__(8) uint64_t full_bar[S::kStages];      // used in the leader: both CTAs' tiles have landed
   __shared__ __align__(8) uint64_t empty_bar[S::kStages];     // in each CTA: the products that read its stage are done
@@ -600,6 +634,7 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
   __shared__ __align__(8) uint64_t accum_empty[S::kSlots];    // used in the leader: both CTAs have taken an accumulator's sums
   __shared__ __align__(8) uint64_t factor_full[kBatches], factor_empty[kBatches];      // in each CTA, its own
   __shared__ float factor[kBatches][kBatch][WIDE ? 2 : 1][kBlock];                     // by token
+  __shared__ uint32_t largest[kQuantised ? 2 : 1][4][kQuantised ? kBlock : 1];
   __shared__ uint32_t tmem_base_s;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -751,12 +786,46 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
           if (++batch == kBatches) batch = 0, batch_par ^= 1;
         }
       }
-      if (ok && token < t.end) {
+      if (EPI == kGated) {
+        if (p.gate.act == kGateSilu) {       // (one gate for all, outside the loop)
+#pragma unroll
+          for (int c = 0; c < 32; ++c) acc[c] = silu_fast(acc[c]) * other[c];
+        } else {
+#pragma unroll
+          for (int c = 0; c < 32; ++c) acc[c] = gated_product(acc[c], other[c], p.gate);
+        }
+      }
+      if constexpr (kQuantised) {
+        // the gated products are the next product's input: a block of 128 features is four threads' (both sets, both parts)
+        const int m = t.tile_m * kBlock + set * 64 + part * 32, buffer = (tile / pairs) & 1, mine = quarter * 32 + lane;
+        uint32_t amax = 0;
+#pragma unroll
+        for (int c = 0; c < 32; ++c) amax = m + c < p.half_rows ? max(amax, __float_as_uint(acc[c]) & 0x7FFFFFFFu) : amax;
+        largest[buffer][set * 2 + part][mine] = amax;
+        asm volatile("bar.sync 1, 512;" ::: "memory");           // (the buffers alternate: who writes one again has passed the barrier behind its readers)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) amax = max(amax, largest[buffer][j][mine]);
+        const bool finite = amax < 0x7F800000u;
+        const int e = finite ? scale_exponent(amax) : 0;
+        const float inverse = power_of_two(-e);
+        if (ok && token < t.end) {
+          uint8_t* to = static_cast<uint8_t*>(p.out) + static_cast<int64_t>(token) * p.ldo + m;
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            uint32_t q[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const float* f = acc + 16 * h + 4 * j;
+              q[j] = e4m3x2(f[0] * inverse, f[1] * inverse) | (e4m3x2(f[2] * inverse, f[3] * inverse) << 16);
+            }
+            if (m + 16 * h < p.ldo) *reinterpret_cast<uint4*>(to + 16 * h) = make_uint4(q[0], q[1], q[2], q[3]);      // (rows are padded to 16 bytes)
+          }
+          if (set + part == 0) p.z_scales[static_cast<int64_t>(t.tile_m) * p.ldxs + token] = finite ? power_of_two(e) : __uint_as_float(0x7FC00000u);
+        }
+      } else if (ok && token < t.end) {
         OUT* out = static_cast<OUT*>(p.out);
         if (EPI == kGated) {
           const int m = t.tile_m * kBlock + set * 64 + part * 32;
-#pragma unroll
-          for (int c = 0; c < 32; ++c) acc[c] = gated_product(acc[c], other[c], p.gate);
           store_token<kStore>(out + static_cast<int64_t>(token) * p.ldo + m, acc, m, p.half_rows, p.vec_out);
         } else {
           int64_t row = token;
@@ -785,22 +854,28 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
 }
 
 // ------------------------------------------------------------------ experts
-// choice [n][top] -> the pairs p = k n + token in expert order, and the row tiles of the products. An id outside [0, E) is no expert: its pair
-// is left out. list: [0] tiles, [1] rows, then (expert, first row, end row) of every tile. (Which of an expert's pairs comes first does not
-// matter: every row is computed on its own.)
+// choice [n][top] -> the pairs p = k n + token in expert order, the row of every choice (place [n][top]; -1: none), and the row tiles of the
+// products. An id outside [0, E) is no expert: its pair is left out. list: [0] tiles, [1] rows, then (expert, first row, end row) of every tile.
+// (Which of an expert's pairs comes first does not matter: every row is computed on its own.) One CTA; a thread holds kHeld choices, loaded
+// together, and reads those beyond twice.
 constexpr int kMaxExperts = 1024;
-constexpr int kOrderThreads = 1024;
-__global__ void __launch_bounds__(kOrderThreads) expert_order_kernel(const int32_t* __restrict__ choice, int n, int top, int E, int tile,
-                                                                     int32_t* __restrict__ order, int32_t* __restrict__ list) {
-  __shared__ int count[kMaxExperts], place[kMaxExperts], tile_at[kMaxExperts];
+constexpr int kOrderThreads = 1024, kHeld = 16;
+__global__ void __launch_bounds__(kOrderThreads) expert_order_kernel(const int32_t* choice, int n, int top, int E, int tile,
+                                                                     int32_t* order, int32_t* place, int32_t* list) {
+  __shared__ int count[kMaxExperts], next[kMaxExperts], tile_at[kMaxExperts];
   sb::grid_launch_dependents();
   for (int e = threadIdx.x; e < E; e += blockDim.x) count[e] = 0;
   __syncthreads();
   sb::grid_dependency_wait();
-  const int pairs = n * top;
-  auto expert_of = [&](int p) { return static_cast<uint32_t>(choice[static_cast<int64_t>(p % n) * top + p / n]); };
-  for (int p = threadIdx.x; p < pairs; p += blockDim.x) {
-    const uint32_t e = expert_of(p);
+  const int pairs = n * top, t = threadIdx.x;
+  uint32_t held[kHeld];
+#pragma unroll
+  for (int j = 0; j < kHeld; ++j) held[j] = t + j * kOrderThreads < pairs ? static_cast<uint32_t>(choice[t + j * kOrderThreads]) : 0xFFFFFFFFu;
+#pragma unroll
+  for (int j = 0; j < kHeld; ++j)
+    if (held[j] < static_cast<uint32_t>(E)) atomicAdd(&count[held[j]], 1);
+  for (int i = t + kHeld * kOrderThreads; i < pairs; i += kOrderThreads) {
+    const uint32_t e = static_cast<uint32_t>(choice[i]);
     if (e < static_cast<uint32_t>(E)) atomicAdd(&count[e], 1);
   }
   __syncthreads();
@@ -808,43 +883,74 @@ __global__ void __launch_bounds__(kOrderThreads) expert_order_kernel(const int32
     const int lane = threadIdx.x;
     int rows_before = 0, tiles_before = 0;
     for (int e0 = 0; e0 < E; e0 += 32) {
-      const int e = e0 + lane, c = e < E ? count[e] : 0, t = (c + tile - 1) / tile;
-      int cs = c, ts = t;
+      const int e = e0 + lane, c = e < E ? count[e] : 0, ct = (c + tile - 1) / tile;
+      int cs = c, ts = ct;
       for (int o = 1; o < 32; o <<= 1) {
         const int a = __shfl_up_sync(0xffffffffu, cs, o), b = __shfl_up_sync(0xffffffffu, ts, o);
         if (lane >= o) cs += a, ts += b;
       }
-      if (e < E) place[e] = rows_before + cs - c, tile_at[e] = tiles_before + ts - t;
+      if (e < E) next[e] = rows_before + cs - c, tile_at[e] = tiles_before + ts - ct;
       rows_before += __shfl_sync(0xffffffffu, cs, 31), tiles_before += __shfl_sync(0xffffffffu, ts, 31);
     }
     if (lane == 0) list[0] = tiles_before, list[1] = rows_before;
   }
   __syncthreads();
   for (int e = threadIdx.x; e < E; e += blockDim.x) {
-    const int first = place[e], end = first + count[e];
+    const int first = next[e], end = first + count[e];
     int32_t* to = list + 2 + 3 * static_cast<int64_t>(tile_at[e]);
     for (int r = first; r < end; r += tile, to += 3) to[0] = e, to[1] = r, to[2] = end;
   }
   __syncthreads();
-  for (int p = threadIdx.x; p < pairs; p += blockDim.x) {
-    const uint32_t e = expert_of(p);
-    if (e < static_cast<uint32_t>(E)) order[atomicAdd(&place[e], 1)] = p;
-  }
+  auto put = [&](int i, uint32_t e) {
+    int at = -1;
+    if (e < static_cast<uint32_t>(E)) {
+      at = atomicAdd(&next[e], 1);
+      order[at] = i % top * n + i / top;
+    }
+    place[i] = at;
+  };
+#pragma unroll
+  for (int j = 0; j < kHeld; ++j)
+    if (t + j * kOrderThreads < pairs) put(t + j * kOrderThreads, held[j]);
+  for (int i = t + kHeld * kOrderThreads; i < pairs; i += kOrderThreads) put(i, static_cast<uint32_t>(choice[i]));
 }
 
-// out[t] = the token's weighted results in the order of its choices; a choice that is no expert has none.
-template <class OUT>
-__global__ void __launch_bounds__(256) expert_combine_kernel(const float* __restrict__ parts, const int32_t* __restrict__ choice, int n, int top, int E,
-                                                             int W, OUT* __restrict__ out, int64_t ldo) {
+// out[t] = the token's weighted results in the order of its choices; a choice that is no expert has none. parts [top][n][ldp], rows 16-byte
+// aligned. Four features a thread (VEC: so is the result), the choices' loads together.
+template <class OUT, bool VEC>
+__global__ void __launch_bounds__(128) expert_combine_kernel(const float* parts, int64_t ldp, const int32_t* choice, int n, int top,
+                                                             int E, int W, OUT* out, int64_t ldo) {
   sb::grid_launch_dependents();
   sb::grid_dependency_wait();
-  const int t = blockIdx.x;
+  const int t = blockIdx.x, m = (blockIdx.y * blockDim.x + threadIdx.x) * 4;
+  if (m >= W) return;
   const int32_t* mine = choice + static_cast<int64_t>(t) * top;
-  for (int m = blockIdx.y * blockDim.x + threadIdx.x; m < W; m += gridDim.y * blockDim.x) {
-    float sum = 0.0f;
-    for (int k = 0; k < top; ++k)
-      if (static_cast<uint32_t>(mine[k]) < static_cast<uint32_t>(E)) sum += parts[(static_cast<int64_t>(k) * n + t) * W + m];
-    out[static_cast<int64_t>(t) * ldo + m] = sb::narrow<OUT>(sum);
+  const float* from = parts + static_cast<int64_t>(t) * ldp + m;
+  float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+  constexpr int kTogether = 8;
+  for (int k0 = 0; k0 < top; k0 += kTogether) {
+    float4 v[kTogether];
+    bool there[kTogether];
+#pragma unroll
+    for (int k = 0; k < kTogether; ++k) {
+      there[k] = k0 + k < top && static_cast<uint32_t>(mine[min(k0 + k, top - 1)]) < static_cast<uint32_t>(E);
+      if (there[k]) v[k] = *reinterpret_cast<const float4*>(from + static_cast<int64_t>(k0 + k) * n * ldp);
+    }
+#pragma unroll
+    for (int k = 0; k < kTogether; ++k)
+      if (there[k]) sum[0] += v[k].x, sum[1] += v[k].y, sum[2] += v[k].z, sum[3] += v[k].w;
+  }
+  OUT* to = out + static_cast<int64_t>(t) * ldo + m;
+  if (VEC && m + 4 <= W) {
+    alignas(16) OUT r[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r[i] = sb::narrow<OUT>(sum[i]);
+    if (sizeof(OUT) == 4) *reinterpret_cast<uint4*>(to) = *reinterpret_cast<const uint4*>(r);
+    else *reinterpret_cast<uint2*>(to) = *reinterpret_cast<const uint2*>(r);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (m + i < W) to[i] = sb::narrow<OUT>(sum[i]);
   }
 }
 
@@ -880,15 +986,15 @@ int launch_tile(const void* w, int64_t rows_w, int64_t ldw, const void* q, int64
   if (!byte_map(w, rows_w, p.K, ldw, EPI == kGated ? 64 : kBlock, &map_w) || (!quant && !byte_map(q, rows_q, p.K, ldq, BN, &map_x)))
     return sb::fail("gemm_fp8: no tensor map for a weight of %lld x %d (stride %lld)", (long long)rows_w, p.K, (long long)ldw);
   if (quant) map_x = map_w;                  // (not read)
-  p.stages = std::min(kMaxStages, (S::kSmem - (quant && p.x_f32 ? kCopies * BN * kBlock * 4 : quant ? kCopies * BN * kBlock * 2 : 0)) / S::kStage);
-  const int copies = quant ? kCopies * BN * kBlock * (p.x_f32 ? 4 : 2) : 0;
+  // (quantising: a whole number of stages a warp, see the kernel; sixteen rows leave room for two CTAs an SM, 32 do not)
+  const int copies = quant ? quant_bytes(BN, p.x_f32) : 0;
+  p.stages = !quant ? std::min(kMaxStages, S::kSmem / S::kStage) : BN == 16 ? kQuantWarps : (kSmemBudget - copies) / S::kStage / kQuantWarps * kQuantWarps;
   const size_t smem = static_cast<size_t>(p.stages) * S::kStage + copies + 1024;
   const bool split = !GROUPED && p.ranges > 1 && p.n <= kSplitTokens;
   const dim3 grid(tiles_m, tiles_n, split ? p.ranges : 1);
   auto run = [&](auto kernel, sb::DeviceOnce& once) {
     if (once.needed()) {
-      const int most = std::min(kMaxStages, S::kSmem / S::kStage) * S::kStage + kCopies * (BN <= kQuantRows ? BN : 0) * kBlock * 4 + 1024;
-      if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most) != cudaSuccess) return sb::check_launch("gemm_fp8");
+      if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBudget + 1024) != cudaSuccess) return sb::check_launch("gemm_fp8");
       once.done();
     }
     if (split) sb::launch_pdl_cluster(kernel, grid, dim3(S::threads(quant)), smem, st, dim3(1, 1, p.ranges), map_w, map_x, p);
@@ -937,7 +1043,7 @@ template <int EPI, class OUT, bool GROUPED>
 int launch_product(const void* w, int64_t rows_w, int64_t ldw, const void* q, int64_t rows_q, int64_t ldq, const Fp8Params& p, int tile_n, int tiles_n,
                    cudaStream_t st) {
   const int tiles_m = EPI == kGated ? (p.half_rows + 63) / 64 : (p.M + kBlock - 1) / kBlock;
-  if (tile_n == kPairTokens) {
+  if (tile_n == kPairTokens && !(GROUPED && EPI == kGated)) {
     if (p.ranges == 1) return launch_pair<EPI, true, OUT, GROUPED>(w, rows_w, ldw, q, rows_q, ldq, p, tiles_n, st);
     if constexpr (EPI != kGated && !GROUPED) return launch_pair<EPI, false, OUT, GROUPED>(w, rows_w, ldw, q, rows_q, ldq, p, tiles_n, st);
   }
@@ -949,25 +1055,19 @@ int launch_product(const void* w, int64_t rows_w, int64_t ldw, const void* q, in
   }
 }
 
-int launch_quantize(const void* x, int xdtype, int64_t ldx, const int32_t* order, const int32_t* used, int n, int rows, int K, void* q, int64_t ldq, float* scales, int64_t lds,
-                    cudaStream_t st) {
+int launch_quantize(const void* x, int xdtype, int64_t ldx, const int32_t* used, const int32_t* place, int copies, int n, int K, void* q, int64_t ldq,
+                    float* scales, int64_t lds, cudaStream_t st) {
   const int blocks = (K + kBlock - 1) / kBlock;
-  const int64_t items = static_cast<int64_t>(rows) * blocks;
-  if ((items + 7) / 8 > 0x7FFFFFFF) return sb::fail("quantize_fp8: %d rows of %d columns are too many", rows, K);
-  const dim3 grid(static_cast<unsigned>((items + 7) / 8)), block(256);
-  const int size = xdtype == 0 ? 4 : 2;
-  const bool vec = K % 4 == 0 && ldx % 4 == 0 && (reinterpret_cast<uintptr_t>(x) & (4 * size - 1)) == 0;
+  const dim3 grid((n + 7) / 8, (blocks + 1) / 2), block(256);
+  if (grid.y > 65535) return sb::fail("quantize_fp8: %d columns are too many", K);
+  const bool vec = ldx * (xdtype == 0 ? 4 : 2) % 16 == 0 && (reinterpret_cast<uintptr_t>(x) & 15) == 0;
   uint8_t* to = static_cast<uint8_t*>(q);
-  if (xdtype == 0) {
-    const float* f = static_cast<const float*>(x);
-    if (vec) sb::launch_pdl(quantize_kernel<float, true>, grid, block, 0, st, f, ldx, order, used, n, rows, K, blocks, to, ldq, scales, lds);
-    else sb::launch_pdl(quantize_kernel<float, false>, grid, block, 0, st, f, ldx, order, used, n, rows, K, blocks, to, ldq, scales, lds);
-  } else {
-    const bf16* h = static_cast<const bf16*>(x);
-    if (vec) sb::launch_pdl(quantize_kernel<bf16, true>, grid, block, 0, st, h, ldx, order, used, n, rows, K, blocks, to, ldq, scales, lds);
-    else sb::launch_pdl(quantize_kernel<bf16, false>, grid, block, 0, st, h, ldx, order, used, n, rows, K, blocks, to, ldq, scales, lds);
-  }
-  return sb::check_launch("quantize_fp8");
+  auto run = [&](auto kernel, auto from) {
+    sb::launch_pdl(kernel, grid, block, 0, st, from, ldx, used, place, copies, n, K, blocks, to, ldq, scales, lds);
+    return sb::check_launch("quantize_fp8");
+  };
+  if (xdtype == 0) return vec ? run(quantize_kernel<float, true>, static_cast<const float*>(x)) : run(quantize_kernel<float, false>, static_cast<const float*>(x));
+  return vec ? run(quantize_kernel<bf16, true>, static_cast<const bf16*>(x)) : run(quantize_kernel<bf16, false>, static_cast<const bf16*>(x));
 }
 
 // Tokens of a tile of the product.
@@ -1028,7 +1128,7 @@ int most_tiles(int pairs, int E, int tile) { return std::min(pairs, pairs / tile
 
 // Where an expert call's intermediate results lie in its scratch buffer, every one 256-byte aligned.
 struct ExpertScratch {
-  int64_t order, list, xq, xs, z, zq, zs, parts, bytes, ldx, ldz;
+  int64_t order, place, list, xq, xs, z, zq, zs, parts, bytes, ldx, ldz, ldp;
 };
 ExpertScratch expert_scratch(int64_t n, int64_t top, int64_t E, int64_t W, int64_t F) {
   ExpertScratch s;
@@ -1039,11 +1139,11 @@ ExpertScratch expert_scratch(int64_t n, int64_t top, int64_t E, int64_t W, int64
     at += (bytes + 255) / 256 * 256;
     return here;
   };
-  s.ldx = (W + 15) / 16 * 16, s.ldz = (F + 15) / 16 * 16;
-  s.order = take(4 * pairs), s.list = take(4 * (2 + 3 * pairs));
+  s.ldx = (W + 15) / 16 * 16, s.ldz = (F + 15) / 16 * 16, s.ldp = (W + 3) / 4 * 4;
+  s.order = take(4 * pairs), s.place = take(4 * pairs), s.list = take(4 * (2 + 3 * pairs));
   s.xq = take(pairs * s.ldx), s.xs = take(4 * pairs * ((W + kBlock - 1) / kBlock));
   s.z = take(4 * pairs * s.ldz), s.zq = take(pairs * s.ldz), s.zs = take(4 * pairs * ((F + kBlock - 1) / kBlock));
-  s.parts = take(4 * pairs * W);
+  s.parts = take(4 * pairs * s.ldp);
   s.bytes = at;
   return s;
 }
@@ -1057,7 +1157,7 @@ SB_EXPORT int sb_quantize_fp8(const void* x, int xdtype, int64_t ldx, void* q, i
   if (int rc = check_quantized("quantize_fp8", q, ldq, lds, n, K)) return rc;
   if (xdtype < 0 || xdtype > 1 || ldx < K) return sb::fail("quantize_fp8: rows of %lld elements, %d columns", (long long)ldx, K);
   if (n == 0) return 0;
-  return launch_quantize(x, xdtype, ldx, nullptr, nullptr, n, n, K, q, ldq, scales, lds, static_cast<cudaStream_t>(stream));
+  return launch_quantize(x, xdtype, ldx, nullptr, nullptr, 1, n, K, q, ldq, scales, lds, static_cast<cudaStream_t>(stream));
 }
 
 // out = x . w^T of quantised x; epilogue 0 store, 1 add, 2 gated (w: half_rows gate rows, then as many up rows; act, limit, slope: the gate).
@@ -1071,21 +1171,33 @@ SB_EXPORT int sb_gemm_fp8(const void* q, int64_t ldq, const float* xs, int64_t l
   return launch_gemm(nullptr, 0, 0, q, ldq, xs, ldxs, w, ldw, ws, out, out_dtype, ldo, n, M, K, epilogue, half_rows, gate, static_cast<cudaStream_t>(stream));
 }
 
-// Both: x is quantised into the buffers q and xs first (of few tokens on the way into the product, which leaves the buffers alone).
-SB_EXPORT int sb_linear_fp8(const void* x, int xdtype, int64_t ldx, void* q, int64_t ldq, float* xs, int64_t ldxs, const void* w, int64_t ldw, const float* ws,
-                            void* out, int out_dtype, int64_t ldo, int n, int M, int K, int epilogue, int half_rows, int act, float limit, float slope,
-                            void* stream) {
-  if (int rc = check_quantized("linear_fp8", q, ldq, ldxs, n, K)) return rc;
-  if (int rc = check_product("linear_fp8", w, ldw, out_dtype, ldo, M, K, epilogue, half_rows)) return rc;
-  if (xdtype < 0 || xdtype > 1 || ldx < K) return sb::fail("linear_fp8: rows of %lld elements, %d columns", (long long)ldx, K);
+// What a layer hands over with every call: buffers for the quantised input, q [rows][ldq] and x_scales [ceil(K / 128)][ldxs], and the weight.
+typedef struct SbFp8Layer {
+  void* q;
+  int64_t ldq;
+  float* x_scales;
+  int64_t ldxs;
+  const void* w;
+  int64_t ldw;
+  const float* w_scales;
+  int32_t M, K, half_rows;
+} SbFp8Layer;
+
+// x is quantised, of few tokens on the way into the product (which leaves the buffers alone), then multiplied.
+SB_EXPORT int sb_linear_fp8(const SbFp8Layer* l, const void* x, int xdtype, int64_t ldx, void* out, int out_dtype, int64_t ldo, int n, int epilogue, int act,
+                            float limit, float slope, void* stream) {
+  if (int rc = check_quantized("linear_fp8", l->q, l->ldq, l->ldxs, n, l->K)) return rc;
+  if (int rc = check_product("linear_fp8", l->w, l->ldw, out_dtype, ldo, l->M, l->K, epilogue, l->half_rows)) return rc;
+  if (xdtype < 0 || xdtype > 1 || ldx < l->K) return sb::fail("linear_fp8: rows of %lld elements, %d columns", (long long)ldx, l->K);
   if (n == 0) return 0;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (n > kQuantRows || !copied_input(x, xdtype, ldx)) {
-    if (int rc = launch_quantize(x, xdtype, ldx, nullptr, nullptr, n, n, K, q, ldq, xs, ldxs, st)) return rc;
+    if (int rc = launch_quantize(x, xdtype, ldx, nullptr, nullptr, 1, n, l->K, l->q, l->ldq, l->x_scales, l->ldxs, st)) return rc;
   }
   Gate gate;
   gate.act = act, gate.limit = limit, gate.slope = slope;
-  return launch_gemm(x, xdtype, ldx, q, ldq, xs, ldxs, w, ldw, ws, out, out_dtype, ldo, n, M, K, epilogue, half_rows, gate, st);
+  return launch_gemm(x, xdtype, ldx, l->q, l->ldq, l->x_scales, l->ldxs, l->w, l->ldw, l->w_scales, out, out_dtype, ldo, n, l->M, l->K, epilogue,
+                     epilogue == kGated ? l->half_rows : 0, gate, st);
 }
 
 // Bytes of scratch that `sb_experts_fp8` needs for n tokens.
@@ -1094,9 +1206,22 @@ SB_EXPORT int64_t sb_experts_fp8_scratch(int n, int top, int E, int W, int F) { 
 // out[t] = sum over k of weights[k][t] D_e (silu(G_e x_t) * (U_e x_t)), e = choice[t][k] (no expert: no term). gate_up [E 2F][ldg] e4m3 (an
 // expert's gate rows, then its up rows) with scales [E 2 ceil(F / 128)][ceil(W / 128)], down [E W][ldd] with [E ceil(W / 128)][ceil(F / 128)].
 // The gated products stay in 32-bit until they are quantised.
-SB_EXPORT int sb_experts_fp8(const void* x, int xdtype, int64_t ldx, const int32_t* choice, const float* weights, const void* gate_up, int64_t ldg,
-                             const float* gate_up_scales, const void* down, int64_t ldd, const float* down_scales, void* out, int out_dtype, int64_t ldo,
-                             int n, int top, int E, int W, int F, void* scratch, int64_t scratch_bytes, void* stream) {
+typedef struct SbFp8Experts {
+  const void* gate_up;
+  int64_t ldg;
+  const float* gate_up_scales;
+  const void* down;
+  int64_t ldd;
+  const float* down_scales;
+  int32_t experts, width, inner;
+} SbFp8Experts;
+
+SB_EXPORT int sb_experts_fp8(const SbFp8Experts* l, const void* x, int xdtype, int64_t ldx, const int32_t* choice, const float* weights, void* out,
+                             int out_dtype, int64_t ldo, int n, int top, void* scratch, int64_t scratch_bytes, void* stream) {
+  const void *gate_up = l->gate_up, *down = l->down;
+  const float *gate_up_scales = l->gate_up_scales, *down_scales = l->down_scales;
+  const int64_t ldg = l->ldg, ldd = l->ldd;
+  const int E = l->experts, W = l->width, F = l->inner;
   const char* who = "experts_fp8";
   if (n < 0 || top < 1 || E < 1 || E > kMaxExperts || W < 1 || F < 1) return sb::fail("%s: %d of %d experts (at most %d), %d tokens, sizes %d and %d", who, top, E, kMaxExperts, n, W, F);
   if (static_cast<int64_t>(n) * top > (1 << 24) || static_cast<int64_t>(E) * std::max(2 * F, W) > 0x7FFFFFFF)
@@ -1111,32 +1236,41 @@ SB_EXPORT int sb_experts_fp8(const void* x, int xdtype, int64_t ldx, const int32
   if (status == nullptr) return sb::fail("%s: no status word on this device", who);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   uint8_t* base = static_cast<uint8_t*>(scratch);
-  int32_t *order = reinterpret_cast<int32_t*>(base + s.order), *list = reinterpret_cast<int32_t*>(base + s.list);
+  int32_t *order = reinterpret_cast<int32_t*>(base + s.order), *place = reinterpret_cast<int32_t*>(base + s.place), *list = reinterpret_cast<int32_t*>(base + s.list);
   float *xs = reinterpret_cast<float*>(base + s.xs), *z = reinterpret_cast<float*>(base + s.z), *zs = reinterpret_cast<float*>(base + s.zs);
   float* parts = reinterpret_cast<float*>(base + s.parts);
   const int pairs = n * top, tile = expert_tile(pairs, E), tiles = most_tiles(pairs, E, tile);
   if (tiles > 65535) return sb::fail("%s: %d tiles of rows are too many", who, tiles);
-  sb::launch_pdl(expert_order_kernel, dim3(1), dim3(kOrderThreads), 0, st, choice, n, top, E, tile, order, list);
+  sb::launch_pdl(expert_order_kernel, dim3(1), dim3(kOrderThreads), 0, st, choice, n, top, E, tile, order, place, list);
   if (int rc = sb::check_launch(who)) return rc;
   const bool quant = tile <= kQuantRows, quant_x = quant && copied_input(x, xdtype, ldx);
   if (!quant_x) {
-    if (int rc = launch_quantize(x, xdtype, ldx, order, list + 1, n, pairs, W, base + s.xq, s.ldx, xs, pairs, st)) return rc;
+    if (int rc = launch_quantize(x, xdtype, ldx, nullptr, place, top, n, W, base + s.xq, s.ldx, xs, pairs, st)) return rc;
   }
   Fp8Params p = {};
   if (quant_x) set_input(p, x, xdtype, ldx), p.x_gathered = 1;
   p.tiles = list, p.order = order, p.status = status, p.n = n, p.ranges = 1;
   p.out = z, p.ldo = s.ldz, p.x_scales = xs, p.ldxs = pairs, p.w_scales = gate_up_scales, p.M = 2 * F, p.K = W, p.half_rows = F;
   p.blocks = p.range_blocks = (W + kBlock - 1) / kBlock, p.scale_rows = 2 * ((F + kBlock - 1) / kBlock);
-  if (int rc = launch_product<kGated, float, true>(gate_up, static_cast<int64_t>(E) * 2 * F, ldg, base + s.xq, pairs, s.ldx, p, tile, tiles, st)) return rc;
-  if (quant) set_input(p, z, 0, s.ldz), p.x_gathered = 0;
-  else if (int rc = launch_quantize(z, 0, s.ldz, nullptr, list + 1, pairs, pairs, F, base + s.zq, s.ldz, zs, pairs, st)) return rc;
-  p.out = parts, p.ldo = W, p.x_scales = zs, p.w_scales = down_scales, p.M = W, p.K = F, p.half_rows = 0, p.pair_weight = weights;
+  if (tile == kPairTokens) {         // (the pairs' epilogue quantises the gated products itself)
+    p.out = base + s.zq, p.ldo = s.ldz, p.z_scales = zs;
+    if (int rc = launch_pair<kGated, true, uint8_t, true>(gate_up, static_cast<int64_t>(E) * 2 * F, ldg, base + s.xq, pairs, s.ldx, p, tiles, st)) return rc;
+  } else {
+    if (int rc = launch_product<kGated, float, true>(gate_up, static_cast<int64_t>(E) * 2 * F, ldg, base + s.xq, pairs, s.ldx, p, tile, tiles, st)) return rc;
+    if (quant) set_input(p, z, 0, s.ldz), p.x_gathered = 0;
+    else if (int rc = launch_quantize(z, 0, s.ldz, list + 1, nullptr, 1, pairs, F, base + s.zq, s.ldz, zs, pairs, st)) return rc;
+  }
+  p.out = parts, p.ldo = s.ldp, p.x_scales = zs, p.w_scales = down_scales, p.M = W, p.K = F, p.half_rows = 0, p.pair_weight = weights;
   p.blocks = p.range_blocks = (F + kBlock - 1) / kBlock, p.scale_rows = (W + kBlock - 1) / kBlock;
   if (int rc = launch_product<kStore, float, true>(down, static_cast<int64_t>(E) * W, ldd, base + s.zq, pairs, s.ldz, p, tile, tiles, st)) return rc;
-  const dim3 grid(n, n >= 296 ? 1 : std::min((W + 255) / 256, (296 + n - 1) / n));
-  if (out_dtype == 0)
-    sb::launch_pdl(expert_combine_kernel<float>, grid, dim3(256), 0, st, static_cast<const float*>(parts), choice, n, top, E, W, static_cast<float*>(out), ldo);
-  else
-    sb::launch_pdl(expert_combine_kernel<bf16>, grid, dim3(256), 0, st, static_cast<const float*>(parts), choice, n, top, E, W, static_cast<bf16*>(out), ldo);
+  const dim3 grid(n, (W + 511) / 512);
+  if (grid.y > 65535) return sb::fail("%s: %d features are too many", who, W);
+  auto combine = [&](auto kernel, auto to) {
+    sb::launch_pdl(kernel, grid, dim3(128), 0, st, static_cast<const float*>(parts), s.ldp, choice, n, top, E, W, to, ldo);
+  };
+  const int size = out_dtype == 0 ? 4 : 2;
+  const bool vec = ldo % 4 == 0 && (reinterpret_cast<uintptr_t>(out) & (4 * size - 1)) == 0;
+  if (out_dtype == 0) vec ? combine(expert_combine_kernel<float, true>, static_cast<float*>(out)) : combine(expert_combine_kernel<float, false>, static_cast<float*>(out));
+  else vec ? combine(expert_combine_kernel<bf16, true>, static_cast<bf16*>(out)) : combine(expert_combine_kernel<bf16, false>, static_cast<bf16*>(out));
   return sb::check_launch(who);
 }

@@ -14,6 +14,8 @@ kernel adds them itself, in the same order: a token's result has the same bits e
 """
 from __future__ import annotations
 
+import ctypes
+
 import torch
 
 from . import ops
@@ -108,6 +110,9 @@ class Fp8Experts:
         self.gate_up_scales = torch.cat([w.scales for w in gate_up])
         self.down = torch.cat([w.q.view(torch.uint8) for w in down]).view(torch.float8_e4m3fn)
         self.down_scales = torch.cat([w.scales for w in down])
+        self._layout = ops._Fp8ExpertsLayout(self.gate_up.data_ptr(), self.gate_up.stride(0), self.gate_up_scales.data_ptr(), self.down.data_ptr(),
+                                             self.down.stride(0), self.down_scales.data_ptr(), self.experts, self.width, self.inner)
+        self.address = ctypes.addressof(self._layout)
 
     def weight_bytes(self) -> int:
         """Of one expert."""
@@ -126,7 +131,7 @@ class Linear:
             weight = weight.to(torch.float32)          # the 32-bit engine: what the 8-bit weight stands for, in true 32-bit products
         self.fp8 = weight if isinstance(weight, Fp8Weight) else None
         if self.fp8 is not None:
-            self.weight = None
+            self.weight = self._call = self._call_workspace = None
             self.out_features, self.in_features = weight.shape
             self.compute_dtype, self.tensor_core, self.splits = compute_dtype, False, 1
             return
@@ -142,19 +147,18 @@ class Linear:
     def weight_bytes(self) -> int:
         return self.fp8.nbytes() if self.fp8 is not None else self.weight.numel() * self.weight.element_size()
 
-    def _quantised(self, workspace, n: int):
-        """The workspace's buffers for n quantised rows of this layer's input: (values, scales)."""
+    def _buffers(self, workspace):
+        """The workspace's buffers for the quantised rows of this layer's input: (values, scales)."""
         if workspace is None:
             raise ValueError("a linear layer with an 8-bit weight takes the workspace that its quantised input is kept in")
         T, K = workspace.max_tokens, self.in_features
-        if n > T:
-            raise ValueError(f"a step of {n} tokens exceeds the workspace's {T}")
         q = workspace.raw("linear.fp8", (T, -(-K // 16) * 16), torch.float8_e4m3fn)
         return q, workspace.raw("linear.fp8_scales", (-(-K // ops.FP8_BLOCK), T), torch.float32)
 
     def _fp8(self, x: torch.Tensor, out: torch.Tensor, epilogue: int, workspace, constants=(0.0, 0.0)) -> None:
-        q, scales = self._quantised(workspace, x.shape[0])
-        ops.linear_fp8(x, q[:x.shape[0]], scales, self.fp8, out, epilogue, constants)
+        if self._call is None or self._call_workspace is not workspace:
+            self._call, self._call_workspace = ops.Fp8Linear(self.fp8, *self._buffers(workspace)), workspace
+        self._call(x, out, epilogue, constants)
 
     def _tc(self, x: torch.Tensor) -> bool:
         return self.tensor_core and x.dtype == torch.bfloat16 and x.stride(0) % 8 == 0

@@ -784,19 +784,48 @@ def gemm_fp8(q: torch.Tensor, scales: torch.Tensor, weight, out: torch.Tensor, e
                    dtype_code(out.dtype), _row_stride(out), n, M, K, code, half, max(epilogue - SWIGLU, 0), *constants, _stream()))
 
 
-def linear_fp8(x: torch.Tensor, q: torch.Tensor, scales: torch.Tensor, weight, out: torch.Tensor, epilogue: int = STORE, constants=(0.0, 0.0)) -> None:
-    """`quantize_fp8` of x into the buffers q and scales, then `gemm_fp8`, in one call."""
-    _cuda(x, q, scales, weight.q, out)
-    n, K = x.shape
-    if K != weight.shape[1] or (K > 1 and x.stride(1) != 1):
-        raise ValueError(f"linear_fp8 shapes: x {tuple(x.shape)}, weight {tuple(weight.shape)}")
-    _check_fp8_rows("linear_fp8", q, scales, n, K)
-    M, code, half = _fp8_product(weight, out, epilogue, n)
-    lib, fn = _fn("gemm_fp8", "sb_linear_fp8", [c_void_p, c_int, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p,
-                                                c_int, c_int64, c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_float, c_void_p])
-    _check(lib, fn(_ptr(x), dtype_code(x.dtype), _row_stride(x), _ptr(q), _row_stride(q), _ptr(scales), _row_stride(scales), _ptr(weight.q), weight.stride,
-                   _ptr(weight.scales), _ptr(out), dtype_code(out.dtype), _row_stride(out), n, M, K, code, half, max(epilogue - SWIGLU, 0), *constants,
-                   _stream()))
+class _Fp8Layer(ctypes.Structure):
+    """What a layer with an 8-bit weight hands over with every call (csrc/gemm_fp8.cu: SbFp8Layer)."""
+    _fields_ = [("q", c_void_p), ("ldq", c_int64), ("x_scales", c_void_p), ("ldxs", c_int64), ("w", c_void_p), ("ldw", c_int64), ("w_scales", c_void_p),
+                ("M", c_int), ("K", c_int), ("half_rows", c_int)]
+
+
+class Fp8Linear:
+    """`quantize_fp8` and `gemm_fp8` in one call: `Fp8Linear(weight, q, scales)(x, out)` with buffers q [max rows, columns] and scales
+    [column blocks, max rows] for the quantised input. What does not change from call to call is checked and laid out once, here."""
+
+    def __init__(self, weight, q: torch.Tensor, scales: torch.Tensor):
+        _cuda(q, scales, weight.q)
+        self.M, self.K = weight.shape
+        _check_fp8_rows("linear_fp8", q, scales, q.shape[0], self.K)
+        self.rows, self.halves, self.in_blocks = min(q.shape[0], scales.shape[1]), weight.halves, weight.in_blocks
+        self._keep = (weight, q, scales)
+        half = self.M // 2 if weight.halves == 2 else 0
+        self._layer = _Fp8Layer(q.data_ptr(), _row_stride(q), scales.data_ptr(), _row_stride(scales), weight.q.data_ptr(), weight.stride,
+                                weight.scales.data_ptr(), self.M, self.K, half)
+        self._address = ctypes.addressof(self._layer)
+        self._lib, self._fn = _fn("gemm_fp8", "sb_linear_fp8", [c_void_p, c_void_p, c_int, c_int64, c_void_p, c_int, c_int64, c_int, c_int, c_int,
+                                                                c_float, c_float, c_void_p])
+
+    def __call__(self, x: torch.Tensor, out: torch.Tensor, epilogue: int = STORE, constants=(0.0, 0.0)) -> None:
+        if not (x.is_cuda and out.is_cuda):
+            _cuda(x, out)
+        gated = epilogue >= SWIGLU
+        (n, K), (rows, M) = x.shape, out.shape
+        ldx, step_x = x.stride()
+        ldo, step_o = out.stride()
+        if K != self.K or rows != n or M != (self.M // 2 if gated else self.M) or n > self.rows or (K > 1 and step_x != 1) or (M > 1 and step_o != 1):
+            raise ValueError(f"linear_fp8: x {tuple(x.shape)}, weight {(self.M, self.K)}, out {tuple(out.shape)}, at most {self.rows} rows, "
+                             f"rows of consecutive elements")
+        if gated and self.halves != 2:
+            raise ValueError("a gated product takes a weight stacked from a gate and an up matrix of one shape")
+        if not gated and not self.in_blocks:
+            raise ValueError("a stacked weight whose matrices are no whole number of 128 rows only has the gated product")
+        if n <= 1:
+            ldx, ldo = max(ldx, K), max(ldo, M)          # (of a single row the stride says nothing)
+        rc = self._fn(self._address, x.data_ptr(), dtype_code(x.dtype), ldx, out.data_ptr(), dtype_code(out.dtype), ldo, n, epilogue if epilogue < SWIGLU else 2,
+                      epilogue - SWIGLU if gated else 0, *constants, _stream())
+        _check(self._lib, rc)
 
 
 ROUTER_SCORES = {"sigmoid": 0, "softmax": 1}
@@ -812,18 +841,18 @@ def route_experts(logits: torch.Tensor, choice: torch.Tensor, weights: torch.Ten
     _cuda(logits, bias, choice, weights)
     if score not in ROUTER_SCORES:
         raise ValueError(f"route_experts: unknown score '{score}' (known: {', '.join(ROUTER_SCORES)})")
-    n, E = logits.shape
-    top = choice.shape[1]
-    if logits.dtype != torch.float32 or weights.dtype != torch.float32 or choice.dtype != torch.int32 or (bias is not None and bias.dtype != torch.float32):
+    (n, E), (rows, top), f32 = logits.shape, choice.shape, torch.float32
+    (ldz, step_z), (ldw, step_w) = logits.stride(), weights.stride()
+    if logits.dtype != f32 or weights.dtype != f32 or choice.dtype != torch.int32 or (bias is not None and bias.dtype != f32):
         raise TypeError("route_experts takes float32 logits, bias and weights and an int32 choice")
-    if tuple(choice.shape) != (n, top) or not choice.is_contiguous() or tuple(weights.shape) != (top, n) or (n > 1 and weights.stride(1) != 1) \
-            or (E > 1 and logits.stride(1) != 1) or (bias is not None and (tuple(bias.shape) != (E,) or not bias.is_contiguous())):
+    if rows != n or weights.shape != (top, n) or not choice.is_contiguous() or (n > 1 and step_w != 1) or (E > 1 and step_z != 1) \
+            or (bias is not None and (bias.shape != (E,) or not bias.is_contiguous())):
         raise ValueError(f"route_experts shapes: logits {tuple(logits.shape)}, choice {tuple(choice.shape)}, weights {tuple(weights.shape)}"
                          + (f", bias {tuple(bias.shape)}" if bias is not None else ""))
     lib, fn = _fn("router", "sb_route_experts", [c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_int64, c_int, c_int, c_int, c_int, c_int, c_int, c_int,
                                                  c_int, c_float, c_void_p])
-    _check(lib, fn(_ptr(logits), _row_stride(logits), _ptr(bias), _ptr(choice), _ptr(weights), _row_stride(weights), n, E, top, ROUTER_SCORES[score], groups,
-                   top_groups, group_best, int(renormalise), scale, _stream()))
+    _check(lib, fn(logits.data_ptr(), ldz if n > 1 else max(ldz, E), 0 if bias is None else bias.data_ptr(), choice.data_ptr(), weights.data_ptr(),
+                   ldw if top > 1 else max(ldw, n), n, E, top, ROUTER_SCORES[score], groups, top_groups, group_best, int(renormalise), scale, _stream()))
 
 
 def experts_fp8_scratch(n: int, top: int, experts: int, width: int, inner: int) -> int:
@@ -837,18 +866,24 @@ def experts_fp8(x: torch.Tensor, choice: torch.Tensor, weights: torch.Tensor, ex
     """out[t] = sum over k of weights[k, t] * down_e (silu(gate_e x_t) * (up_e x_t)), e = choice[t, k], in the order of the choices; an id that is no
     expert's has no term. x [n, width] float32 or bfloat16, choice [n, top] int32, weights [top, n] float32, `experts` an `Fp8Experts`, out float32 or
     bfloat16 [n, width], scratch uint8 of `experts_fp8_scratch` bytes. Inputs of both projections are quantised as `quantize_fp8` does."""
-    _cuda(x, choice, weights, experts.gate_up, out, scratch)
-    n, W = x.shape
-    top = choice.shape[1]
+    _cuda(x, choice, weights, out, scratch)
+    (n, W), (rows, top) = x.shape, choice.shape
+    (ldx, step_x), (ldo, step_o) = x.stride(), out.stride()
     if choice.dtype != torch.int32 or weights.dtype != torch.float32 or scratch.dtype != torch.uint8:
         raise TypeError("experts_fp8 takes an int32 choice, float32 weights and uint8 scratch")
-    if W != experts.width or tuple(out.shape) != (n, W) or tuple(choice.shape) != (n, top) or tuple(weights.shape) != (top, n) \
-            or not choice.is_contiguous() or not weights.is_contiguous() or not scratch.is_contiguous() \
-            or (W > 1 and (x.stride(1) != 1 or out.stride(1) != 1)):
+    if W != experts.width or out.shape != (n, W) or rows != n or weights.shape != (top, n) or not choice.is_contiguous() or not weights.is_contiguous() \
+            or not scratch.is_contiguous() or (W > 1 and (step_x != 1 or step_o != 1)):
         raise ValueError(f"experts_fp8 shapes: x {tuple(x.shape)}, choice {tuple(choice.shape)}, weights {tuple(weights.shape)}, out {tuple(out.shape)}, "
                          f"experts of width {experts.width}")
-    lib, fn = _fn("gemm_fp8", "sb_experts_fp8", [c_void_p, c_int, c_int64, c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_void_p,
-                                                 c_void_p, c_int, c_int64, c_int, c_int, c_int, c_int, c_int, c_void_p, c_int64, c_void_p])
-    _check(lib, fn(_ptr(x), dtype_code(x.dtype), _row_stride(x), _ptr(choice), _ptr(weights), _ptr(experts.gate_up), experts.gate_up.stride(0),
-                   _ptr(experts.gate_up_scales), _ptr(experts.down), experts.down.stride(0), _ptr(experts.down_scales), _ptr(out), dtype_code(out.dtype),
-                   _row_stride(out), n, top, experts.experts, W, experts.inner, _ptr(scratch), scratch.numel(), _stream()))
+    if n <= 1:
+        ldx, ldo = max(ldx, W), max(ldo, W)
+    lib, fn = _fn("gemm_fp8", "sb_experts_fp8", [c_void_p, c_void_p, c_int, c_int64, c_void_p, c_void_p, c_void_p, c_int, c_int64, c_int, c_int, c_void_p,
+                                                 c_int64, c_void_p])
+    _check(lib, fn(experts.address, x.data_ptr(), dtype_code(x.dtype), ldx, choice.data_ptr(), weights.data_ptr(), out.data_ptr(), dtype_code(out.dtype), ldo,
+                   n, top, scratch.data_ptr(), scratch.numel(), _stream()))
+
+
+class _Fp8ExpertsLayout(ctypes.Structure):
+    """The experts' weights as csrc/gemm_fp8.cu takes them (SbFp8Experts)."""
+    _fields_ = [("gate_up", c_void_p), ("ldg", c_int64), ("gate_up_scales", c_void_p), ("down", c_void_p), ("ldd", c_int64), ("down_scales", c_void_p),
+                ("experts", c_int), ("width", c_int), ("inner", c_int)]
