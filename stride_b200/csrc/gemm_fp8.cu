@@ -228,7 +228,7 @@ template <int BN>
 struct Shape {
   static constexpr int kEpilogueWarps = BN >= 64 ? 8 : 4;
   static constexpr int kColumns = BN * 4 / kEpilogueWarps;             // columns of a thread's row of the tile
-  static constexpr int threads(bool quant) { return 128 + 32 * kEpilogueWarps + (quant ? 64 : 0); }
+  static constexpr int threads(bool quant) { return 128 + 32 * kEpilogueWarps + (quant ? 192 : 0); }
   static constexpr int kSlots = BN <= 32 ? 8 : 4;                      // accumulators under way
   static constexpr int kStage = kStageA + BN * 128;
   static constexpr int kTmem = kSlots * BN;                            // (a power of two)
@@ -239,15 +239,14 @@ struct Shape {
 // blockIdx = (weight tile, token tile, K range: the rank in the cluster when SPLIT). Warp 0 loads, warp 1 issues the products, warps 2 and 3
 // multiply the scales, the others are the epilogue: four of them see all 128 rows, with eight each half takes half of the columns. QUANT (few
 // tokens): the input comes as it is, and four warps quantise it, the same arithmetic as `quantize_kernel`, straight into the ring's stages. A
-// block is one warp's, so that four are on their way at a time (all four warps on one block at a time took 1.2 us for it), and where there is
-// room the warp's next block is copied meanwhile; a lane copies the columns that it reads. The ring's stages are a multiple of the warps: every
-// stage (and every accumulator, of which there are eight) then belongs to one warp, which sees each of its barriers' phases; a warp that met a
-// barrier only now and then could take a phase for the one two further on.
-constexpr int kQuantWarps = 4;
-__host__ __device__ constexpr int quant_depth(int bn, bool f32) { return bn * (f32 ? 4 : 2) <= 32 ? 2 : 1; }
-__host__ __device__ constexpr int quant_bytes(int bn, bool f32) { return kQuantWarps * quant_depth(bn, f32) * bn * kBlock * (f32 ? 4 : 2); }
+// block is one warp's, so that eight (of float32 four) are on their way at a time; all warps on one block at a time took 1.2 us for it. A lane
+// copies the columns that it reads. A warp meets a stage's barrier only now and then, and could take one phase for the one two further on:
+// it looks there only once its accumulator, of which there are eight, is free, and with it the last but one block of that stage.
+constexpr int kQuantWarps = 8;
+__host__ __device__ constexpr int quant_warps(bool f32) { return f32 ? 4 : 8; }        // (of float32 there is no room for more)
+__host__ __device__ constexpr int quant_bytes(int bn, bool f32) { return quant_warps(f32) * bn * kBlock * (f32 ? 4 : 2); }
 template <int EPI, int BN, class OUT, bool GROUPED, bool SPLIT, bool QUANT>
-__global__ void __launch_bounds__(Shape<BN>::threads(QUANT), Shape<BN>::kCtas)
+__global__ void __launch_bounds__(Shape<BN>::threads(QUANT), QUANT && BN > 16 ? 1 : Shape<BN>::kCtas)
 gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const Fp8Params p) {
   using S = Shape<BN>;
   constexpr int kScaleWarps = QUANT ? kQuantWarps : 2, kFirst = 2 + kScaleWarps;        // the epilogue's first warp
@@ -347,30 +346,28 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
     if (!GROUPED) sb::grid_dependency_wait();
     if constexpr (QUANT) {
       constexpr int kPerRow = 32 / BN, kColumns = 128 / kPerRow;            // lanes of a row of the tile, columns of a lane
-      const int r = lane / kPerRow, part = lane % kPerRow, first = warp - 2, size = p.x_f32 ? 4 : 2, pieces = kColumns * size / 16;
-      const bool live = n0 + r < end, two = quant_depth(BN, p.x_f32) == 2;
+      const int r = lane / kPerRow, part = lane % kPerRow, first = warp - 2, warps = quant_warps(p.x_f32), size = p.x_f32 ? 4 : 2,
+                pieces = kColumns * size / 16;
+      const bool live = n0 + r < end;
       const int64_t row = !live ? 0 : GROUPED && p.x_gathered ? pair_s[GROUPED ? r : 0] % p.n : n0 + r;
       const uint8_t* from = static_cast<const uint8_t*>(p.x) + (row * p.ldx + b0 * kBlock + part * kColumns) * size;
       const int columns = live ? p.K - b0 * kBlock - part * kColumns : 0;        // what the row has from there on
-      const int mine = p.stages * S::kStage + first * (two ? 2 : 1) * pieces * 512 + lane * 16;      // this lane's pieces, 32 x 16 bytes from one to the next
-      auto copy = [&](int i, int buffer) {
+      const int mine = p.stages * S::kStage + first * pieces * 512 + lane * 16;      // this lane's pieces, 32 x 16 bytes from one to the next
+      auto copy = [&](int i) {
         if (i < iters) {
           for (int j = 0; j < pieces; ++j) {
             const int there = (columns - i * kBlock) * size - 16 * j;
-            copy16_async(smem0 + mine + (buffer * pieces + j) * 512, there > 0 ? from + i * kBlock * size + 16 * j : static_cast<const uint8_t*>(p.x),
+            copy16_async(smem0 + mine + j * 512, there > 0 ? from + i * kBlock * size + 16 * j : static_cast<const uint8_t*>(p.x),
                          min(max(there, 0), 16));
           }
         }
         copies_commit();
       };
-      copy(first, 0);
-      if (two) copy(first + kQuantWarps, 1);
-      int buffer = 0;
-      for (int i = first; i < iters; i += kQuantWarps) {
+      if (first < warps) copy(first);
+      for (int i = first; i < iters && first < warps; i += warps) {
         const float w0 = __ldg(ws0 + i), w1 = EPI == kGated ? __ldg(ws1 + i) : 0.0f;
-        if (two) copies_wait<1>();
-        else copies_wait<0>();
-        const uint8_t* piece = smem0_p + mine + buffer * pieces * 512;
+        copies_wait<0>();
+        const uint8_t* piece = smem0_p + mine;
         uint32_t amax = 0;
         if (p.x_f32) {
 #pragma unroll 8
@@ -391,6 +388,7 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
         const bool finite = amax < 0x7F800000u;
         const int e = finite ? scale_exponent(amax) : 0, st = i % p.stages, slot = i % S::kSlots;
         const float inverse = power_of_two(-e), scale = finite ? power_of_two(e) : __uint_as_float(0x7FC00000u);
+        mbar_wait(smem_u32(&slot_empty[slot]), ((i / S::kSlots) & 1) ^ 1, p.status, 44);
         mbar_wait(smem_u32(&empty_bar[st]), ((i / p.stages) & 1) ^ 1, p.status, 47);
         uint8_t* to = smem0_p + st * S::kStage + kStageA + r * 128;
 #pragma unroll 2
@@ -417,9 +415,7 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
         fence_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(smem_u32(&full_bar[st]));
-        copy(i + (two ? 2 : 1) * kQuantWarps, buffer);
-        if (two) buffer ^= 1;
-        mbar_wait(smem_u32(&slot_empty[slot]), ((i / S::kSlots) & 1) ^ 1, p.status, 44);
+        copy(i + warps);
         if (part == 0) {
           factor[slot][0][r] = scale * w0;
           if (EPI == kGated) factor[slot][1][r] = scale * w1;
@@ -986,9 +982,9 @@ int launch_tile(const void* w, int64_t rows_w, int64_t ldw, const void* q, int64
   if (!byte_map(w, rows_w, p.K, ldw, EPI == kGated ? 64 : kBlock, &map_w) || (!quant && !byte_map(q, rows_q, p.K, ldq, BN, &map_x)))
     return sb::fail("gemm_fp8: no tensor map for a weight of %lld x %d (stride %lld)", (long long)rows_w, p.K, (long long)ldw);
   if (quant) map_x = map_w;                  // (not read)
-  // (quantising: a whole number of stages a warp, see the kernel; sixteen rows leave room for two CTAs an SM, 32 do not)
+  // (quantising: at least half as many stages as accumulators, see the kernel; sixteen rows leave room for two CTAs an SM, 32 do not)
   const int copies = quant ? quant_bytes(BN, p.x_f32) : 0;
-  p.stages = !quant ? std::min(kMaxStages, S::kSmem / S::kStage) : BN == 16 ? kQuantWarps : (kSmemBudget - copies) / S::kStage / kQuantWarps * kQuantWarps;
+  p.stages = !quant ? std::min(kMaxStages, S::kSmem / S::kStage) : BN == 16 ? 4 : std::min(kMaxStages, (kSmemBudget - copies) / S::kStage);
   const size_t smem = static_cast<size_t>(p.stages) * S::kStage + copies + 1024;
   const bool split = !GROUPED && p.ranges > 1 && p.n <= kSplitTokens;
   const dim3 grid(tiles_m, tiles_n, split ? p.ranges : 1);

@@ -111,15 +111,26 @@ __device__ __forceinline__ uint32_t keep_groups(const Routing& r, int lane, cons
   for (int i = 0; i < PER; ++i)
     if (lane + 32 * i < r.E) held[lane + 32 * i] = (open >> i) & 1u ? c[i] : static_cast<T>(-INFINITY);
   __syncwarp();
-  T a = -INFINITY, b = -INFINITY;              // lane g: the two largest of group g
-  if (lane < r.groups) {
-    for (int j = 0, at = lane % size; j < size; ++j) {        // (lanes begin at different places: fewer meet in a bank)
-      const T v = held[lane * size + at];
+  // the two largest of every group: `share` neighbouring lanes (a power of two) look through a group's experts by turns, then join
+  int share = 1;
+  while (2 * share * r.groups <= 32) share *= 2;
+  T a = -INFINITY, b = -INFINITY;
+  const int g = lane / share;
+  if (g < r.groups) {
+    const T* from = held + g * size;
+    for (int j = lane % share; j < size; j += share) {
+      const T v = from[j];
       b = v > a ? a : (v > b ? v : b);
       a = v > a ? v : a;
-      if (++at == size) at = 0;
     }
   }
+  for (int o = 1; o < share; o <<= 1) {
+    const T oa = __shfl_xor_sync(0xffffffffu, a, o), ob = __shfl_xor_sync(0xffffffffu, b, o);
+    b = oa > a ? (a > ob ? a : ob) : (oa > b ? oa : b);
+    a = oa > a ? oa : a;
+  }
+  a = __shfl_sync(0xffffffffu, a, lane * share & 31), b = __shfl_sync(0xffffffffu, b, lane * share & 31);      // lane g: group g's
+  if (lane >= r.groups) a = b = -INFINITY;
   __syncwarp();
   const T mine = r.group_best > 1 && b > static_cast<T>(-INFINITY) ? a + b : a;
   int before = 0;                              // groups that come before this lane's
@@ -175,19 +186,21 @@ __device__ __noinline__ void route_row_64(const Routing& r, int row, int lane, d
   write_row(r, row, lane, kept_e, r.renormalise ? kept_s * r.scale / (sum + 1e-20) : kept_s * r.scale);
 }
 
-// A warp a token. In 32-bit first: a score is off by less than 2^-19 of the largest, a sum with a bias by 2^-22 of its size more; where two
+// A warp a token. In 32-bit first: a score is off by less than 2^-20 of the largest (the exponential by two units in the last place of
+// 2^-23, sum and division by half of one an operation), a sum with a bias by 2^-23 of its size more; where two
 // candidates that follow one another, or the last group that stays and the first that does not, are closer than twice that, the token is routed
 // again in 64-bit. So the choice is that of 64-bit scores always, at the price of 32-bit ones for nearly all tokens (16,384 tokens of 256 experts in
 // eight groups, everything in 64-bit: 87 us).
 constexpr int kWarps = 4;
 template <int PER>
 __global__ void __launch_bounds__(32 * kWarps) route_kernel(const Routing r) {
-  __shared__ double held_s[kWarps][32 * PER];
+  __shared__ double held_s[kWarps][32 * PER];       // (64-bit scores, or 32-bit sums with the bias in front of 32-bit scores)
   sb::grid_launch_dependents();
   sb::grid_dependency_wait();
   const int row = blockIdx.x * kWarps + (threadIdx.x >> 5), lane = threadIdx.x & 31;
   if (row >= r.n) return;
   double* held = held_s[threadIdx.x >> 5];
+  float* held_scores = reinterpret_cast<float*>(held) + 32 * PER;
   float s[PER], c[PER];
   uint32_t open = scores<float, PER>(r, r.logits + row * r.ldz, lane, s, c);
   float high_s = 0.0f, high_c = 0.0f;
@@ -197,46 +210,50 @@ __global__ void __launch_bounds__(32 * kWarps) route_kernel(const Routing r) {
   // (both are not negative: their bits are ordered as they are)
   high_s = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(high_s)));
   high_c = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(high_c)));
-  const float near = 2.0f * (0x1p-19f * high_s + 0x1p-22f * high_c);
+  const float near = 2.0f * (0x1p-20f * high_s + 0x1p-23f * high_c);
   bool sure = high_c < INFINITY;
   if (r.groups > 1) {
     float gap;
     open = keep_groups<float, PER>(r, lane, c, open, reinterpret_cast<float*>(held), gap);
     sure = sure && gap > 2.0f * near;           // (sums of two)
   }
+  uint32_t key[PER];                             // this lane's candidates, largest first: the order of c's bits (0: none) and the place
+  int place[PER];
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    key[i] = (open >> i) & 1u ? order_key(c[i]) : 0u, place[i] = i;
+    held_scores[lane + 32 * i] = s[i];
+  }
+#pragma unroll
+  for (int i = 0; i + 1 < PER; ++i)
+#pragma unroll
+    for (int j = 0; j + 1 < PER - i; ++j) {
+      const bool turned = key[j] < key[j + 1];
+      const uint32_t k = key[j];
+      const int at = place[j];
+      key[j] = turned ? key[j + 1] : k, key[j + 1] = turned ? k : key[j + 1];
+      place[j] = turned ? place[j + 1] : at, place[j + 1] = turned ? at : place[j + 1];
+    }
+  __syncwarp();
   float sum = 0.0f, kept_s = 0.0f, before = INFINITY;
   int kept_e = -1;
-  uint32_t key = 0;                              // this lane's best that is left; 0: nothing
-  int at = 0;
-  auto look = [&]() {
-    key = 0;
-#pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      const uint32_t k = order_key(c[i]);
-      if (((open >> i) & 1u) && k > key) key = k, at = i;
-    }
-  };
-  look();
   for (int k = 0; k <= r.top && sure; ++k) {     // (one more than is chosen: it may not be too close)
-    const uint32_t best = __reduce_max_sync(0xffffffffu, key);
+    const uint32_t best = __reduce_max_sync(0xffffffffu, key[0]);
     if (best == 0) break;
-    const int owner = __ffs(__ballot_sync(0xffffffffu, key == best)) - 1;      // (equal ones are too close anyway)
+    const int owner = __ffs(__ballot_sync(0xffffffffu, key[0] == best)) - 1;      // (equal ones are too close anyway)
     const float value = __uint_as_float((best & 0x80000000u) ? (best & 0x7FFFFFFFu) : ~best);
     sure = before - value > near;
     before = value;
     if (k == r.top) break;
-    float score = 0.0f;
-    if (lane == owner) {
-#pragma unroll
-      for (int i = 0; i < PER; ++i)
-        if (i == at) score = s[i];
-      open &= ~(1u << at);
-    }
-    score = __shfl_sync(0xffffffffu, score, owner);
-    const int e = __shfl_sync(0xffffffffu, lane + 32 * at, owner);
+    const int e = owner + 32 * __shfl_sync(0xffffffffu, place[0], owner);
+    const float score = held_scores[e];
     sum += score;
     if (lane == k) kept_s = score, kept_e = e;      // (at most 32 choices)
-    if (lane == owner) look();
+    if (lane == owner) {
+#pragma unroll
+      for (int i = 0; i + 1 < PER; ++i) key[i] = key[i + 1], place[i] = place[i + 1];
+      key[PER - 1] = 0;
+    }
   }
   if (r.renormalise && kept_e >= 0 && sum < 0x1p-50f) sure = false;      // (scores below the smallest floats count where all are)
   sure = __all_sync(0xffffffffu, sure);
