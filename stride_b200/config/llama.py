@@ -74,6 +74,12 @@ class LlamaConfig:
         for key in ("attention_bias", "mlp_bias"):
             if j.get(key):
                 raise ConfigError(f"config.json: '{key}' = true is not supported (the decoder has no bias terms)")
+        quantised = j.get("quantization_config")
+        if quantised is not None:
+            known = {"quant_method": "fp8", "weight_block_size": [128, 128], "activation_scheme": "dynamic", "fmt": "e4m3"}
+            for key, only in known.items():
+                if not isinstance(quantised, dict) or quantised.get(key, only if key == "fmt" else None) != only:
+                    raise ConfigError(f"config.json: quantization_config needs '{key}' = {only!r} (weights in 8 bits with a scale per block of 128 x 128)")
         act = j.get("hidden_act", "silu")
         if act != "silu":
             raise ConfigError(f"config.json: hidden_act '{act}' is not supported (only 'silu')")

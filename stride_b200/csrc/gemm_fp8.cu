@@ -1270,3 +1270,26 @@ SB_EXPORT int sb_experts_fp8(const SbFp8Experts* l, const void* x, int xdtype, i
   else vec ? combine(expert_combine_kernel<bf16, true>, static_cast<bf16*>(out)) : combine(expert_combine_kernel<bf16, false>, static_cast<bf16*>(out));
   return sb::check_launch(who);
 }
+
+// i: 0 q, 1 ldq, 2 x scales, 3 ldxs, 4 w, 5 ldw, 6 w scales, 7 M, 8 K, 9 half_rows, 10 x, 11 x dtype, 12 ldx, 13 out, 14 out dtype, 15 ldo,
+// 16 epilogue, 17 act, 18 wanted rows (else the step's tokens). f: 0 limit, 1 slope
+SB_EXPORT int sb_op_linear_fp8(const SbOp* op, const SbStep* s, void* stream) {
+  using namespace sbstep;
+  const int n = op->i[18] != 0 ? s->wanted : s->n;
+  if (n <= 0) return SB_OP_SKIPPED;
+  const SbFp8Layer l = {ptr<void>(op->i[0]), op->i[1], ptr<float>(op->i[2]), op->i[3], ptr<void>(op->i[4]), op->i[5], ptr<float>(op->i[6]),
+                        (int)op->i[7], (int)op->i[8], (int)op->i[9]};
+  return sb_linear_fp8(&l, ptr<void>(op->i[10]), (int)op->i[11], op->i[12], ptr<void>(op->i[13]), (int)op->i[14], op->i[15], n, (int)op->i[16],
+                       (int)op->i[17], (float)op->f[0], (float)op->f[1], stream) != 0 ? SB_OP_FAILED : SB_OP_LAUNCHED;
+}
+
+// i: 0 gate_up, 1 ldg, 2 gate_up scales, 3 down, 4 ldd, 5 down scales, 6 experts, 7 width, 8 inner, 9 x, 10 x dtype, 11 ldx, 12 choice [n][top],
+// 13 weights [top][n], 14 out, 15 out dtype, 16 ldo, 17 top, 18 scratch, 19 its bytes
+SB_EXPORT int sb_op_experts_fp8(const SbOp* op, const SbStep* s, void* stream) {
+  using namespace sbstep;
+  if (s->n <= 0) return SB_OP_SKIPPED;
+  const SbFp8Experts l = {ptr<void>(op->i[0]), op->i[1], ptr<float>(op->i[2]), ptr<void>(op->i[3]), op->i[4], ptr<float>(op->i[5]), (int)op->i[6],
+                          (int)op->i[7], (int)op->i[8]};
+  return sb_experts_fp8(&l, ptr<void>(op->i[9]), (int)op->i[10], op->i[11], ptr<int32_t>(op->i[12]), ptr<float>(op->i[13]), ptr<void>(op->i[14]),
+                        (int)op->i[15], op->i[16], s->n, (int)op->i[17], ptr<void>(op->i[18]), op->i[19], stream) != 0 ? SB_OP_FAILED : SB_OP_LAUNCHED;
+}

@@ -25,10 +25,12 @@ import torch
 
 from ..cache.manager import CacheManager
 from ..config import resolve_architecture
+from ..kernels import ops
 from ..kernels.build import build_all
+from ..kernels.linear import Fp8Weight
 from ..kernels.native import NotNative, StepProgram
 from ..parts import BuildEnv, DecoderModel, StepContext, Workspace
-from ..weights.loader import check_plan, load_weights, tensor_shapes
+from ..weights.loader import check_plan, join_scales, load_weights, tensor_shapes, with_scales
 
 
 class EngineError(RuntimeError):
@@ -119,15 +121,16 @@ class Engine:
         build_all(sorted(libraries))      # what this model needs, compiled side by side if missing
         # the word into which the tensor-core kernels' bounded waits report; the sampling kernels pass it on to the host
         self._status_device = None
-        if self.device.type == "cuda" and libraries & {"gemm_tc", "attention_tc5", "decode_chain", "grouped_gemm"}:
-            from ..kernels import ops
+        if self.device.type == "cuda" and libraries & {"gemm_tc", "attention_tc5", "decode_chain", "grouped_gemm", "gemm_fp8"}:
             self._status_device = ops.shared_status_word(libraries | {"sampling"})
         plan = self.model.tensor_plan()
         if tensors is None:
             tensors = load_weights(model_dir, plan, self.device)
         else:
-            check_plan(plan, {n: tuple(t.shape) for n, t in tensors.items()}, "the given tensors")
-            tensors = {n: t.to(self.device) for n, t in tensors.items()}
+            check_plan(with_scales(plan, {n: t.dtype for n, t in tensors.items()}), {n: tuple(t.shape) for n, t in tensors.items()}, "the given tensors")
+            tensors = join_scales({n: t.to(self.device) for n, t in tensors.items()})
+        if self._status_device is not None and any(isinstance(t, Fp8Weight) for t in tensors.values()):
+            ops.shared_status_word({"gemm_fp8"})
         self.model.bind(tensors)
         self.cache = CacheManager(self.model.cache_needs(), device=self.device, max_slots=o.max_slots,
                                   max_context=self.max_context, page_size=o.page_size,
@@ -171,7 +174,6 @@ class Engine:
         # model to the Python driver (`DecoderModel.forward`), which launches the same kernels part by part.
         self._program, self._program_logits = None, None
         if o.native_step:
-            from ..kernels import ops
             program = StepProgram(self.workspace, o.max_rows, self._work_ints, ops.gemm_tc_partial_tokens() if self.compute_dtype == torch.bfloat16 else 0)
             try:
                 self._program_logits = self.model.emit(program, self.caches, self.sampled)
@@ -336,7 +338,6 @@ class Engine:
                 self._graph_generation = self.workspace.generation
             torch.cuda.synchronize()
             g = torch.cuda.CUDAGraph()
-            from ..kernels import ops
             before = ops.launches
             with torch.cuda.graph(g):
                 static_logits = run()
@@ -346,7 +347,6 @@ class Engine:
             graph[0].replay()
             logits = graph[1]
             self.graph_replays += 1
-            from ..kernels import ops
             ops.launches += graph[2]
         self.logit_slots = d[8 * R:8 * R + E]
         self.steps += 1

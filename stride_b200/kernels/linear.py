@@ -2,6 +2,9 @@
 
 float32 engine: true 32-bit FMA (`csrc/gemm_f32.cu`) on float32 activations; the weight stays
 as stored (bfloat16 is widened exactly inside the kernel).
+A weight in 8 bits with a scale per block of 128 x 128 (`Fp8Weight`): in the bfloat16 engine the input is quantised per token and block of
+128 columns, and the products run on the tensor cores in 8 bits (`csrc/gemm_fp8.cu`); the float32 engine takes what the weight stands for
+into true 32-bit products.
 bfloat16 engine: bfloat16 activations and weights with float32 accumulation on the tcgen05
 tensor cores (`csrc/gemm_tc.cu`); a weight stored in float32, or a K that TMA cannot
 address (not a multiple of 8), falls back to the SIMT kernel, which takes any size.
@@ -19,6 +22,24 @@ import ctypes
 import torch
 
 from . import ops
+
+
+FP8_SCALES = "_scale_inv"        # what the name of an 8-bit weight's scales in a checkpoint ends with
+
+
+def fp8_scales_shape(rows: int, columns: int) -> tuple:
+    return -(-rows // ops.FP8_BLOCK), -(-columns // ops.FP8_BLOCK)
+
+
+def stack_rows(weights, compute_dtype: torch.dtype):
+    """The matrices one below the other: tensors, or 8-bit weights (for the float32 engine what they stand for); of several kinds, all as float32."""
+    weights = list(weights)
+    if compute_dtype == torch.bfloat16 and all(isinstance(w, Fp8Weight) for w in weights):
+        return Fp8Weight.stack(weights)
+    weights = [w.to(torch.float32) if isinstance(w, Fp8Weight) else w for w in weights]
+    if len({w.dtype for w in weights}) > 1:
+        weights = [w.to(torch.float32) for w in weights]
+    return torch.cat(weights, dim=0)
 
 
 class Fp8Weight:
@@ -233,9 +254,17 @@ class Linear:
         program.add("gemm_tc", "sb_op_linear_tc", [x, x.stride(0), self.weight, self.weight.stride(0), out, self.out_features,
                                                     self.in_features, mode, splits, int(wanted_rows)], constants, chain=phase)
 
+    def _fp8_op(self, program, x, out, ldo: int, epilogue: int, wanted_rows: bool = False, act: int = 0, constants=()) -> None:
+        q, scales = self._buffers(program.workspace)
+        w = self.fp8
+        program.add("gemm_fp8", "sb_op_linear_fp8", [q, q.stride(0), scales, scales.stride(0), w.q, w.stride, w.scales, *w.shape, w.shape[0] // 2,
+                                                     x, x.dtype, x.stride(0), out, out.dtype, ldo, epilogue, act, int(wanted_rows)], constants)
+
     def emit(self, program, x: torch.Tensor, out: torch.Tensor, wanted_rows: bool = False) -> None:
         """`forward`; with `wanted_rows` the rows are the step's wanted rows (the head), not its tokens."""
-        if self._tc(x):
+        if self.fp8 is not None:
+            self._fp8_op(program, x, out, out.stride(0), 0, wanted_rows)
+        elif self._tc(x):
             self._tc_op(program, x, out, 0, wanted_rows=wanted_rows)
         else:
             self._f32_op(program, x, out, out.stride(0), False, wanted_rows)
@@ -243,6 +272,9 @@ class Linear:
     def emit_partials(self, program, x: torch.Tensor, flat: torch.Tensor) -> int:
         """`forward_partials`; returns the number of K ranges S that the reader of `flat` has to expect
         ([S, n, out_features] up to `program.few_tokens` tokens, [1, n, out_features] beyond)."""
+        if self.fp8 is not None:
+            self._fp8_op(program, x, flat, self.out_features, 0)
+            return 1
         if not self._tc(x):
             self._f32_op(program, x, flat, self.out_features, False, False)
             return 1
@@ -260,7 +292,9 @@ class Linear:
         fresh = program.take_fresh()        # a branch that holds nothing yet: the result is stored, not added
         if fresh is not None:
             return self.emit(program, x, fresh)
-        if self._tc(x):
+        if self.fp8 is not None:
+            self._fp8_op(program, x, program.h, program.h.stride(0), 1)
+        elif self._tc(x):
             self._tc_op(program, x, program.h, 2)
         else:
             self._f32_op(program, x, program.h, program.h.stride(0), True, False)
@@ -268,7 +302,9 @@ class Linear:
     def emit_swiglu(self, program, x: torch.Tensor, z: torch.Tensor, scratch_fn, activation: str = "silu", constants=()) -> None:
         """`forward_swiglu`."""
         act = ops.GATE_ACTIVATIONS[activation]
-        if self._tc(x) and z.dtype == torch.bfloat16:
+        if self.fp8 is not None:
+            self._fp8_op(program, x, z, z.stride(0), 2, act=act, constants=constants)
+        elif self._tc(x) and z.dtype == torch.bfloat16:
             self._tc_op(program, x, z, 3 + act, constants=constants)
         else:
             gate_up = scratch_fn()

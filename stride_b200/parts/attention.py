@@ -17,7 +17,7 @@ import numpy as np
 import torch
 
 from ..kernels import ops
-from ..kernels.linear import Linear
+from ..kernels.linear import Linear, stack_rows
 from ..kernels.native import NO_PHASE
 from .base import CacheNeed, Mixer, part_class, register_part
 from .spec import TensorPlan
@@ -87,11 +87,11 @@ class AttentionMixer(Mixer):
 
     def tensor_plan(self):
         t, D = self.spec.tensors, self.head_dim
-        plan = {t["q"]: TensorPlan((self.num_heads * D, self.hidden)),
-                t["k"]: TensorPlan((self.num_kv_heads * D, self.hidden)),
-                t["o"]: TensorPlan((self.hidden, self.num_heads * D))}
+        plan = {t["q"]: TensorPlan((self.num_heads * D, self.hidden), fp8=True),
+                t["k"]: TensorPlan((self.num_kv_heads * D, self.hidden), fp8=True),
+                t["o"]: TensorPlan((self.hidden, self.num_heads * D), fp8=True)}
         if not self.values_from_keys:
-            plan[t["v"]] = TensorPlan((self.num_kv_heads * D, self.hidden))
+            plan[t["v"]] = TensorPlan((self.num_kv_heads * D, self.hidden), fp8=True)
         if self.position is not None:
             plan.update(self.position.tensor_plan())      # a position part may have tensors of its own (a learned table)
         return plan
@@ -99,9 +99,7 @@ class AttentionMixer(Mixer):
     def bind(self, tensors):
         t = self.spec.tensors
         ws = [tensors[t[r]] for r in (("q", "k") if self.values_from_keys else ("q", "k", "v"))]
-        if len({w.dtype for w in ws}) > 1:
-            ws = [w.to(torch.float32) for w in ws]
-        self.qkv = Linear(torch.cat(ws, dim=0), self.env.compute_dtype)
+        self.qkv = Linear(stack_rows(ws, self.env.compute_dtype), self.env.compute_dtype)
         self.o = Linear(tensors[t["o"]], self.env.compute_dtype)
         if self.position is None:
             # No rotation: a table of cos = 1, sin = 0 is never read because rotary_dim is 0.
@@ -133,7 +131,7 @@ class AttentionMixer(Mixer):
 
     def forward(self, ctx, x, stream, cache):
         n, ws, D = ctx.n, ctx.workspace, self.head_dim
-        qkv = self.qkv.forward_partials(x, ws.raw("attn.qkv", (self.qkv.partial_elems(ws.max_tokens),), torch.float32))
+        qkv = self.qkv.forward_partials(x, ws.raw("attn.qkv", (self.qkv.partial_elems(ws.max_tokens),), torch.float32), ws)
         mixed = ws.get("attn.out", n, (self.num_heads * D,), ctx.act_dtype)
         G = self.num_heads // self.num_kv_heads
         tensor_core = tensor_core_head(ctx.act_dtype, self.num_heads, self.num_kv_heads, D)
@@ -150,7 +148,7 @@ class AttentionMixer(Mixer):
             counters = ws.raw("attn.counters", (ws.max_tokens * self.num_kv_heads,), torch.int32)
             ops.attention_decode_rope(qkv, self._cos_sin, mixed, cache.pages, cache.block_table, ctx.entry_meta, work, n_items,
                                       chunks, scratch, counters, self.num_heads, self.num_kv_heads, D, self.window, self.scale)
-            self.o.forward_add(mixed, stream, ws.raw("attn.o_partials", (self.o.partial_elems(ws.max_tokens),), torch.float32))
+            self.o.forward_add(mixed, stream, ws.raw("attn.o_partials", (self.o.partial_elems(ws.max_tokens),), torch.float32), ws)
             return
         q = ws.get("attn.q", n, (self.num_heads * D,), ctx.act_dtype)
         ops.rope_append(qkv, ctx.positions, ctx.slots, self._cos_sin, self._rotary, q, cache.pages, cache.block_table,
@@ -171,7 +169,7 @@ class AttentionMixer(Mixer):
         else:
             ops.attention_generic(q, mixed, cache.pages, cache.block_table, ctx.positions, ctx.slots,
                                   self.num_heads, self.num_kv_heads, D, self.window, self.scale)
-        self.o.forward_add(mixed, stream, ws.raw("attn.o_partials", (self.o.partial_elems(ws.max_tokens),), torch.float32))
+        self.o.forward_add(mixed, stream, ws.raw("attn.o_partials", (self.o.partial_elems(ws.max_tokens),), torch.float32), ws)
 
     def emit(self, program, x, cache):
         """`forward` as operations of the native step program: the projection, then rotation and append, the

@@ -15,6 +15,9 @@ Two parameters make other routed designs of it. `weights_from` "logits": the sto
 `top` largest z are chosen and weigh by the softmax over the chosen z alone. `expert` "silu_gated": an expert is
 W_down (silu(W_gate x) * (W_up x)); its gate and up matrices lie one above the other in the side-by-side product.
 
+"scored_experts": gated experts with weights in 8 bits behind a router with a bias for balance and groups of experts; the chosen ones' results are
+added by their weights (csrc/router.cu, csrc/gemm_fp8.cu).
+
 "table_experts": gated experts without a router, chosen by a stored table of token ids; the products run grouped, every expert on the rows
 that chose it (csrc/grouped_gemm.cu). "sigmoid_experts": the same grouped products behind a router, whose chosen scores are sigmoids taken as
 they are and multiply the experts' inputs."""
@@ -23,7 +26,7 @@ from __future__ import annotations
 import torch
 
 from ..kernels import ops
-from ..kernels.linear import Linear
+from ..kernels.linear import Fp8Experts, Fp8Weight, Linear
 from ..kernels.native import ImmediateProgram
 from .base import FeedForward, register_part
 from .branch import ALWAYS, emit_fold, emit_on_branch
@@ -302,6 +305,98 @@ class SigmoidExpertsFeedForward(GroupedExpertsFeedForward):
         sources = self._emit_grouped(program, x, choice, 0, weights, 1.0)
         if gate is not None:
             sources[1] = (*sources[1][:2], gate)
+        return sources
+
+
+@register_part("feed_forward", "scored_experts")
+class ScoredExpertsFeedForward(FeedForward):
+    """Gated experts with weights in 8 bits behind a router in 32-bit: z = W_r x, s = sigmoid(z) or softmax(z); the `top` experts with the largest
+    s + bias, of the `top_groups` groups with the largest sums of their `group_best` largest s + bias, are chosen; the result is the sum of
+    w_e expert_e(x), w_e = s_e, divided by the chosen ones' sum if `renormalise`, times `scale`; and perhaps a shared expert's.
+    params: hidden_size, intermediate_size (of one expert), experts, top, score ("sigmoid" by default, or "softmax"), groups, top_groups,
+    group_best (1, 1 and 2 by default), renormalise (True by default), scale (1.0), shared (the shared expert's intermediate size; 0: none).
+    tensors: router [experts, hidden], bias [experts] (may be absent), gate, up, down (lists of names, one per expert: matrices stored in 8 bits),
+    shared_gate, shared_up, shared_down. Runs in the bfloat16 engine."""
+    graph_safe = True
+
+    def __init__(self, spec, env):
+        super().__init__(spec, env)
+        p, t = spec.params, spec.tensors
+        self.hidden, self.intermediate = int(p["hidden_size"]), int(p["intermediate_size"])
+        self.experts, self.top, self.shared_size = int(p["experts"]), int(p["top"]), int(p.get("shared", 0) or 0)
+        self.score, self.renormalise, self.scale = str(p.get("score", "sigmoid")), bool(p.get("renormalise", True)), float(p.get("scale", 1.0))
+        self.groups, self.top_groups, self.group_best = (int(p.get(k, d)) for k, d in (("groups", 1), ("top_groups", 1), ("group_best", 2)))
+        if self.score not in ops.ROUTER_SCORES:
+            raise ValueError(f"scored experts: unknown score '{self.score}' (known: {', '.join(ops.ROUTER_SCORES)})")
+        if not 0 < self.top <= min(self.experts, 32) or self.experts > 1024 or self.groups < 1 or self.experts % self.groups or self.groups > 32 \
+                or not 0 < self.top_groups <= self.groups or self.group_best not in (1, 2) or self.top > self.top_groups * (self.experts // self.groups):
+            raise ValueError(f"scored experts: {self.top} (at most 32) of {self.experts} experts (at most 1024), {self.top_groups} of {self.groups} groups "
+                             f"(at most 32, of one size) judged by their best {self.group_best} (1 or 2)")
+        if env.compute_dtype != torch.bfloat16:
+            raise ValueError("scored experts run in the bfloat16 engine only: their products are 8-bit ones")
+        self.shared = SwiGLU(PartSpec("gated", {"hidden_size": self.hidden, "intermediate_size": self.shared_size},
+                                      {"gate": t["shared_gate"], "up": t["shared_up"], "down": t["shared_down"]}), env) if self.shared_size else None
+        self.router = self.bias = self.layer = None
+
+    def tensor_plan(self):
+        t = self.spec.tensors
+        plan = {t["router"]: TensorPlan((self.experts, self.hidden))}
+        if "bias" in t:
+            plan[t["bias"]] = TensorPlan((self.experts,), zero_mean=True)
+        for name in (*t["gate"], *t["up"]):
+            plan[name] = TensorPlan((self.intermediate, self.hidden), fp8=True)
+        for name in t["down"]:
+            plan[name] = TensorPlan((self.hidden, self.intermediate), fp8=True)
+        if self.shared is not None:
+            plan.update(self.shared.tensor_plan())
+        return plan
+
+    def bind(self, tensors):
+        t = self.spec.tensors
+        for name in (*t["gate"], *t["up"], *t["down"]):
+            if not isinstance(tensors[name], Fp8Weight):
+                raise TypeError(f"scored experts take matrices stored in 8 bits; '{name}' is {tensors[name].dtype}")
+        self.router = tensors[t["router"]].contiguous()
+        self.bias = tensors[t["bias"]].to(torch.float32).contiguous() if "bias" in t else None
+        self.layer = Fp8Experts([tensors[name] for pair in zip(t["gate"], t["up"]) for name in pair], [tensors[name] for name in t["down"]])
+        if self.shared is not None:
+            self.shared.bind(tensors)
+
+    def weight_bytes(self):
+        """Of a step of one token: its `top` experts, the shared one and the router."""
+        own = self.top * self.layer.weight_bytes() + self.router.numel() * self.router.element_size()
+        return own + (self.shared.weight_bytes() if self.shared is not None else 0)
+
+    def kernel_libraries(self):
+        return {"gemm_f32", "router", "gemm_fp8", "branch"} | (self.shared.kernel_libraries() if self.shared is not None else set())
+
+    def forward(self, ctx, x, stream):
+        with ImmediateProgram(ctx, stream) as program:
+            self.emit(program, x)
+
+    def emit(self, program, x):
+        program.need_folded("scored experts")
+        emit_fold(program, self.emit_sources(program, x), None, self.hidden, fresh=True)
+
+    def emit_sources(self, program, x):
+        """The result as branches with constants, left to the caller to add."""
+        ws, E, top, W, f32 = program.workspace, self.experts, self.top, self.hidden, torch.float32
+        T, layer = ws.max_tokens, self.layer
+        logits = ws.get("experts.logits", T, (E,), f32)
+        program.add("gemm_f32", "sb_op_linear_f32", [x, x.dtype, x.stride(0), self.router, self.router.dtype, self.router.stride(0), logits, E, E, W, 0, 0])
+        choice = ws.raw("experts.choice", (T * top,), torch.int32)
+        weights = ws.raw("experts.weights", (T * top,), f32)
+        program.add("router", "sb_op_route_experts", [logits, E, self.bias, choice, weights, E, top, ops.ROUTER_SCORES[self.score], self.groups,
+                                                      self.top_groups, self.group_best, int(self.renormalise)], [self.scale])
+        out = ws.raw("experts.out", (T * W,), f32)
+        scratch = ws.raw("experts.scratch", (ops.experts_fp8_scratch(T, top, E, W, self.intermediate),), torch.uint8)
+        program.add("gemm_fp8", "sb_op_experts_fp8", [layer.gate_up, layer.gate_up.stride(0), layer.gate_up_scales, layer.down, layer.down.stride(0),
+                                                      layer.down_scales, E, W, self.intermediate, x, x.dtype, x.stride(0), choice, weights, out, out.dtype, W,
+                                                      top, scratch, scratch.numel()])
+        sources = [(None, (out, 1, W, ALWAYS), 1.0)]
+        if self.shared is not None:
+            branch = ws.get("experts.shared", T, (W,), f32)
+            sources.append((*emit_on_branch(program, branch, lambda: self.shared.emit(program, x), fresh=True), 1.0))
         return sources
 
 

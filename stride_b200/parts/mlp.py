@@ -8,7 +8,7 @@ from __future__ import annotations
 import torch
 
 from ..kernels import ops
-from ..kernels.linear import Linear
+from ..kernels.linear import Linear, stack_rows
 from .base import FeedForward, register_part
 from .spec import TensorPlan
 
@@ -33,16 +33,13 @@ class SwiGLU(FeedForward):
 
     def tensor_plan(self):
         t = self.spec.tensors
-        return {t["gate"]: TensorPlan((self.intermediate, self.hidden)),
-                t["up"]: TensorPlan((self.intermediate, self.hidden)),
-                t["down"]: TensorPlan((self.hidden, self.intermediate))}
+        return {t["gate"]: TensorPlan((self.intermediate, self.hidden), fp8=True),
+                t["up"]: TensorPlan((self.intermediate, self.hidden), fp8=True),
+                t["down"]: TensorPlan((self.hidden, self.intermediate), fp8=True)}
 
     def bind(self, tensors):
         t = self.spec.tensors
-        gate, up = tensors[t["gate"]], tensors[t["up"]]
-        if gate.dtype != up.dtype:
-            gate, up = gate.to(torch.float32), up.to(torch.float32)
-        self.gate_up = Linear(torch.cat([gate, up], dim=0), self.env.compute_dtype)
+        self.gate_up = Linear(stack_rows([tensors[t["gate"]], tensors[t["up"]]], self.env.compute_dtype), self.env.compute_dtype)
         self.down = Linear(tensors[t["down"]], self.env.compute_dtype)
 
     def weight_bytes(self):
@@ -55,8 +52,8 @@ class SwiGLU(FeedForward):
         n, ws = ctx.n, ctx.workspace
         z = ws.get("mlp.z", n, (self.intermediate,), ctx.act_dtype)
         self.gate_up.forward_swiglu(x, z, lambda: ws.get("mlp.gate_up", n, (2 * self.intermediate,), torch.float32),
-                                    self.activation, self.constants)
-        self.down.forward_add(z, stream, ws.raw("mlp.down_partials", (self.down.partial_elems(ws.max_tokens),), torch.float32))
+                                    self.activation, self.constants, ws)
+        self.down.forward_add(z, stream, ws.raw("mlp.down_partials", (self.down.partial_elems(ws.max_tokens),), torch.float32), ws)
 
     def emit(self, program, x):
         ws = program.workspace

@@ -102,3 +102,4 @@ class TensorPlan:
     below: int = 0               # integers: random ones lie in 0 .. below - 1, those of a row differ
     zero_mean: bool = False      # a vector that is added, not multiplied (a bias): random weights are N(0, .), not 1 + N(0, .)
     near_identity: bool = False  # a square matrix whose random weights are the identity + N(0, .)
+    fp8: bool = False            # a matrix that may be stored in 8 bits (`weights.loader`): its layer then runs on 8-bit products

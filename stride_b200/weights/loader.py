@@ -5,6 +5,8 @@ The model's parts say which tensors they expect and with what shape
 raises ONE error that lists every missing tensor, every unexpected tensor and every
 wrong shape. Floating tensors stored in 16 bits are kept (or made) bfloat16; a tensor
 stored in 32 bits stays float32; integer tables become int32.
+A matrix whose plan allows it may be stored in 8 bits (F8_E4M3) beside a float32 tensor `<name>_scale_inv` with one factor per block of 128
+rows and 128 columns, [ceil(rows / 128), ceil(columns / 128)]: it comes as a `kernels.linear.Fp8Weight`.
 Counterpart in arhaamatiq/stride: the Weights constructor (src/model.cpp:149-238), which
 reads the same names and fails on the first missing one.
 """
@@ -14,6 +16,7 @@ from pathlib import Path
 
 import torch
 
+from ..kernels.linear import FP8_SCALES, Fp8Weight, fp8_scales_shape
 from .safetensors_io import SafetensorsFile
 
 
@@ -40,6 +43,27 @@ def check_plan(plan: dict, available: dict, source: str) -> None:
         lines.append(f"  wrong shapes ({len(wrong)}): " + "; ".join(
             f"{n} is {list(have)}, expected {list(want)}" for n, have, want in sorted(wrong)))
     raise WeightsError("\n".join(lines), missing, unexpected, wrong)
+
+
+def with_scales(plan: dict, dtypes: dict) -> dict:
+    """`plan` with a scale tensor beside every matrix that is stored in 8 bits. `dtypes`: name -> dtype of the stored tensors."""
+    out = {}
+    for name, want in plan.items():
+        out[name] = want
+        if dtypes.get(name) == torch.float8_e4m3fn:
+            if not want.fp8:
+                raise WeightsError(f"{name} is stored in 8 bits, which its layer does not take", wrong_shape=())
+            out[name + FP8_SCALES] = type(want)(fp8_scales_shape(*want.shape))
+    return out
+
+
+def join_scales(tensors: dict) -> dict:
+    """`tensors` (name -> tensor, checked) with every 8-bit matrix and its scales as one `Fp8Weight`."""
+    out = {n: t for n, t in tensors.items() if not (n.endswith(FP8_SCALES) and n[:-len(FP8_SCALES)] in tensors)}
+    for name, t in out.items():
+        if t.dtype == torch.float8_e4m3fn:
+            out[name] = Fp8Weight(t, tensors[name + FP8_SCALES].to(torch.float32))
+    return out
 
 
 def storage_dtype(dtype: torch.dtype, integer: bool) -> torch.dtype:
@@ -94,14 +118,19 @@ def load_weights(model_dir, plan: dict, device) -> dict:
     """Read the model folder's safetensors (one file or shards), check them against `plan`, return name -> device tensor."""
     where = _open_files(model_dir)
     try:
-        check_plan(plan, {n: f.shape(n) for n, f in where.items()}, str(Path(model_dir)))
+        dtypes = {n: f.dtype(n) for n, f in where.items()}
+        check_plan(with_scales(plan, dtypes), {n: f.shape(n) for n, f in where.items()}, str(Path(model_dir)))
         out = {}
         for name, want in plan.items():
             if name not in where:
                 continue
             t = where[name].get(name)
+            if dtypes[name] == torch.float8_e4m3fn:
+                out[name] = t.to(device=device, copy=True)
+                out[name + FP8_SCALES] = where[name + FP8_SCALES].get(name + FP8_SCALES).to(device=device, copy=True)
+                continue
             out[name] = t.to(device=device, dtype=storage_dtype(t.dtype, want.integer), copy=True)
-        return out
+        return join_scales(out)
     finally:
         for f in {id(f): f for f in where.values()}.values():
             f.close()

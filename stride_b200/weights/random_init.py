@@ -17,6 +17,7 @@ from pathlib import Path
 import torch
 
 from ..config import resolve_architecture
+from ..kernels.linear import FP8_SCALES, Fp8Weight
 from ..parts import BuildEnv, DecoderModel
 from .safetensors_io import write_safetensors
 
@@ -36,11 +37,13 @@ def model_plan(config: dict) -> dict:
 def random_tensors(config: dict, seed: int, device="cpu", dtype=torch.bfloat16, std: float = 0.02,
                    gain_std: float = 0.1, include_optional: bool | None = None) -> dict:
     """name -> tensor for every tensor of the plan. Optional tensors (an untied head) are made when
-    `include_optional`, which defaults to config['tie_word_embeddings'] being false."""
+    `include_optional`, which defaults to config['tie_word_embeddings'] being false. With a
+    `quantization_config`, matrices that may be stored in 8 bits are, rounded from those values, each beside its scales."""
     plan = model_plan(config)
     if include_optional is None:
         include_optional = config.get("tie_word_embeddings") is False
     device = torch.device(device)
+    quantised = config.get("quantization_config") is not None
     out = {}
     for name, want in plan.items():
         if want.optional and not include_optional:
@@ -61,6 +64,9 @@ def random_tensors(config: dict, seed: int, device="cpu", dtype=torch.bfloat16, 
             out[name] = (torch.eye(want.shape[0], device=device) + noise).to(dtype)
         else:
             out[name] = (std * torch.randn(want.shape, generator=gen, device=device, dtype=torch.float32)).to(dtype)
+            if quantised and want.fp8:
+                weight = Fp8Weight.quantize(out[name])
+                out[name], out[name + FP8_SCALES] = weight.q[:, :weight.shape[1]].contiguous(), weight.scales
     return out
 
 

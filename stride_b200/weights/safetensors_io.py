@@ -26,7 +26,7 @@ class SafetensorsError(RuntimeError):
 _DTYPES = {
     "BF16": (torch.bfloat16, 2), "F16": (torch.float16, 2), "F32": (torch.float32, 4), "F64": (torch.float64, 8),
     "I8": (torch.int8, 1), "U8": (torch.uint8, 1), "I16": (torch.int16, 2), "I32": (torch.int32, 4),
-    "I64": (torch.int64, 8), "BOOL": (torch.bool, 1),
+    "I64": (torch.int64, 8), "BOOL": (torch.bool, 1), "F8_E4M3": (torch.float8_e4m3fn, 1),
 }
 _NAMES = {v[0]: k for k, v in _DTYPES.items()}
 
@@ -88,7 +88,7 @@ class SafetensorsFile:
         buf = memoryview(self._map)[self._data_start + begin:self._data_start + end]
         with warnings.catch_warnings():
             warnings.simplefilter("ignore", UserWarning)     # the map is read-only; callers copy, never write
-            flat = torch.frombuffer(buf, dtype=tdt)
+            flat = torch.frombuffer(buf, dtype=torch.uint8 if tdt == torch.float8_e4m3fn else tdt).view(tdt)
         return flat.reshape(shape)
 
     def close(self):

@@ -1,0 +1,175 @@
+"""8-bit weights on the CPU: what they stand for, how matrices are stacked, checkpoints that hold them, and what is refused."""
+from __future__ import annotations
+
+import json
+
+import pytest
+import torch
+
+import plain_fp8 as plain
+
+CONFIG = {
+    "architectures": ["LlamaForCausalLM"], "hidden_size": 256, "intermediate_size": 200, "num_hidden_layers": 2, "num_attention_heads": 4,
+    "num_key_value_heads": 2, "head_dim": 64, "vocab_size": 300, "rope_theta": 10000.0, "tie_word_embeddings": True, "rms_norm_eps": 1e-5,
+    "max_position_embeddings": 512, "quantization_config": {"quant_method": "fp8", "weight_block_size": [128, 128], "activation_scheme": "dynamic"},
+}
+
+
+def _weight(M, K, seed=0):
+    from stride_b200.kernels.linear import Fp8Weight
+    return Fp8Weight.quantize(torch.randn(M, K, generator=torch.Generator().manual_seed(seed)))
+
+
+@pytest.mark.parametrize("M,K", [(1, 1), (128, 128), (130, 257), (300, 15), (64, 640)])
+def test_what_a_weight_stands_for(M, K):
+    w = torch.randn(M, K, generator=torch.Generator().manual_seed(M))
+    from stride_b200.kernels.linear import Fp8Weight
+    got = Fp8Weight.quantize(w)
+    values = plain.weight_values(got.q[:, :K].float(), got.scales)
+    assert (values - w.double()).abs().max() <= 2.0 ** -4 * w.abs().max()           # half a step of the largest element
+    assert (got.to(torch.float32).double() - values).abs().max() <= 2.0 ** -24 * values.abs().max()
+    assert got.stride % 16 == 0 and got.stride >= K and got.q.data_ptr() % 16 == 0
+    if got.stride > K:
+        assert (got.q.view(torch.uint8)[:, K:] == 0).all()
+
+
+def test_a_block_of_zeros_and_columns_of_a_wider_matrix():
+    from stride_b200.kernels.linear import Fp8Weight
+    w = torch.zeros(200, 300)
+    w[130:, :100] = 3.0
+    got = Fp8Weight.quantize(w)
+    assert torch.equal(got.to(torch.float32), w)
+    inner = Fp8Weight(got.q[:, :300], got.scales)
+    assert torch.equal(inner.to(torch.float32), w)
+    narrow = Fp8Weight(got.q[:64, :128], got.scales[:1, :1])
+    assert torch.equal(narrow.to(torch.float32), w[:64, :128])
+
+
+def test_stacked_weights():
+    from stride_b200.kernels.linear import Fp8Weight
+    a, b, c = _weight(256, 100, 1), _weight(128, 100, 2), _weight(70, 100, 3)
+    stacked = Fp8Weight.stack([a, b, c])
+    assert stacked.in_blocks and stacked.halves == 1
+    assert torch.equal(stacked.to(torch.float32), torch.cat([w.to(torch.float32) for w in (a, b, c)]))
+    pair = Fp8Weight.stack([c, _weight(70, 100, 4)])
+    assert pair.halves == 2 and not pair.in_blocks
+    assert torch.equal(pair.to(torch.float32)[:70], c.to(torch.float32))
+    assert torch.equal(pair.to(torch.float32)[70:], _weight(70, 100, 4).to(torch.float32))
+    with pytest.raises(ValueError, match="cannot be stacked"):
+        Fp8Weight.stack([c, a])
+    with pytest.raises(ValueError, match="same number of columns"):
+        Fp8Weight.stack([a, _weight(128, 101)])
+    with pytest.raises(ValueError, match="plain matrices"):
+        Fp8Weight.stack([pair, c])
+
+
+def test_weights_that_are_refused():
+    from stride_b200.kernels.linear import Fp8Experts, Fp8Weight
+    w = _weight(130, 129)
+    with pytest.raises(TypeError):
+        Fp8Weight(torch.zeros(4, 4), torch.zeros(1, 1))
+    with pytest.raises(ValueError, match="scales"):
+        Fp8Weight(w.q[:, :129], w.scales[:1])
+    with pytest.raises(ValueError, match="scales"):
+        Fp8Weight(w.q[:, :129], w.scales.double())
+    with pytest.raises(ValueError, match="gate and an up matrix"):
+        Fp8Experts([w, w], [w])
+    with pytest.raises(ValueError, match="gate and an up matrix"):
+        Fp8Experts([_weight(8, 16)], [_weight(16, 8)])
+
+
+def test_calls_without_a_device_are_refused():
+    from stride_b200.kernels import ops
+    from stride_b200.kernels.linear import Linear
+    from stride_b200.parts.context import Workspace
+    with pytest.raises(RuntimeError, match="CUDA tensors only"):
+        ops.route_experts(torch.zeros(2, 4), torch.zeros(2, 1, dtype=torch.int32), torch.zeros(1, 2))
+    with pytest.raises(RuntimeError, match="CUDA tensors only"):
+        ops.quantize_fp8(torch.zeros(2, 16), torch.zeros(2, 16).to(torch.float8_e4m3fn), torch.zeros(1, 2))
+    layer = Linear(_weight(128, 64), torch.bfloat16)
+    with pytest.raises(ValueError, match="workspace"):
+        layer.forward(torch.zeros(2, 64), torch.zeros(2, 128))
+    with pytest.raises(RuntimeError, match="CUDA tensors only"):
+        layer.forward(torch.zeros(2, 64), torch.zeros(2, 128), workspace=Workspace(torch.device("cpu"), 2))
+
+
+def test_the_float32_engine_takes_what_the_weight_stands_for():
+    from stride_b200.kernels.linear import Linear
+    w = _weight(130, 200)
+    layer = Linear(w, torch.float32)
+    assert layer.fp8 is None and torch.equal(layer.weight, w.to(torch.float32))
+
+
+def test_checkpoint_with_8_bit_matrices(tmp_path):
+    from stride_b200.kernels.linear import Fp8Weight
+    from stride_b200.weights.loader import load_weights
+    from stride_b200.weights.random_init import model_plan, random_tensors, write_random_model
+    folder = write_random_model(tmp_path / "m", CONFIG, 3)
+    plan = model_plan(CONFIG)
+    loaded = load_weights(folder, plan, "cpu")
+    assert set(loaded) == {n for n in plan if n != "lm_head.weight"}
+    given = random_tensors(CONFIG, 3)
+    for name, want in plan.items():
+        if name not in loaded:
+            continue
+        assert isinstance(loaded[name], Fp8Weight) == want.fp8
+        if want.fp8:
+            assert torch.equal(loaded[name].q[:, :want.shape[1]].view(torch.uint8), given[name].view(torch.uint8))
+            assert torch.equal(loaded[name].scales, given[name + "_scale_inv"])
+        else:
+            assert torch.equal(loaded[name], given[name])
+    header = json.loads((folder / "model.safetensors").read_bytes()[8:8 + int.from_bytes((folder / "model.safetensors").read_bytes()[:8], "little")])
+    assert header["model.layers.0.mlp.up_proj.weight"]["dtype"] == "F8_E4M3"
+
+
+@pytest.mark.parametrize("break_it,match", [
+    (lambda t: t.pop("model.layers.0.mlp.up_proj.weight_scale_inv"), "missing tensors"),
+    (lambda t: t.update({"model.layers.0.mlp.up_proj.weight_scale_inv": torch.ones(1, 2)}), "wrong shapes"),
+    (lambda t: t.update({"model.norm.weight_scale_inv": torch.ones(1, 1)}), "unexpected tensors"),
+    (lambda t: t.update({"model.embed_tokens.weight": t["model.embed_tokens.weight"].to(torch.float8_e4m3fn),
+                         "model.embed_tokens.weight_scale_inv": torch.ones(3, 2)}), "does not take")])
+def test_checkpoints_that_do_not_fit(tmp_path, break_it, match):
+    from stride_b200.weights.loader import WeightsError, load_weights
+    from stride_b200.weights.random_init import model_plan, random_tensors
+    from stride_b200.weights.safetensors_io import write_safetensors
+    tensors = random_tensors(CONFIG, 3)
+    break_it(tensors)
+    write_safetensors(tmp_path / "model.safetensors", tensors)
+    with pytest.raises(WeightsError, match=match):
+        load_weights(tmp_path, model_plan(CONFIG), "cpu")
+
+
+@pytest.mark.parametrize("change", [{"quant_method": "awq"}, {"weight_block_size": [64, 128]}, {"weight_block_size": None}, {"activation_scheme": "static"},
+                                    {"fmt": "e5m2"}])
+def test_quantisations_that_are_refused(change):
+    from stride_b200.config.llama import ConfigError, LlamaConfig
+    LlamaConfig.from_dict(CONFIG)
+    with pytest.raises(ConfigError, match="quantization_config"):
+        LlamaConfig.from_dict({**CONFIG, "quantization_config": {**CONFIG["quantization_config"], **change}})
+
+
+def _experts_spec(**params):
+    from stride_b200.parts import PartSpec
+    names = {r: tuple(f"e{e}.{r}" for e in range(8)) for r in ("gate", "up", "down")}
+    return PartSpec("scored_experts", {"hidden_size": 64, "intermediate_size": 32, "experts": 8, "top": 2, **params}, {"router": "router", **names})
+
+
+@pytest.mark.parametrize("params", [{"top": 9}, {"top": 0}, {"groups": 3}, {"groups": 4, "top_groups": 5}, {"groups": 4, "top_groups": 1, "top": 3},
+                                    {"group_best": 3}, {"score": "relu"}])
+def test_scored_experts_that_are_refused(params):
+    from stride_b200.parts import BuildEnv, part_class
+    env = BuildEnv(torch.device("cpu"), torch.bfloat16, 8, 64)
+    part_class("feed_forward", "scored_experts")(_experts_spec(groups=4, top_groups=2), env)
+    with pytest.raises(ValueError, match="scored experts"):
+        part_class("feed_forward", "scored_experts")(_experts_spec(**params), env)
+
+
+def test_scored_experts_take_8_bit_matrices_in_the_bfloat16_engine():
+    from stride_b200.parts import BuildEnv, part_class
+    make = part_class("feed_forward", "scored_experts")
+    with pytest.raises(ValueError, match="bfloat16 engine"):
+        make(_experts_spec(), BuildEnv(torch.device("cpu"), torch.float32, 8, 64))
+    part = make(_experts_spec(), BuildEnv(torch.device("cpu"), torch.bfloat16, 8, 64))
+    tensors = {n: torch.zeros(p.shape, dtype=torch.bfloat16) for n, p in part.tensor_plan().items()}
+    with pytest.raises(TypeError, match="8 bits"):
+        part.bind(tensors)
