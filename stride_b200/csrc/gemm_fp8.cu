@@ -118,7 +118,7 @@ struct Fp8Params {
   int64_t ldxs;
   const void* x;             // for the forms that quantise it themselves: float32 (x_f32) or bfloat16 [n][ldx], rows 16-byte aligned
   int64_t ldx;
-  int x_f32, x_gathered;     // x_gathered: row i is token order[i] % n
+  int x_f32, x_gathered;     // x_gathered: row i is token order[i]
   const float* w_scales;     // [blocks of rows][blocks]
   int n, M, K, blocks;       // M: rows of the weight (of one expert); kGated: gate rows, then up rows
   int half_rows;
@@ -127,8 +127,7 @@ struct Fp8Params {
   int stages;
   int tiles_m, tiles_n, vec_out;      // (the kernel on pairs; vec_out: the result takes 16-byte stores)
   const int32_t* tiles;      // experts: the list of `expert_order_kernel`; else null
-  const int32_t* order;      // experts: row -> pair k n + token
-  const float* pair_weight;  // experts: a factor on every pair's result, by pair, or null
+  const int32_t* order;      // experts: row -> token
   float* z_scales;           // experts, gated products quantised by the epilogue: [blocks of features][ldxs]
   Gate gate;
   int* status;
@@ -254,8 +253,7 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
   __shared__ __align__(8) uint64_t full_bar[kMaxStages], empty_bar[kMaxStages];
   __shared__ __align__(8) uint64_t accum_full[S::kSlots], scale_full[S::kSlots], slot_empty[S::kSlots];
   __shared__ __align__(16) float factor[S::kSlots][2][BN];
-  __shared__ int pair_s[GROUPED ? BN : 1];           // the tile's rows' pairs and the factors on their results
-  __shared__ float weight_s[GROUPED ? BN : 1];
+  __shared__ int token_s[GROUPED && QUANT ? BN : 1];         // the tokens of the tile's rows
   __shared__ uint32_t tmem_base_s;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -282,9 +280,9 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
     }
     mbar_init_fence();
   }
-  if (GROUPED && threadIdx.x >= 128 && threadIdx.x < 128 + BN) {
-    const int c = threadIdx.x - 128, pair = n0 + c < end ? p.order[n0 + c] : 0;
-    pair_s[c] = pair, weight_s[c] = p.pair_weight != nullptr ? p.pair_weight[pair] : 1.0f;
+  if (GROUPED && QUANT && p.x_gathered && threadIdx.x >= 128 && threadIdx.x < 128 + BN) {
+    const int c = threadIdx.x - 128;
+    token_s[c] = n0 + c < end ? p.order[n0 + c] : 0;
   }
   if (warp == 1) tmem_alloc(smem_u32(&tmem_base_s), S::kTmem);
   fence_before_sync();
@@ -349,7 +347,7 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
       const int r = lane / kPerRow, part = lane % kPerRow, first = warp - 2, warps = quant_warps(p.x_f32), size = p.x_f32 ? 4 : 2,
                 pieces = kColumns * size / 16;
       const bool live = n0 + r < end;
-      const int64_t row = !live ? 0 : GROUPED && p.x_gathered ? pair_s[GROUPED ? r : 0] % p.n : n0 + r;
+      const int64_t row = !live ? 0 : GROUPED && p.x_gathered ? token_s[GROUPED ? r : 0] : n0 + r;
       const uint8_t* from = static_cast<const uint8_t*>(p.x) + (row * p.ldx + b0 * kBlock + part * kColumns) * size;
       const int columns = live ? p.K - b0 * kBlock - part * kColumns : 0;        // what the row has from there on
       const int mine = p.stages * S::kStage + first * pieces * 512 + lane * 16;      // this lane's pieces, 32 x 16 bytes from one to the next
@@ -510,10 +508,8 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
       if (tile != nullptr && m < (EPI == kGated ? p.half_rows : p.M)) {
         for (int c = thread / kFeatures; c < BN && n0 + c < end; c += kStride) {
           float v = tile[c * kBlock + j];
-          int64_t to = n0 + c;
           if (EPI == kGated) v = gated_product(v, tile[c * kBlock + 64 + j], p.gate);
-          if (GROUPED && EPI != kGated) to = pair_s[GROUPED ? c : 0], v *= weight_s[GROUPED ? c : 0];
-          OUT* o = static_cast<OUT*>(p.out) + to * p.ldo + m;
+          OUT* o = static_cast<OUT*>(p.out) + static_cast<int64_t>(n0 + c) * p.ldo + m;
           if (EPI == kAdd) v += sb::widen(*o);
           *o = sb::narrow<OUT>(v);
         }
@@ -577,7 +573,7 @@ struct PairShape {
   static constexpr int kColumns = kRows / 2;                 // of a chain
   static constexpr int kStage = kStageA + kRows / 2 * 128;
   static constexpr int kSlots = 512 / kColumns;              // accumulators under way, all of tensor memory; even ones are the first chain's
-  static constexpr int kStages = WIDE ? 6 : 8;
+  static constexpr int kStages = WIDE ? 5 : 6;
 };
 
 // The tiles of a launch in the order in which the pairs walk them. Dense: the tiles of tokens first, so that the pairs of a round share few weight
@@ -596,25 +592,45 @@ struct PairTile {
   }
 };
 
-// 32 results of a token, features m .. m + 31 of `rows`, to `to` (the address of the first).
+// A warp's results, a token a lane, 32 features m .. m + 31 of M each, to rows first .. of `out`, of which `count` exist. They pass through shared
+// memory (`staged`, 32 rows of kPitch bytes), 64 bytes a token at a time, so that a store of the warp fills whole sectors of eight tokens: stored from
+// the registers, half a sector a lane of 32 tokens, a tile's stores took as long as eight of its blocks.
+constexpr int kPitch = 80;
+constexpr int kStaged = 16 * 32 * kPitch;       // of all the epilogue's warps
 template <int EPI, class OUT>
-__device__ __forceinline__ void store_token(OUT* to, const float* v, int m, int rows, bool vec) {
-  constexpr int kPer = 16 / sizeof(OUT);
-  if (vec && m + 32 <= rows) {
+__device__ __forceinline__ void store_rows(OUT* out, int64_t ldo, int64_t first, int count, int m, int M, bool vec, const float* v, uint8_t* staged, int lane) {
+  constexpr int kPer = 16 / sizeof(OUT), kChunk = 4 * kPer;      // elements of a piece of 16 bytes, of a token's 64 bytes
 #pragma unroll
-    for (int c = 0; c < 32; c += kPer) {
-      float r[kPer];
-      uint4 raw = EPI == kAdd ? *reinterpret_cast<const uint4*>(to + c) : make_uint4(0, 0, 0, 0);
+  for (int c0 = 0; c0 < 32; c0 += kChunk) {
+    __syncwarp();
 #pragma unroll
-      for (int i = 0; i < kPer; ++i) r[i] = v[c + i] + (EPI == kAdd ? sb::widen(reinterpret_cast<const OUT*>(&raw)[i]) : 0.0f);
+    for (int j = 0; j < 4; ++j) {
+      alignas(16) OUT r[kPer];
 #pragma unroll
-      for (int i = 0; i < kPer; ++i) reinterpret_cast<OUT*>(&raw)[i] = sb::narrow<OUT>(EPI == kAdd ? r[i] : v[c + i]);
-      *reinterpret_cast<uint4*>(to + c) = raw;
+      for (int i = 0; i < kPer; ++i) r[i] = sb::narrow<OUT>(v[c0 + j * kPer + i]);
+      *reinterpret_cast<uint4*>(staged + lane * kPitch + j * 16) = *reinterpret_cast<const uint4*>(r);
     }
-  } else {
+    __syncwarp();
 #pragma unroll
-    for (int c = 0; c < 32; ++c)
-      if (m + c < rows) to[c] = sb::narrow<OUT>(EPI == kAdd ? v[c] + sb::widen(to[c]) : v[c]);
+    for (int j = 0; j < 4; ++j) {
+      const int token = j * 8 + (lane >> 2), at = m + c0 + (lane & 3) * kPer;
+      if (token >= count || at >= M) continue;
+      uint4 raw = *reinterpret_cast<const uint4*>(staged + token * kPitch + (lane & 3) * 16);
+      OUT* to = out + (first + token) * ldo + at;
+      if (vec && at + kPer <= M) {
+        if (EPI == kAdd) {
+          const uint4 old = *reinterpret_cast<const uint4*>(to);
+#pragma unroll
+          for (int i = 0; i < kPer; ++i)
+            reinterpret_cast<OUT*>(&raw)[i] = sb::narrow<OUT>(sb::widen(reinterpret_cast<const OUT*>(&raw)[i]) + sb::widen(reinterpret_cast<const OUT*>(&old)[i]));
+        }
+        *reinterpret_cast<uint4*>(to) = raw;
+      } else {
+#pragma unroll
+        for (int i = 0; i < kPer; ++i)
+          if (at + i < M) to[i] = EPI == kAdd ? sb::narrow<OUT>(sb::widen(reinterpret_cast<const OUT*>(&raw)[i]) + sb::widen(to[i])) : reinterpret_cast<const OUT*>(&raw)[i];
+      }
+    }
   }
 }
 
@@ -636,6 +652,7 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = static_cast<int>(sb::cluster_rank());
   const uint32_t smem0 = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  uint8_t* smem0_p = smem_raw + (smem0 - smem_u32(smem_raw));
   const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
   if (threadIdx.x == 0) {
     prefetch_tensormap(&map_w);
@@ -818,23 +835,16 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
           }
           if (set + part == 0) p.z_scales[static_cast<int64_t>(t.tile_m) * p.ldxs + token] = finite ? power_of_two(e) : __uint_as_float(0x7FC00000u);
         }
-      } else if (ok && token < t.end) {
+      } else if (__all_sync(0xffffffffu, ok)) {
         OUT* out = static_cast<OUT*>(p.out);
+        uint8_t* staged = smem0_p + S::kStages * S::kStage + (warp - 4) * 32 * kPitch;
+        const int first = token - lane, count = min(t.end - first, 32);
         if (EPI == kGated) {
-          const int m = t.tile_m * kBlock + set * 64 + part * 32;
-          store_token<kStore>(out + static_cast<int64_t>(token) * p.ldo + m, acc, m, p.half_rows, p.vec_out);
+          store_rows<kStore>(out, p.ldo, first, count, t.tile_m * kBlock + set * 64 + part * 32, p.half_rows, p.vec_out, acc, staged, lane);
         } else {
-          int64_t row = token;
-          if (GROUPED) {
-            row = p.order[token];
-            const float by = p.pair_weight[row];
-#pragma unroll
-            for (int c = 0; c < 32; ++c) acc[c] *= by, other[c] *= by;
-          }
           const int m = t.tile_m * S::kRows + (WIDE ? set * 64 + part * 32 : part * 64 + set * 32);
-          OUT* o = out + row * p.ldo + m;
-          store_token<EPI>(o, WIDE ? acc : other, m, p.M, p.vec_out);
-          if (WIDE) store_token<EPI>(o + kBlock, other, m + kBlock, p.M, p.vec_out);
+          store_rows<EPI>(out, p.ldo, first, count, m, p.M, p.vec_out, WIDE ? acc : other, staged, lane);
+          if (WIDE) store_rows<EPI>(out, p.ldo, first, count, m + kBlock, p.M, p.vec_out, other, staged, lane);
         }
       }
       __syncwarp();
@@ -850,9 +860,9 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
 }
 
 // ------------------------------------------------------------------ experts
-// choice [n][top] -> the pairs p = k n + token in expert order, the row of every choice (place [n][top]; -1: none), and the row tiles of the
-// products. An id outside [0, E) is no expert: its pair is left out. list: [0] tiles, [1] rows, then (expert, first row, end row) of every tile.
-// (Which of an expert's pairs comes first does not matter: every row is computed on its own.) One CTA; a thread holds kHeld choices, loaded
+// choice [n][top] -> the choices' tokens in expert order, the row of every choice (place [n][top]; -1: none), and the row tiles of the
+// products. An id outside [0, E) is no expert: it is left out. list: [0] tiles, [1] rows, then (expert, first row, end row) of every tile.
+// (Which of an expert's rows comes first does not matter: every row is computed on its own.) One CTA; a thread holds kHeld choices, loaded
 // together, and reads those beyond twice.
 constexpr int kMaxExperts = 1024;
 constexpr int kOrderThreads = 1024, kHeld = 16;
@@ -901,7 +911,7 @@ __global__ void __launch_bounds__(kOrderThreads) expert_order_kernel(const int32
     int at = -1;
     if (e < static_cast<uint32_t>(E)) {
       at = atomicAdd(&next[e], 1);
-      order[at] = i % top * n + i / top;
+      order[at] = i / top;
     }
     place[i] = at;
   };
@@ -911,30 +921,30 @@ __global__ void __launch_bounds__(kOrderThreads) expert_order_kernel(const int32
   for (int i = t + kHeld * kOrderThreads; i < pairs; i += kOrderThreads) put(i, static_cast<uint32_t>(choice[i]));
 }
 
-// out[t] = the token's weighted results in the order of its choices; a choice that is no expert has none. parts [top][n][ldp], rows 16-byte
-// aligned. Four features a thread (VEC: so is the result), the choices' loads together.
+// out[t] = the sum over the token's choices, in their order, of weight times result: parts [rows][ldp], rows 16-byte aligned, by `place` [n][top] (-1:
+// no expert, no term), weights [top][n]. Four features a thread (VEC: so is the result), the choices' loads together.
 template <class OUT, bool VEC>
-__global__ void __launch_bounds__(128) expert_combine_kernel(const float* parts, int64_t ldp, const int32_t* choice, int n, int top,
-                                                             int E, int W, OUT* out, int64_t ldo) {
+__global__ void __launch_bounds__(128) expert_combine_kernel(const float* parts, int64_t ldp, const int32_t* place, const float* weights, int n, int top, int W,
+                                                             OUT* out, int64_t ldo) {
   sb::grid_launch_dependents();
   sb::grid_dependency_wait();
   const int t = blockIdx.x, m = (blockIdx.y * blockDim.x + threadIdx.x) * 4;
   if (m >= W) return;
-  const int32_t* mine = choice + static_cast<int64_t>(t) * top;
-  const float* from = parts + static_cast<int64_t>(t) * ldp + m;
+  const int32_t* mine = place + static_cast<int64_t>(t) * top;
   float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
   constexpr int kTogether = 8;
   for (int k0 = 0; k0 < top; k0 += kTogether) {
     float4 v[kTogether];
-    bool there[kTogether];
+    float w[kTogether];
+    int row[kTogether];
 #pragma unroll
     for (int k = 0; k < kTogether; ++k) {
-      there[k] = k0 + k < top && static_cast<uint32_t>(mine[min(k0 + k, top - 1)]) < static_cast<uint32_t>(E);
-      if (there[k]) v[k] = *reinterpret_cast<const float4*>(from + static_cast<int64_t>(k0 + k) * n * ldp);
+      row[k] = k0 + k < top ? mine[k0 + k] : -1;
+      if (row[k] >= 0) w[k] = weights[static_cast<int64_t>(k0 + k) * n + t], v[k] = *reinterpret_cast<const float4*>(parts + row[k] * ldp + m);
     }
 #pragma unroll
     for (int k = 0; k < kTogether; ++k)
-      if (there[k]) sum[0] += v[k].x, sum[1] += v[k].y, sum[2] += v[k].z, sum[3] += v[k].w;
+      if (row[k] >= 0) sum[0] = fmaf(w[k], v[k].x, sum[0]), sum[1] = fmaf(w[k], v[k].y, sum[1]), sum[2] = fmaf(w[k], v[k].z, sum[2]), sum[3] = fmaf(w[k], v[k].w, sum[3]);
   }
   OUT* to = out + static_cast<int64_t>(t) * ldo + m;
   if (VEC && m + 4 <= W) {
@@ -1024,7 +1034,7 @@ int launch_pair(const void* w, int64_t rows_w, int64_t ldw, const void* q, int64
   const long long tiles = static_cast<long long>(p.tiles_m) * tiles_n;
   if (tiles > (1ll << 30)) return sb::fail("gemm_fp8: too many tiles");
   auto kernel = gemm_fp8_pair_kernel<EPI, WIDE, OUT, GROUPED>;
-  const size_t smem = static_cast<size_t>(S::kStages) * S::kStage + 1024;
+  const size_t smem = static_cast<size_t>(S::kStages) * S::kStage + (std::is_same<OUT, uint8_t>::value ? 0 : kStaged) + 1024;
   static sb::DeviceOnce once;
   if (once.needed()) {
     if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)) != cudaSuccess) return sb::check_launch("gemm_fp8");
@@ -1256,13 +1266,13 @@ SB_EXPORT int sb_experts_fp8(const SbFp8Experts* l, const void* x, int xdtype, i
     if (quant) set_input(p, z, 0, s.ldz), p.x_gathered = 0;
     else if (int rc = launch_quantize(z, 0, s.ldz, list + 1, nullptr, 1, pairs, F, base + s.zq, s.ldz, zs, pairs, st)) return rc;
   }
-  p.out = parts, p.ldo = s.ldp, p.x_scales = zs, p.w_scales = down_scales, p.M = W, p.K = F, p.half_rows = 0, p.pair_weight = weights;
+  p.out = parts, p.ldo = s.ldp, p.x_scales = zs, p.w_scales = down_scales, p.M = W, p.K = F, p.half_rows = 0;
   p.blocks = p.range_blocks = (F + kBlock - 1) / kBlock, p.scale_rows = (W + kBlock - 1) / kBlock;
   if (int rc = launch_product<kStore, float, true>(down, static_cast<int64_t>(E) * W, ldd, base + s.zq, pairs, s.ldz, p, tile, tiles, st)) return rc;
   const dim3 grid(n, (W + 511) / 512);
   if (grid.y > 65535) return sb::fail("%s: %d features are too many", who, W);
   auto combine = [&](auto kernel, auto to) {
-    sb::launch_pdl(kernel, grid, dim3(128), 0, st, static_cast<const float*>(parts), s.ldp, choice, n, top, E, W, to, ldo);
+    sb::launch_pdl(kernel, grid, dim3(128), 0, st, static_cast<const float*>(parts), s.ldp, place, weights, n, top, W, to, ldo);
   };
   const int size = out_dtype == 0 ? 4 : 2;
   const bool vec = ldo % 4 == 0 && (reinterpret_cast<uintptr_t>(out) & (4 * size - 1)) == 0;

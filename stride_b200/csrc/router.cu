@@ -86,7 +86,7 @@ __device__ __forceinline__ uint32_t scores(const Routing& r, const float* z, int
       s[i] = 0;
       if ((open >> i) & 1u) {
         if constexpr (sizeof(T) == 8) s[i] = 1.0 / (1.0 + exp(-static_cast<double>(v[i])));
-        else s[i] = 1.0f / (1.0f + expf(-v[i]));
+        else s[i] = __fdividef(1.0f, 1.0f + __expf(fminf(-v[i], 80.0f)));      // (to choose by; a chosen one's weight is computed anew)
       }
     }
   }
@@ -186,8 +186,31 @@ __device__ __noinline__ void route_row_64(const Routing& r, int row, int lane, d
   write_row(r, row, lane, kept_e, r.renormalise ? kept_s * r.scale / (sum + 1e-20) : kept_s * r.scale);
 }
 
-// A warp a token. In 32-bit first: a score is off by less than 2^-20 of the largest (the exponential by two units in the last place of
-// 2^-23, sum and division by half of one an operation), a sum with a bias by 2^-23 of its size more; where two
+// Both arrays by descending key: Batcher's merge exchanges.
+template <int N, int P, int K>
+__device__ __forceinline__ void merge_exchange(uint32_t* key, int* place) {
+#pragma unroll
+  for (int a = 0; a + K < N; ++a) {
+    constexpr int kFirst = K % P;
+    const int b = a + K;
+    if (a >= kFirst && (a - kFirst) % (2 * K) < K && a / (2 * P) == b / (2 * P)) {
+      const bool turned = key[a] < key[b];
+      const uint32_t low = min(key[a], key[b]);
+      const int at = place[a];
+      key[a] = max(key[a], key[b]), key[b] = low;
+      place[a] = turned ? place[b] : at, place[b] = turned ? at : place[b];
+    }
+  }
+  if constexpr (K > 1) merge_exchange<N, P, K / 2>(key, place);
+  else if constexpr (2 * P < N) merge_exchange<N, 2 * P, 2 * P>(key, place);
+}
+template <int N>
+__device__ __forceinline__ void sort_descending(uint32_t* key, int* place) {
+  if constexpr (N > 1) merge_exchange<N, 1, 1>(key, place);
+}
+
+// A warp a token. In 32-bit first: a score is off by less than 2^-20 of the largest (a sigmoid's approximated exponential is off by 2 + 1.2 |z| units
+// in the last place, which near and above 1/2 counts for a quarter at most, its division by two; where all scores are small, 2^-16), a sum with a bias by 2^-23 of its size more; where two
 // candidates that follow one another, or the last group that stays and the first that does not, are closer than twice that, the token is routed
 // again in 64-bit. So the choice is that of 64-bit scores always, at the price of 32-bit ones for nearly all tokens (16,384 tokens of 256 experts in
 // eight groups, everything in 64-bit: 87 us).
@@ -201,8 +224,9 @@ __global__ void __launch_bounds__(32 * kWarps) route_kernel(const Routing r) {
   if (row >= r.n) return;
   double* held = held_s[threadIdx.x >> 5];
   float* held_scores = reinterpret_cast<float*>(held) + 32 * PER;
+  const float* z = r.logits + row * r.ldz;
   float s[PER], c[PER];
-  uint32_t open = scores<float, PER>(r, r.logits + row * r.ldz, lane, s, c);
+  uint32_t open = scores<float, PER>(r, z, lane, s, c);
   float high_s = 0.0f, high_c = 0.0f;
 #pragma unroll
   for (int i = 0; i < PER; ++i)
@@ -210,7 +234,7 @@ __global__ void __launch_bounds__(32 * kWarps) route_kernel(const Routing r) {
   // (both are not negative: their bits are ordered as they are)
   high_s = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(high_s)));
   high_c = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(high_c)));
-  const float near = 2.0f * (0x1p-20f * high_s + 0x1p-23f * high_c);
+  const float near = 2.0f * ((high_s > 0.125f ? 0x1p-20f : 0x1p-16f) * high_s + 0x1p-23f * high_c);
   bool sure = high_c < INFINITY;
   if (r.groups > 1) {
     float gap;
@@ -222,18 +246,9 @@ __global__ void __launch_bounds__(32 * kWarps) route_kernel(const Routing r) {
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
     key[i] = (open >> i) & 1u ? order_key(c[i]) : 0u, place[i] = i;
-    held_scores[lane + 32 * i] = s[i];
+    if (r.softmax) held_scores[lane + 32 * i] = s[i];
   }
-#pragma unroll
-  for (int i = 0; i + 1 < PER; ++i)
-#pragma unroll
-    for (int j = 0; j + 1 < PER - i; ++j) {
-      const bool turned = key[j] < key[j + 1];
-      const uint32_t k = key[j];
-      const int at = place[j];
-      key[j] = turned ? key[j + 1] : k, key[j + 1] = turned ? k : key[j + 1];
-      place[j] = turned ? place[j + 1] : at, place[j + 1] = turned ? at : place[j + 1];
-    }
+  sort_descending<PER>(key, place);
   __syncwarp();
   float sum = 0.0f, kept_s = 0.0f, before = INFINITY;
   int kept_e = -1;
@@ -246,15 +261,15 @@ __global__ void __launch_bounds__(32 * kWarps) route_kernel(const Routing r) {
     before = value;
     if (k == r.top) break;
     const int e = owner + 32 * __shfl_sync(0xffffffffu, place[0], owner);
-    const float score = held_scores[e];
-    sum += score;
-    if (lane == k) kept_s = score, kept_e = e;      // (at most 32 choices)
+    if (lane == k) kept_e = e;                      // (at most 32 choices)
     if (lane == owner) {
 #pragma unroll
       for (int i = 0; i + 1 < PER; ++i) key[i] = key[i + 1], place[i] = place[i + 1];
       key[PER - 1] = 0;
     }
   }
+  if (kept_e >= 0) kept_s = r.softmax ? held_scores[kept_e] : 1.0f / (1.0f + expf(-fminf(z[kept_e], FLT_MAX)));
+  if (r.renormalise) sum = warp_sum(kept_s);
   if (r.renormalise && kept_e >= 0 && sum < 0x1p-50f) sure = false;      // (scores below the smallest floats count where all are)
   sure = __all_sync(0xffffffffu, sure);
   if (!sure) {
