@@ -37,7 +37,7 @@ using sb::gemm_tile::silu_fast;
 constexpr int kBlock = 128;            // columns (and weight rows) of a scale
 constexpr int kStageA = kBlock * 128;  // bytes of a weight tile's block
 constexpr int kMaxStages = 8;
-constexpr int kMaxRanges = 8;
+constexpr int kMaxRanges = 4;
 constexpr int kSmemBudget = 200 * 1024;
 
 enum Epilogue { kStore = 0, kAdd = 1, kGated = 2 };
@@ -173,6 +173,19 @@ __device__ __forceinline__ void issue_signal(uint32_t bar) {
                  "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(bar)
                  : "memory");
 }
+// Whether a barrier's phase is over, asked ahead of the wait for it: the answer is on its way while other work is issued (a wait that finds its phase
+// over takes some hundred cycles, as long as a quarter of a block).
+__device__ __forceinline__ bool mbar_over(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
 // Waits for this warp's loads from tensor memory; what they brought passes through, so that no use of it can be moved in front of the wait.
 __device__ __forceinline__ void tmem_arrived16(uint32_t* r) {
   asm volatile("tcgen05.wait::ld.sync.aligned;"
@@ -232,7 +245,6 @@ struct Shape {
   static constexpr int kStage = kStageA + BN * 128;
   static constexpr int kTmem = kSlots * BN;                            // (a power of two)
   static constexpr int kCtas = BN <= 32 ? 2 : 1;                       // of an SM: with few tokens one fills its ring while the other drains
-  static constexpr int kSmem = kCtas == 2 ? 100 * 1024 : kSmemBudget;
 };
 
 // blockIdx = (weight tile, token tile, K range: the rank in the cluster when SPLIT). Warp 0 loads, warp 1 issues the products, warps 2 and 3
@@ -253,16 +265,9 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
   __shared__ __align__(8) uint64_t full_bar[kMaxStages], empty_bar[kMaxStages];
   __shared__ __align__(8) uint64_t accum_full[S::kSlots], scale_full[S::kSlots], slot_empty[S::kSlots];
   __shared__ __align__(16) float factor[S::kSlots][2][BN];
-  __shared__ int token_s[GROUPED && QUANT ? BN : 1];         // the tokens of the tile's rows
   __shared__ uint32_t tmem_base_s;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  int expert = 0, n0 = blockIdx.y * BN, end = p.n;
-  if (GROUPED) {
-    sb::grid_dependency_wait();        // whose rows this tile holds is an earlier kernel's result
-    if (static_cast<int>(blockIdx.y) >= p.tiles[0]) return;
-    expert = p.tiles[2 + 3 * blockIdx.y], n0 = p.tiles[3 + 3 * blockIdx.y], end = p.tiles[4 + 3 * blockIdx.y];
-  }
   const uint32_t smem0 = (smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* smem0_p = smem_raw + (smem0 - smem_u32(smem_raw));
   const int tile_m = blockIdx.x;
@@ -280,18 +285,22 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
     }
     mbar_init_fence();
   }
-  if (GROUPED && QUANT && p.x_gathered && threadIdx.x >= 128 && threadIdx.x < 128 + BN) {
-    const int c = threadIdx.x - 128;
-    token_s[c] = n0 + c < end ? p.order[n0 + c] : 0;
-  }
   if (warp == 1) tmem_alloc(smem_u32(&tmem_base_s), S::kTmem);
   fence_before_sync();
   __syncthreads();
   fence_after_sync();
   const uint32_t tmem_base = tmem_base_s;
   sb::grid_launch_dependents();        // (behind the allocation: a kernel let in before it could take the columns and wait for this one)
+  int expert = 0, n0 = blockIdx.y * BN, end = p.n;
+  bool empty = false;
+  if (GROUPED) {
+    sb::grid_dependency_wait();        // whose rows this tile holds is an earlier kernel's result
+    empty = static_cast<int>(blockIdx.y) >= p.tiles[0];
+    if (!empty) expert = p.tiles[2 + 3 * blockIdx.y], n0 = p.tiles[3 + 3 * blockIdx.y], end = p.tiles[4 + 3 * blockIdx.y];
+  }
 
-  if (warp == 0) {
+  if (empty) {
+  } else if (warp == 0) {
     if (lane == 0) {
       const int row_w = expert * p.M + tile_m * (EPI == kGated ? 64 : kBlock);
       auto load_w = [&](int i, int st) {
@@ -323,10 +332,13 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
     const uint64_t first = smem_desc_sw128(smem0);
     int st = 0, slot = 0;
     uint32_t par = 0, slot_par = 1;
+    bool ready = false;
     for (int i = 0; i < iters; ++i) {
-      mbar_wait(smem_u32(&slot_empty[slot]), slot_par, p.status, 42);
-      mbar_wait(smem_u32(&full_bar[st]), par, p.status, 43);
-      __syncwarp();
+      if (!__all_sync(0xffffffffu, ready)) {
+        mbar_wait(smem_u32(&slot_empty[slot]), slot_par, p.status, 42);
+        mbar_wait(smem_u32(&full_bar[st]), par, p.status, 43);
+        __syncwarp();
+      }
       fence_after_sync();
       const uint64_t da = first + static_cast<uint64_t>(st * (S::kStage >> 4));
       issue_products<false>(tmem_base + slot * BN, da, da + (kStageA >> 4), idesc);
@@ -334,6 +346,7 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
       issue_signal<false>(smem_u32(&accum_full[slot]));
       if (++st == p.stages) st = 0, par ^= 1;
       if (++slot == S::kSlots) slot = 0, slot_par ^= 1;
+      ready = mbar_over(smem_u32(&slot_empty[slot]), slot_par) && mbar_over(smem_u32(&full_bar[st]), par);
     }
   } else if (warp < kFirst) {
     // the scales' products, two columns a thread; four blocks are read ahead of their turn
@@ -347,7 +360,7 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
       const int r = lane / kPerRow, part = lane % kPerRow, first = warp - 2, warps = quant_warps(p.x_f32), size = p.x_f32 ? 4 : 2,
                 pieces = kColumns * size / 16;
       const bool live = n0 + r < end;
-      const int64_t row = !live ? 0 : GROUPED && p.x_gathered ? token_s[GROUPED ? r : 0] : n0 + r;
+      const int64_t row = !live ? 0 : GROUPED && p.x_gathered ? p.order[n0 + r] : n0 + r;
       const uint8_t* from = static_cast<const uint8_t*>(p.x) + (row * p.ldx + b0 * kBlock + part * kColumns) * size;
       const int columns = live ? p.K - b0 * kBlock - part * kColumns : 0;        // what the row has from there on
       const int mine = p.stages * S::kStage + first * pieces * 512 + lane * 16;      // this lane's pieces, 32 x 16 bytes from one to the next
@@ -469,9 +482,13 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
     bool ok = true;
     int slot = 0, left = p.range_blocks;
     uint32_t slot_par = 0;
+    bool ready = false;
     for (int i = 0; i < iters; ++i) {
-      ok = mbar_wait(smem_u32(&accum_full[slot]), slot_par, p.status, 45) && ok;
-      ok = mbar_wait(smem_u32(&scale_full[slot]), slot_par, p.status, 46) && ok;
+      if (!__all_sync(0xffffffffu, ready)) {
+        ok = mbar_wait(smem_u32(&accum_full[slot]), slot_par, p.status, 45) && ok;
+        ok = mbar_wait(smem_u32(&scale_full[slot]), slot_par, p.status, 46) && ok;
+        __syncwarp();
+      }
       fence_after_sync();
       const uint32_t from = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + slot * BN + half * C;
       const float* f = factor[slot][EPI == kGated && quarter >= 2 ? 1 : 0] + half * C;
@@ -486,6 +503,7 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
       __syncwarp();
       if (lane == 0) mbar_arrive(smem_u32(&slot_empty[slot]));
       if (++slot == S::kSlots) slot = 0, slot_par ^= 1;
+      ready = mbar_over(smem_u32(&accum_full[slot]), slot_par) && mbar_over(smem_u32(&scale_full[slot]), slot_par);
       if (!SPLIT && (--left == 0 || i + 1 == iters)) {
         left = p.range_blocks;
 #pragma unroll
@@ -701,11 +719,14 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
       const uint32_t idesc = (1u << 4) | (static_cast<uint32_t>(S::kColumns >> 3) << 17) | (static_cast<uint32_t>(256 >> 4) << 24);
       int st = 0, slot = chain;
       uint32_t par = 0, slot_par = 1;
+      bool ready = false;
       for (int tile = pair; tile < total; tile += pairs) {
         for (int i = 0; i < p.blocks; ++i) {
-          mbar_wait(smem_u32(&accum_empty[slot]), slot_par, p.status, 52);
-          mbar_wait(smem_u32(&full_bar[st]), par, p.status, 53);
-          __syncwarp();
+          if (WIDE || !__all_sync(0xffffffffu, ready)) {
+            mbar_wait(smem_u32(&accum_empty[slot]), slot_par, p.status, 52);
+            mbar_wait(smem_u32(&full_bar[st]), par, p.status, 53);
+            __syncwarp();
+          }
           fence_after_sync();
           const uint64_t da = first + static_cast<uint64_t>(st * (S::kStage >> 4));
           issue_products<true>(tmem_base + slot * S::kColumns, da, da + (kStageA >> 4) + chain * (S::kColumns / 2 * 128 >> 4), idesc);
@@ -713,6 +734,7 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
           issue_signal<true>(smem_u32(&accum_full[slot]));
           if (++st == S::kStages) st = 0, par ^= 1;
           if ((slot += 2) >= S::kSlots) slot = chain, slot_par ^= 1;
+          if (!WIDE) ready = mbar_over(smem_u32(&accum_empty[slot]), slot_par) && mbar_over(smem_u32(&full_bar[st]), par);
         }
       }
     }
@@ -760,6 +782,7 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
     float acc[32], other[32];            // the sums; WIDE: of the second 128 rows, else: the ranges' totals
     int slot = set, batch = 0;
     uint32_t slot_par = 0, batch_par = 0;
+    bool ready = false;
     for (int tile = pair; tile < total; tile += pairs) {
       const PairTile t(p, GROUPED, tile);
       const int token = t.n0 + rank * kBlock + quarter * 32 + lane, blocks = p.blocks;
@@ -771,7 +794,8 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
       for (int i = 0, in_batch = 0; i < blocks; ++i) {
         if (in_batch == 0) ok = mbar_wait(smem_u32(&factor_full[batch]), batch_par, p.status, 56) && ok;
         const float f0 = factor[batch][in_batch][0][quarter * 32 + lane], f1 = factor[batch][in_batch][WIDE ? 1 : 0][quarter * 32 + lane];
-        ok = mbar_wait(smem_u32(&accum_full[slot]), slot_par, p.status, 55) && ok;
+        if (WIDE || !__all_sync(0xffffffffu, ready)) ok = mbar_wait(smem_u32(&accum_full[slot]), slot_par, p.status, 55) && ok;
+        if (!WIDE) __syncwarp();
         fence_after_sync();
         const uint32_t from = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + slot * S::kColumns + part * 32;
         uint32_t v[16];
@@ -783,10 +807,11 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
             fence_before_sync();
             __syncwarp();
             if (lane == 0) mbar_arrive_leader(smem_u32(&accum_empty[slot]));
+            if ((slot += 2) >= S::kSlots) slot = set, slot_par ^= 1;
+            if (!WIDE) ready = mbar_over(smem_u32(&accum_full[slot]), slot_par);       // (WIDE: two accumulators a set, the next is never there yet)
           }
           add_scaled<16>((c0 & 32 ? other : acc) + (c0 & 31), v, c0 & 32 ? f1 : f0);
         }
-        if ((slot += 2) >= S::kSlots) slot = set, slot_par ^= 1;
         if (!WIDE && (--left == 0 || i + 1 == blocks)) {
           left = p.range_blocks;
 #pragma unroll
@@ -980,8 +1005,11 @@ int fp8_ranges(int tiles, int blocks) {
 
 // Up to this many tokens the ranges run on CTAs of their own.
 constexpr int kSplitTokens = 128;
-// Up to this many rows of a tile the product quantises its input itself.
-constexpr int kQuantRows = 32;
+// Up to this many rows of a tile the product can quantise its input itself. Of a dense product it does where a CTA has few blocks of columns: that
+// saves a launch, but a block takes longer (2,048 x 2,048 of one token 7.7 us with a launch, 4.6 without; 16,384 x 2,048, 16 blocks a CTA, of eight
+// 10.1 and 12.1). The experts' two inputs would need two launches.
+constexpr int kQuantRows = 16;
+constexpr int kQuantBlocks = 6;
 
 template <int EPI, int BN, class OUT, bool GROUPED>
 int launch_tile(const void* w, int64_t rows_w, int64_t ldw, const void* q, int64_t rows_q, int64_t ldq, Fp8Params p, int tiles_m, int tiles_n,
@@ -992,12 +1020,15 @@ int launch_tile(const void* w, int64_t rows_w, int64_t ldw, const void* q, int64
   if (!byte_map(w, rows_w, p.K, ldw, EPI == kGated ? 64 : kBlock, &map_w) || (!quant && !byte_map(q, rows_q, p.K, ldq, BN, &map_x)))
     return sb::fail("gemm_fp8: no tensor map for a weight of %lld x %d (stride %lld)", (long long)rows_w, p.K, (long long)ldw);
   if (quant) map_x = map_w;                  // (not read)
-  // (quantising: at least half as many stages as accumulators, see the kernel; sixteen rows leave room for two CTAs an SM, 32 do not)
-  const int copies = quant ? quant_bytes(BN, p.x_f32) : 0;
-  p.stages = !quant ? std::min(kMaxStages, S::kSmem / S::kStage) : BN == 16 ? 4 : std::min(kMaxStages, (kSmemBudget - copies) / S::kStage);
-  const size_t smem = static_cast<size_t>(p.stages) * S::kStage + copies + 1024;
   const bool split = !GROUPED && p.ranges > 1 && p.n <= kSplitTokens;
   const dim3 grid(tiles_m, tiles_n, split ? p.ranges : 1);
+  // (few CTAs have an SM each: the longest ring then brings most of the weights on their way while the kernel in front still runs. Else two share
+  // one where they can. Quantising: at least half as many stages as accumulators, see the kernel)
+  const int copies = quant ? quant_bytes(BN, p.x_f32) : 0;
+  const bool alone = static_cast<long long>(tiles_m) * tiles_n * grid.z <= sb::sm_count();
+  const int room = (alone || S::kCtas == 1 ? kSmemBudget : quant ? 4 * S::kStage + copies : 100 * 1024) - copies;
+  p.stages = std::min(kMaxStages, room / S::kStage);
+  const size_t smem = static_cast<size_t>(p.stages) * S::kStage + copies + 1024;
   auto run = [&](auto kernel, sb::DeviceOnce& once) {
     if (once.needed()) {
       if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBudget + 1024) != cudaSuccess) return sb::check_launch("gemm_fp8");
@@ -1088,7 +1119,14 @@ void set_input(Fp8Params& p, const void* x, int xdtype, int64_t ldx) {
   p.x = x, p.ldx = ldx, p.x_f32 = xdtype == 0;
 }
 
-// One product; x (or null): the input that q and xs are to hold, where the form does not quantise it itself. out_dtype 0 float32, 1 bfloat16.
+// Whether a layer's product of n tokens quantises its input itself.
+bool quantises_itself(const void* x, int xdtype, int64_t ldx, int n, int M, int K) {
+  if (n > kQuantRows || !copied_input(x, xdtype, ldx)) return false;
+  const int blocks = (K + kBlock - 1) / kBlock, ranges = fp8_ranges((M + kBlock - 1) / kBlock, blocks);
+  return (blocks + ranges - 1) / ranges <= kQuantBlocks;
+}
+
+// One product; x: the input that it quantises itself, or null: q and xs hold it. out_dtype 0 float32, 1 bfloat16.
 int launch_gemm(const void* x, int xdtype, int64_t ldx, const void* q, int64_t ldq, const float* xs, int64_t ldxs, const void* w, int64_t ldw, const float* ws, void* out, int out_dtype,
                 int64_t ldo, int n, int M, int K, int epilogue, int half_rows, const Gate& gate, cudaStream_t st) {
   Fp8Params p = {};
@@ -1098,7 +1136,7 @@ int launch_gemm(const void* x, int xdtype, int64_t ldx, const void* q, int64_t l
   p.ranges = fp8_ranges((M + kBlock - 1) / kBlock, p.blocks);
   p.range_blocks = (p.blocks + p.ranges - 1) / p.ranges;
   p.gate = gate;
-  if (x != nullptr && copied_input(x, xdtype, ldx)) set_input(p, x, xdtype, ldx);
+  if (x != nullptr) set_input(p, x, xdtype, ldx);
   p.status = status_word();
   if (p.status == nullptr) return sb::fail("gemm_fp8: no status word on this device");
   const int tile = token_tile(p, epilogue), tiles_n = (n + tile - 1) / tile;
@@ -1189,7 +1227,7 @@ typedef struct SbFp8Layer {
   int32_t M, K, half_rows;
 } SbFp8Layer;
 
-// x is quantised, of few tokens on the way into the product (which leaves the buffers alone), then multiplied.
+// x is quantised, of few tokens perhaps on the way into the product (which leaves the buffers alone), and multiplied.
 SB_EXPORT int sb_linear_fp8(const SbFp8Layer* l, const void* x, int xdtype, int64_t ldx, void* out, int out_dtype, int64_t ldo, int n, int epilogue, int act,
                             float limit, float slope, void* stream) {
   if (int rc = check_quantized("linear_fp8", l->q, l->ldq, l->ldxs, n, l->K)) return rc;
@@ -1197,12 +1235,13 @@ SB_EXPORT int sb_linear_fp8(const SbFp8Layer* l, const void* x, int xdtype, int6
   if (xdtype < 0 || xdtype > 1 || ldx < l->K) return sb::fail("linear_fp8: rows of %lld elements, %d columns", (long long)ldx, l->K);
   if (n == 0) return 0;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (n > kQuantRows || !copied_input(x, xdtype, ldx)) {
+  const bool itself = quantises_itself(x, xdtype, ldx, n, l->M, l->K);
+  if (!itself) {
     if (int rc = launch_quantize(x, xdtype, ldx, nullptr, nullptr, 1, n, l->K, l->q, l->ldq, l->x_scales, l->ldxs, st)) return rc;
   }
   Gate gate;
   gate.act = act, gate.limit = limit, gate.slope = slope;
-  return launch_gemm(x, xdtype, ldx, l->q, l->ldq, l->x_scales, l->ldxs, l->w, l->ldw, l->w_scales, out, out_dtype, ldo, n, l->M, l->K, epilogue,
+  return launch_gemm(itself ? x : nullptr, xdtype, ldx, l->q, l->ldq, l->x_scales, l->ldxs, l->w, l->ldw, l->w_scales, out, out_dtype, ldo, n, l->M, l->K, epilogue,
                      epilogue == kGated ? l->half_rows : 0, gate, st);
 }
 

@@ -29,7 +29,10 @@ struct Routing {
   int n, E, top, groups, top_groups, group_best;
   int softmax, renormalise;
   float scale;
+  int size;                   // experts of a group, and 2^32 / size rounded up: e / size = the upper half of e times it, for e and size below 2^11
+  uint32_t inverse_size;
 };
+__device__ __forceinline__ int group_of(const Routing& r, int e) { return r.size == 1 ? e : __umulhi(e, r.inverse_size); }
 
 // float -> a word whose unsigned order is the values' (no NaN comes here).
 __device__ __forceinline__ uint32_t order_key(float v) {
@@ -106,7 +109,7 @@ __device__ __forceinline__ uint32_t scores(const Routing& r, const float* z, int
 // minus the best that does not.
 template <class T, int PER>
 __device__ __forceinline__ uint32_t keep_groups(const Routing& r, int lane, const T* c, uint32_t open, T* held, T& gap) {
-  const int size = r.E / r.groups;
+  const int size = r.size;
 #pragma unroll
   for (int i = 0; i < PER; ++i)
     if (lane + 32 * i < r.E) held[lane + 32 * i] = (open >> i) & 1u ? c[i] : static_cast<T>(-INFINITY);
@@ -134,6 +137,7 @@ __device__ __forceinline__ uint32_t keep_groups(const Routing& r, int lane, cons
   __syncwarp();
   const T mine = r.group_best > 1 && b > static_cast<T>(-INFINITY) ? a + b : a;
   int before = 0;                              // groups that come before this lane's
+#pragma unroll 4
   for (int g = 0; g < r.groups; ++g) {
     const T other = __shfl_sync(0xffffffffu, mine, g);
     before += other > mine || (other == mine && g < lane);
@@ -146,7 +150,7 @@ __device__ __forceinline__ uint32_t keep_groups(const Routing& r, int lane, cons
   if (score == static_cast<T>(-INFINITY)) gap = INFINITY;       // (groups with nothing in them: it does not matter which)
 #pragma unroll
   for (int i = 0; i < PER; ++i)
-    if ((open >> i) & 1u && !((kept >> ((lane + 32 * i) / size)) & 1u)) open &= ~(1u << i);
+    if ((open >> i) & 1u && !((kept >> group_of(r, lane + 32 * i)) & 1u)) open &= ~(1u << i);
   return open;
 }
 
@@ -279,7 +283,7 @@ __global__ void __launch_bounds__(32 * kWarps) route_kernel(const Routing r) {
   write_row(r, row, lane, kept_e, r.renormalise ? kept_s * (r.scale / (sum + 1e-20f)) : kept_s * r.scale);
 }
 
-int launch(const Routing& r, cudaStream_t st) {
+int launch(Routing r, cudaStream_t st) {
   if (r.n < 0 || r.E < 1 || r.E > kMaxExperts || r.top < 1 || r.top > 32 || r.top > r.E || r.ldz < r.E || r.ldw < r.n)
     return sb::fail("route_experts: %d of %d experts (at most 32 of %d), %d tokens, rows of %lld logits, of %lld weights", r.top, r.E, kMaxExperts, r.n,
                     (long long)r.ldz, (long long)r.ldw);
@@ -287,6 +291,7 @@ int launch(const Routing& r, cudaStream_t st) {
     return sb::fail("route_experts: %d of %d groups (at most %d) of %d experts, judged by their best %d (1 or 2)", r.top_groups, r.groups, kMaxGroups, r.E, r.group_best);
   if (r.top > r.top_groups * (r.E / r.groups)) return sb::fail("route_experts: %d experts of %d groups of %d", r.top, r.top_groups, r.E / r.groups);
   if (r.n == 0) return 0;
+  r.size = r.E / r.groups, r.inverse_size = r.size == 1 ? 0u : static_cast<uint32_t>((0x100000000ull + r.size - 1) / r.size);
   const dim3 grid((r.n + kWarps - 1) / kWarps), block(32 * kWarps);
   const int per = (r.E + 31) / 32;
   if (per <= 1) sb::launch_pdl(route_kernel<1>, grid, block, 0, st, r);
