@@ -119,6 +119,7 @@ struct Fp8Params {
   const void* x;             // for the forms that quantise it themselves: float32 (x_f32) or bfloat16 [n][ldx], rows 16-byte aligned
   int64_t ldx;
   int x_f32, x_gathered;     // x_gathered: row i is token order[i]
+  int quant_warps;           // how many of the warps quantise
   const float* w_scales;     // [blocks of rows][blocks]
   int n, M, K, blocks;       // M: rows of the weight (of one expert); kGated: gate rows, then up rows
   int half_rows;
@@ -171,6 +172,24 @@ __device__ __forceinline__ void issue_signal(uint32_t bar) {
   else
     asm volatile("{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\t"
                  "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(bar)
+                 : "memory");
+}
+// The same for loads: by one thread of a warp that is here as a whole, with addresses and coordinates that are values of the warp.
+__device__ __forceinline__ void issue_expect(uint32_t bar, uint32_t bytes) {
+  asm volatile("{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\t@e mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n\t}" ::"r"(bar), "r"(bytes)
+               : "memory");
+}
+template <bool PAIR>
+__device__ __forceinline__ void issue_load(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, int y) {
+  if (PAIR)
+    asm volatile("{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\t"
+                 "@e cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];\n\t}" ::"r"(dst),
+                 "l"(reinterpret_cast<uint64_t>(map)), "r"(bar & kPeerBitMask), "r"(x), "r"(y)
+                 : "memory");
+  else
+    asm volatile("{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\t"
+                 "@e cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];\n\t}" ::"r"(dst),
+                 "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y)
                  : "memory");
 }
 // Whether a barrier's phase is over, asked ahead of the wait for it: the answer is on its way while other work is issued (a wait that finds its phase
@@ -250,12 +269,10 @@ struct Shape {
 // blockIdx = (weight tile, token tile, K range: the rank in the cluster when SPLIT). Warp 0 loads, warp 1 issues the products, warps 2 and 3
 // multiply the scales, the others are the epilogue: four of them see all 128 rows, with eight each half takes half of the columns. QUANT (few
 // tokens): the input comes as it is, and four warps quantise it, the same arithmetic as `quantize_kernel`, straight into the ring's stages. A
-// block is one warp's, so that eight (of float32 four) are on their way at a time; all warps on one block at a time took 1.2 us for it. A lane
+// block is one warp's, so that eight (of float32, where two CTAs share an SM's memory, four) are on their way at a time; all warps on one block at a time took 1.2 us for it. A lane
 // copies the columns that it reads. A warp meets a stage's barrier only now and then, and could take one phase for the one two further on:
 // it looks there only once its accumulator, of which there are eight, is free, and with it the last but one block of that stage.
 constexpr int kQuantWarps = 8;
-__host__ __device__ constexpr int quant_warps(bool f32) { return f32 ? 4 : 8; }        // (of float32 there is no room for more)
-__host__ __device__ constexpr int quant_bytes(int bn, bool f32) { return quant_warps(f32) * bn * kBlock * (f32 ? 4 : 2); }
 template <int EPI, int BN, class OUT, bool GROUPED, bool SPLIT, bool QUANT>
 __global__ void __launch_bounds__(Shape<BN>::threads(QUANT), QUANT && BN > 16 ? 1 : Shape<BN>::kCtas)
 gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const Fp8Params p) {
@@ -301,32 +318,30 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
 
   if (empty) {
   } else if (warp == 0) {
-    if (lane == 0) {
-      const int row_w = expert * p.M + tile_m * (EPI == kGated ? 64 : kBlock);
-      auto load_w = [&](int i, int st) {
-        const uint32_t bar = smem_u32(&full_bar[st]), a = smem0 + st * S::kStage;
-        mbar_expect_tx(bar, QUANT ? kStageA : S::kStage);
-        tma_load_2d(a, &map_w, bar, (b0 + i) * kBlock, row_w);
-        if (EPI == kGated) tma_load_2d(a + kStageA / 2, &map_w, bar, (b0 + i) * kBlock, row_w + p.half_rows);
-      };
-      auto load_x = [&](int i, int st) {
-        if (!QUANT) tma_load_2d(smem0 + st * S::kStage + kStageA, &map_x, smem_u32(&full_bar[st]), (b0 + i) * kBlock, n0);
-      };
-      // (the weights are nobody's result: the first ring of them is under way before the kernels in front have ended)
-      const int ahead = min(iters, p.stages);
-      for (int i = 0; i < ahead; ++i) load_w(i, i);
-      if (!GROUPED && !QUANT) sb::grid_dependency_wait();
-      for (int i = 0; i < ahead; ++i) load_x(i, i);
-      int st = ahead == p.stages ? 0 : ahead;
-      uint32_t par = 0;
-      for (int i = ahead; i < iters; ++i) {
-        mbar_wait(smem_u32(&empty_bar[st]), par, p.status, 41);
-        load_w(i, st);
-        load_x(i, st);
-        if (++st == p.stages) st = 0, par ^= 1;
-      }
+    const int row_w = expert * p.M + tile_m * (EPI == kGated ? 64 : kBlock);
+    auto load_w = [&](int i, int st) {
+      const uint32_t bar = smem_u32(&full_bar[st]), a = smem0 + st * S::kStage;
+      issue_expect(bar, QUANT ? kStageA : S::kStage);
+      issue_load<false>(a, &map_w, bar, (b0 + i) * kBlock, row_w);
+      if (EPI == kGated) issue_load<false>(a + kStageA / 2, &map_w, bar, (b0 + i) * kBlock, row_w + p.half_rows);
+    };
+    auto load_x = [&](int i, int st) {
+      if (!QUANT) issue_load<false>(smem0 + st * S::kStage + kStageA, &map_x, smem_u32(&full_bar[st]), (b0 + i) * kBlock, n0);
+    };
+    // (the weights are nobody's result: the first ring of them is under way before the kernels in front have ended)
+    const int ahead = min(iters, p.stages);
+    for (int i = 0; i < ahead; ++i) load_w(i, i);
+    if (!GROUPED && !QUANT) sb::grid_dependency_wait();
+    for (int i = 0; i < ahead; ++i) load_x(i, i);
+    int st = ahead == p.stages ? 0 : ahead;
+    uint32_t par = 0;
+    for (int i = ahead; i < iters; ++i) {
+      mbar_wait(smem_u32(&empty_bar[st]), par, p.status, 41);
+      __syncwarp();
+      load_w(i, st);
+      load_x(i, st);
+      if (++st == p.stages) st = 0, par ^= 1;
     }
-    __syncwarp();
   } else if (warp == 1) {
     const uint32_t idesc = instr_desc_e4m3(BN);
     const uint64_t first = smem_desc_sw128(smem0);
@@ -357,7 +372,7 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
     if (!GROUPED) sb::grid_dependency_wait();
     if constexpr (QUANT) {
       constexpr int kPerRow = 32 / BN, kColumns = 128 / kPerRow;            // lanes of a row of the tile, columns of a lane
-      const int r = lane / kPerRow, part = lane % kPerRow, first = warp - 2, warps = quant_warps(p.x_f32), size = p.x_f32 ? 4 : 2,
+      const int r = lane / kPerRow, part = lane % kPerRow, first = warp - 2, warps = p.quant_warps, size = p.x_f32 ? 4 : 2,
                 pieces = kColumns * size / 16;
       const bool live = n0 + r < end;
       const int64_t row = !live ? 0 : GROUPED && p.x_gathered ? p.order[n0 + r] : n0 + r;
@@ -694,24 +709,24 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
   const int total = p.tiles_m * (GROUPED ? p.tiles[0] : p.tiles_n);
 
   if (warp == 0) {
-    if (lane == 0) {
-      int st = 0;
-      uint32_t par = 1;
-      for (int tile = pair; tile < total; tile += pairs) {
-        const PairTile t(p, GROUPED, tile);
-        const int row = t.expert * p.M + (EPI == kGated ? t.tile_m * kBlock + rank * p.half_rows : t.tile_m * S::kRows + rank * (S::kRows / 2));
-        const int token = t.n0 + rank * kBlock;
-        for (int i = 0; i < p.blocks; ++i) {
-          mbar_wait(smem_u32(&empty_bar[st]), par, p.status, 51);
-          const uint32_t bar = smem_u32(&full_bar[st]), a = smem0 + st * S::kStage;
-          if (rank == 0) mbar_expect_tx(bar, 2 * S::kStage);
-          tma_load_2d_pair(a, &map_x, bar, i * kBlock, token);
-          tma_load_2d_pair(a + kStageA, &map_w, bar, i * kBlock, row);
-          if (++st == S::kStages) st = 0, par ^= 1;
-        }
+    int st = 0;
+    uint32_t par = 1;
+    PairTile t(p, GROUPED, max(min(pair, total - 1), 0));
+    for (int tile = pair; tile < total; tile += pairs) {
+      const PairTile next(p, GROUPED, min(tile + pairs, total - 1));        // (on its way while this one is loaded)
+      const int row = t.expert * p.M + (EPI == kGated ? t.tile_m * kBlock + rank * p.half_rows : t.tile_m * S::kRows + rank * (S::kRows / 2));
+      const int token = t.n0 + rank * kBlock;
+      for (int i = 0; i < p.blocks; ++i) {
+        mbar_wait(smem_u32(&empty_bar[st]), par, p.status, 51);
+        __syncwarp();
+        const uint32_t bar = smem_u32(&full_bar[st]), a = smem0 + st * S::kStage;
+        if (rank == 0) issue_expect(bar, 2 * S::kStage);
+        issue_load<true>(a, &map_x, bar, i * kBlock, token);
+        issue_load<true>(a + kStageA, &map_w, bar, i * kBlock, row);
+        if (++st == S::kStages) st = 0, par ^= 1;
       }
+      t = next;
     }
-    __syncwarp();
   } else if (warp < 3) {
     if (rank == 0) {
       const int chain = warp - 1;
@@ -742,8 +757,9 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
     // the scales' products, four tokens a lane, a batch ahead of those that wait in shared memory (a trip to L2 takes longer than a block)
     int slot = 0;
     uint32_t slot_par = 1;
+    PairTile t(p, GROUPED, max(min(pair, total - 1), 0));
     for (int tile = pair; tile < total; tile += pairs) {
-      const PairTile t(p, GROUPED, tile);
+      const PairTile next(p, GROUPED, min(tile + pairs, total - 1));
       const int last = (EPI == kGated ? p.scale_rows / 2 : p.scale_rows) - 1;      // (rows beyond the weight: their sums are nobody's)
       const float* base = p.w_scales + static_cast<int64_t>(t.expert) * p.scale_rows * p.blocks;
       const float* ws0 = base + static_cast<int64_t>(min(EPI == kGated || !WIDE ? t.tile_m : 2 * t.tile_m, last)) * p.blocks;
@@ -775,6 +791,7 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
         fetch(i0 + kBatch);
         if (++slot == kBatches) slot = 0, slot_par ^= 1;
       }
+      t = next;
     }
   } else {
     // a token a thread; WIDE: 32 weight rows of each CTA, else 32 of the CTA `part`
@@ -783,8 +800,9 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
     int slot = set, batch = 0;
     uint32_t slot_par = 0, batch_par = 0;
     bool ready = false;
+    PairTile t(p, GROUPED, max(min(pair, total - 1), 0));
     for (int tile = pair; tile < total; tile += pairs) {
-      const PairTile t(p, GROUPED, tile);
+      const PairTile next(p, GROUPED, min(tile + pairs, total - 1));
       const int token = t.n0 + rank * kBlock + quarter * 32 + lane, blocks = p.blocks;
 #pragma unroll
       for (int c = 0; c < 32; ++c) acc[c] = 0.0f, other[c] = WIDE ? 0.0f : -0.0f;
@@ -873,6 +891,7 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
         }
       }
       __syncwarp();
+      t = next;
     }
   }
   fence_before_sync();
@@ -947,41 +966,55 @@ __global__ void __launch_bounds__(kOrderThreads) expert_order_kernel(const int32
 }
 
 // out[t] = the sum over the token's choices, in their order, of weight times result: parts [rows][ldp], rows 16-byte aligned, by `place` [n][top] (-1:
-// no expert, no term), weights [top][n]. Four features a thread (VEC: so is the result), the choices' loads together.
+// no expert, no term), weights [top][n]. Twice four features a thread (VEC: the result takes them together), the loads of several choices under way.
 template <class OUT, bool VEC>
 __global__ void __launch_bounds__(128) expert_combine_kernel(const float* parts, int64_t ldp, const int32_t* place, const float* weights, int n, int top, int W,
                                                              OUT* out, int64_t ldo) {
   sb::grid_launch_dependents();
   sb::grid_dependency_wait();
-  const int t = blockIdx.x, m = (blockIdx.y * blockDim.x + threadIdx.x) * 4;
-  if (m >= W) return;
+  const int t = blockIdx.x, m0 = (blockIdx.y * 2 * blockDim.x + threadIdx.x) * 4;
   const int32_t* mine = place + static_cast<int64_t>(t) * top;
-  float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-  constexpr int kTogether = 8;
+  float sum[2][4] = {};
+  constexpr int kTogether = 4;
   for (int k0 = 0; k0 < top; k0 += kTogether) {
-    float4 v[kTogether];
+    float4 v[kTogether][2];
     float w[kTogether];
     int row[kTogether];
 #pragma unroll
     for (int k = 0; k < kTogether; ++k) {
       row[k] = k0 + k < top ? mine[k0 + k] : -1;
-      if (row[k] >= 0) w[k] = weights[static_cast<int64_t>(k0 + k) * n + t], v[k] = *reinterpret_cast<const float4*>(parts + row[k] * ldp + m);
+      w[k] = k0 + k < top ? weights[static_cast<int64_t>(k0 + k) * n + t] : 0.0f;
     }
 #pragma unroll
     for (int k = 0; k < kTogether; ++k)
-      if (row[k] >= 0) sum[0] = fmaf(w[k], v[k].x, sum[0]), sum[1] = fmaf(w[k], v[k].y, sum[1]), sum[2] = fmaf(w[k], v[k].z, sum[2]), sum[3] = fmaf(w[k], v[k].w, sum[3]);
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        if (row[k] >= 0 && m0 + h * 512 < W) v[k][h] = *reinterpret_cast<const float4*>(parts + row[k] * ldp + m0 + h * 512);
+#pragma unroll
+    for (int k = 0; k < kTogether; ++k)
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        if (row[k] >= 0 && m0 + h * 512 < W) {
+          sum[h][0] = fmaf(w[k], v[k][h].x, sum[h][0]), sum[h][1] = fmaf(w[k], v[k][h].y, sum[h][1]);
+          sum[h][2] = fmaf(w[k], v[k][h].z, sum[h][2]), sum[h][3] = fmaf(w[k], v[k][h].w, sum[h][3]);
+        }
   }
-  OUT* to = out + static_cast<int64_t>(t) * ldo + m;
-  if (VEC && m + 4 <= W) {
-    alignas(16) OUT r[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) r[i] = sb::narrow<OUT>(sum[i]);
-    if (sizeof(OUT) == 4) *reinterpret_cast<uint4*>(to) = *reinterpret_cast<const uint4*>(r);
-    else *reinterpret_cast<uint2*>(to) = *reinterpret_cast<const uint2*>(r);
-  } else {
+  for (int h = 0; h < 2; ++h) {
+    const int m = m0 + h * 512;
+    if (m >= W) break;
+    OUT* to = out + static_cast<int64_t>(t) * ldo + m;
+    if (VEC && m + 4 <= W) {
+      alignas(16) OUT r[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (m + i < W) to[i] = sb::narrow<OUT>(sum[i]);
+      for (int i = 0; i < 4; ++i) r[i] = sb::narrow<OUT>(sum[h][i]);
+      if (sizeof(OUT) == 4) *reinterpret_cast<uint4*>(to) = *reinterpret_cast<const uint4*>(r);
+      else *reinterpret_cast<uint2*>(to) = *reinterpret_cast<const uint2*>(r);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (m + i < W) to[i] = sb::narrow<OUT>(sum[h][i]);
+    }
   }
 }
 
@@ -1024,8 +1057,9 @@ int launch_tile(const void* w, int64_t rows_w, int64_t ldw, const void* q, int64
   const dim3 grid(tiles_m, tiles_n, split ? p.ranges : 1);
   // (few CTAs have an SM each: the longest ring then brings most of the weights on their way while the kernel in front still runs. Else two share
   // one where they can. Quantising: at least half as many stages as accumulators, see the kernel)
-  const int copies = quant ? quant_bytes(BN, p.x_f32) : 0;
   const bool alone = static_cast<long long>(tiles_m) * tiles_n * grid.z <= sb::sm_count();
+  p.quant_warps = p.x_f32 && !alone ? kQuantWarps / 2 : kQuantWarps;
+  const int copies = quant ? p.quant_warps * BN * kBlock * (p.x_f32 ? 4 : 2) : 0;
   const int room = (alone || S::kCtas == 1 ? kSmemBudget : quant ? 4 * S::kStage + copies : 100 * 1024) - copies;
   p.stages = std::min(kMaxStages, room / S::kStage);
   const size_t smem = static_cast<size_t>(p.stages) * S::kStage + copies + 1024;
@@ -1308,7 +1342,7 @@ SB_EXPORT int sb_experts_fp8(const SbFp8Experts* l, const void* x, int xdtype, i
   p.out = parts, p.ldo = s.ldp, p.x_scales = zs, p.w_scales = down_scales, p.M = W, p.K = F, p.half_rows = 0;
   p.blocks = p.range_blocks = (F + kBlock - 1) / kBlock, p.scale_rows = (W + kBlock - 1) / kBlock;
   if (int rc = launch_product<kStore, float, true>(down, static_cast<int64_t>(E) * W, ldd, base + s.zq, pairs, s.ldz, p, tile, tiles, st)) return rc;
-  const dim3 grid(n, (W + 511) / 512);
+  const dim3 grid(n, (W + 1023) / 1024);
   if (grid.y > 65535) return sb::fail("%s: %d features are too many", who, W);
   auto combine = [&](auto kernel, auto to) {
     sb::launch_pdl(kernel, grid, dim3(128), 0, st, static_cast<const float*>(parts), s.ldp, place, weights, n, top, W, to, ldo);
