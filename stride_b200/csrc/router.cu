@@ -54,18 +54,31 @@ __device__ __forceinline__ float exp_difference(float z, float top) {
   return fabsf(dropped) < 1.0f ? expf(d) * (1.0f + dropped) : expf(d);
 }
 
-// Scores s and c of this lane's experts, e = lane + 32 i; `open`: bit i, the expert may be chosen. T: float or double.
+// This lane's values of a row of E: places lane PER .. lane PER + PER - 1 (`other` beyond). VEC: the row begins at a 16-byte border.
+template <int PER, bool VEC>
+__device__ __forceinline__ void load_lane(const float* row, int E, int lane, float other, float* v) {
+  if (VEC && (lane + 1) * PER <= E) {
+#pragma unroll
+    for (int i = 0; i < PER; i += 4) {
+      const float4 a = *reinterpret_cast<const float4*>(row + lane * PER + i);
+      v[i] = a.x, v[i + 1] = a.y, v[i + 2] = a.z, v[i + 3] = a.w;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < PER; ++i) v[i] = lane * PER + i < E ? row[lane * PER + i] : other;
+  }
+}
+
+// Scores s and c of this lane's experts from its logits and biases; bit i of the result: the expert may be chosen. T: float or double.
 template <class T, int PER>
-__device__ __forceinline__ uint32_t scores(const Routing& r, const float* z, int lane, T* s, T* c) {
+__device__ __forceinline__ uint32_t scores(const Routing& r, const float* logits, const float* bias, T* s, T* c) {
   uint32_t open = 0;
   float v[PER];
-#pragma unroll
-  for (int i = 0; i < PER; ++i) v[i] = lane + 32 * i < r.E ? z[lane + 32 * i] : -INFINITY;
   float top = -INFINITY;
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
-    if (v[i] > -INFINITY) open |= 1u << i;              // (not NaN either)
-    v[i] = fminf(v[i], FLT_MAX);
+    if (logits[i] > -INFINITY) open |= 1u << i;              // (not NaN either)
+    v[i] = fminf(logits[i], FLT_MAX);
     if ((open >> i) & 1u) top = fmaxf(top, v[i]);
   }
   if (r.softmax) {
@@ -86,21 +99,14 @@ __device__ __forceinline__ uint32_t scores(const Routing& r, const float* z, int
   } else {
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-      s[i] = 0;
-      if ((open >> i) & 1u) {
-        if constexpr (sizeof(T) == 8) s[i] = 1.0 / (1.0 + exp(-static_cast<double>(v[i])));
-        else s[i] = __fdividef(1.0f, 1.0f + __expf(fminf(-v[i], 80.0f)));      // (to choose by; a chosen one's weight is computed anew)
-      }
+      if constexpr (sizeof(T) == 8) s[i] = (open >> i) & 1u ? 1.0 / (1.0 + exp(-static_cast<double>(v[i]))) : 0.0;
+      else s[i] = __fdividef(1.0f, 1.0f + __expf(fminf(-v[i], 80.0f)));      // (to choose by; a chosen one's weight is computed anew)
     }
   }
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
-    c[i] = s[i];
-    if (((open >> i) & 1u) && r.bias != nullptr) {
-      const float b = __ldg(r.bias + lane + 32 * i);
-      if (!(b > -INFINITY)) open &= ~(1u << i);
-      c[i] += static_cast<T>(b);
-    }
+    if (!(bias[i] > -INFINITY)) open &= ~(1u << i);
+    c[i] = s[i] + static_cast<T>(bias[i]);
   }
   return open;
 }
@@ -110,21 +116,31 @@ __device__ __forceinline__ uint32_t scores(const Routing& r, const float* z, int
 template <class T, int PER>
 __device__ __forceinline__ uint32_t keep_groups(const Routing& r, int lane, const T* c, uint32_t open, T* held, T& gap) {
   const int size = r.size;
-#pragma unroll
-  for (int i = 0; i < PER; ++i)
-    if (lane + 32 * i < r.E) held[lane + 32 * i] = (open >> i) & 1u ? c[i] : static_cast<T>(-INFINITY);
-  __syncwarp();
-  // the two largest of every group: `share` neighbouring lanes (a power of two) look through a group's experts by turns, then join
-  int share = 1;
-  while (2 * share * r.groups <= 32) share *= 2;
   T a = -INFINITY, b = -INFINITY;
-  const int g = lane / share;
-  if (g < r.groups) {
-    const T* from = held + g * size;
-    for (int j = lane % share; j < size; j += share) {
-      const T v = from[j];
+  int share = 1;              // neighbouring lanes that look through a group, a power of two
+  const bool whole = size % PER == 0 && (size / PER & (size / PER - 1)) == 0;        // a lane's experts are of one group, a group's lanes that many
+  if (whole) {
+    share = size / PER;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const T v = (open >> i) & 1u ? c[i] : static_cast<T>(-INFINITY);
       b = v > a ? a : (v > b ? v : b);
       a = v > a ? v : a;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
+      if (lane * PER + i < r.E) held[lane * PER + i] = (open >> i) & 1u ? c[i] : static_cast<T>(-INFINITY);
+    __syncwarp();
+    while (2 * share * r.groups <= 32) share *= 2;
+    const int g = lane / share;
+    if (g < r.groups) {
+      const T* from = held + g * size;
+      for (int j = lane % share; j < size; j += share) {
+        const T v = from[j];
+        b = v > a ? a : (v > b ? v : b);
+        a = v > a ? v : a;
+      }
     }
   }
   for (int o = 1; o < share; o <<= 1) {
@@ -148,9 +164,10 @@ __device__ __forceinline__ uint32_t keep_groups(const Routing& r, int lane, cons
   const T score = __shfl_sync(0xffffffffu, mine, __ffs(last) - 1);
   gap = next != 0 ? score - __shfl_sync(0xffffffffu, mine, __ffs(next) - 1) : static_cast<T>(INFINITY);
   if (score == static_cast<T>(-INFINITY)) gap = INFINITY;       // (groups with nothing in them: it does not matter which)
+  if (whole) return (kept >> (lane / share)) & 1u ? open : 0u;
 #pragma unroll
   for (int i = 0; i < PER; ++i)
-    if ((open >> i) & 1u && !((kept >> group_of(r, lane + 32 * i)) & 1u)) open &= ~(1u << i);
+    if ((open >> i) & 1u && !((kept >> group_of(r, lane * PER + i)) & 1u)) open &= ~(1u << i);
   return open;
 }
 
@@ -165,7 +182,11 @@ __device__ __forceinline__ void write_row(const Routing& r, int row, int lane, i
 template <int PER>
 __device__ __noinline__ void route_row_64(const Routing& r, int row, int lane, double* held) {
   double s[PER], c[PER], gap;
-  uint32_t open = scores<double, PER>(r, r.logits + row * r.ldz, lane, s, c);
+  float z[PER], bias[PER];
+  load_lane<PER, false>(r.logits + row * r.ldz, r.E, lane, -INFINITY, z);
+#pragma unroll
+  for (int i = 0; i < PER; ++i) bias[i] = r.bias != nullptr && lane * PER + i < r.E ? r.bias[lane * PER + i] : 0.0f;
+  uint32_t open = scores<double, PER>(r, z, bias, s, c);
   if (r.groups > 1) open = keep_groups<double, PER>(r, lane, c, open, held, gap);
   double sum = 0.0, kept_s = 0.0;
   int kept_e = -1;
@@ -174,7 +195,7 @@ __device__ __noinline__ void route_row_64(const Routing& r, int row, int lane, d
     int at = 0x7fffffff;
 #pragma unroll
     for (int i = 0; i < PER; ++i)
-      if (((open >> i) & 1u) && (at == 0x7fffffff || c[i] > best)) best = c[i], at = lane + 32 * i, score = s[i];
+      if (((open >> i) & 1u) && (at == 0x7fffffff || c[i] > best)) best = c[i], at = lane * PER + i, score = s[i];
     for (int o = 16; o > 0; o >>= 1) {
       const double ob = __shfl_xor_sync(0xffffffffu, best, o), os = __shfl_xor_sync(0xffffffffu, score, o);
       const int oa = __shfl_xor_sync(0xffffffffu, at, o);
@@ -183,7 +204,7 @@ __device__ __noinline__ void route_row_64(const Routing& r, int row, int lane, d
     if (at == 0x7fffffff) at = -1, score = 0.0;
 #pragma unroll
     for (int i = 0; i < PER; ++i)
-      if (at == lane + 32 * i) open &= ~(1u << i);
+      if (at == lane * PER + i) open &= ~(1u << i);
     sum += score;
     if (lane == k) kept_s = score, kept_e = at;      // (at most 32 choices)
   }
@@ -218,19 +239,10 @@ __device__ __forceinline__ void sort_descending(uint32_t* key, int* place) {
 // candidates that follow one another, or the last group that stays and the first that does not, are closer than twice that, the token is routed
 // again in 64-bit. So the choice is that of 64-bit scores always, at the price of 32-bit ones for nearly all tokens (16,384 tokens of 256 experts in
 // eight groups, everything in 64-bit: 87 us).
-constexpr int kWarps = 4;
 template <int PER>
-__global__ void __launch_bounds__(32 * kWarps) route_kernel(const Routing r) {
-  __shared__ double held_s[kWarps][32 * PER];       // (64-bit scores, or 32-bit sums with the bias in front of 32-bit scores)
-  sb::grid_launch_dependents();
-  sb::grid_dependency_wait();
-  const int row = blockIdx.x * kWarps + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-  if (row >= r.n) return;
-  double* held = held_s[threadIdx.x >> 5];
-  float* held_scores = reinterpret_cast<float*>(held) + 32 * PER;
-  const float* z = r.logits + row * r.ldz;
+__device__ __forceinline__ void route_row(const Routing& r, int row, int lane, const float* z, const float* bias, double* held, float* held_scores) {
   float s[PER], c[PER];
-  uint32_t open = scores<float, PER>(r, z, lane, s, c);
+  uint32_t open = scores<float, PER>(r, z, bias, s, c);
   float high_s = 0.0f, high_c = 0.0f;
 #pragma unroll
   for (int i = 0; i < PER; ++i)
@@ -250,7 +262,7 @@ __global__ void __launch_bounds__(32 * kWarps) route_kernel(const Routing r) {
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
     key[i] = (open >> i) & 1u ? order_key(c[i]) : 0u, place[i] = i;
-    if (r.softmax) held_scores[lane + 32 * i] = s[i];
+    held_scores[lane * PER + i] = r.softmax ? s[i] : z[i];
   }
   sort_descending<PER>(key, place);
   __syncwarp();
@@ -264,7 +276,7 @@ __global__ void __launch_bounds__(32 * kWarps) route_kernel(const Routing r) {
     sure = before - value > near;
     before = value;
     if (k == r.top) break;
-    const int e = owner + 32 * __shfl_sync(0xffffffffu, place[0], owner);
+    const int e = owner * PER + __shfl_sync(0xffffffffu, place[0], owner);
     if (lane == k) kept_e = e;                      // (at most 32 choices)
     if (lane == owner) {
 #pragma unroll
@@ -272,7 +284,7 @@ __global__ void __launch_bounds__(32 * kWarps) route_kernel(const Routing r) {
       key[PER - 1] = 0;
     }
   }
-  if (kept_e >= 0) kept_s = r.softmax ? held_scores[kept_e] : 1.0f / (1.0f + expf(-fminf(z[kept_e], FLT_MAX)));
+  if (kept_e >= 0) kept_s = r.softmax ? held_scores[kept_e] : 1.0f / (1.0f + expf(-fminf(held_scores[kept_e], FLT_MAX)));
   if (r.renormalise) sum = warp_sum(kept_s);
   if (r.renormalise && kept_e >= 0 && sum < 0x1p-50f) sure = false;      // (scores below the smallest floats count where all are)
   sure = __all_sync(0xffffffffu, sure);
@@ -281,6 +293,23 @@ __global__ void __launch_bounds__(32 * kWarps) route_kernel(const Routing r) {
     return route_row_64<PER>(r, row, lane, held);
   }
   write_row(r, row, lane, kept_e, r.renormalise ? kept_s * (r.scale / (sum + 1e-20f)) : kept_s * r.scale);
+}
+
+constexpr int kWarps = 4;
+template <int PER, bool VEC>
+__global__ void __launch_bounds__(32 * kWarps, PER <= 8 ? 8 : 1) route_kernel(const Routing r) {
+  __shared__ double held_s[kWarps][32 * PER];       // (64-bit scores, or 32-bit sums with the bias in front of 32-bit scores)
+  sb::grid_launch_dependents();
+  const int lane = threadIdx.x & 31, row = blockIdx.x * kWarps + (threadIdx.x >> 5);
+  sb::grid_dependency_wait();
+  if (row >= r.n) return;
+  double* held = held_s[threadIdx.x >> 5];
+  float bias[PER], z[PER];
+#pragma unroll
+  for (int i = 0; i < PER; ++i) bias[i] = 0.0f;
+  load_lane<PER, VEC>(r.logits + row * r.ldz, r.E, lane, -INFINITY, z);
+  if (r.bias != nullptr) load_lane<PER, VEC>(r.bias, r.E, lane, 0.0f, bias);
+  route_row<PER>(r, row, lane, z, bias, held, reinterpret_cast<float*>(held) + 32 * PER);
 }
 
 int launch(Routing r, cudaStream_t st) {
@@ -292,14 +321,15 @@ int launch(Routing r, cudaStream_t st) {
   if (r.top > r.top_groups * (r.E / r.groups)) return sb::fail("route_experts: %d experts of %d groups of %d", r.top, r.top_groups, r.E / r.groups);
   if (r.n == 0) return 0;
   r.size = r.E / r.groups, r.inverse_size = r.size == 1 ? 0u : static_cast<uint32_t>((0x100000000ull + r.size - 1) / r.size);
-  const dim3 grid((r.n + kWarps - 1) / kWarps), block(32 * kWarps);
   const int per = (r.E + 31) / 32;
-  if (per <= 1) sb::launch_pdl(route_kernel<1>, grid, block, 0, st, r);
-  else if (per <= 2) sb::launch_pdl(route_kernel<2>, grid, block, 0, st, r);
-  else if (per <= 4) sb::launch_pdl(route_kernel<4>, grid, block, 0, st, r);
-  else if (per <= 8) sb::launch_pdl(route_kernel<8>, grid, block, 0, st, r);
-  else if (per <= 16) sb::launch_pdl(route_kernel<16>, grid, block, 0, st, r);
-  else sb::launch_pdl(route_kernel<32>, grid, block, 0, st, r);
+  const dim3 grid((r.n + kWarps - 1) / kWarps), block(32 * kWarps);
+  const bool vec = r.ldz % 4 == 0 && ((reinterpret_cast<uintptr_t>(r.logits) | reinterpret_cast<uintptr_t>(r.bias)) & 15) == 0;
+  if (per <= 1) sb::launch_pdl(route_kernel<1, false>, grid, block, 0, st, r);
+  else if (per <= 2) sb::launch_pdl(route_kernel<2, false>, grid, block, 0, st, r);
+  else if (per <= 4) vec ? sb::launch_pdl(route_kernel<4, true>, grid, block, 0, st, r) : sb::launch_pdl(route_kernel<4, false>, grid, block, 0, st, r);
+  else if (per <= 8) vec ? sb::launch_pdl(route_kernel<8, true>, grid, block, 0, st, r) : sb::launch_pdl(route_kernel<8, false>, grid, block, 0, st, r);
+  else if (per <= 16) vec ? sb::launch_pdl(route_kernel<16, true>, grid, block, 0, st, r) : sb::launch_pdl(route_kernel<16, false>, grid, block, 0, st, r);
+  else vec ? sb::launch_pdl(route_kernel<32, true>, grid, block, 0, st, r) : sb::launch_pdl(route_kernel<32, false>, grid, block, 0, st, r);
   return sb::check_launch("route_experts");
 }
 
