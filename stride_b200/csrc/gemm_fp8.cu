@@ -125,6 +125,7 @@ struct Fp8Params {
   int half_rows;
   int scale_rows;            // blocks of rows of one expert's scales
   int ranges, range_blocks;  // K ranges and blocks of columns in each
+  int split;                 // the ranges run on CTAs of their own
   int stages;
   int tiles_m, tiles_n, vec_out;      // (the kernel on pairs; vec_out: the result takes 16-byte stores)
   const int32_t* tiles;      // experts: the list of `expert_order_kernel`; else null
@@ -903,6 +904,264 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
   }
 }
 
+// The same for more tokens than a few and fewer than many, with tokens as the product's rows too (a thread of the epilogue holds one token's sums and
+// needs one factor a block; with weight rows as the product's rows, a factor from shared memory for every four sums, a block of 128 tokens took
+// twice as long): up to 128 tokens (BOX: how many are loaded; the rows behind them multiply whatever lies there, nobody reads them) by 128
+// weight rows, or 64 gate rows and their 64 up rows. SPLIT: the K ranges are the CTAs of a cluster. Warp 0 loads, warp 1 issues the
+// products, warp 2 multiplies the scales, sixteen warps are the epilogue, a token a lane and 32 columns each; those without tokens pass over.
+constexpr int kTokenThreads = 640, kTokenRows = 128, kTokenSlots = 4;
+constexpr int kRowPitch = 132;                   // floats from a token's sums to the next one's: 16-byte pieces of eight tokens meet in no bank
+template <int BOX>
+struct TokenShape {
+  static constexpr int kStage = BOX * 128 + kStageA;
+  static constexpr int kStages = BOX == 64 ? 8 : 6;
+};
+
+template <int EPI, class OUT, bool GROUPED, bool SPLIT, int BOX>
+__global__ void __launch_bounds__(kTokenThreads, 1)
+gemm_fp8_token_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const Fp8Params p) {
+  using S = TokenShape<BOX>;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  __shared__ __align__(8) uint64_t full_bar[S::kStages], empty_bar[S::kStages];
+  __shared__ __align__(8) uint64_t accum_full[kTokenSlots], accum_empty[kTokenSlots];
+  __shared__ __align__(8) uint64_t factor_full[kBatches], factor_empty[kBatches];
+  __shared__ float factor[kBatches][kBatch][EPI == kGated ? 2 : 1][kTokenRows];
+  __shared__ uint32_t tmem_base_s;
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t smem0 = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  uint8_t* smem0_p = smem_raw + (smem0 - smem_u32(smem_raw));
+  const int tile_m = blockIdx.x;
+  const int b0 = SPLIT ? blockIdx.z * p.range_blocks : 0;
+  const int iters = (SPLIT ? min(p.blocks, b0 + p.range_blocks) : p.blocks) - b0;
+
+  if (warp == 1) tmem_alloc(smem_u32(&tmem_base_s), 512);
+  __syncthreads();
+  sb::grid_launch_dependents();        // (behind the allocation, as above)
+  int expert = 0, n0 = blockIdx.y * BOX, end = p.n;
+  bool empty = false;
+  if (GROUPED) {
+    sb::grid_dependency_wait();        // whose rows this tile holds is an earlier kernel's result
+    empty = static_cast<int>(blockIdx.y) >= p.tiles[0];
+    if (!empty) expert = p.tiles[2 + 3 * blockIdx.y], n0 = p.tiles[3 + 3 * blockIdx.y], end = p.tiles[4 + 3 * blockIdx.y];
+  }
+  const int count = min(end - n0, BOX), quarters = (count + 31) / 32;        // the tile's tokens, and the lanes' quarters that have some
+  if (threadIdx.x == 0) {
+    prefetch_tensormap(&map_w);
+    prefetch_tensormap(&map_x);
+    for (int s = 0; s < S::kStages; ++s) mbar_init(smem_u32(&full_bar[s]), 1), mbar_init(smem_u32(&empty_bar[s]), 1);
+    for (int s = 0; s < kTokenSlots; ++s) mbar_init(smem_u32(&accum_full[s]), 1), mbar_init(smem_u32(&accum_empty[s]), max(4 * quarters, 1));
+    for (int s = 0; s < kBatches; ++s) mbar_init(smem_u32(&factor_full[s]), 32), mbar_init(smem_u32(&factor_empty[s]), max(4 * quarters, 1));
+    mbar_init_fence();
+  }
+  fence_before_sync();
+  __syncthreads();
+  fence_after_sync();
+  const uint32_t tmem_base = tmem_base_s;
+  float* sums = reinterpret_cast<float*>(smem0_p);
+
+  if (empty) {
+  } else if (warp == 0) {
+    const int row_w = expert * p.M + tile_m * (EPI == kGated ? 64 : kBlock);
+    auto load_w = [&](int i, int st) {
+      const uint32_t bar = smem_u32(&full_bar[st]), to = smem0 + st * S::kStage + BOX * 128;
+      issue_expect(bar, S::kStage);
+      issue_load<false>(to, &map_w, bar, (b0 + i) * kBlock, row_w);
+      if (EPI == kGated) issue_load<false>(to + kStageA / 2, &map_w, bar, (b0 + i) * kBlock, row_w + p.half_rows);
+    };
+    auto load_x = [&](int i, int st) { issue_load<false>(smem0 + st * S::kStage, &map_x, smem_u32(&full_bar[st]), (b0 + i) * kBlock, n0); };
+    // (the weights are nobody's result: the first ring of them is under way before the kernels in front have ended)
+    const int ahead = min(iters, S::kStages);
+    for (int i = 0; i < ahead; ++i) load_w(i, i);
+    if (!GROUPED) sb::grid_dependency_wait();
+    for (int i = 0; i < ahead; ++i) load_x(i, i);
+    int st = ahead == S::kStages ? 0 : ahead;
+    uint32_t par = 0;
+    for (int i = ahead; i < iters; ++i) {
+      mbar_wait(smem_u32(&empty_bar[st]), par, p.status, 61);
+      __syncwarp();
+      load_w(i, st);
+      load_x(i, st);
+      if (++st == S::kStages) st = 0, par ^= 1;
+    }
+  } else if (warp == 1) {
+    const uint32_t idesc = instr_desc_e4m3(kBlock);
+    const uint64_t first = smem_desc_sw128(smem0);
+    int st = 0, slot = 0;
+    uint32_t par = 0, slot_par = 1;
+    bool ready = false;
+    for (int i = 0; i < iters; ++i) {
+      if (!__all_sync(0xffffffffu, ready)) {
+        mbar_wait(smem_u32(&accum_empty[slot]), slot_par, p.status, 62);
+        mbar_wait(smem_u32(&full_bar[st]), par, p.status, 63);
+        __syncwarp();
+      }
+      fence_after_sync();
+      const uint64_t da = first + static_cast<uint64_t>(st * (S::kStage >> 4));
+      issue_products<false>(tmem_base + slot * kBlock, da, da + (BOX * 128 >> 4), idesc);
+      issue_signal<false>(smem_u32(&empty_bar[st]));
+      issue_signal<false>(smem_u32(&accum_full[slot]));
+      if (++st == S::kStages) st = 0, par ^= 1;
+      if (++slot == kTokenSlots) slot = 0, slot_par ^= 1;
+      ready = mbar_over(smem_u32(&accum_empty[slot]), slot_par) && mbar_over(smem_u32(&full_bar[st]), par);
+    }
+  } else if (warp == 2) {
+    // the scales' products, four tokens a lane, a batch ahead of those that wait in shared memory
+    const float* ws0 = p.w_scales + static_cast<int64_t>(expert * p.scale_rows + (EPI == kGated ? tile_m / 2 : tile_m)) * p.blocks + b0;
+    const float* ws1 = ws0 + static_cast<int64_t>(EPI == kGated ? p.scale_rows / 2 : 0) * p.blocks;
+    const float* xs = p.x_scales + b0 * p.ldxs + n0 + lane;
+    if (!GROUPED) sb::grid_dependency_wait();
+    float x[kBatch][4], w0[kBatch], w1[kBatch];
+    auto fetch = [&](int i0) {
+#pragma unroll
+      for (int a = 0; a < kBatch; ++a) {
+        const int i = i0 + a;
+        const bool there = i < iters;
+        w0[a] = there ? __ldg(ws0 + i) : 0.0f, w1[a] = EPI == kGated && there ? __ldg(ws1 + i) : 0.0f;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) x[a][c] = there && lane + 32 * c < count ? xs[i * p.ldxs + 32 * c] : 0.0f;
+      }
+    };
+    fetch(0);
+    int slot = 0;
+    uint32_t slot_par = 1;
+    for (int i0 = 0; i0 < iters; i0 += kBatch) {
+      mbar_wait(smem_u32(&factor_empty[slot]), slot_par, p.status, 64);
+#pragma unroll
+      for (int a = 0; a < kBatch; ++a)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          factor[slot][a][0][lane + 32 * c] = x[a][c] * w0[a];
+          if (EPI == kGated) factor[slot][a][EPI == kGated ? 1 : 0][lane + 32 * c] = x[a][c] * w1[a];
+        }
+      mbar_arrive(smem_u32(&factor_full[slot]));
+      fetch(i0 + kBatch);
+      if (++slot == kBatches) slot = 0, slot_par ^= 1;
+    }
+  } else if (warp >= 4 && (warp & 3) < quarters) {
+    const int quarter = warp & 3, part = (warp - 4) >> 2, token = quarter * 32 + lane;
+    float acc[32], total[SPLIT ? 1 : 32];
+#pragma unroll
+    for (int c = 0; c < 32; ++c) acc[c] = 0.0f;
+    if (!SPLIT) {
+#pragma unroll
+      for (int c = 0; c < 32; ++c) total[c] = -0.0f;          // (the first range is added to nothing: -0 + v = v, signs of zeros too)
+    }
+    int slot = 0, batch = 0, left = p.range_blocks;
+    uint32_t slot_par = 0, batch_par = 0;
+    bool ready = false;
+#pragma unroll 1
+    for (int i = 0, in_batch = 0; i < iters; ++i) {
+      if (in_batch == 0) mbar_wait(smem_u32(&factor_full[batch]), batch_par, p.status, 66);
+      const float f = factor[batch][in_batch][EPI == kGated && part >= 2 ? 1 : 0][token];
+      if (!__all_sync(0xffffffffu, ready)) mbar_wait(smem_u32(&accum_full[slot]), slot_par, p.status, 65);
+      __syncwarp();
+      fence_after_sync();
+      const uint32_t from = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + slot * kBlock + part * 32;
+      constexpr int kChunk = SPLIT ? 32 : 16;          // (the totals leave fewer registers)
+      uint32_t v[kChunk];
+#pragma unroll
+      for (int c0 = 0; c0 < 32; c0 += kChunk) {
+        if (kChunk == 32) tmem_load32_nowait(from, v), tmem_arrived32(v);
+        else tmem_load16_nowait(from + c0, v), tmem_arrived16(v);
+        if (c0 + kChunk == 32) {
+          fence_before_sync();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(smem_u32(&accum_empty[slot]));
+          if (++slot == kTokenSlots) slot = 0, slot_par ^= 1;
+          ready = mbar_over(smem_u32(&accum_full[slot]), slot_par);
+        }
+        add_scaled<kChunk>(acc + c0, v, f);
+      }
+      if (++in_batch == kBatch || i + 1 == iters) {
+        in_batch = 0;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&factor_empty[batch]));
+        if (++batch == kBatches) batch = 0, batch_par ^= 1;
+      }
+      if (!SPLIT && (--left == 0 || i + 1 == iters)) {
+        left = p.range_blocks;
+#pragma unroll
+        for (int c = 0; c < 32; ++c) total[c] += acc[c], acc[c] = 0.0f;
+      }
+    }
+    // the sums to shared memory, a row a token: every load has arrived and every product that reads the ring is done
+    const float* done = SPLIT ? acc : total;
+#pragma unroll
+    for (int c = 0; c < 32; c += 4)
+      *reinterpret_cast<float4*>(sums + token * kRowPitch + part * 32 + c) = make_float4(done[c], done[c + 1], done[c + 2], done[c + 3]);
+  }
+  __syncwarp();
+  if (SPLIT) sb::cluster_sync();
+  else __syncthreads();
+  if (!empty && warp >= 4 && *reinterpret_cast<volatile int*>(p.status) == 0) {      // (a wait that gave up has left no sums)
+    if (!GROUPED) sb::grid_dependency_wait();
+    const int rank = SPLIT ? static_cast<int>(sb::cluster_rank()) : 0, ranges = SPLIT ? p.ranges : 1;
+    constexpr int kPer = EPI == kGated ? 2 : 4;                  // features of a lane
+    const int m = tile_m * (EPI == kGated ? 64 : kBlock) + lane * kPer, M = EPI == kGated ? p.half_rows : p.M;
+    for (int t = rank + ranges * (warp - 4); t < count; t += ranges * 16) {
+      float v[kPer], u[EPI == kGated ? 2 : 1];
+      const uint32_t here = smem0 + (t * kRowPitch + lane * kPer) * 4;
+      for (int r = 0; r < ranges; ++r) {
+        float a[kPer], b[2] = {0.0f, 0.0f};
+        if (SPLIT) {
+          uint32_t peer;
+          asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(peer) : "r"(here), "r"(r));
+#pragma unroll
+          for (int i = 0; i < kPer; i += 2) {
+            const float2 x = sb::cluster_load_float2(peer + 4 * i);
+            a[i] = x.x, a[i + 1] = x.y;
+          }
+          if (EPI == kGated) {
+            const float2 x = sb::cluster_load_float2(peer + 64 * 4);
+            b[0] = x.x, b[1] = x.y;
+          }
+        } else {
+          const float* at = sums + t * kRowPitch + lane * kPer;
+#pragma unroll
+          for (int i = 0; i < kPer; ++i) a[i] = at[i];
+          if (EPI == kGated) b[0] = at[64], b[1] = at[65];
+        }
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) v[i] = r == 0 ? a[i] : v[i] + a[i];
+        if (EPI == kGated) {
+#pragma unroll
+          for (int i = 0; i < 2; ++i) u[EPI == kGated ? i : 0] = r == 0 ? b[i] : u[EPI == kGated ? i : 0] + b[i];
+        }
+      }
+      if (EPI == kGated) {
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) v[i] = gated_product(v[i], u[EPI == kGated ? i : 0], p.gate);
+      }
+      OUT* o = static_cast<OUT*>(p.out) + static_cast<int64_t>(n0 + t) * p.ldo + m;
+      if (p.vec_out && m + kPer <= M) {
+        struct alignas(kPer * sizeof(OUT)) Piece {
+          OUT e[kPer];
+        } piece;
+        if (EPI == kAdd) {
+          piece = *reinterpret_cast<const Piece*>(o);
+#pragma unroll
+          for (int i = 0; i < kPer; ++i) v[i] += sb::widen(piece.e[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) piece.e[i] = sb::narrow<OUT>(v[i]);
+        *reinterpret_cast<Piece*>(o) = piece;
+      } else {
+#pragma unroll
+        for (int i = 0; i < kPer; ++i)
+          if (m + i < M) o[i] = sb::narrow<OUT>(EPI == kAdd ? v[i] + sb::widen(o[i]) : v[i]);
+      }
+    }
+  }
+  if (SPLIT) sb::cluster_sync();       // (nobody leaves while another reads its sums)
+  fence_before_sync();
+  __syncthreads();
+  if (warp == 1) {
+    fence_after_sync();
+    tmem_dealloc(tmem_base, 512);
+  }
+}
+
 // ------------------------------------------------------------------ experts
 // choice [n][top] -> the choices' tokens in expert order, the row of every choice (place [n][top]; -1: none), and the row tiles of the
 // products. An id outside [0, E) is no expert: it is left out. list: [0] tiles, [1] rows, then (expert, first row, end row) of every tile.
@@ -1036,8 +1295,6 @@ int fp8_ranges(int tiles, int blocks) {
   return (blocks + (blocks + s - 1) / s - 1) / ((blocks + s - 1) / s);        // (no empty range)
 }
 
-// Up to this many tokens the ranges run on CTAs of their own.
-constexpr int kSplitTokens = 128;
 // Up to this many rows of a tile the product can quantise its input itself. Of a dense product it does where a CTA has few blocks of columns: that
 // saves a launch, but a block takes longer (2,048 x 2,048 of one token 7.7 us with a launch, 4.6 without; 16,384 x 2,048, 16 blocks a CTA, of eight
 // 10.1 and 12.1). The experts' two inputs would need two launches.
@@ -1053,7 +1310,7 @@ int launch_tile(const void* w, int64_t rows_w, int64_t ldw, const void* q, int64
   if (!byte_map(w, rows_w, p.K, ldw, EPI == kGated ? 64 : kBlock, &map_w) || (!quant && !byte_map(q, rows_q, p.K, ldq, BN, &map_x)))
     return sb::fail("gemm_fp8: no tensor map for a weight of %lld x %d (stride %lld)", (long long)rows_w, p.K, (long long)ldw);
   if (quant) map_x = map_w;                  // (not read)
-  const bool split = !GROUPED && p.ranges > 1 && p.n <= kSplitTokens;
+  const bool split = !GROUPED && p.split;
   const dim3 grid(tiles_m, tiles_n, split ? p.ranges : 1);
   // (few CTAs have an SM each: the longest ring then brings most of the weights on their way while the kernel in front still runs. Else two share
   // one where they can. Quantising: at least half as many stages as accumulators, see the kernel)
@@ -1085,6 +1342,33 @@ int launch_tile(const void* w, int64_t rows_w, int64_t ldw, const void* q, int64
     if (split) return run(gemm_fp8_kernel<EPI, BN, OUT, GROUPED, true, false>, once[2]);
   }
   return run(gemm_fp8_kernel<EPI, BN, OUT, GROUPED, false, false>, once[3]);
+}
+
+template <int EPI, class OUT, bool GROUPED, int BOX>
+int launch_token(const void* w, int64_t rows_w, int64_t ldw, const void* q, int64_t rows_q, int64_t ldq, Fp8Params p, int tiles_m, int tiles_n, cudaStream_t st) {
+  using S = TokenShape<BOX>;
+  CUtensorMap map_w, map_x;
+  if (!byte_map(w, rows_w, p.K, ldw, EPI == kGated ? 64 : kBlock, &map_w) || !byte_map(q, rows_q, p.K, ldq, BOX, &map_x))
+    return sb::fail("gemm_fp8: no tensor map for a weight of %lld x %d (stride %lld)", (long long)rows_w, p.K, (long long)ldw);
+  const int piece = (EPI == kGated ? 2 : 4) * static_cast<int>(sizeof(OUT));
+  p.vec_out = p.ldo * sizeof(OUT) % piece == 0 && (reinterpret_cast<uintptr_t>(p.out) & (piece - 1)) == 0;
+  const size_t smem = static_cast<size_t>(S::kStages) * S::kStage + 1024;
+  const bool split = !GROUPED && p.split;
+  const dim3 grid(tiles_m, tiles_n, split ? p.ranges : 1);
+  static sb::DeviceOnce once[2];
+  auto run = [&](auto kernel, sb::DeviceOnce& first) {
+    if (first.needed()) {
+      if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)) != cudaSuccess) return sb::check_launch("gemm_fp8");
+      first.done();
+    }
+    if (split) sb::launch_pdl_cluster(kernel, grid, dim3(kTokenThreads), smem, st, dim3(1, 1, p.ranges), map_w, map_x, p);
+    else sb::launch_pdl(kernel, grid, dim3(kTokenThreads), smem, st, map_w, map_x, p);
+    return sb::check_launch("gemm_fp8");
+  };
+  if constexpr (!GROUPED) {
+    if (split) return run(gemm_fp8_token_kernel<EPI, OUT, false, true, BOX>, once[0]);
+  }
+  return run(gemm_fp8_token_kernel<EPI, OUT, GROUPED, false, BOX>, once[1]);
 }
 
 template <int EPI, bool WIDE, class OUT, bool GROUPED>
@@ -1122,7 +1406,7 @@ int launch_product(const void* w, int64_t rows_w, int64_t ldw, const void* q, in
     case 16: return launch_tile<EPI, 16, OUT, GROUPED>(w, rows_w, ldw, q, rows_q, ldq, p, tiles_m, tiles_n, st);
     case 32: return launch_tile<EPI, 32, OUT, GROUPED>(w, rows_w, ldw, q, rows_q, ldq, p, tiles_m, tiles_n, st);
     case 64: return launch_tile<EPI, 64, OUT, GROUPED>(w, rows_w, ldw, q, rows_q, ldq, p, tiles_m, tiles_n, st);
-    default: return launch_tile<EPI, 128, OUT, GROUPED>(w, rows_w, ldw, q, rows_q, ldq, p, tiles_m, tiles_n, st);
+    default: return launch_token<EPI, OUT, GROUPED, 128>(w, rows_w, ldw, q, rows_q, ldq, p, tiles_m, tiles_n, st);
   }
 }
 
@@ -1141,10 +1425,24 @@ int launch_quantize(const void* x, int xdtype, int64_t ldx, const int32_t* used,
   return vec ? run(quantize_kernel<bf16, true>, static_cast<const bf16*>(x)) : run(quantize_kernel<bf16, false>, static_cast<const bf16*>(x));
 }
 
-// Tokens of a tile of the product.
-int token_tile(const Fp8Params& p, int epilogue) {
+// Tokens of a tile of the product; sets whether its K ranges run on CTAs of their own. Up to 128 tokens they do, more are for pairs of CTAs (gated
+// with ranges, whose sums and totals would not fit a pair's registers: for single ones), unless a weight of several ranges has so few tiles that
+// most pairs had none: then whichever takes fewer rounds of the SMs, a block of columns costing a pair some 0.43 us and a CTA of a
+// cluster 0.6, a round's beginning and end 5 and 3.5 ([4096, 14336] of 256 tokens: 49.7 us on pairs, 39.0 on clusters; [4096, 4096] 18.8 and 24.1;
+// [6144, 4096] of 333 32.8 and 26.1).
+int token_tile(Fp8Params& p, int epilogue) {
+  p.split = p.ranges > 1;
   if (p.n <= 64) return p.n <= 16 ? 16 : p.n <= 32 ? 32 : 64;
-  return p.n <= kSplitTokens || (epilogue == kGated && p.ranges > 1) ? 128 : kPairTokens;
+  if (p.n <= kTokenRows) return kTokenRows;
+  const bool gated = epilogue == kGated;
+  if (p.split && !gated) {
+    const long long sms = sb::sm_count(), tiles = (p.M + kBlock - 1) / kBlock;
+    const long long pair_rounds = (tiles * ((p.n + kPairTokens - 1) / kPairTokens) + sms / 2 - 1) / (sms / 2);
+    const long long split_rounds = (tiles * ((p.n + kTokenRows - 1) / kTokenRows) * p.ranges + sms - 1) / sms;
+    if (split_rounds * (60 * p.range_blocks + 350) < pair_rounds * 43 * p.blocks + 500) return kTokenRows;
+  }
+  p.split = 0;
+  return gated && p.ranges > 1 ? kTokenRows : kPairTokens;
 }
 
 // The input as it is, for the forms that quantise it themselves: they copy 16 bytes at a time.
