@@ -127,7 +127,7 @@ struct Fp8Params {
   int ranges, range_blocks;  // K ranges and blocks of columns in each
   int split;                 // the ranges run on CTAs of their own
   int stages;
-  int tiles_m, tiles_n, vec_out;      // (the kernel on pairs; vec_out: the result takes 16-byte stores)
+  int tiles_m, tiles_n, vec_out;      // (kernels that walk tiles; vec_out: the result takes 16-byte stores)
   const int32_t* tiles;      // experts: the list of `expert_order_kernel`; else null
   const int32_t* order;      // experts: row -> token
   float* z_scales;           // experts, gated products quantised by the epilogue: [blocks of features][ldxs]
@@ -601,13 +601,18 @@ constexpr int kBatch = 4, kBatches = 3;          // blocks whose factors are han
 // A block's product is issued as two chains, each with half of both CTAs' weight rows (of a gated product: a feature's gate row and its up row
 // in the same chain) and accumulators of its own, and the epilogue's warps as two sets, one a chain: a set's way from one accumulator to the
 // next (signals, first loads) then falls into the other's additions. (All sixteen warps on one accumulator at a time: 526 us.)
-template <bool WIDE>
+//
+// PAIR false (experts, whose rows rarely fill 256): one CTA with the pair's weight rows and 128 tokens, 48 KB a block for the same 512 cycles. The
+// weight rows lie in shared memory as the pair's CTAs would have them, 64 of the first chain's each, then the second's.
+template <bool WIDE, bool PAIR>
 struct PairShape {
   static constexpr int kRows = WIDE ? 256 : 128;             // weight rows of a tile
   static constexpr int kColumns = kRows / 2;                 // of a chain
-  static constexpr int kStage = kStageA + kRows / 2 * 128;
+  static constexpr int kTokens = PAIR ? 256 : 128;
+  static constexpr int kStage = kStageA + (PAIR ? kRows / 2 : kRows) * 128;
+  static constexpr int kChainB = (PAIR ? kColumns / 2 : kColumns) * 128;      // bytes from one chain's weight rows to the other's
   static constexpr int kSlots = 512 / kColumns;              // accumulators under way, all of tensor memory; even ones are the first chain's
-  static constexpr int kStages = WIDE ? 5 : 6;
+  __host__ __device__ static constexpr int stages(bool staged) { return !PAIR ? (staged ? 3 : 4) : WIDE ? 5 : 6; }
 };
 
 // The tiles of a launch in the order in which the pairs walk them. Dense: the tiles of tokens first, so that the pairs of a round share few weight
@@ -668,14 +673,15 @@ __device__ __forceinline__ void store_rows(OUT* out, int64_t ldo, int64_t first,
   }
 }
 
-template <int EPI, bool WIDE, class OUT, bool GROUPED>
+template <int EPI, bool WIDE, class OUT, bool GROUPED, bool PAIR>
 __global__ void __launch_bounds__(kPairThreads, 1)
 gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const Fp8Params p) {
-  using S = PairShape<WIDE>;
+  using S = PairShape<WIDE, PAIR>;
   constexpr bool kQuantised = std::is_same<OUT, uint8_t>::value;       // the gated products leave as e4m3 with scales of their own
+  constexpr int kStages = S::stages(!kQuantised);
   extern __shared__ __align__(1024) uint8_t smem_raw[];
-  __shared__ __align__(8) uint64_t full_bar[S::kStages];      // used in the leader: both CTAs' tiles have landed
-  __shared__ __align__(8) uint64_t empty_bar[S::kStages];     // in each CTA: the products that read its stage are done
+  __shared__ __align__(8) uint64_t full_bar[kStages];      // used in the leader: both CTAs' tiles have landed
+  __shared__ __align__(8) uint64_t empty_bar[kStages];     // in each CTA: the products that read its stage are done
   __shared__ __align__(8) uint64_t accum_full[S::kSlots];     // in each CTA
   __shared__ __align__(8) uint64_t accum_empty[S::kSlots];    // used in the leader: both CTAs have taken an accumulator's sums
   __shared__ __align__(8) uint64_t factor_full[kBatches], factor_empty[kBatches];      // in each CTA, its own
@@ -684,25 +690,28 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
   __shared__ uint32_t tmem_base_s;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int rank = static_cast<int>(sb::cluster_rank());
+  const int rank = PAIR ? static_cast<int>(sb::cluster_rank()) : 0;
   const uint32_t smem0 = (smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* smem0_p = smem_raw + (smem0 - smem_u32(smem_raw));
-  const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+  const int pair = PAIR ? blockIdx.x >> 1 : blockIdx.x, pairs = PAIR ? gridDim.x >> 1 : gridDim.x;
   if (threadIdx.x == 0) {
     prefetch_tensormap(&map_w);
     prefetch_tensormap(&map_x);
-    for (int s = 0; s < S::kStages; ++s) mbar_init(smem_u32(&full_bar[s]), 1), mbar_init(smem_u32(&empty_bar[s]), 2);      // (both chains')
+    for (int s = 0; s < kStages; ++s) mbar_init(smem_u32(&full_bar[s]), 1), mbar_init(smem_u32(&empty_bar[s]), 2);      // (both chains')
     for (int s = 0; s < S::kSlots; ++s) {
       mbar_init(smem_u32(&accum_full[s]), 1);
-      mbar_init(smem_u32(&accum_empty[s]), 2 * 8);       // one arrival a warp of either CTA's set
+      mbar_init(smem_u32(&accum_empty[s]), PAIR ? 2 * 8 : 8);       // one arrival a warp of either CTA's set
     }
     for (int s = 0; s < kBatches; ++s) mbar_init(smem_u32(&factor_full[s]), 32), mbar_init(smem_u32(&factor_empty[s]), 16);
     mbar_init_fence();
   }
-  if (warp == 1) tmem_alloc_pair(smem_u32(&tmem_base_s), 512);
+  if (warp == 1) {
+    if (PAIR) tmem_alloc_pair(smem_u32(&tmem_base_s), 512);
+    else tmem_alloc(smem_u32(&tmem_base_s), 512);
+  }
   fence_before_sync();
   __syncthreads();
-  sb::cluster_sync();          // the peer's barriers exist before anything signals them
+  if (PAIR) sb::cluster_sync();          // the peer's barriers exist before anything signals them
   fence_after_sync();
   const uint32_t tmem_base = tmem_base_s;
   sb::grid_launch_dependents();
@@ -721,10 +730,16 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
         mbar_wait(smem_u32(&empty_bar[st]), par, p.status, 51);
         __syncwarp();
         const uint32_t bar = smem_u32(&full_bar[st]), a = smem0 + st * S::kStage;
-        if (rank == 0) issue_expect(bar, 2 * S::kStage);
-        issue_load<true>(a, &map_x, bar, i * kBlock, token);
-        issue_load<true>(a + kStageA, &map_w, bar, i * kBlock, row);
-        if (++st == S::kStages) st = 0, par ^= 1;
+        if (rank == 0) issue_expect(bar, (PAIR ? 2 : 1) * S::kStage);
+        issue_load<PAIR>(a, &map_x, bar, i * kBlock, token);
+        issue_load<PAIR>(a + kStageA, &map_w, bar, i * kBlock, row);
+        if (!PAIR) {           // (boxes of 64 rows: the first chain's of the first and of the second half, then the second chain's)
+          const int second = row + (EPI == kGated ? p.half_rows : kBlock);
+          issue_load<false>(a + kStageA + 64 * 128, &map_w, bar, i * kBlock, second);
+          issue_load<false>(a + kStageA + 128 * 128, &map_w, bar, i * kBlock, row + 64);
+          issue_load<false>(a + kStageA + 192 * 128, &map_w, bar, i * kBlock, second + 64);
+        }
+        if (++st == kStages) st = 0, par ^= 1;
       }
       t = next;
     }
@@ -732,7 +747,7 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
     if (rank == 0) {
       const int chain = warp - 1;
       const uint64_t first = smem_desc_sw128(smem0);
-      const uint32_t idesc = (1u << 4) | (static_cast<uint32_t>(S::kColumns >> 3) << 17) | (static_cast<uint32_t>(256 >> 4) << 24);
+      const uint32_t idesc = (1u << 4) | (static_cast<uint32_t>(S::kColumns >> 3) << 17) | (static_cast<uint32_t>(S::kTokens >> 4) << 24);
       int st = 0, slot = chain;
       uint32_t par = 0, slot_par = 1;
       bool ready = false;
@@ -745,10 +760,10 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
           }
           fence_after_sync();
           const uint64_t da = first + static_cast<uint64_t>(st * (S::kStage >> 4));
-          issue_products<true>(tmem_base + slot * S::kColumns, da, da + (kStageA >> 4) + chain * (S::kColumns / 2 * 128 >> 4), idesc);
-          issue_signal<true>(smem_u32(&empty_bar[st]));
-          issue_signal<true>(smem_u32(&accum_full[slot]));
-          if (++st == S::kStages) st = 0, par ^= 1;
+          issue_products<PAIR>(tmem_base + slot * S::kColumns, da, da + (kStageA >> 4) + chain * (S::kChainB >> 4), idesc);
+          issue_signal<PAIR>(smem_u32(&empty_bar[st]));
+          issue_signal<PAIR>(smem_u32(&accum_full[slot]));
+          if (++st == kStages) st = 0, par ^= 1;
           if ((slot += 2) >= S::kSlots) slot = chain, slot_par ^= 1;
           if (!WIDE) ready = mbar_over(smem_u32(&accum_empty[slot]), slot_par) && mbar_over(smem_u32(&full_bar[st]), par);
         }
@@ -825,7 +840,10 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
           if (c0 + 16 == (WIDE ? 64 : 32)) {         // (the last of them: the accumulator is free)
             fence_before_sync();
             __syncwarp();
-            if (lane == 0) mbar_arrive_leader(smem_u32(&accum_empty[slot]));
+            if (lane == 0) {
+              if (PAIR) mbar_arrive_leader(smem_u32(&accum_empty[slot]));
+              else mbar_arrive(smem_u32(&accum_empty[slot]));
+            }
             if ((slot += 2) >= S::kSlots) slot = set, slot_par ^= 1;
             if (!WIDE) ready = mbar_over(smem_u32(&accum_full[slot]), slot_par);       // (WIDE: two accumulators a set, the next is never there yet)
           }
@@ -881,7 +899,7 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
         }
       } else if (__all_sync(0xffffffffu, ok)) {
         OUT* out = static_cast<OUT*>(p.out);
-        uint8_t* staged = smem0_p + S::kStages * S::kStage + (warp - 4) * 32 * kPitch;
+        uint8_t* staged = smem0_p + kStages * S::kStage + (warp - 4) * 32 * kPitch;
         const int first = token - lane, count = min(t.end - first, 32);
         if (EPI == kGated) {
           store_rows<kStore>(out, p.ldo, first, count, t.tile_m * kBlock + set * 64 + part * 32, p.half_rows, p.vec_out, acc, staged, lane);
@@ -897,32 +915,28 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
   }
   fence_before_sync();
   __syncthreads();
-  sb::cluster_sync();          // neither CTA frees the pair's tensor memory, or leaves, while the other still works
+  if (PAIR) sb::cluster_sync();          // neither CTA frees the pair's tensor memory, or leaves, while the other still works
   if (warp == 1) {
     fence_after_sync();
-    tmem_dealloc_pair(tmem_base, 512);
+    if (PAIR) tmem_dealloc_pair(tmem_base, 512);
+    else tmem_dealloc(tmem_base, 512);
   }
 }
 
 // The same for more tokens than a few and fewer than many, with tokens as the product's rows too (a thread of the epilogue holds one token's sums and
 // needs one factor a block; with weight rows as the product's rows, a factor from shared memory for every four sums, a block of 128 tokens took
-// twice as long): up to 128 tokens (BOX: how many are loaded; the rows behind them multiply whatever lies there, nobody reads them) by 128
+// twice as long): up to 128 tokens by 128
 // weight rows, or 64 gate rows and their 64 up rows. SPLIT: the K ranges are the CTAs of a cluster. Warp 0 loads, warp 1 issues the
 // products, warp 2 multiplies the scales, sixteen warps are the epilogue, a token a lane and 32 columns each; those without tokens pass over.
 constexpr int kTokenThreads = 640, kTokenRows = 128, kTokenSlots = 4;
 constexpr int kRowPitch = 132;                   // floats from a token's sums to the next one's: 16-byte pieces of eight tokens meet in no bank
-template <int BOX>
-struct TokenShape {
-  static constexpr int kStage = BOX * 128 + kStageA;
-  static constexpr int kStages = BOX == 64 ? 8 : 6;
-};
+constexpr int kTokenStage = 2 * kStageA, kTokenStages = 6;
 
-template <int EPI, class OUT, bool GROUPED, bool SPLIT, int BOX>
+template <int EPI, class OUT, bool SPLIT>
 __global__ void __launch_bounds__(kTokenThreads, 1)
 gemm_fp8_token_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const Fp8Params p) {
-  using S = TokenShape<BOX>;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
-  __shared__ __align__(8) uint64_t full_bar[S::kStages], empty_bar[S::kStages];
+  __shared__ __align__(8) uint64_t full_bar[kTokenStages], empty_bar[kTokenStages];
   __shared__ __align__(8) uint64_t accum_full[kTokenSlots], accum_empty[kTokenSlots];
   __shared__ __align__(8) uint64_t factor_full[kBatches], factor_empty[kBatches];
   __shared__ float factor[kBatches][kBatch][EPI == kGated ? 2 : 1][kTokenRows];
@@ -938,20 +952,14 @@ gemm_fp8_token_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_co
   if (warp == 1) tmem_alloc(smem_u32(&tmem_base_s), 512);
   __syncthreads();
   sb::grid_launch_dependents();        // (behind the allocation, as above)
-  int expert = 0, n0 = blockIdx.y * BOX, end = p.n;
-  bool empty = false;
-  if (GROUPED) {
-    sb::grid_dependency_wait();        // whose rows this tile holds is an earlier kernel's result
-    empty = static_cast<int>(blockIdx.y) >= p.tiles[0];
-    if (!empty) expert = p.tiles[2 + 3 * blockIdx.y], n0 = p.tiles[3 + 3 * blockIdx.y], end = p.tiles[4 + 3 * blockIdx.y];
-  }
-  const int count = min(end - n0, BOX), quarters = (count + 31) / 32;        // the tile's tokens, and the lanes' quarters that have some
+  const int n0 = blockIdx.y * kTokenRows;
+  const int count = min(p.n - n0, kTokenRows), quarters = (count + 31) / 32;        // the tile's tokens, and the lanes' quarters that have some
   if (threadIdx.x == 0) {
     prefetch_tensormap(&map_w);
     prefetch_tensormap(&map_x);
-    for (int s = 0; s < S::kStages; ++s) mbar_init(smem_u32(&full_bar[s]), 1), mbar_init(smem_u32(&empty_bar[s]), 1);
-    for (int s = 0; s < kTokenSlots; ++s) mbar_init(smem_u32(&accum_full[s]), 1), mbar_init(smem_u32(&accum_empty[s]), max(4 * quarters, 1));
-    for (int s = 0; s < kBatches; ++s) mbar_init(smem_u32(&factor_full[s]), 32), mbar_init(smem_u32(&factor_empty[s]), max(4 * quarters, 1));
+    for (int s = 0; s < kTokenStages; ++s) mbar_init(smem_u32(&full_bar[s]), 1), mbar_init(smem_u32(&empty_bar[s]), 1);
+    for (int s = 0; s < kTokenSlots; ++s) mbar_init(smem_u32(&accum_full[s]), 1), mbar_init(smem_u32(&accum_empty[s]), 4 * quarters);
+    for (int s = 0; s < kBatches; ++s) mbar_init(smem_u32(&factor_full[s]), 32), mbar_init(smem_u32(&factor_empty[s]), 4 * quarters);
     mbar_init_fence();
   }
   fence_before_sync();
@@ -960,29 +968,28 @@ gemm_fp8_token_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_co
   const uint32_t tmem_base = tmem_base_s;
   float* sums = reinterpret_cast<float*>(smem0_p);
 
-  if (empty) {
-  } else if (warp == 0) {
-    const int row_w = expert * p.M + tile_m * (EPI == kGated ? 64 : kBlock);
+  if (warp == 0) {
+    const int row_w = tile_m * (EPI == kGated ? 64 : kBlock);
     auto load_w = [&](int i, int st) {
-      const uint32_t bar = smem_u32(&full_bar[st]), to = smem0 + st * S::kStage + BOX * 128;
-      issue_expect(bar, S::kStage);
+      const uint32_t bar = smem_u32(&full_bar[st]), to = smem0 + st * kTokenStage + kStageA;
+      issue_expect(bar, kTokenStage);
       issue_load<false>(to, &map_w, bar, (b0 + i) * kBlock, row_w);
       if (EPI == kGated) issue_load<false>(to + kStageA / 2, &map_w, bar, (b0 + i) * kBlock, row_w + p.half_rows);
     };
-    auto load_x = [&](int i, int st) { issue_load<false>(smem0 + st * S::kStage, &map_x, smem_u32(&full_bar[st]), (b0 + i) * kBlock, n0); };
+    auto load_x = [&](int i, int st) { issue_load<false>(smem0 + st * kTokenStage, &map_x, smem_u32(&full_bar[st]), (b0 + i) * kBlock, n0); };
     // (the weights are nobody's result: the first ring of them is under way before the kernels in front have ended)
-    const int ahead = min(iters, S::kStages);
+    const int ahead = min(iters, kTokenStages);
     for (int i = 0; i < ahead; ++i) load_w(i, i);
-    if (!GROUPED) sb::grid_dependency_wait();
+    sb::grid_dependency_wait();
     for (int i = 0; i < ahead; ++i) load_x(i, i);
-    int st = ahead == S::kStages ? 0 : ahead;
+    int st = ahead == kTokenStages ? 0 : ahead;
     uint32_t par = 0;
     for (int i = ahead; i < iters; ++i) {
       mbar_wait(smem_u32(&empty_bar[st]), par, p.status, 61);
       __syncwarp();
       load_w(i, st);
       load_x(i, st);
-      if (++st == S::kStages) st = 0, par ^= 1;
+      if (++st == kTokenStages) st = 0, par ^= 1;
     }
   } else if (warp == 1) {
     const uint32_t idesc = instr_desc_e4m3(kBlock);
@@ -997,20 +1004,20 @@ gemm_fp8_token_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_co
         __syncwarp();
       }
       fence_after_sync();
-      const uint64_t da = first + static_cast<uint64_t>(st * (S::kStage >> 4));
-      issue_products<false>(tmem_base + slot * kBlock, da, da + (BOX * 128 >> 4), idesc);
+      const uint64_t da = first + static_cast<uint64_t>(st * (kTokenStage >> 4));
+      issue_products<false>(tmem_base + slot * kBlock, da, da + (kStageA >> 4), idesc);
       issue_signal<false>(smem_u32(&empty_bar[st]));
       issue_signal<false>(smem_u32(&accum_full[slot]));
-      if (++st == S::kStages) st = 0, par ^= 1;
+      if (++st == kTokenStages) st = 0, par ^= 1;
       if (++slot == kTokenSlots) slot = 0, slot_par ^= 1;
       ready = mbar_over(smem_u32(&accum_empty[slot]), slot_par) && mbar_over(smem_u32(&full_bar[st]), par);
     }
   } else if (warp == 2) {
     // the scales' products, four tokens a lane, a batch ahead of those that wait in shared memory
-    const float* ws0 = p.w_scales + static_cast<int64_t>(expert * p.scale_rows + (EPI == kGated ? tile_m / 2 : tile_m)) * p.blocks + b0;
+    const float* ws0 = p.w_scales + static_cast<int64_t>(EPI == kGated ? tile_m / 2 : tile_m) * p.blocks + b0;
     const float* ws1 = ws0 + static_cast<int64_t>(EPI == kGated ? p.scale_rows / 2 : 0) * p.blocks;
     const float* xs = p.x_scales + b0 * p.ldxs + n0 + lane;
-    if (!GROUPED) sb::grid_dependency_wait();
+    sb::grid_dependency_wait();
     float x[kBatch][4], w0[kBatch], w1[kBatch];
     auto fetch = [&](int i0) {
 #pragma unroll
@@ -1094,8 +1101,8 @@ gemm_fp8_token_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_co
   __syncwarp();
   if (SPLIT) sb::cluster_sync();
   else __syncthreads();
-  if (!empty && warp >= 4 && *reinterpret_cast<volatile int*>(p.status) == 0) {      // (a wait that gave up has left no sums)
-    if (!GROUPED) sb::grid_dependency_wait();
+  if (warp >= 4 && *reinterpret_cast<volatile int*>(p.status) == 0) {      // (a wait that gave up has left no sums)
+    sb::grid_dependency_wait();
     const int rank = SPLIT ? static_cast<int>(sb::cluster_rank()) : 0, ranges = SPLIT ? p.ranges : 1;
     constexpr int kPer = EPI == kGated ? 2 : 4;                  // features of a lane
     const int m = tile_m * (EPI == kGated ? 64 : kBlock) + lane * kPer, M = EPI == kGated ? p.half_rows : p.M;
@@ -1344,16 +1351,15 @@ int launch_tile(const void* w, int64_t rows_w, int64_t ldw, const void* q, int64
   return run(gemm_fp8_kernel<EPI, BN, OUT, GROUPED, false, false>, once[3]);
 }
 
-template <int EPI, class OUT, bool GROUPED, int BOX>
+template <int EPI, class OUT>
 int launch_token(const void* w, int64_t rows_w, int64_t ldw, const void* q, int64_t rows_q, int64_t ldq, Fp8Params p, int tiles_m, int tiles_n, cudaStream_t st) {
-  using S = TokenShape<BOX>;
   CUtensorMap map_w, map_x;
-  if (!byte_map(w, rows_w, p.K, ldw, EPI == kGated ? 64 : kBlock, &map_w) || !byte_map(q, rows_q, p.K, ldq, BOX, &map_x))
+  if (!byte_map(w, rows_w, p.K, ldw, EPI == kGated ? 64 : kBlock, &map_w) || !byte_map(q, rows_q, p.K, ldq, kTokenRows, &map_x))
     return sb::fail("gemm_fp8: no tensor map for a weight of %lld x %d (stride %lld)", (long long)rows_w, p.K, (long long)ldw);
   const int piece = (EPI == kGated ? 2 : 4) * static_cast<int>(sizeof(OUT));
   p.vec_out = p.ldo * sizeof(OUT) % piece == 0 && (reinterpret_cast<uintptr_t>(p.out) & (piece - 1)) == 0;
-  const size_t smem = static_cast<size_t>(S::kStages) * S::kStage + 1024;
-  const bool split = !GROUPED && p.split;
+  const size_t smem = static_cast<size_t>(kTokenStages) * kTokenStage + 1024;
+  const bool split = p.split != 0;
   const dim3 grid(tiles_m, tiles_n, split ? p.ranges : 1);
   static sb::DeviceOnce once[2];
   auto run = [&](auto kernel, sb::DeviceOnce& first) {
@@ -1365,32 +1371,31 @@ int launch_token(const void* w, int64_t rows_w, int64_t ldw, const void* q, int6
     else sb::launch_pdl(kernel, grid, dim3(kTokenThreads), smem, st, map_w, map_x, p);
     return sb::check_launch("gemm_fp8");
   };
-  if constexpr (!GROUPED) {
-    if (split) return run(gemm_fp8_token_kernel<EPI, OUT, false, true, BOX>, once[0]);
-  }
-  return run(gemm_fp8_token_kernel<EPI, OUT, GROUPED, false, BOX>, once[1]);
+  return split ? run(gemm_fp8_token_kernel<EPI, OUT, true>, once[0]) : run(gemm_fp8_token_kernel<EPI, OUT, false>, once[1]);
 }
 
-template <int EPI, bool WIDE, class OUT, bool GROUPED>
+template <int EPI, bool WIDE, class OUT, bool GROUPED, bool PAIR>
 int launch_pair(const void* w, int64_t rows_w, int64_t ldw, const void* q, int64_t rows_q, int64_t ldq, Fp8Params p, int tiles_n, cudaStream_t st) {
-  using S = PairShape<WIDE>;
+  using S = PairShape<WIDE, PAIR>;
   CUtensorMap map_w, map_x;
-  if (!byte_map(w, rows_w, p.K, ldw, S::kRows / 2, &map_w) || !byte_map(q, rows_q, p.K, ldq, kBlock, &map_x))
+  if (!byte_map(w, rows_w, p.K, ldw, PAIR ? S::kRows / 2 : 64, &map_w) || !byte_map(q, rows_q, p.K, ldq, kBlock, &map_x))
     return sb::fail("gemm_fp8: no tensor map for a weight of %lld x %d (stride %lld)", (long long)rows_w, p.K, (long long)ldw);
   p.tiles_m = EPI == kGated ? (p.half_rows + kBlock - 1) / kBlock : (p.M + S::kRows - 1) / S::kRows;
   p.tiles_n = tiles_n;
   p.vec_out = p.ldo * sizeof(OUT) % 16 == 0 && (reinterpret_cast<uintptr_t>(p.out) & 15) == 0;
   const long long tiles = static_cast<long long>(p.tiles_m) * tiles_n;
   if (tiles > (1ll << 30)) return sb::fail("gemm_fp8: too many tiles");
-  auto kernel = gemm_fp8_pair_kernel<EPI, WIDE, OUT, GROUPED>;
-  const size_t smem = static_cast<size_t>(S::kStages) * S::kStage + (std::is_same<OUT, uint8_t>::value ? 0 : kStaged) + 1024;
+  auto kernel = gemm_fp8_pair_kernel<EPI, WIDE, OUT, GROUPED, PAIR>;
+  constexpr bool kThrough = !std::is_same<OUT, uint8_t>::value;          // results pass through shared memory
+  const size_t smem = static_cast<size_t>(S::stages(kThrough)) * S::kStage + (kThrough ? kStaged : 0) + 1024;
   static sb::DeviceOnce once;
   if (once.needed()) {
     if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)) != cudaSuccess) return sb::check_launch("gemm_fp8");
     once.done();
   }
-  const int pairs = static_cast<int>(std::min<long long>(tiles, sb::sm_count() / 2));
-  sb::launch_pdl_cluster(kernel, dim3(2 * pairs), dim3(kPairThreads), smem, st, dim3(2, 1, 1), map_w, map_x, p);
+  const int units = static_cast<int>(std::min<long long>(tiles, PAIR ? sb::sm_count() / 2 : sb::sm_count()));
+  if (PAIR) sb::launch_pdl_cluster(kernel, dim3(2 * units), dim3(kPairThreads), smem, st, dim3(2, 1, 1), map_w, map_x, p);
+  else sb::launch_pdl(kernel, dim3(units), dim3(kPairThreads), smem, st, map_w, map_x, p);
   return sb::check_launch("gemm_fp8");
 }
 
@@ -1398,16 +1403,17 @@ template <int EPI, class OUT, bool GROUPED>
 int launch_product(const void* w, int64_t rows_w, int64_t ldw, const void* q, int64_t rows_q, int64_t ldq, const Fp8Params& p, int tile_n, int tiles_n,
                    cudaStream_t st) {
   const int tiles_m = EPI == kGated ? (p.half_rows + 63) / 64 : (p.M + kBlock - 1) / kBlock;
-  if (tile_n == kPairTokens && !(GROUPED && EPI == kGated)) {
-    if (p.ranges == 1) return launch_pair<EPI, true, OUT, GROUPED>(w, rows_w, ldw, q, rows_q, ldq, p, tiles_n, st);
-    if constexpr (EPI != kGated && !GROUPED) return launch_pair<EPI, false, OUT, GROUPED>(w, rows_w, ldw, q, rows_q, ldq, p, tiles_n, st);
-  }
   switch (tile_n) {
     case 16: return launch_tile<EPI, 16, OUT, GROUPED>(w, rows_w, ldw, q, rows_q, ldq, p, tiles_m, tiles_n, st);
     case 32: return launch_tile<EPI, 32, OUT, GROUPED>(w, rows_w, ldw, q, rows_q, ldq, p, tiles_m, tiles_n, st);
     case 64: return launch_tile<EPI, 64, OUT, GROUPED>(w, rows_w, ldw, q, rows_q, ldq, p, tiles_m, tiles_n, st);
-    default: return launch_token<EPI, OUT, GROUPED, 128>(w, rows_w, ldw, q, rows_q, ldq, p, tiles_m, tiles_n, st);
   }
+  if constexpr (!GROUPED) {
+    if (tile_n == kTokenRows) return launch_token<EPI, OUT>(w, rows_w, ldw, q, rows_q, ldq, p, tiles_m, tiles_n, st);
+    if (p.ranges == 1) return launch_pair<EPI, true, OUT, false, true>(w, rows_w, ldw, q, rows_q, ldq, p, tiles_n, st);
+    if constexpr (EPI != kGated) return launch_pair<EPI, false, OUT, false, true>(w, rows_w, ldw, q, rows_q, ldq, p, tiles_n, st);
+  }
+  return sb::fail("gemm_fp8: no form for tiles of %d tokens", tile_n);
 }
 
 int launch_quantize(const void* x, int xdtype, int64_t ldx, const int32_t* used, const int32_t* place, int copies, int n, int K, void* q, int64_t ldq,
@@ -1498,7 +1504,7 @@ int check_product(const char* who, const void* w, int64_t ldw, int out_dtype, in
 // Rows of a tile of the experts' products: near the rows an expert gets on average (a row's result does not depend on it).
 int expert_tile(int pairs, int E) {
   const int mean = (pairs + E - 1) / E;
-  return mean <= 16 ? 16 : mean <= 32 ? 32 : mean <= 64 ? 64 : mean <= 128 ? 128 : kPairTokens;
+  return mean <= 16 ? 16 : mean <= 32 ? 32 : mean <= 64 ? 64 : mean <= 512 ? kTokenRows : kPairTokens;
 }
 int most_tiles(int pairs, int E, int tile) { return std::min(pairs, pairs / tile + std::min(pairs, E)); }
 
@@ -1629,17 +1635,24 @@ SB_EXPORT int sb_experts_fp8(const SbFp8Experts* l, const void* x, int xdtype, i
   p.tiles = list, p.order = order, p.status = status, p.n = n, p.ranges = 1;
   p.out = z, p.ldo = s.ldz, p.x_scales = xs, p.ldxs = pairs, p.w_scales = gate_up_scales, p.M = 2 * F, p.K = W, p.half_rows = F;
   p.blocks = p.range_blocks = (W + kBlock - 1) / kBlock, p.scale_rows = 2 * ((F + kBlock - 1) / kBlock);
-  if (tile == kPairTokens) {         // (the pairs' epilogue quantises the gated products itself)
+  const int64_t rows_g = static_cast<int64_t>(E) * 2 * F, rows_d = static_cast<int64_t>(E) * W;
+  const bool walks = tile >= kTokenRows;          // (kernels that walk tiles quantise the gated products themselves)
+  if (walks) {
     p.out = base + s.zq, p.ldo = s.ldz, p.z_scales = zs;
-    if (int rc = launch_pair<kGated, true, uint8_t, true>(gate_up, static_cast<int64_t>(E) * 2 * F, ldg, base + s.xq, pairs, s.ldx, p, tiles, st)) return rc;
+    if (int rc = tile == kPairTokens ? launch_pair<kGated, true, uint8_t, true, true>(gate_up, rows_g, ldg, base + s.xq, pairs, s.ldx, p, tiles, st)
+                                     : launch_pair<kGated, true, uint8_t, true, false>(gate_up, rows_g, ldg, base + s.xq, pairs, s.ldx, p, tiles, st))
+      return rc;
   } else {
-    if (int rc = launch_product<kGated, float, true>(gate_up, static_cast<int64_t>(E) * 2 * F, ldg, base + s.xq, pairs, s.ldx, p, tile, tiles, st)) return rc;
+    if (int rc = launch_product<kGated, float, true>(gate_up, rows_g, ldg, base + s.xq, pairs, s.ldx, p, tile, tiles, st)) return rc;
     if (quant) set_input(p, z, 0, s.ldz), p.x_gathered = 0;
     else if (int rc = launch_quantize(z, 0, s.ldz, list + 1, nullptr, 1, pairs, F, base + s.zq, s.ldz, zs, pairs, st)) return rc;
   }
   p.out = parts, p.ldo = s.ldp, p.x_scales = zs, p.w_scales = down_scales, p.M = W, p.K = F, p.half_rows = 0;
   p.blocks = p.range_blocks = (F + kBlock - 1) / kBlock, p.scale_rows = (W + kBlock - 1) / kBlock;
-  if (int rc = launch_product<kStore, float, true>(down, static_cast<int64_t>(E) * W, ldd, base + s.zq, pairs, s.ldz, p, tile, tiles, st)) return rc;
+  if (int rc = !walks                ? launch_product<kStore, float, true>(down, rows_d, ldd, base + s.zq, pairs, s.ldz, p, tile, tiles, st)
+               : tile == kPairTokens ? launch_pair<kStore, true, float, true, true>(down, rows_d, ldd, base + s.zq, pairs, s.ldz, p, tiles, st)
+                                     : launch_pair<kStore, true, float, true, false>(down, rows_d, ldd, base + s.zq, pairs, s.ldz, p, tiles, st))
+    return rc;
   const dim3 grid(n, (W + 1023) / 1024);
   if (grid.y > 65535) return sb::fail("%s: %d features are too many", who, W);
   auto combine = [&](auto kernel, auto to) {
