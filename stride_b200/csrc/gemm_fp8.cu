@@ -6,15 +6,21 @@
 // same however it is computed (a scale a / 448 uses up to one more bit of the largest elements' range, but rounds the quotient twice). A block
 // with an infinity or a NaN gets the scale NaN, so the token's whole result is NaN.
 //
-// `gemm_fp8_kernel`: y[t, m] = sum over blocks b of columns of s[t, b] w_s[m / 128, b] (sum of q w over the block). The inner sum runs on the
-// tensor cores (tcgen05.mma kind::f8f6f4, float32 accumulators, 128 weight rows by BN tokens): every block of 128 columns, one row of the
-// 128-byte swizzle, is a fresh accumulator in tensor memory, of which there is a ring; the epilogue's warps take it from there and add it,
-// times its two scales, to the tile's sum in registers, one fused multiply-add an element, in 32 bits. The scales' products s w_s come
-// from two warps of their own through shared memory.
+// The product: y[t, m] = sum over blocks b of columns of s[t, b] w_s[m / 128, b] (sum of q w over the block). The inner sum runs on the tensor cores
+// (tcgen05.mma kind::f8f6f4, float32 accumulators): every block of 128 columns, one row of the 128-byte swizzle, is a fresh accumulator in
+// tensor memory, of which there is a ring; the epilogue's warps take it from there and add it, times its two scales, to the tile's sum in
+// registers, one fused multiply-add an element, in 32 bits. That addition is what bounds large products (one multiply-add an element and
+// block beside 128 products on the tensor cores: 4,096 tokens through 28,672 gate and up rows of 4,096 470 to 530 us, with the clock, 2.0
+// PFLOP/s at best; without it, as a trial, 348), the weights' bytes the small ones.
 //
 // K is cut into ranges, a function of the weight's shape alone (`fp8_ranges`): few weight tiles leave SMs without work. The sum of a range
 // starts from zero, the ranges are added in ascending order. With few tokens the ranges are the CTAs of a cluster, which add up through
-// distributed shared memory; with many one CTA walks them all. So a token's bits depend neither on the step it is part of nor on the tile.
+// distributed shared memory; with many one CTA walks them all. So a token's bits depend neither on the step it is part of nor on the tile,
+// nor on which of the forms made them:
+//   `gemm_fp8_kernel`        up to 64 tokens: 128 weight rows by 16, 32 or 64 tokens; of 16 it may quantise its input itself
+//   `gemm_fp8_token_kernel`  up to 128, and more where that takes fewer rounds: tokens are the product's rows
+//   `gemm_fp8_pair_kernel`   many, and the experts': tokens are the product's rows, CTAs or pairs of CTAs walk the tiles
+// An expert's products are those of a tile of its rows (`expert_order_kernel` sorts the choices by expert).
 #include <algorithm>
 #include <type_traits>
 
@@ -74,16 +80,15 @@ __device__ __forceinline__ void load8(const T* from, int k, int K, float* v) {
 }
 
 // x [n][ldx] -> q bytes [rows][ldq], scales [ceil(K / 128)][lds]. Sixteen lanes take a block of 128 columns of a row, a warp two blocks; the CTA's
-// warps take neighbouring rows, whose scales lie side by side. used (or null): how many of the n rows there are. place (or null): a row is
-// stored `copies` times, as rows place[row copies + i] (left out where that is negative).
+// warps take neighbouring rows, whose scales lie side by side. place (or null): a row is stored `copies` times, as rows place[row copies + i] (left out where that is negative).
 template <class T, bool VEC>
-__global__ void __launch_bounds__(256) quantize_kernel(const T* x, int64_t ldx, const int32_t* used, const int32_t* place,
+__global__ void __launch_bounds__(256) quantize_kernel(const T* x, int64_t ldx, const int32_t* place,
                                                        int copies, int n, int K, int blocks, uint8_t* q, int64_t ldq,
                                                        float* scales, int64_t lds) {
   sb::grid_launch_dependents();
   sb::grid_dependency_wait();
   const int row = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31, b = blockIdx.y * 2 + (lane >> 4), k = b * kBlock + (lane & 15) * 8;
-  if (row >= n || (used != nullptr && row >= *used)) return;
+  if (row >= n) return;
   float v[8];
   load8<T, VEC>(x + static_cast<int64_t>(row) * ldx + k, k, K, v);
   uint32_t amax = 0;               // (the bit patterns of |x| are ordered as the values are, infinity and NaN above them)
@@ -594,16 +599,18 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
 // for every four sums, the gated product of 4,096 tokens, 2 x 14,336 rows of 4,096, took 870 us.) WIDE: 256 weight rows a tile, or 128 gate rows
 // and their 128 up rows: each CTA loads 128 of them and 128 tokens, 32 KB a block for 512 cycles of the tensor cores. A weight with several K
 // ranges needs its totals beside the sums in registers and has 128 rows a tile.
-constexpr int kPairTokens = 256;
-constexpr int kPairThreads = 640;                // a warp that loads, two that issue the products, one for the scales, sixteen of the epilogue
-constexpr int kBatch = 4, kBatches = 3;          // blocks whose factors are handed over together; batches under way
 //
 // A block's product is issued as two chains, each with half of both CTAs' weight rows (of a gated product: a feature's gate row and its up row
 // in the same chain) and accumulators of its own, and the epilogue's warps as two sets, one a chain: a set's way from one accumulator to the
-// next (signals, first loads) then falls into the other's additions. (All sixteen warps on one accumulator at a time: 526 us.)
+// next (signals, first loads) then falls into the other's additions. Each chain has a warp that issues it: one for both took longer than the
+// tensor cores (574 us, with a warp each 524, at the time).
 //
-// PAIR false (experts, whose rows rarely fill 256): one CTA with the pair's weight rows and 128 tokens, 48 KB a block for the same 512 cycles. The
-// weight rows lie in shared memory as the pair's CTAs would have them, 64 of the first chain's each, then the second's.
+// PAIR false (experts, whose rows rarely fill 256, and dense products that need fewer rounds so): one CTA with the pair's weight rows and 128
+// tokens, 48 KB a block for the same 512 cycles (2,000 tokens through 64 experts, six each: 280 us on pairs, 238 so). The weight rows lie in
+// shared memory as the pair's CTAs would have them, 64 of the first chain's each, then the second's.
+constexpr int kPairTokens = 256;
+constexpr int kPairThreads = 640;                // a warp that loads, two that issue the products, one for the scales, sixteen of the epilogue
+constexpr int kBatch = 4, kBatches = 3;          // blocks whose factors are handed over together; batches under way
 template <bool WIDE, bool PAIR>
 struct PairShape {
   static constexpr int kRows = WIDE ? 256 : 128;             // weight rows of a tile
@@ -619,14 +626,14 @@ struct PairShape {
 // rows and every tile of tokens (which stay in L2); experts: the weight tiles of a tile of rows first.
 struct PairTile {
   int tile_m, expert, n0, end;
-  __device__ __forceinline__ PairTile(const Fp8Params& p, bool grouped, int tile) {
+  __device__ __forceinline__ PairTile(const Fp8Params& p, bool grouped, int tile, int tokens) {
     if (grouped) {
       const int t = tile / p.tiles_m;
       tile_m = tile - t * p.tiles_m;
       expert = p.tiles[2 + 3 * t], n0 = p.tiles[3 + 3 * t], end = p.tiles[4 + 3 * t];
     } else {
       tile_m = tile / p.tiles_n;
-      expert = 0, n0 = (tile - tile_m * p.tiles_n) * kPairTokens, end = p.n;
+      expert = 0, n0 = (tile - tile_m * p.tiles_n) * tokens, end = p.n;
     }
   }
 };
@@ -721,9 +728,9 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
   if (warp == 0) {
     int st = 0;
     uint32_t par = 1;
-    PairTile t(p, GROUPED, max(min(pair, total - 1), 0));
+    PairTile t(p, GROUPED, max(min(pair, total - 1), 0), S::kTokens);
     for (int tile = pair; tile < total; tile += pairs) {
-      const PairTile next(p, GROUPED, min(tile + pairs, total - 1));        // (on its way while this one is loaded)
+      const PairTile next(p, GROUPED, min(tile + pairs, total - 1), S::kTokens);        // (on its way while this one is loaded)
       const int row = t.expert * p.M + (EPI == kGated ? t.tile_m * kBlock + rank * p.half_rows : t.tile_m * S::kRows + rank * (S::kRows / 2));
       const int token = t.n0 + rank * kBlock;
       for (int i = 0; i < p.blocks; ++i) {
@@ -773,9 +780,9 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
     // the scales' products, four tokens a lane, a batch ahead of those that wait in shared memory (a trip to L2 takes longer than a block)
     int slot = 0;
     uint32_t slot_par = 1;
-    PairTile t(p, GROUPED, max(min(pair, total - 1), 0));
+    PairTile t(p, GROUPED, max(min(pair, total - 1), 0), S::kTokens);
     for (int tile = pair; tile < total; tile += pairs) {
-      const PairTile next(p, GROUPED, min(tile + pairs, total - 1));
+      const PairTile next(p, GROUPED, min(tile + pairs, total - 1), S::kTokens);
       const int last = (EPI == kGated ? p.scale_rows / 2 : p.scale_rows) - 1;      // (rows beyond the weight: their sums are nobody's)
       const float* base = p.w_scales + static_cast<int64_t>(t.expert) * p.scale_rows * p.blocks;
       const float* ws0 = base + static_cast<int64_t>(min(EPI == kGated || !WIDE ? t.tile_m : 2 * t.tile_m, last)) * p.blocks;
@@ -816,9 +823,9 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
     int slot = set, batch = 0;
     uint32_t slot_par = 0, batch_par = 0;
     bool ready = false;
-    PairTile t(p, GROUPED, max(min(pair, total - 1), 0));
+    PairTile t(p, GROUPED, max(min(pair, total - 1), 0), S::kTokens);
     for (int tile = pair; tile < total; tile += pairs) {
-      const PairTile next(p, GROUPED, min(tile + pairs, total - 1));
+      const PairTile next(p, GROUPED, min(tile + pairs, total - 1), S::kTokens);
       const int token = t.n0 + rank * kBlock + quarter * 32 + lane, blocks = p.blocks;
 #pragma unroll
       for (int c = 0; c < 32; ++c) acc[c] = 0.0f, other[c] = WIDE ? 0.0f : -0.0f;
@@ -923,9 +930,8 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
   }
 }
 
-// The same for more tokens than a few and fewer than many, with tokens as the product's rows too (a thread of the epilogue holds one token's sums and
-// needs one factor a block; with weight rows as the product's rows, a factor from shared memory for every four sums, a block of 128 tokens took
-// twice as long): up to 128 tokens by 128
+// The same for more tokens than a few and fewer than many, with tokens as the product's rows too (with weight rows as the product's rows [6144, 4096] of
+// 128 tokens took 20.4 us, so 13.9): up to 128 tokens by 128
 // weight rows, or 64 gate rows and their 64 up rows. SPLIT: the K ranges are the CTAs of a cluster. Warp 0 loads, warp 1 issues the
 // products, warp 2 multiplies the scales, sixteen warps are the epilogue, a token a lane and 32 columns each; those without tokens pass over.
 constexpr int kTokenThreads = 640, kTokenRows = 128, kTokenSlots = 4;
@@ -1295,7 +1301,8 @@ bool byte_map(const void* base, int64_t rows, int64_t K, int64_t ld, int box_row
             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// K ranges of a weight of `tiles` tiles of 128 rows and `blocks` blocks of columns.
+// K ranges of a weight of `tiles` tiles of 128 rows and `blocks` blocks of columns: as many CTAs as there are SMs, four ranges at most (of eight, a
+// cluster's CTAs found places late: [2048, 2048] of 40 tokens 10.5 us, in four ranges 7.1).
 int fp8_ranges(int tiles, int blocks) {
   int s = 1;
   while (s < kMaxRanges && tiles * s * 2 <= 148 && blocks >= s * 4) s *= 2;
@@ -1403,20 +1410,26 @@ template <int EPI, class OUT, bool GROUPED>
 int launch_product(const void* w, int64_t rows_w, int64_t ldw, const void* q, int64_t rows_q, int64_t ldq, const Fp8Params& p, int tile_n, int tiles_n,
                    cudaStream_t st) {
   const int tiles_m = EPI == kGated ? (p.half_rows + 63) / 64 : (p.M + kBlock - 1) / kBlock;
-  switch (tile_n) {
-    case 16: return launch_tile<EPI, 16, OUT, GROUPED>(w, rows_w, ldw, q, rows_q, ldq, p, tiles_m, tiles_n, st);
-    case 32: return launch_tile<EPI, 32, OUT, GROUPED>(w, rows_w, ldw, q, rows_q, ldq, p, tiles_m, tiles_n, st);
-    case 64: return launch_tile<EPI, 64, OUT, GROUPED>(w, rows_w, ldw, q, rows_q, ldq, p, tiles_m, tiles_n, st);
-  }
+  if (tile_n == 16) return launch_tile<EPI, 16, OUT, GROUPED>(w, rows_w, ldw, q, rows_q, ldq, p, tiles_m, tiles_n, st);
   if constexpr (!GROUPED) {
+    if (tile_n == 32) return launch_tile<EPI, 32, OUT, false>(w, rows_w, ldw, q, rows_q, ldq, p, tiles_m, tiles_n, st);
+    if (tile_n == 64) return launch_tile<EPI, 64, OUT, false>(w, rows_w, ldw, q, rows_q, ldq, p, tiles_m, tiles_n, st);
     if (tile_n == kTokenRows) return launch_token<EPI, OUT>(w, rows_w, ldw, q, rows_q, ldq, p, tiles_m, tiles_n, st);
-    if (p.ranges == 1) return launch_pair<EPI, true, OUT, false, true>(w, rows_w, ldw, q, rows_q, ldq, p, tiles_n, st);
+    if (p.ranges == 1) {
+      // (a round of tiles takes pairs and single CTAs the same, within 5%, single CTAs a little longer: they are for where they need fewer of them.
+      // [12000, 4096] of 300 tokens: 46 us on pairs, two rounds, 27.7 on single CTAs)
+      const long long sms = sb::sm_count(), wide = EPI == kGated ? (p.half_rows + kBlock - 1) / kBlock : (p.M + 255) / 256;
+      const int single_n = (p.n + kTokenRows - 1) / kTokenRows;
+      if ((wide * single_n + sms - 1) / sms < (wide * tiles_n + sms / 2 - 1) / (sms / 2))
+        return launch_pair<EPI, true, OUT, false, false>(w, rows_w, ldw, q, rows_q, ldq, p, single_n, st);
+      return launch_pair<EPI, true, OUT, false, true>(w, rows_w, ldw, q, rows_q, ldq, p, tiles_n, st);
+    }
     if constexpr (EPI != kGated) return launch_pair<EPI, false, OUT, false, true>(w, rows_w, ldw, q, rows_q, ldq, p, tiles_n, st);
   }
   return sb::fail("gemm_fp8: no form for tiles of %d tokens", tile_n);
 }
 
-int launch_quantize(const void* x, int xdtype, int64_t ldx, const int32_t* used, const int32_t* place, int copies, int n, int K, void* q, int64_t ldq,
+int launch_quantize(const void* x, int xdtype, int64_t ldx, const int32_t* place, int copies, int n, int K, void* q, int64_t ldq,
                     float* scales, int64_t lds, cudaStream_t st) {
   const int blocks = (K + kBlock - 1) / kBlock;
   const dim3 grid((n + 7) / 8, (blocks + 1) / 2), block(256);
@@ -1424,7 +1437,7 @@ int launch_quantize(const void* x, int xdtype, int64_t ldx, const int32_t* used,
   const bool vec = ldx * (xdtype == 0 ? 4 : 2) % 16 == 0 && (reinterpret_cast<uintptr_t>(x) & 15) == 0;
   uint8_t* to = static_cast<uint8_t*>(q);
   auto run = [&](auto kernel, auto from) {
-    sb::launch_pdl(kernel, grid, block, 0, st, from, ldx, used, place, copies, n, K, blocks, to, ldq, scales, lds);
+    sb::launch_pdl(kernel, grid, block, 0, st, from, ldx, place, copies, n, K, blocks, to, ldq, scales, lds);
     return sb::check_launch("quantize_fp8");
   };
   if (xdtype == 0) return vec ? run(quantize_kernel<float, true>, static_cast<const float*>(x)) : run(quantize_kernel<float, false>, static_cast<const float*>(x));
@@ -1501,10 +1514,13 @@ int check_product(const char* who, const void* w, int64_t ldw, int out_dtype, in
   return 0;
 }
 
-// Rows of a tile of the experts' products: near the rows an expert gets on average (a row's result does not depend on it).
+// Rows of a tile of the experts' products (a row's result does not depend on it). 16, quantised on the way in, where an expert gets few, else 128 on
+// CTAs that walk tiles, which pays from nine or so on average if there are many pairs in all (64 experts of 2,048 x 1,408, six a token: 100 tokens
+// 131 us in tiles of 16, 123 walked, 150 tokens 157 and 127; 20 tokens, two of four experts of 1,024 x 512: 24.3 and 28.2). Tiles of 256 on pairs
+// of CTAs were no faster even with 1,000 rows an expert (82.6 us, 80.4 walked by single ones).
 int expert_tile(int pairs, int E) {
   const int mean = (pairs + E - 1) / E;
-  return mean <= 16 ? 16 : mean <= 32 ? 32 : mean <= 64 ? 64 : mean <= 512 ? kTokenRows : kPairTokens;
+  return mean <= 8 || (mean <= 16 && pairs <= 256) ? 16 : kTokenRows;
 }
 int most_tiles(int pairs, int E, int tile) { return std::min(pairs, pairs / tile + std::min(pairs, E)); }
 
@@ -1539,7 +1555,7 @@ SB_EXPORT int sb_quantize_fp8(const void* x, int xdtype, int64_t ldx, void* q, i
   if (int rc = check_quantized("quantize_fp8", q, ldq, lds, n, K)) return rc;
   if (xdtype < 0 || xdtype > 1 || ldx < K) return sb::fail("quantize_fp8: rows of %lld elements, %d columns", (long long)ldx, K);
   if (n == 0) return 0;
-  return launch_quantize(x, xdtype, ldx, nullptr, nullptr, 1, n, K, q, ldq, scales, lds, static_cast<cudaStream_t>(stream));
+  return launch_quantize(x, xdtype, ldx, nullptr, 1, n, K, q, ldq, scales, lds, static_cast<cudaStream_t>(stream));
 }
 
 // out = x . w^T of quantised x; epilogue 0 store, 1 add, 2 gated (w: half_rows gate rows, then as many up rows; act, limit, slope: the gate).
@@ -1575,7 +1591,7 @@ SB_EXPORT int sb_linear_fp8(const SbFp8Layer* l, const void* x, int xdtype, int6
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const bool itself = quantises_itself(x, xdtype, ldx, n, l->M, l->K);
   if (!itself) {
-    if (int rc = launch_quantize(x, xdtype, ldx, nullptr, nullptr, 1, n, l->K, l->q, l->ldq, l->x_scales, l->ldxs, st)) return rc;
+    if (int rc = launch_quantize(x, xdtype, ldx, nullptr, 1, n, l->K, l->q, l->ldq, l->x_scales, l->ldxs, st)) return rc;
   }
   Gate gate;
   gate.act = act, gate.limit = limit, gate.slope = slope;
@@ -1626,9 +1642,9 @@ SB_EXPORT int sb_experts_fp8(const SbFp8Experts* l, const void* x, int xdtype, i
   if (tiles > 65535) return sb::fail("%s: %d tiles of rows are too many", who, tiles);
   sb::launch_pdl(expert_order_kernel, dim3(1), dim3(kOrderThreads), 0, st, choice, n, top, E, tile, order, place, list);
   if (int rc = sb::check_launch(who)) return rc;
-  const bool quant = tile <= kQuantRows, quant_x = quant && copied_input(x, xdtype, ldx);
+  const bool quant_x = tile <= kQuantRows && copied_input(x, xdtype, ldx);
   if (!quant_x) {
-    if (int rc = launch_quantize(x, xdtype, ldx, nullptr, place, top, n, W, base + s.xq, s.ldx, xs, pairs, st)) return rc;
+    if (int rc = launch_quantize(x, xdtype, ldx, place, top, n, W, base + s.xq, s.ldx, xs, pairs, st)) return rc;
   }
   Fp8Params p = {};
   if (quant_x) set_input(p, x, xdtype, ldx), p.x_gathered = 1;
@@ -1636,22 +1652,18 @@ SB_EXPORT int sb_experts_fp8(const SbFp8Experts* l, const void* x, int xdtype, i
   p.out = z, p.ldo = s.ldz, p.x_scales = xs, p.ldxs = pairs, p.w_scales = gate_up_scales, p.M = 2 * F, p.K = W, p.half_rows = F;
   p.blocks = p.range_blocks = (W + kBlock - 1) / kBlock, p.scale_rows = 2 * ((F + kBlock - 1) / kBlock);
   const int64_t rows_g = static_cast<int64_t>(E) * 2 * F, rows_d = static_cast<int64_t>(E) * W;
-  const bool walks = tile >= kTokenRows;          // (kernels that walk tiles quantise the gated products themselves)
+  const bool walks = tile == kTokenRows;          // (those quantise the gated products themselves)
   if (walks) {
     p.out = base + s.zq, p.ldo = s.ldz, p.z_scales = zs;
-    if (int rc = tile == kPairTokens ? launch_pair<kGated, true, uint8_t, true, true>(gate_up, rows_g, ldg, base + s.xq, pairs, s.ldx, p, tiles, st)
-                                     : launch_pair<kGated, true, uint8_t, true, false>(gate_up, rows_g, ldg, base + s.xq, pairs, s.ldx, p, tiles, st))
-      return rc;
+    if (int rc = launch_pair<kGated, true, uint8_t, true, false>(gate_up, rows_g, ldg, base + s.xq, pairs, s.ldx, p, tiles, st)) return rc;
   } else {
     if (int rc = launch_product<kGated, float, true>(gate_up, rows_g, ldg, base + s.xq, pairs, s.ldx, p, tile, tiles, st)) return rc;
-    if (quant) set_input(p, z, 0, s.ldz), p.x_gathered = 0;
-    else if (int rc = launch_quantize(z, 0, s.ldz, list + 1, nullptr, 1, pairs, F, base + s.zq, s.ldz, zs, pairs, st)) return rc;
+    set_input(p, z, 0, s.ldz), p.x_gathered = 0;
   }
   p.out = parts, p.ldo = s.ldp, p.x_scales = zs, p.w_scales = down_scales, p.M = W, p.K = F, p.half_rows = 0;
   p.blocks = p.range_blocks = (F + kBlock - 1) / kBlock, p.scale_rows = (W + kBlock - 1) / kBlock;
-  if (int rc = !walks                ? launch_product<kStore, float, true>(down, rows_d, ldd, base + s.zq, pairs, s.ldz, p, tile, tiles, st)
-               : tile == kPairTokens ? launch_pair<kStore, true, float, true, true>(down, rows_d, ldd, base + s.zq, pairs, s.ldz, p, tiles, st)
-                                     : launch_pair<kStore, true, float, true, false>(down, rows_d, ldd, base + s.zq, pairs, s.ldz, p, tiles, st))
+  if (int rc = walks ? launch_pair<kStore, true, float, true, false>(down, rows_d, ldd, base + s.zq, pairs, s.ldz, p, tiles, st)
+                     : launch_product<kStore, float, true>(down, rows_d, ldd, base + s.zq, pairs, s.ldz, p, tile, tiles, st))
     return rc;
   const dim3 grid(n, (W + 1023) / 1024);
   if (grid.y > 65535) return sb::fail("%s: %d features are too many", who, W);

@@ -234,11 +234,13 @@ __device__ __forceinline__ void sort_descending(uint32_t* key, int* place) {
   if constexpr (N > 1) merge_exchange<N, 1, 1>(key, place);
 }
 
-// A warp a token. In 32-bit first: a score is off by less than 2^-20 of the largest (a sigmoid's approximated exponential is off by 2 + 1.2 |z| units
-// in the last place, which near and above 1/2 counts for a quarter at most, its division by two; where all scores are small, 2^-16), a sum with a bias by 2^-23 of its size more; where two
-// candidates that follow one another, or the last group that stays and the first that does not, are closer than twice that, the token is routed
-// again in 64-bit. So the choice is that of 64-bit scores always, at the price of 32-bit ones for nearly all tokens (16,384 tokens of 256 experts in
-// eight groups, everything in 64-bit: 87 us).
+// A warp a token. In 32-bit first, where a score is off by less than a known share of the largest: a sigmoid by 2^-20 (its approximated exponential is
+// off by 2 + 1.2 |z| units in the last place, of which a quarter counts at most near and above 1/2, its division by two; 2^-16 where all scores
+// are small), a softmax by PER + 16 times 2^-24 (PER + 4 additions, four units in the last place of the exponential, a division); a sum with a bias
+// by 2^-23 of its size more. Where two candidates that follow one another, or the last group that stays and the first that does not, are
+// closer than twice that, the token is routed again in 64-bit. So the choice is that of 64-bit scores always, at the price of 32-bit ones for
+// nearly all tokens. 16,384 tokens of 256 experts in eight groups, eight chosen: everything in 64-bit 87 us, so 30 (560 GB/s; issue slots bound it,
+// some 1,000 instructions a token, eleven times the time of its bytes); one token 12.6 and 2.7.
 template <int PER>
 __device__ __forceinline__ void route_row(const Routing& r, int row, int lane, const float* z, const float* bias, double* held, float* held_scores) {
   float s[PER], c[PER];
@@ -250,7 +252,8 @@ __device__ __forceinline__ void route_row(const Routing& r, int row, int lane, c
   // (both are not negative: their bits are ordered as they are)
   high_s = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(high_s)));
   high_c = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(high_c)));
-  const float near = 2.0f * ((high_s > 0.125f ? 0x1p-20f : 0x1p-16f) * high_s + 0x1p-23f * high_c);
+  const float off = r.softmax ? (PER + 16) * 0x1p-24f : high_s > 0.125f ? 0x1p-20f : 0x1p-16f;
+  const float near = 2.0f * (off * high_s + 0x1p-23f * high_c);
   bool sure = high_c < INFINITY;
   if (r.groups > 1) {
     float gap;
