@@ -263,7 +263,7 @@ __device__ __forceinline__ float cluster_load_float(uint32_t addr) {
 
 template <int BN>
 struct Shape {
-  static constexpr int kEpilogueWarps = BN >= 64 ? 8 : 4;
+  static constexpr int kEpilogueWarps = BN >= 64 ? 16 : BN >= 32 ? 8 : 4;
   static constexpr int kColumns = BN * 4 / kEpilogueWarps;             // columns of a thread's row of the tile
   static constexpr int threads(bool quant) { return 128 + 32 * kEpilogueWarps + (quant ? 192 : 0); }
   static constexpr int kSlots = BN <= 32 ? 8 : 4;                      // accumulators under way
@@ -1449,13 +1449,22 @@ int launch_quantize(const void* x, int xdtype, int64_t ldx, const int32_t* place
 // most pairs had none: then whichever takes fewer rounds of the SMs, a block of columns costing a pair some 0.43 us and a CTA of a
 // cluster 0.6, a round's beginning and end 5 and 3.5 ([4096, 14336] of 256 tokens: 49.7 us on pairs, 39.0 on clusters; [4096, 4096] 18.8 and 24.1;
 // [6144, 4096] of 333 32.8 and 26.1).
+//
+// More than 32 tokens of a weight with more tiles than SMs: walked too if the wide tiles then take half the rounds (a round of those takes half as
+// long again). 64 tokens, [20000, 2048]: 19.8 and 15.6 us, [28000, 4096]: 31.2 and 26.6; [14000, 8192], one round either way: 27.1 and 39.6.
 int token_tile(Fp8Params& p, int epilogue) {
-  p.split = p.ranges > 1;
-  if (p.n <= 64) return p.n <= 16 ? 16 : p.n <= 32 ? 32 : 64;
-  if (p.n <= kTokenRows) return kTokenRows;
   const bool gated = epilogue == kGated;
+  const long long sms = sb::sm_count();
+  p.split = p.ranges > 1;
+  if (p.n <= 32) return p.n <= 16 ? 16 : 32;
+  if (p.n <= kTokenRows) {
+    const int rows = gated ? p.half_rows : p.M, narrow = gated ? 64 : kBlock;
+    const long long tiles = (rows + narrow - 1) / narrow, wide = (rows + 2 * narrow - 1) / (2 * narrow);
+    if (p.ranges == 1 && (tiles + sms - 1) / sms >= 2 * ((wide + sms - 1) / sms)) return kPairTokens;
+    return p.n <= 64 ? 64 : kTokenRows;
+  }
   if (p.split && !gated) {
-    const long long sms = sb::sm_count(), tiles = (p.M + kBlock - 1) / kBlock;
+    const long long tiles = (p.M + kBlock - 1) / kBlock;
     const long long pair_rounds = (tiles * ((p.n + kPairTokens - 1) / kPairTokens) + sms / 2 - 1) / (sms / 2);
     const long long split_rounds = (tiles * ((p.n + kTokenRows - 1) / kTokenRows) * p.ranges + sms - 1) / sms;
     if (split_rounds * (60 * p.range_blocks + 350) < pair_rounds * 43 * p.blocks + 500) return kTokenRows;
@@ -1582,8 +1591,23 @@ typedef struct SbFp8Layer {
 } SbFp8Layer;
 
 // x is quantised, of few tokens perhaps on the way into the product (which leaves the buffers alone), and multiplied.
-SB_EXPORT int sb_linear_fp8(const SbFp8Layer* l, const void* x, int xdtype, int64_t ldx, void* out, int out_dtype, int64_t ldo, int n, int epilogue, int act,
-                            float limit, float slope, void* stream) {
+typedef struct SbFp8Call {
+  const SbFp8Layer* layer;
+  const void* x;
+  int64_t ldx;
+  void* out;
+  int64_t ldo;
+  int32_t x_dtype, out_dtype, n, epilogue, act;
+  float limit, slope;
+} SbFp8Call;
+
+SB_EXPORT int sb_linear_fp8(const SbFp8Call* call, void* stream) {
+  const SbFp8Call c = *call;
+  const SbFp8Layer* l = c.layer;
+  const void* x = c.x;
+  void* out = c.out;
+  const int64_t ldx = c.ldx, ldo = c.ldo;
+  const int xdtype = c.x_dtype, out_dtype = c.out_dtype, n = c.n, epilogue = c.epilogue;
   if (int rc = check_quantized("linear_fp8", l->q, l->ldq, l->ldxs, n, l->K)) return rc;
   if (int rc = check_product("linear_fp8", l->w, l->ldw, out_dtype, ldo, l->M, l->K, epilogue, l->half_rows)) return rc;
   if (xdtype < 0 || xdtype > 1 || ldx < l->K) return sb::fail("linear_fp8: rows of %lld elements, %d columns", (long long)ldx, l->K);
@@ -1594,7 +1618,7 @@ SB_EXPORT int sb_linear_fp8(const SbFp8Layer* l, const void* x, int xdtype, int6
     if (int rc = launch_quantize(x, xdtype, ldx, nullptr, 1, n, l->K, l->q, l->ldq, l->x_scales, l->ldxs, st)) return rc;
   }
   Gate gate;
-  gate.act = act, gate.limit = limit, gate.slope = slope;
+  gate.act = c.act, gate.limit = c.limit, gate.slope = c.slope;
   return launch_gemm(itself ? x : nullptr, xdtype, ldx, l->q, l->ldq, l->x_scales, l->ldxs, l->w, l->ldw, l->w_scales, out, out_dtype, ldo, n, l->M, l->K, epilogue,
                      epilogue == kGated ? l->half_rows : 0, gate, st);
 }
@@ -1615,8 +1639,28 @@ typedef struct SbFp8Experts {
   int32_t experts, width, inner;
 } SbFp8Experts;
 
-SB_EXPORT int sb_experts_fp8(const SbFp8Experts* l, const void* x, int xdtype, int64_t ldx, const int32_t* choice, const float* weights, void* out,
-                             int out_dtype, int64_t ldo, int n, int top, void* scratch, int64_t scratch_bytes, void* stream) {
+typedef struct SbFp8ExpertsCall {
+  const SbFp8Experts* experts;
+  const void* x;
+  int64_t ldx;
+  const int32_t* choice;
+  const float* weights;
+  void* out;
+  int64_t ldo;
+  void* scratch;
+  int64_t scratch_bytes;
+  int32_t x_dtype, out_dtype, n, top;
+} SbFp8ExpertsCall;
+
+SB_EXPORT int sb_experts_fp8(const SbFp8ExpertsCall* call, void* stream) {
+  const SbFp8ExpertsCall c = *call;
+  const SbFp8Experts* l = c.experts;
+  const void* x = c.x;
+  const int32_t* choice = c.choice;
+  const float* weights = c.weights;
+  void *out = c.out, *scratch = c.scratch;
+  const int64_t ldx = c.ldx, ldo = c.ldo, scratch_bytes = c.scratch_bytes;
+  const int xdtype = c.x_dtype, out_dtype = c.out_dtype, n = c.n, top = c.top;
   const void *gate_up = l->gate_up, *down = l->down;
   const float *gate_up_scales = l->gate_up_scales, *down_scales = l->down_scales;
   const int64_t ldg = l->ldg, ldd = l->ldd;
@@ -1685,8 +1729,9 @@ SB_EXPORT int sb_op_linear_fp8(const SbOp* op, const SbStep* s, void* stream) {
   if (n <= 0) return SB_OP_SKIPPED;
   const SbFp8Layer l = {ptr<void>(op->i[0]), op->i[1], ptr<float>(op->i[2]), op->i[3], ptr<void>(op->i[4]), op->i[5], ptr<float>(op->i[6]),
                         (int)op->i[7], (int)op->i[8], (int)op->i[9]};
-  return sb_linear_fp8(&l, ptr<void>(op->i[10]), (int)op->i[11], op->i[12], ptr<void>(op->i[13]), (int)op->i[14], op->i[15], n, (int)op->i[16],
-                       (int)op->i[17], (float)op->f[0], (float)op->f[1], stream) != 0 ? SB_OP_FAILED : SB_OP_LAUNCHED;
+  const SbFp8Call c = {&l, ptr<void>(op->i[10]), op->i[12], ptr<void>(op->i[13]), op->i[15], (int)op->i[11], (int)op->i[14], n, (int)op->i[16], (int)op->i[17],
+                       (float)op->f[0], (float)op->f[1]};
+  return sb_linear_fp8(&c, stream) != 0 ? SB_OP_FAILED : SB_OP_LAUNCHED;
 }
 
 // i: 0 gate_up, 1 ldg, 2 gate_up scales, 3 down, 4 ldd, 5 down scales, 6 experts, 7 width, 8 inner, 9 x, 10 x dtype, 11 ldx, 12 choice [n][top],
@@ -1696,6 +1741,7 @@ SB_EXPORT int sb_op_experts_fp8(const SbOp* op, const SbStep* s, void* stream) {
   if (s->n <= 0) return SB_OP_SKIPPED;
   const SbFp8Experts l = {ptr<void>(op->i[0]), op->i[1], ptr<float>(op->i[2]), ptr<void>(op->i[3]), op->i[4], ptr<float>(op->i[5]), (int)op->i[6],
                           (int)op->i[7], (int)op->i[8]};
-  return sb_experts_fp8(&l, ptr<void>(op->i[9]), (int)op->i[10], op->i[11], ptr<int32_t>(op->i[12]), ptr<float>(op->i[13]), ptr<void>(op->i[14]),
-                        (int)op->i[15], op->i[16], s->n, (int)op->i[17], ptr<void>(op->i[18]), op->i[19], stream) != 0 ? SB_OP_FAILED : SB_OP_LAUNCHED;
+  const SbFp8ExpertsCall c = {&l, ptr<void>(op->i[9]), op->i[11], ptr<int32_t>(op->i[12]), ptr<float>(op->i[13]), ptr<void>(op->i[14]), op->i[16],
+                              ptr<void>(op->i[18]), op->i[19], (int)op->i[10], (int)op->i[15], s->n, (int)op->i[17]};
+  return sb_experts_fp8(&c, stream) != 0 ? SB_OP_FAILED : SB_OP_LAUNCHED;
 }

@@ -339,9 +339,21 @@ int launch(Routing r, cudaStream_t st) {
 }  // namespace
 
 // logits [n][ldz] float32, bias [E] float32 or null, choice [n][top] int32, weights [top][ldw] float32. score: 0 sigmoid, 1 softmax.
-SB_EXPORT int sb_route_experts(const float* logits, int64_t ldz, const float* bias, int32_t* choice, float* weights, int64_t ldw, int n, int E, int top,
-                               int score, int groups, int top_groups, int group_best, int renormalise, float scale, void* stream) {
-  const Routing r = {logits, ldz, bias, choice, weights, ldw, n, E, top, groups, top_groups, group_best, score, renormalise, scale};
+typedef struct SbRouteCall {
+  const float* logits;
+  int64_t ldz;
+  const float* bias;
+  int32_t* choice;
+  float* weights;
+  int64_t ldw;
+  int32_t n, experts, top, score, groups, top_groups, group_best, renormalise;
+  float scale;
+} SbRouteCall;
+
+SB_EXPORT int sb_route_experts(const SbRouteCall* call, void* stream) {
+  const SbRouteCall c = *call;
+  const Routing r = {c.logits, c.ldz, c.bias, c.choice, c.weights, c.ldw, c.n, c.experts, c.top, c.groups, c.top_groups, c.group_best, c.score,
+                     c.renormalise, c.scale};
   return launch(r, static_cast<cudaStream_t>(stream));
 }
 

@@ -7,7 +7,8 @@ tensor that is not on a CUDA device, or a library that cannot be built, raises.
 from __future__ import annotations
 
 import ctypes
-from ctypes import c_float, c_int, c_int64, c_void_p
+import struct
+from ctypes import c_char_p, c_float, c_int, c_int64, c_void_p
 
 import torch
 
@@ -784,6 +785,13 @@ def gemm_fp8(q: torch.Tensor, scales: torch.Tensor, weight, out: torch.Tensor, e
                    dtype_code(out.dtype), _row_stride(out), n, M, K, code, half, max(epilogue - SWIGLU, 0), *constants, _stream()))
 
 
+# Calls with many arguments hand them over as one record (the structures of the same names in csrc): as separate arguments they took ctypes
+# 2.4 us a call, packed 0.9.
+_LINEAR_CALL = struct.Struct("@PPqPqiiiiiff")          # SbFp8Call
+_EXPERTS_CALL = struct.Struct("@PPqPPPqPqiiii")        # SbFp8ExpertsCall
+_ROUTE_CALL = struct.Struct("@PqPPPqiiiiiiiif")        # SbRouteCall
+
+
 class _Fp8Layer(ctypes.Structure):
     """What a layer with an 8-bit weight hands over with every call (csrc/gemm_fp8.cu: SbFp8Layer)."""
     _fields_ = [("q", c_void_p), ("ldq", c_int64), ("x_scales", c_void_p), ("ldxs", c_int64), ("w", c_void_p), ("ldw", c_int64), ("w_scales", c_void_p),
@@ -804,8 +812,7 @@ class Fp8Linear:
         self._layer = _Fp8Layer(q.data_ptr(), _row_stride(q), scales.data_ptr(), _row_stride(scales), weight.q.data_ptr(), weight.stride,
                                 weight.scales.data_ptr(), self.M, self.K, half)
         self._address = ctypes.addressof(self._layer)
-        self._lib, self._fn = _fn("gemm_fp8", "sb_linear_fp8", [c_void_p, c_void_p, c_int, c_int64, c_void_p, c_int, c_int64, c_int, c_int, c_int,
-                                                                c_float, c_float, c_void_p])
+        self._lib, self._fn = _fn("gemm_fp8", "sb_linear_fp8", [c_char_p, c_void_p])
 
     def __call__(self, x: torch.Tensor, out: torch.Tensor, epilogue: int = STORE, constants=(0.0, 0.0)) -> None:
         if not (x.is_cuda and out.is_cuda):
@@ -823,8 +830,9 @@ class Fp8Linear:
             raise ValueError("a stacked weight whose matrices are no whole number of 128 rows only has the gated product")
         if n <= 1:
             ldx, ldo = max(ldx, K), max(ldo, M)          # (of a single row the stride says nothing)
-        rc = self._fn(self._address, x.data_ptr(), dtype_code(x.dtype), ldx, out.data_ptr(), dtype_code(out.dtype), ldo, n, epilogue if epilogue < SWIGLU else 2,
-                      epilogue - SWIGLU if gated else 0, *constants, _stream())
+        call = _LINEAR_CALL.pack(self._address, x.data_ptr(), ldx, out.data_ptr(), ldo, dtype_code(x.dtype), dtype_code(out.dtype), n,
+                                 epilogue if epilogue < SWIGLU else 2, epilogue - SWIGLU if gated else 0, *constants)
+        rc = self._fn(call, _stream())
         _check(self._lib, rc)
 
 
@@ -849,10 +857,10 @@ def route_experts(logits: torch.Tensor, choice: torch.Tensor, weights: torch.Ten
             or (bias is not None and (bias.shape != (E,) or not bias.is_contiguous())):
         raise ValueError(f"route_experts shapes: logits {tuple(logits.shape)}, choice {tuple(choice.shape)}, weights {tuple(weights.shape)}"
                          + (f", bias {tuple(bias.shape)}" if bias is not None else ""))
-    lib, fn = _fn("router", "sb_route_experts", [c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_int64, c_int, c_int, c_int, c_int, c_int, c_int, c_int,
-                                                 c_int, c_float, c_void_p])
-    _check(lib, fn(logits.data_ptr(), ldz if n > 1 else max(ldz, E), 0 if bias is None else bias.data_ptr(), choice.data_ptr(), weights.data_ptr(),
-                   ldw if top > 1 else max(ldw, n), n, E, top, ROUTER_SCORES[score], groups, top_groups, group_best, int(renormalise), scale, _stream()))
+    lib, fn = _fn("router", "sb_route_experts", [c_char_p, c_void_p])
+    call = _ROUTE_CALL.pack(logits.data_ptr(), ldz if n > 1 else max(ldz, E), 0 if bias is None else bias.data_ptr(), choice.data_ptr(), weights.data_ptr(),
+                            ldw if top > 1 else max(ldw, n), n, E, top, ROUTER_SCORES[score], groups, top_groups, group_best, int(renormalise), scale)
+    _check(lib, fn(call, _stream()))
 
 
 def experts_fp8_scratch(n: int, top: int, experts: int, width: int, inner: int) -> int:
@@ -877,10 +885,10 @@ def experts_fp8(x: torch.Tensor, choice: torch.Tensor, weights: torch.Tensor, ex
                          f"experts of width {experts.width}")
     if n <= 1:
         ldx, ldo = max(ldx, W), max(ldo, W)
-    lib, fn = _fn("gemm_fp8", "sb_experts_fp8", [c_void_p, c_void_p, c_int, c_int64, c_void_p, c_void_p, c_void_p, c_int, c_int64, c_int, c_int, c_void_p,
-                                                 c_int64, c_void_p])
-    _check(lib, fn(experts.address, x.data_ptr(), dtype_code(x.dtype), ldx, choice.data_ptr(), weights.data_ptr(), out.data_ptr(), dtype_code(out.dtype), ldo,
-                   n, top, scratch.data_ptr(), scratch.numel(), _stream()))
+    lib, fn = _fn("gemm_fp8", "sb_experts_fp8", [c_char_p, c_void_p])
+    call = _EXPERTS_CALL.pack(experts.address, x.data_ptr(), ldx, choice.data_ptr(), weights.data_ptr(), out.data_ptr(), ldo, scratch.data_ptr(),
+                              scratch.numel(), dtype_code(x.dtype), dtype_code(out.dtype), n, top)
+    _check(lib, fn(call, _stream()))
 
 
 class _Fp8ExpertsLayout(ctypes.Structure):

@@ -72,8 +72,25 @@ def test_a_block_that_is_not_finite_poisons_its_token_only(bad):
     assert torch.equal(out[[0, 1, 2, 4]], clean[[0, 1, 2, 4]])
 
 
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_quantised_rows_at_the_ends_of_the_range(dtype):
+    """The largest finite values, the smallest normal ones and below: the scale's exponent at both ends."""
+    x = _rand(5, 6, 300, dtype=dtype)
+    top = torch.finfo(dtype).max
+    x[0], x[0, 1] = top, -top
+    x[1], x[1, 200] = 1.0, top / 2
+    x[2] = 2.0 ** -100 * 448
+    x[3] = 2.0 ** -126
+    x[4] = 0
+    x[5, ::2] = 2.0 ** -133
+    q, s = _quantize(x)
+    want, scales = plain.quantised(x.to(F64))
+    assert torch.equal(s.t().to(F64), scales)
+    assert torch.equal(q[:, :300].to(F64), want)
+
+
 SIZES = [(1, 1, 1), (1, 128, 128), (2, 130, 100), (16, 2048, 2048), (17, 500, 1000), (40, 128, 4096), (64, 1000, 900), (65, 300, 2056), (129, 256, 640),
-         (333, 2500, 2056), (1000, 640, 384)]
+         (333, 2500, 2056), (1000, 640, 384), (300, 12000, 256), (3000, 1300, 384), (200, 1000, 4096), (50, 20000, 256), (120, 19000, 130)]
 
 
 @pytest.mark.parametrize("n,M,K", SIZES)
@@ -130,31 +147,101 @@ def test_added_to_the_residual(n):
     assert torch.equal(out, alone + h)
 
 
-@pytest.mark.parametrize("M,K", [(128, 8192), (2048, 2048), (1500, 4104), (640, 260), (20000, 256)])
+@pytest.mark.parametrize("M,K", [(128, 8192), (2048, 2048), (1500, 4104), (640, 260), (20000, 256), (12000, 384)])
 def test_a_tokens_bits_do_not_depend_on_the_step(M, K):
     """Alone, in a few, in tiles of every size, the ranges of K on CTAs of their own and walked by one: the same bits."""
     from stride_b200.kernels.linear import Linear
     x, layer = _rand(M, 300, K, dtype=BF), Linear(_weight(K, M, K), BF)
     whole = torch.empty(300, M, device="cuda")
     layer.forward(x, whole, workspace=_workspace(300))
-    for first, n in [(0, 1), (7, 16), (30, 17), (60, 33), (100, 65), (100, 128), (170, 129)]:
+    for first, n in [(0, 1), (7, 16), (30, 17), (60, 33), (100, 65), (100, 128), (170, 129), (0, 257)]:
         part = torch.full((n, M), float("nan"), device="cuda")
         layer.forward(x[first:first + n], part, workspace=_workspace(300))
         assert torch.equal(part, whole[first:first + n]), (first, n)
 
 
-def test_rows_of_larger_tensors_and_what_lies_around_them():
-    """Input and result as column ranges of wider buffers, a narrow slice that starts off a 16-byte border; what is around the result stays."""
+@pytest.mark.parametrize("n", [1, 9, 16, 30, 50, 100, 300])
+@pytest.mark.parametrize("columns,rows", [(257, 200), (256, 200), (256, 5000)])
+def test_rows_of_larger_tensors_and_what_lies_around_them(n, columns, rows):
+    """Input and result as column ranges of wider buffers, a slice that starts off a 16-byte border; what is around the result stays."""
     from stride_b200.kernels.linear import Linear
-    wide, layer = _rand(3, 50, 1003, dtype=BF), Linear(_weight(4, 200, 257), BF)
-    x = wide[:, 5:262]
-    want = torch.empty(50, 200, device="cuda")
-    layer.forward(x.contiguous(), want, workspace=_workspace(64))
-    held = torch.full((52, 333), 7.0, device="cuda")
-    layer.forward(x, held[1:51, 100:300], workspace=_workspace(64))
-    assert torch.equal(held[1:51, 100:300], want)
-    held[1:51, 100:300] = 7.0
-    assert (held == 7.0).all()
+    wide, layer = _rand(3, n, 1003, dtype=BF), Linear(_weight(4, rows, columns), BF)
+    x = wide[:, 5:5 + columns]
+    want = torch.empty(n, rows, device="cuda")
+    layer.forward(x.contiguous(), want, workspace=_workspace(n))
+    for first in (100, 101):
+        held = torch.full((n + 2, rows + 133), 7.0, device="cuda")
+        layer.forward(x, held[1:n + 1, first:first + rows], workspace=_workspace(n))
+        assert torch.equal(held[1:n + 1, first:first + rows], want)
+        held[1:n + 1, first:first + rows] = 7.0
+        assert (held == 7.0).all()
+
+
+def test_calls_that_are_refused():
+    """Shapes, types and layouts that the entry points do not take: an error, nothing is written."""
+    from stride_b200.kernels import ops
+    from stride_b200.kernels.linear import Fp8Weight, Linear
+    x, w, ws = _rand(1, 4, 256, dtype=BF), _weight(2, 130, 256), _workspace(4)
+    layer, out = Linear(w, BF), torch.full((4, 130), 7.0, device="cuda")
+    with pytest.raises(ValueError):
+        layer.forward(x[:, :255], out, workspace=ws)
+    with pytest.raises(ValueError):
+        layer.forward(x, out[:, :129], workspace=ws)
+    with pytest.raises(ValueError):
+        layer.forward(x.t().contiguous().t(), out, workspace=ws)
+    with pytest.raises(ValueError):
+        layer.forward(_rand(1, 5, 256, dtype=BF), torch.empty(5, 130, device="cuda"), workspace=ws)         # more rows than the workspace
+    with pytest.raises(ValueError):
+        layer.forward_swiglu(x, torch.empty(4, 65, device="cuda"), None, workspace=ws)                       # not stacked from two
+    with pytest.raises(ValueError):
+        Linear(Fp8Weight.stack([w, _weight(3, 130, 256)]), BF).forward(x, torch.empty(4, 260, device="cuda"), workspace=ws)
+    with pytest.raises(TypeError):
+        layer.forward(x.half(), out, workspace=ws)
+    with pytest.raises(TypeError):
+        layer.forward(x, out.half(), workspace=ws)
+    q, s = _quantize(x)
+    with pytest.raises(RuntimeError):
+        ops.gemm_fp8(q, s, w, out.to(BF), ops.ADD)
+    with pytest.raises(ValueError):
+        ops.gemm_fp8(q, s[:1], w, out)
+    with pytest.raises(TypeError):
+        ops.gemm_fp8(q.view(torch.uint8), s, w, out)
+    with pytest.raises(RuntimeError):
+        ops.quantize_fp8(x, torch.zeros(4, 257, dtype=torch.uint8, device="cuda").view(torch.float8_e4m3fn), s)      # rows off their 16-byte borders
+    z, choice, weights = _rand(1, 4, 16), torch.full((4, 2), 7, dtype=torch.int32, device="cuda"), torch.full((2, 4), 7.0, device="cuda")
+    for kw in ({"groups": 3}, {"groups": 0}, {"groups": 4, "top_groups": 5}, {"groups": 16, "top_groups": 1}, {"groups": 4, "top_groups": 2, "group_best": 3}):
+        with pytest.raises(RuntimeError):
+            ops.route_experts(z, choice, weights, **kw)
+    for bad in ((z.double(), choice, weights), (z, choice.long(), weights), (z, choice, weights.t()), (z[:3], choice, weights), (z, choice, weights.to(BF))):
+        with pytest.raises((TypeError, ValueError)):
+            ops.route_experts(*bad)
+    with pytest.raises(ValueError):
+        ops.route_experts(z, choice, weights, score="relu")
+    with pytest.raises(RuntimeError):
+        ops.route_experts(_rand(1, 4, 1025), choice, weights)
+    experts, _ = _experts(4, 256, 128)
+    y = torch.full((4, 256), 7.0, device="cuda")
+    good = experts.scratch(4, 2)
+    with pytest.raises(RuntimeError):
+        experts.forward(x, choice, weights, y, good[:-1])
+    with pytest.raises(ValueError):
+        experts.forward(x[:, :128], choice, weights, y, good)
+    with pytest.raises(ValueError):
+        experts.forward(x, choice, weights.t().contiguous(), y, good)
+    with pytest.raises(TypeError):
+        experts.forward(x, choice.long(), weights, y, good)
+    assert (out == 7.0).all() and (choice == 7).all() and (weights == 7.0).all() and (y == 7.0).all()
+
+
+def test_no_tokens():
+    from stride_b200.kernels import ops
+    from stride_b200.kernels.linear import Linear
+    Linear(_weight(2, 130, 256), BF).forward(_rand(1, 0, 256, dtype=BF), torch.empty(0, 130, device="cuda"), workspace=_workspace(4))
+    choice, weights = torch.empty(0, 2, dtype=torch.int32, device="cuda"), torch.empty(2, 0, device="cuda")
+    ops.route_experts(torch.empty(0, 8, device="cuda"), choice, weights)
+    experts, _ = _experts(4, 256, 128)
+    experts.forward(torch.empty(0, 256, device="cuda"), choice, weights, torch.empty(0, 256, device="cuda"), experts.scratch(0, 2))
+    torch.cuda.synchronize()
 
 
 def test_product_in_a_graph_and_on_another_stream():
@@ -297,6 +384,44 @@ def test_experts(n, E, top, W, F, missing, x_dtype, out_dtype):
         assert (out[1] == 0).all()
 
 
+@pytest.mark.parametrize("n", [2, 40, 300])
+def test_an_expert_chosen_twice_and_one_chosen_by_all(n):
+    """The same id in several of a token's places counts as often; all tokens on one expert, the others idle."""
+    layer, (gate, up, down) = _experts(3, 256, 160)
+    x = _rand(n, n, 256, dtype=BF)
+    choice = torch.full((n, 3), 1, dtype=torch.int32, device="cuda")
+    choice[0] = torch.tensor([2, 2, 0], dtype=torch.int32)
+    weights = _rand(4, 3, n).abs()
+    out = torch.empty(n, 256, device="cuda")
+    layer.forward(x, choice, weights, out, layer.scratch(n, 3))
+    want, bound = plain.experts(x.to(F64), choice, weights, gate, up, down)
+    assert ((out.to(F64) - want).abs() <= bound).all()
+
+
+def test_two_streams_at_once():
+    """Two layers' and two experts' calls side by side, each with buffers of its own."""
+    from stride_b200.kernels.linear import Linear
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    linear = [Linear(_weight(20 + i, 2048, 1024), BF) for i in range(2)]
+    experts = [_experts(8, 256, 264, seed=5000 * i)[0] for i in range(2)]
+    x, rows = [_rand(30 + i, 70, 1024, dtype=BF) for i in range(2)], [_rand(40 + i, 70, 256, dtype=BF) for i in range(2)]
+    routes = [_choices(50 + i, 70, 8, 2) for i in range(2)]
+    work, scratch = [_workspace(70) for _ in range(2)], [experts[i].scratch(70, 2) for i in range(2)]
+    alone, out = ([(torch.empty(70, 2048, device="cuda"), torch.empty(70, 256, device="cuda")) for _ in range(2)] for _ in range(2))
+    for i in range(2):
+        linear[i].forward(x[i], alone[i][0], workspace=work[i])
+        experts[i].forward(rows[i], *routes[i], alone[i][1], scratch[i])
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for i in range(2):
+            with torch.cuda.stream(streams[i]):
+                linear[i].forward(x[i], out[i][0], workspace=work[i])
+                experts[i].forward(rows[i], *routes[i], out[i][1], scratch[i])
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert torch.equal(out[i][0], alone[i][0]) and torch.equal(out[i][1], alone[i][1])
+
+
 def test_experts_of_a_token_do_not_depend_on_the_step():
     """Alone, in a few and in many, whoever else chose the same experts; the same twice over the same scratch."""
     layer, _ = _experts(8, 384, 264)
@@ -307,7 +432,7 @@ def test_experts_of_a_token_do_not_depend_on_the_step():
     layer.forward(x, choice, weights, whole, scratch)
     layer.forward(x, choice, weights, again, scratch)
     assert torch.equal(whole, again)
-    for first, n in [(0, 1), (9, 5), (100, 40), (200, 150)]:
+    for first, n in [(0, 1), (9, 5), (100, 40), (200, 150), (0, 399)]:
         part = torch.full((n, 384), float("nan"), device="cuda")
         rows = slice(first, first + n)
         layer.forward(x[rows], choice[rows].contiguous(), weights[:, rows].contiguous(), part, scratch)
