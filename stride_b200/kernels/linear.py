@@ -257,6 +257,7 @@ class Linear:
     def _fp8_op(self, program, x, out, ldo: int, epilogue: int, wanted_rows: bool = False, act: int = 0, constants=()) -> None:
         q, scales = self._buffers(program.workspace)
         w = self.fp8
+        ops.check_fp8_epilogue(w, epilogue == 2)
         program.add("gemm_fp8", "sb_op_linear_fp8", [q, q.stride(0), scales, scales.stride(0), w.q, w.stride, w.scales, *w.shape, w.shape[0] // 2,
                                                      x, x.dtype, x.stride(0), out, out.dtype, ldo, epilogue, act, int(wanted_rows)], constants)
 

@@ -756,15 +756,20 @@ def quantize_fp8(x: torch.Tensor, q: torch.Tensor, scales: torch.Tensor) -> None
     _check(lib, fn(_ptr(x), dtype_code(x.dtype), _row_stride(x), _ptr(q), _row_stride(q), _ptr(scales), _row_stride(scales), n, K, _stream()))
 
 
+def check_fp8_epilogue(weight, gated: bool) -> None:
+    """Whether a product with the 8-bit weight (its `halves` and `in_blocks`) can be gated, or plain."""
+    if gated and weight.halves != 2:
+        raise ValueError("a gated product takes a weight stacked from a gate and an up matrix of one shape")
+    if not gated and not weight.in_blocks:
+        raise ValueError("a stacked weight whose matrices are no whole number of 128 rows only has the gated product")
+
+
 def _fp8_product(weight, out: torch.Tensor, epilogue: int, n: int):
     """(weight's address, stride, scales, out's address, dtype, stride, M, epilogue code, half rows, gate) of a product, checked."""
     M = weight.shape[0]
     code = _EPILOGUES_FP8[epilogue]
     half = M // 2 if code == 2 else 0
-    if code == 2 and weight.halves != 2:
-        raise ValueError("a gated product takes a weight stacked from a gate and an up matrix of one shape")
-    if code != 2 and not weight.in_blocks:
-        raise ValueError("a stacked weight whose matrices are no whole number of 128 rows only has the gated product")
+    check_fp8_epilogue(weight, code == 2)
     if out.dim() != 2 or out.shape[0] != n or out.shape[1] != (half or M) or (out.shape[1] > 1 and out.stride(1) != 1):
         raise ValueError(f"gemm_fp8 writes [{n}, {half or M}], not {tuple(out.shape)}")
     return M, code, half
@@ -774,7 +779,8 @@ def gemm_fp8(q: torch.Tensor, scales: torch.Tensor, weight, out: torch.Tensor, e
     """out = x . weight^T of rows that `quantize_fp8` made, weight an `Fp8Weight`: sums of blocks of 128 columns times both scales, added in 32-bit.
 
     STORE: out float32 or bfloat16 [n, M]. ADD: out float32 += result. SWIGLU, GEGLU_TANH, CLAMPED_GLU: weight stacked from gate and up rows,
-    out float32 or bfloat16 [n, M / 2] (`gemm_tc`)."""
+    out float32 or bfloat16 [n, M / 2] (`gemm_tc`). out overlaps no input. The weight may be read while this module's kernels in front still run:
+    it is not what one of them writes."""
     _cuda(q, scales, weight.q, out)
     n, K = q.shape[0], weight.shape[1]
     _check_fp8_rows("gemm_fp8", q, scales, n, K)
@@ -800,7 +806,8 @@ class _Fp8Layer(ctypes.Structure):
 
 class Fp8Linear:
     """`quantize_fp8` and `gemm_fp8` in one call: `Fp8Linear(weight, q, scales)(x, out)` with buffers q [max rows, columns] and scales
-    [column blocks, max rows] for the quantised input. What does not change from call to call is checked and laid out once, here."""
+    [column blocks, max rows] for the quantised input. What does not change from call to call is checked and laid out once, here. out does not
+    overlap x. Calls that share buffers run on one stream."""
 
     def __init__(self, weight, q: torch.Tensor, scales: torch.Tensor):
         _cuda(q, scales, weight.q)
@@ -824,10 +831,7 @@ class Fp8Linear:
         if K != self.K or rows != n or M != (self.M // 2 if gated else self.M) or n > self.rows or (K > 1 and step_x != 1) or (M > 1 and step_o != 1):
             raise ValueError(f"linear_fp8: x {tuple(x.shape)}, weight {(self.M, self.K)}, out {tuple(out.shape)}, at most {self.rows} rows, "
                              f"rows of consecutive elements")
-        if gated and self.halves != 2:
-            raise ValueError("a gated product takes a weight stacked from a gate and an up matrix of one shape")
-        if not gated and not self.in_blocks:
-            raise ValueError("a stacked weight whose matrices are no whole number of 128 rows only has the gated product")
+        check_fp8_epilogue(self, gated)
         if n <= 1:
             ldx, ldo = max(ldx, K), max(ldo, M)          # (of a single row the stride says nothing)
         call = _LINEAR_CALL.pack(self._address, x.data_ptr(), ldx, out.data_ptr(), ldo, dtype_code(x.dtype), dtype_code(out.dtype), n,

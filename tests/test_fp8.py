@@ -93,6 +93,24 @@ def test_calls_without_a_device_are_refused():
         layer.forward(torch.zeros(2, 64), torch.zeros(2, 128), workspace=Workspace(torch.device("cpu"), 2))
 
 
+def test_a_stacked_weight_that_has_only_the_gated_product_is_no_plain_layer_of_a_program():
+    from types import SimpleNamespace
+    from stride_b200.kernels.linear import Fp8Weight, Linear
+    from stride_b200.parts.context import Workspace
+    added = []
+    program = SimpleNamespace(workspace=Workspace(torch.device("cpu"), 2), h=torch.zeros(2, 128), take_fresh=lambda: None, need_folded=lambda what: None,
+                              add=lambda *a, **k: added.append(a))
+    layer = Linear(Fp8Weight.stack([_weight(64, 32), _weight(64, 32)]), torch.bfloat16)
+    x, flat = torch.zeros(2, 32), torch.zeros(256)
+    with pytest.raises(ValueError, match="only has the gated product"):
+        layer.emit_partials(program, x, flat)
+    with pytest.raises(ValueError, match="only has the gated product"):
+        layer.emit(program, x, flat.view(2, 128))
+    with pytest.raises(ValueError, match="only has the gated product"):
+        layer.emit_add(program, x)
+    assert not added
+
+
 def test_the_float32_engine_takes_what_the_weight_stands_for():
     from stride_b200.kernels.linear import Linear
     w = _weight(130, 200)
