@@ -54,6 +54,8 @@ __device__ __forceinline__ float exp_difference(float z, float top) {
   return fabsf(dropped) < 1.0f ? expf(d) * (1.0f + dropped) : expf(d);
 }
 
+__device__ __forceinline__ double sigmoid_64(float z) { return 1.0 / (1.0 + exp(-static_cast<double>(z))); }
+
 // This lane's values of a row of E: places lane PER .. lane PER + PER - 1 (`other` beyond). VEC: the row begins at a 16-byte border.
 template <int PER, bool VEC>
 __device__ __forceinline__ void load_lane(const float* row, int E, int lane, float other, float* v) {
@@ -69,9 +71,9 @@ __device__ __forceinline__ void load_lane(const float* row, int E, int lane, flo
   }
 }
 
-// Scores s and c of this lane's experts from its logits and biases; bit i of the result: the expert may be chosen. T: float or double.
+// The scores s of this lane's experts from their logits; bit i of the result: the logit allows a choice. T: double, or float, then of a softmax only.
 template <class T, int PER>
-__device__ __forceinline__ uint32_t scores(const Routing& r, const float* logits, const float* bias, T* s, T* c) {
+__device__ __forceinline__ uint32_t scores(const Routing& r, const float* logits, T* s) {
   uint32_t open = 0;
   float v[PER];
   float top = -INFINITY;
@@ -81,7 +83,7 @@ __device__ __forceinline__ uint32_t scores(const Routing& r, const float* logits
     v[i] = fminf(logits[i], FLT_MAX);
     if ((open >> i) & 1u) top = fmaxf(top, v[i]);
   }
-  if (r.softmax) {
+  if (sizeof(T) == 4 || r.softmax) {
     top = warp_max(top);
     T sum = 0;
 #pragma unroll
@@ -99,56 +101,50 @@ __device__ __forceinline__ uint32_t scores(const Routing& r, const float* logits
   } else {
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-      if constexpr (sizeof(T) == 8) s[i] = (open >> i) & 1u ? 1.0 / (1.0 + exp(-static_cast<double>(v[i]))) : 0.0;
-      else s[i] = __fdividef(1.0f, 1.0f + __expf(fminf(-v[i], 80.0f)));      // (to choose by; a chosen one's weight is computed anew)
+      const double all = sigmoid_64(v[i]);         // (of all: without branches they overlap)
+      s[i] = (open >> i) & 1u ? all : 0.0;
     }
-  }
-#pragma unroll
-  for (int i = 0; i < PER; ++i) {
-    if (!(bias[i] > -INFINITY)) open &= ~(1u << i);
-    c[i] = s[i] + static_cast<T>(bias[i]);
   }
   return open;
 }
 
-// The groups that stay, as bits of `open`. held: the warp's own E values of shared memory. gap (of float): the score of the last group that stays
-// minus the best that does not.
+// Whether a lane's experts are of one group, and a group's lanes a power of two.
+template <int PER>
+__device__ __forceinline__ bool whole_groups(const Routing& r) {
+  return r.size % PER == 0 && (r.size / PER & (r.size / PER - 1)) == 0;
+}
+
+// The experts whose groups stay, as bits. c: -infinity where an expert may not be chosen. held: the warp's own E values of shared memory. a, b: a
+// lane's two largest c, if `whole`. gap (of float): the score of the last group that stays minus the best that does not.
 template <class T, int PER>
-__device__ __forceinline__ uint32_t keep_groups(const Routing& r, int lane, const T* c, uint32_t open, T* held, T& gap) {
+__device__ __forceinline__ uint32_t keep_groups(const Routing& r, int lane, const T* c, T* held, T& gap, bool whole, T a, T b) {
   const int size = r.size;
-  T a = -INFINITY, b = -INFINITY;
-  int share = 1;              // neighbouring lanes that look through a group, a power of two
-  const bool whole = size % PER == 0 && (size / PER & (size / PER - 1)) == 0;        // a lane's experts are of one group, a group's lanes that many
+  int shift = 0;              // of the neighbouring lanes that look through a group: 1 << shift
   if (whole) {
-    share = size / PER;
-#pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      const T v = (open >> i) & 1u ? c[i] : static_cast<T>(-INFINITY);
-      b = v > a ? a : (v > b ? v : b);
-      a = v > a ? v : a;
-    }
+    shift = __ffs(size / PER) - 1;
   } else {
+    a = b = -INFINITY;
 #pragma unroll
     for (int i = 0; i < PER; ++i)
-      if (lane * PER + i < r.E) held[lane * PER + i] = (open >> i) & 1u ? c[i] : static_cast<T>(-INFINITY);
+      if (lane * PER + i < r.E) held[lane * PER + i] = c[i];
     __syncwarp();
-    while (2 * share * r.groups <= 32) share *= 2;
-    const int g = lane / share;
+    while ((2 << shift) * r.groups <= 32) ++shift;
+    const int g = lane >> shift, share = 1 << shift;
     if (g < r.groups) {
       const T* from = held + g * size;
-      for (int j = lane % share; j < size; j += share) {
+      for (int j = lane & (share - 1); j < size; j += share) {
         const T v = from[j];
         b = v > a ? a : (v > b ? v : b);
         a = v > a ? v : a;
       }
     }
   }
-  for (int o = 1; o < share; o <<= 1) {
+  for (int o = 1; o < 1 << shift; o <<= 1) {
     const T oa = __shfl_xor_sync(0xffffffffu, a, o), ob = __shfl_xor_sync(0xffffffffu, b, o);
     b = oa > a ? (a > ob ? a : ob) : (oa > b ? oa : b);
     a = oa > a ? oa : a;
   }
-  a = __shfl_sync(0xffffffffu, a, lane * share & 31), b = __shfl_sync(0xffffffffu, b, lane * share & 31);      // lane g: group g's
+  a = __shfl_sync(0xffffffffu, a, (lane << shift) & 31), b = __shfl_sync(0xffffffffu, b, (lane << shift) & 31);      // lane g: group g's
   if (lane >= r.groups) a = b = -INFINITY;
   __syncwarp();
   const T mine = r.group_best > 1 && b > static_cast<T>(-INFINITY) ? a + b : a;
@@ -164,11 +160,14 @@ __device__ __forceinline__ uint32_t keep_groups(const Routing& r, int lane, cons
   const T score = __shfl_sync(0xffffffffu, mine, __ffs(last) - 1);
   gap = next != 0 ? score - __shfl_sync(0xffffffffu, mine, __ffs(next) - 1) : static_cast<T>(INFINITY);
   if (score == static_cast<T>(-INFINITY)) gap = INFINITY;       // (groups with nothing in them: it does not matter which)
-  if (whole) return (kept >> (lane / share)) & 1u ? open : 0u;
+  if (whole) return (kept >> (lane >> shift)) & 1u ? 0xffffffffu : 0u;
+  uint32_t stay = 0;
 #pragma unroll
-  for (int i = 0; i < PER; ++i)
-    if ((open >> i) & 1u && !((kept >> group_of(r, lane * PER + i)) & 1u)) open &= ~(1u << i);
-  return open;
+  for (int i = 0; i < PER; ++i) {
+    const int g = group_of(r, lane * PER + i);
+    if (g < 32 && ((kept >> g) & 1u)) stay |= 1u << i;
+  }
+  return stay;
 }
 
 __device__ __forceinline__ void write_row(const Routing& r, int row, int lane, int e, double weight) {
@@ -186,8 +185,23 @@ __device__ __noinline__ void route_row_64(const Routing& r, int row, int lane, d
   load_lane<PER, false>(r.logits + row * r.ldz, r.E, lane, -INFINITY, z);
 #pragma unroll
   for (int i = 0; i < PER; ++i) bias[i] = r.bias != nullptr && lane * PER + i < r.E ? r.bias[lane * PER + i] : 0.0f;
-  uint32_t open = scores<double, PER>(r, z, bias, s, c);
-  if (r.groups > 1) open = keep_groups<double, PER>(r, lane, c, open, held, gap);
+  uint32_t open = scores<double, PER>(r, z, s);
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    if (!(bias[i] > -INFINITY)) open &= ~(1u << i);
+    c[i] = s[i] + static_cast<double>(bias[i]);
+  }
+  if (r.groups > 1) {
+    const bool whole = whole_groups<PER>(r);
+    double a = -INFINITY, b = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      if (!((open >> i) & 1u)) c[i] = -INFINITY;
+      b = c[i] > a ? a : (c[i] > b ? c[i] : b);
+      a = c[i] > a ? c[i] : a;
+    }
+    open &= keep_groups<double, PER>(r, lane, c, held, gap, whole, a, b);
+  }
   double sum = 0.0, kept_s = 0.0;
   int kept_e = -1;
   for (int k = 0; k < r.top; ++k) {
@@ -211,82 +225,154 @@ __device__ __noinline__ void route_row_64(const Routing& r, int row, int lane, d
   write_row(r, row, lane, kept_e, r.renormalise ? kept_s * r.scale / (sum + 1e-20) : kept_s * r.scale);
 }
 
-// Both arrays by descending key: Batcher's merge exchanges.
+// A key's value, without the bits that its place took. Below the lowest float's key: -infinity.
+constexpr uint32_t kLowestKey = 0x00800000u;
+__device__ __forceinline__ double score_64(const Routing& r, int e, float z) {
+  return sigmoid_64(fminf(z, FLT_MAX)) + (r.bias != nullptr ? static_cast<double>(r.bias[e]) : 0.0);
+}
+template <int PER>
+__device__ __forceinline__ double score_of_key(const Routing& r, int lane, uint32_t key, const float* z) {
+  const int e = lane * PER + static_cast<int>(key & (PER - 1u));
+  return key < kLowestKey ? -INFINITY : score_64(r, e, z[e]);
+}
+template <int PER>
+__device__ __forceinline__ float key_value(uint32_t key) {
+  const uint32_t k = key & ~(PER - 1u);
+  return key < kLowestKey ? -INFINITY : __uint_as_float((k & 0x80000000u) ? (k & 0x7FFFFFFFu) : ~k);
+}
+
+// By descending key: Batcher's merge exchanges.
 template <int N, int P, int K>
-__device__ __forceinline__ void merge_exchange(uint32_t* key, int* place) {
+__device__ __forceinline__ void merge_exchange(uint32_t* key) {
 #pragma unroll
   for (int a = 0; a + K < N; ++a) {
     constexpr int kFirst = K % P;
     const int b = a + K;
     if (a >= kFirst && (a - kFirst) % (2 * K) < K && a / (2 * P) == b / (2 * P)) {
-      const bool turned = key[a] < key[b];
       const uint32_t low = min(key[a], key[b]);
-      const int at = place[a];
       key[a] = max(key[a], key[b]), key[b] = low;
-      place[a] = turned ? place[b] : at, place[b] = turned ? at : place[b];
     }
   }
-  if constexpr (K > 1) merge_exchange<N, P, K / 2>(key, place);
-  else if constexpr (2 * P < N) merge_exchange<N, 2 * P, 2 * P>(key, place);
+  if constexpr (K > 1) merge_exchange<N, P, K / 2>(key);
+  else if constexpr (2 * P < N) merge_exchange<N, 2 * P, 2 * P>(key);
 }
 template <int N>
-__device__ __forceinline__ void sort_descending(uint32_t* key, int* place) {
-  if constexpr (N > 1) merge_exchange<N, 1, 1>(key, place);
+__device__ __forceinline__ void sort_descending(uint32_t* key) {
+  if constexpr (N > 1) merge_exchange<N, 1, 1>(key);
 }
 
 // A warp a token. In 32-bit first, where a score is off by less than a known share of the largest: a sigmoid by 2^-20 (its approximated exponential is
 // off by 2 + 1.2 |z| units in the last place, of which a quarter counts at most near and above 1/2, its division by two; 2^-16 where all scores
 // are small), a softmax by PER + 16 times 2^-24 (PER + 4 additions, four units in the last place of the exponential, a division); a sum with a bias
-// by 2^-23 of its size more. Where two candidates that follow one another, or the last group that stays and the first that does not, are
-// closer than twice that, the token is routed again in 64-bit. So the choice is that of 64-bit scores always, at the price of 32-bit ones for
-// nearly all tokens. 16,384 tokens of 256 experts in eight groups, eight chosen: everything in 64-bit 87 us, so 30 (560 GB/s; issue slots bound it,
-// some 1,000 instructions a token, eleven times the time of its bytes); one token 12.6 and 2.7.
+// by 2^-23 of its size more, and a key by PER - 1 times that, whose last bits hold the place of the lane's expert. (The sizes of the two that are
+// compared: what lies further down may be off by more, but lies further away by more than that.) Candidates that are closer to their
+// neighbours than both can be off are taken on beyond the last that is chosen, until one is not, and ranked again by 64-bit scores, a candidate a lane;
+// so are groups, if the last that stays is too close to the first that does not. What those do not settle (softmax with a bias or with groups, groups
+// that lie across lanes, too many candidates) is routed again in 64-bit as a whole. So the choice is that of 64-bit scores always, at the price of
+// 32-bit ones. (One token in 64-bit takes 10 us, and of thousands one is always among the last.)
+// 16,384 tokens of 256 experts in eight groups, eight chosen: everything in 64-bit 87 us.
 template <int PER>
 __device__ __forceinline__ void route_row(const Routing& r, int row, int lane, const float* z, const float* bias, double* held, float* held_scores) {
-  float s[PER], c[PER];
-  uint32_t open = scores<float, PER>(r, z, bias, s, c);
-  float high_s = 0.0f, high_c = 0.0f;
+  float c[PER], high_s = 0.0f;                   // c: -infinity if never to be chosen
+  {
+    float s[PER];
+    uint32_t open = 0;
+    if (r.softmax) {
+      open = scores<float, PER>(r, z, s);
+    } else {
 #pragma unroll
-  for (int i = 0; i < PER; ++i)
-    if ((open >> i) & 1u) high_s = fmaxf(high_s, s[i]), high_c = fmaxf(high_c, fabsf(c[i]));
-  // (both are not negative: their bits are ordered as they are)
-  high_s = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(high_s)));
-  high_c = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(high_c)));
-  const float off = r.softmax ? (PER + 16) * 0x1p-24f : high_s > 0.125f ? 0x1p-20f : 0x1p-16f;
-  const float near = 2.0f * (off * high_s + 0x1p-23f * high_c);
-  bool sure = high_c < INFINITY;
-  if (r.groups > 1) {
-    float gap;
-    open = keep_groups<float, PER>(r, lane, c, open, reinterpret_cast<float*>(held), gap);
-    sure = sure && gap > 2.0f * near;           // (sums of two)
-  }
-  uint32_t key[PER];                             // this lane's candidates, largest first: the order of c's bits (0: none) and the place
-  int place[PER];
+      for (int i = 0; i < PER; ++i) s[i] = __fdividef(1.0f, 1.0f + __expf(fminf(-z[i], 80.0f)));      // (to choose by; a chosen one's weight is computed anew)
+    }
 #pragma unroll
-  for (int i = 0; i < PER; ++i) {
-    key[i] = (open >> i) & 1u ? order_key(c[i]) : 0u, place[i] = i;
-    held_scores[lane * PER + i] = r.softmax ? s[i] : z[i];
-  }
-  sort_descending<PER>(key, place);
-  __syncwarp();
-  float sum = 0.0f, kept_s = 0.0f, before = INFINITY;
-  int kept_e = -1;
-  for (int k = 0; k <= r.top && sure; ++k) {     // (one more than is chosen: it may not be too close)
-    const uint32_t best = __reduce_max_sync(0xffffffffu, key[0]);
-    if (best == 0) break;
-    const int owner = __ffs(__ballot_sync(0xffffffffu, key[0] == best)) - 1;      // (equal ones are too close anyway)
-    const float value = __uint_as_float((best & 0x80000000u) ? (best & 0x7FFFFFFFu) : ~best);
-    sure = before - value > near;
-    before = value;
-    if (k == r.top) break;
-    const int e = owner * PER + __shfl_sync(0xffffffffu, place[0], owner);
-    if (lane == k) kept_e = e;                      // (at most 32 choices)
-    if (lane == owner) {
-#pragma unroll
-      for (int i = 0; i + 1 < PER; ++i) key[i] = key[i + 1], place[i] = place[i + 1];
-      key[PER - 1] = 0;
+    for (int i = 0; i < PER; ++i) {
+      c[i] = z[i] > -INFINITY && bias[i] > -INFINITY ? s[i] + bias[i] : -INFINITY;
+      high_s = fmaxf(high_s, s[i]);
+      held_scores[lane * PER + i] = r.softmax ? s[i] : z[i];
     }
   }
+  high_s = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(high_s)));      // (not negative: their bits are ordered as they are)
+  const float near = 2.0f * high_s * (r.softmax ? (PER + 16) * 0x1p-24f : high_s > 0.125f ? 0x1p-20f : 0x1p-16f) + 0x1p-113f;      // (e^-80, where a sigmoid ends)
+  constexpr float kShare = PER * 0x1p-23f;
+  const bool grouped = r.groups > 1, whole = whole_groups<PER>(r);
+  float gap = INFINITY, high_c = 0.0f;
+  bool stays = true;
+  if (grouped && !whole) {
+    const uint32_t stay = keep_groups<float, PER>(r, lane, c, reinterpret_cast<float*>(held), gap, false, 0.0f, 0.0f);
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      if (c[i] > -INFINITY) high_c = fmaxf(high_c, fabsf(c[i]));
+      if (!((stay >> i) & 1u)) c[i] = -INFINITY;
+    }
+  }
+  uint32_t key[PER];                             // this lane's candidates, largest first: the order of c's bits, the last of them the place
+#pragma unroll
+  for (int i = 0; i < PER; ++i) key[i] = (order_key(c[i]) & ~(PER - 1u)) | i;
+  sort_descending<PER>(key);
+  if (grouped && whole) {
+    const float a = key_value<PER>(key[0]), b = PER > 1 ? key_value<PER>(key[PER > 1]) : -INFINITY;
+    high_c = fmaxf(a > -INFINITY ? fabsf(a) : 0.0f, b > -INFINITY ? fabsf(b) : 0.0f);
+    stays = keep_groups<float, PER>(r, lane, c, reinterpret_cast<float*>(held), gap, true, a, b) != 0u;
+  }
+  __syncwarp();
+  bool sure = true;
+  if (grouped) {
+    high_c = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(high_c)));
+    sure = gap > 2.0f * near + 4.0f * kShare * high_c;           // (sums of two)
+    if (!sure && whole && !r.softmax) {
+      // the groups again by 64-bit sums of the lanes' largest two, if no lane's third is too close to its second
+      const float second = PER > 1 ? key_value<PER>(key[PER > 1]) : -INFINITY, third = PER > 2 ? key_value<PER>(key[PER > 2 ? 2 : 0]) : -INFINITY;
+      sure = __all_sync(0xffffffffu, third == -INFINITY || second - third > near + kShare * (fabsf(second) + fabsf(third)));
+      const double a = score_of_key<PER>(r, lane, key[0], held_scores), b = PER > 1 ? score_of_key<PER>(r, lane, key[PER > 1], held_scores) : -INFINITY;
+      double gap_64;
+      stays = keep_groups<double, PER>(r, lane, nullptr, held, gap_64, true, fmax(a, b), fmin(a, b)) != 0u;
+    }
+    if (!stays) {
+#pragma unroll
+      for (int i = 0; i < PER; ++i) key[i] = 0u;
+    }
+  }
+  float before = INFINITY;
+  int kept_e = -1, count = 0;
+  bool close = false;
+  while (sure) {
+    const uint32_t best = __reduce_max_sync(0xffffffffu, key[0]);
+    if (best < kLowestKey) break;
+    const float value = key_value<PER>(best);
+    const bool apart = count == 0 || before - value > near + kShare * (fabsf(before) + fabsf(value));
+    if (count >= r.top && apart) break;
+    close = close || !apart;
+    if (count == 32) sure = false;
+    const int owner = __ffs(__ballot_sync(0xffffffffu, key[0] == best)) - 1;
+    if (lane == count) kept_e = owner * PER + static_cast<int>(best & (PER - 1u));
+    if (lane == owner) {
+#pragma unroll
+      for (int i = 0; i + 1 < PER; ++i) key[i] = key[i + 1];
+      key[PER - 1] = 0;
+    }
+    before = value, ++count;
+  }
+  if (close && r.softmax && r.bias != nullptr) sure = false;
+  if (sure && close) {
+    double mine = -INFINITY;
+    if (r.softmax) {           // (by the exponentials: the sum, which is one for all, does not change their order)
+      const float v = kept_e >= 0 ? fminf(r.logits[row * r.ldz + kept_e], FLT_MAX) : -INFINITY, top = warp_max(v);
+      if (kept_e >= 0) mine = exp(static_cast<double>(v) - static_cast<double>(top));
+      sure = __all_sync(0xffffffffu, kept_e < 0 || mine > 1e-290);      // (where a division by the sum may make equals)
+    } else if (kept_e >= 0) {
+      mine = score_64(r, kept_e, held_scores[kept_e]);
+    }
+    int rank = 0, from = 0;
+    for (int j = 0; j < count; ++j) {
+      const double other = __shfl_sync(0xffffffffu, mine, j);
+      const int e = __shfl_sync(0xffffffffu, kept_e, j);
+      rank += other > mine || (other == mine && e < kept_e);
+    }
+    for (int j = 0; j < count; ++j)
+      if (__shfl_sync(0xffffffffu, rank, j) == lane) from = j;
+    const int e = __shfl_sync(0xffffffffu, kept_e, from);
+    kept_e = lane < min(count, r.top) ? e : -1;
+  }
+  float kept_s = 0.0f, sum = 0.0f;
   if (kept_e >= 0) kept_s = r.softmax ? held_scores[kept_e] : 1.0f / (1.0f + expf(-fminf(held_scores[kept_e], FLT_MAX)));
   if (r.renormalise) sum = warp_sum(kept_s);
   if (r.renormalise && kept_e >= 0 && sum < 0x1p-50f) sure = false;      // (scores below the smallest floats count where all are)

@@ -335,6 +335,34 @@ def test_routes_that_only_64_bits_tell_apart():
         assert torch.equal(choice, want), kw
 
 
+@pytest.mark.parametrize("E,kw", [(256, {"groups": 8, "top_groups": 4}), (64, {"groups": 4, "top_groups": 1, "group_best": 1}), (160, {"groups": 5, "top_groups": 2}),
+                                  (256, {}), (96, {"score": "softmax"}), (64, {"score": "softmax", "groups": 4, "top_groups": 2}), (512, {"groups": 2})])
+@pytest.mark.parametrize("biased", [False, True])
+def test_routes_whose_candidates_or_groups_are_next_to_equal(E, kw, biased):
+    """Some logits one 32-bit step from one another, all over the row or a group's beside another's; few rows of them and whole rows."""
+    n, groups = 48, kw.get("groups", 1)
+    z = _rand(E, n, E, std=1.0)
+    bias = (_rand(E + 1, E, std=0.1) if groups == 1 else _rand(E + 1, E // groups, std=0.1).repeat(groups)) if biased else None
+    up = torch.tensor(float("inf"), device="cuda")
+    size = E // groups
+    for row in range(0, n, 3):                         # a group like its neighbour, one of its logits a step further on
+        first = z[row, :size].clone() if groups > 1 else z[row, :E // 2].clone()
+        z[row, size * (groups > 1) or E // 2:][:first.numel()] = first
+        at = first.topk(2).indices[row % 2]
+        z[row, at] = torch.nextafter(z[row, at], up)
+    for row in range(1, n, 3):                         # the largest ones within a few steps
+        at = z[row].topk(12 if row % 2 else 40).indices
+        top = z[row].max()
+        for i, a in enumerate(at.flip(0)):
+            z[row, a] = top
+            if i % 2:
+                top = torch.nextafter(top, up)
+    choice, weights = _route(z, 8, bias, **kw)
+    want, want_weights = plain.route(z.cpu(), 8, kw.get("score", "sigmoid"), None if bias is None else bias.cpu(), **{k: v for k, v in kw.items() if k != "score"})
+    assert torch.equal(choice, want)
+    assert _close(weights, want_weights)
+
+
 def test_routes_of_rows_of_a_wider_tensor():
     from stride_b200.kernels import ops
     wide = _rand(6, 21, 77)
