@@ -114,21 +114,26 @@ __device__ __forceinline__ bool whole_groups(const Routing& r) {
   return r.size % PER == 0 && (r.size / PER & (r.size / PER - 1)) == 0;
 }
 
+template <int PER>
+__device__ __forceinline__ int lanes_of_group(const Routing& r, bool whole) {
+  if (whole) return __ffs(r.size / PER) - 1;
+  int shift = 0;
+  while ((2 << shift) * r.groups <= 32) ++shift;
+  return shift;
+}
+
 // The experts whose groups stay, as bits. c: -infinity where an expert may not be chosen. held: the warp's own E values of shared memory. a, b: a
-// lane's two largest c, if `whole`. gap (of float): the score of the last group that stays minus the best that does not.
+// lane's two largest c, if `given`. gap (of float): the score of the last group that stays minus the best that does not. 1 << shift neighbouring
+// lanes look through a group.
 template <class T, int PER>
-__device__ __forceinline__ uint32_t keep_groups(const Routing& r, int lane, const T* c, T* held, T& gap, bool whole, T a, T b) {
+__device__ __forceinline__ uint32_t keep_groups(const Routing& r, int lane, const T* c, T* held, T& gap, bool whole, int shift, bool given, T a, T b) {
   const int size = r.size;
-  int shift = 0;              // of the neighbouring lanes that look through a group: 1 << shift
-  if (whole) {
-    shift = __ffs(size / PER) - 1;
-  } else {
+  if (!given) {
     a = b = -INFINITY;
 #pragma unroll
     for (int i = 0; i < PER; ++i)
       if (lane * PER + i < r.E) held[lane * PER + i] = c[i];
     __syncwarp();
-    while ((2 << shift) * r.groups <= 32) ++shift;
     const int g = lane >> shift, share = 1 << shift;
     if (g < r.groups) {
       const T* from = held + g * size;
@@ -200,7 +205,7 @@ __device__ __noinline__ void route_row_64(const Routing& r, int row, int lane, d
       b = c[i] > a ? a : (c[i] > b ? c[i] : b);
       a = c[i] > a ? c[i] : a;
     }
-    open &= keep_groups<double, PER>(r, lane, c, held, gap, whole, a, b);
+    open &= keep_groups<double, PER>(r, lane, c, held, gap, whole, lanes_of_group<PER>(r, whole), whole, a, b);
   }
   double sum = 0.0, kept_s = 0.0;
   int kept_e = -1;
@@ -227,13 +232,33 @@ __device__ __noinline__ void route_row_64(const Routing& r, int row, int lane, d
 
 // A key's value, without the bits that its place took. Below the lowest float's key: -infinity.
 constexpr uint32_t kLowestKey = 0x00800000u;
-__device__ __forceinline__ double score_64(const Routing& r, int e, float z) {
-  return sigmoid_64(fminf(z, FLT_MAX)) + (r.bias != nullptr ? static_cast<double>(r.bias[e]) : 0.0);
-}
+
+// A row's largest logit and, in the order of `scores`, the 64-bit sum of its exponentials.
+struct Softmax64 {
+  float top;
+  double sum;
+};
 template <int PER>
-__device__ __forceinline__ double score_of_key(const Routing& r, int lane, uint32_t key, const float* z) {
-  const int e = lane * PER + static_cast<int>(key & (PER - 1u));
-  return key < kLowestKey ? -INFINITY : score_64(r, e, z[e]);
+__device__ __noinline__ Softmax64 softmax_64(const float* logits, int E, int lane) {
+  float z[PER], top = -INFINITY;
+  load_lane<PER, false>(logits, E, lane, -INFINITY, z);
+#pragma unroll
+  for (int i = 0; i < PER; ++i)
+    if (z[i] > -INFINITY) top = fmaxf(top, fminf(z[i], FLT_MAX));
+  top = warp_max(top);
+  double sum = 0.0;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const double all = exp(static_cast<double>(fminf(z[i], FLT_MAX)) - static_cast<double>(top));
+    sum += z[i] > -INFINITY ? all : 0.0;
+  }
+  return {top, warp_sum(sum)};
+}
+// An expert's 64-bit score with its bias, as `route_row_64` has it.
+__device__ __forceinline__ double score_64(const Routing& r, const float* logits, int e, const Softmax64& of) {
+  const float v = fminf(logits[e], FLT_MAX);
+  const double s = !r.softmax ? sigmoid_64(v) : of.sum > 0 ? exp(static_cast<double>(v) - static_cast<double>(of.top)) / of.sum : 0.0;
+  return s + (r.bias != nullptr ? static_cast<double>(r.bias[e]) : 0.0);
 }
 template <int PER>
 __device__ __forceinline__ float key_value(uint32_t key) {
@@ -267,10 +292,11 @@ __device__ __forceinline__ void sort_descending(uint32_t* key) {
 // by 2^-23 of its size more, and a key by PER - 1 times that, whose last bits hold the place of the lane's expert. (The sizes of the two that are
 // compared: what lies further down may be off by more, but lies further away by more than that.) Candidates that are closer to their
 // neighbours than both can be off are taken on beyond the last that is chosen, until one is not, and ranked again by 64-bit scores, a candidate a lane;
-// so are groups, if the last that stays is too close to the first that does not. What those do not settle (softmax with a bias or with groups, groups
-// that lie across lanes, too many candidates) is routed again in 64-bit as a whole. So the choice is that of 64-bit scores always, at the price of
+// so are groups, if the last that stays is too close to the first that does not. What that does not settle (more than 32 candidates, a group whose
+// third expert is as close to its second) is routed again in 64-bit as a whole. So the choice is that of 64-bit scores always, at the price of
 // 32-bit ones. (One token in 64-bit takes 10 us, and of thousands one is always among the last.)
-// 16,384 tokens of 256 experts in eight groups, eight chosen: everything in 64-bit 87 us.
+// 16,384 tokens of 256 experts in eight groups, eight chosen: everything in 64-bit 87 us, the close ones as a whole 30, so 18.7 (900 GB/s; issue slots
+// bound it, some 900 instructions a token: seven times the time of its bytes); one token 12.6 and 2.7; 8,192 of 160, six chosen of three groups of eight, 12.9.
 template <int PER>
 __device__ __forceinline__ void route_row(const Routing& r, int row, int lane, const float* z, const float* bias, double* held, float* held_scores) {
   float c[PER], high_s = 0.0f;                   // c: -infinity if never to be chosen
@@ -294,43 +320,57 @@ __device__ __forceinline__ void route_row(const Routing& r, int row, int lane, c
   const float near = 2.0f * high_s * (r.softmax ? (PER + 16) * 0x1p-24f : high_s > 0.125f ? 0x1p-20f : 0x1p-16f) + 0x1p-113f;      // (e^-80, where a sigmoid ends)
   constexpr float kShare = PER * 0x1p-23f;
   const bool grouped = r.groups > 1, whole = whole_groups<PER>(r);
-  float gap = INFINITY, high_c = 0.0f;
-  bool stays = true;
-  if (grouped && !whole) {
-    const uint32_t stay = keep_groups<float, PER>(r, lane, c, reinterpret_cast<float*>(held), gap, false, 0.0f, 0.0f);
-#pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      if (c[i] > -INFINITY) high_c = fmaxf(high_c, fabsf(c[i]));
-      if (!((stay >> i) & 1u)) c[i] = -INFINITY;
-    }
-  }
+  const float* logits = r.logits + row * r.ldz;
+  Softmax64 of = {0.0f, -1.0};                   // (once it is needed)
+  bool sure = true;
   uint32_t key[PER];                             // this lane's candidates, largest first: the order of c's bits, the last of them the place
 #pragma unroll
   for (int i = 0; i < PER; ++i) key[i] = (order_key(c[i]) & ~(PER - 1u)) | i;
-  sort_descending<PER>(key);
-  if (grouped && whole) {
-    const float a = key_value<PER>(key[0]), b = PER > 1 ? key_value<PER>(key[PER > 1]) : -INFINITY;
-    high_c = fmaxf(a > -INFINITY ? fabsf(a) : 0.0f, b > -INFINITY ? fabsf(b) : 0.0f);
-    stays = keep_groups<float, PER>(r, lane, c, reinterpret_cast<float*>(held), gap, true, a, b) != 0u;
-  }
-  __syncwarp();
-  bool sure = true;
   if (grouped) {
-    high_c = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(high_c)));
-    sure = gap > 2.0f * near + 4.0f * kShare * high_c;           // (sums of two)
-    if (!sure && whole && !r.softmax) {
-      // the groups again by 64-bit sums of the lanes' largest two, if no lane's third is too close to its second
-      const float second = PER > 1 ? key_value<PER>(key[PER > 1]) : -INFINITY, third = PER > 2 ? key_value<PER>(key[PER > 2 ? 2 : 0]) : -INFINITY;
-      sure = __all_sync(0xffffffffu, third == -INFINITY || second - third > near + kShare * (fabsf(second) + fabsf(third)));
-      const double a = score_of_key<PER>(r, lane, key[0], held_scores), b = PER > 1 ? score_of_key<PER>(r, lane, key[PER > 1], held_scores) : -INFINITY;
-      double gap_64;
-      stays = keep_groups<double, PER>(r, lane, nullptr, held, gap_64, true, fmax(a, b), fmin(a, b)) != 0u;
-    }
-    if (!stays) {
+    const int shift = lanes_of_group<PER>(r, whole);
+    float a = 0.0f, b = 0.0f, gap, high_c = 0.0f;
+    if (whole) {
+      sort_descending<PER>(key);
+      a = key_value<PER>(key[0]), b = PER > 1 ? key_value<PER>(key[PER > 1]) : -INFINITY;
+      high_c = fmaxf(a > -INFINITY ? fabsf(a) : 0.0f, b > -INFINITY ? fabsf(b) : 0.0f);
+    } else {
 #pragma unroll
-      for (int i = 0; i < PER; ++i) key[i] = 0u;
+      for (int i = 0; i < PER; ++i)
+        if (c[i] > -INFINITY) high_c = fmaxf(high_c, fabsf(c[i]));
     }
+    uint32_t stay = keep_groups<float, PER>(r, lane, c, reinterpret_cast<float*>(held), gap, whole, shift, whole, a, b);
+    high_c = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(high_c)));
+    if (!(gap > 2.0f * near + 4.0f * kShare * high_c)) {           // (sums of two)
+      // the groups again by 64-bit sums of the lanes' largest two, if no lane's third is too close to its second
+      float high[3] = {-INFINITY, -INFINITY, -INFINITY};
+      int at[2] = {0, 0};
+      if (whole) {
+        high[0] = a, high[1] = b, high[2] = PER > 2 ? key_value<PER>(key[PER > 2 ? 2 : 0]) : -INFINITY;
+        at[0] = lane * PER + static_cast<int>(key[0] & (PER - 1u)), at[1] = lane * PER + static_cast<int>(key[PER > 1] & (PER - 1u));
+      } else {
+        const float* from = reinterpret_cast<float*>(held);
+        const int g = lane >> shift, share = 1 << shift;
+#pragma unroll 1
+        for (int e = g * r.size + (lane & (share - 1)); e < (g + 1) * r.size && g < r.groups; e += share) {
+          const float v = from[e];
+          if (v > high[0]) high[2] = high[1], high[1] = high[0], at[1] = at[0], high[0] = v, at[0] = e;
+          else if (v > high[1]) high[2] = high[1], high[1] = v, at[1] = e;
+          else if (v > high[2]) high[2] = v;
+        }
+      }
+      const bool clear = high[2] == -INFINITY || high[1] - high[2] > near + kShare * (fabsf(high[1]) + fabsf(high[2]));
+      sure = __all_sync(0xffffffffu, clear);
+      if (r.softmax) of = softmax_64<PER>(logits, r.E, lane);
+      const double a64 = high[0] > -INFINITY ? score_64(r, logits, at[0], of) : -INFINITY, b64 = high[1] > -INFINITY ? score_64(r, logits, at[1], of) : -INFINITY;
+      double gap_64;
+      stay = keep_groups<double, PER>(r, lane, nullptr, nullptr, gap_64, whole, shift, true, fmax(a64, b64), fmin(a64, b64));
+    }
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
+      if (whole ? stay == 0u : !((stay >> i) & 1u)) key[i] = 0u;
   }
+  if (!grouped || !whole) sort_descending<PER>(key);
+  __syncwarp();
   float before = INFINITY;
   int kept_e = -1, count = 0;
   bool close = false;
@@ -351,16 +391,9 @@ __device__ __forceinline__ void route_row(const Routing& r, int row, int lane, c
     }
     before = value, ++count;
   }
-  if (close && r.softmax && r.bias != nullptr) sure = false;
   if (sure && close) {
-    double mine = -INFINITY;
-    if (r.softmax) {           // (by the exponentials: the sum, which is one for all, does not change their order)
-      const float v = kept_e >= 0 ? fminf(r.logits[row * r.ldz + kept_e], FLT_MAX) : -INFINITY, top = warp_max(v);
-      if (kept_e >= 0) mine = exp(static_cast<double>(v) - static_cast<double>(top));
-      sure = __all_sync(0xffffffffu, kept_e < 0 || mine > 1e-290);      // (where a division by the sum may make equals)
-    } else if (kept_e >= 0) {
-      mine = score_64(r, kept_e, held_scores[kept_e]);
-    }
+    if (r.softmax && of.sum < 0.0) of = softmax_64<PER>(logits, r.E, lane);
+    const double mine = kept_e >= 0 ? score_64(r, logits, kept_e, of) : -INFINITY;
     int rank = 0, from = 0;
     for (int j = 0; j < count; ++j) {
       const double other = __shfl_sync(0xffffffffu, mine, j);
