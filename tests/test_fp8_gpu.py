@@ -450,6 +450,29 @@ def test_two_streams_at_once():
         assert torch.equal(out[i][0], alone[i][0]) and torch.equal(out[i][1], alone[i][1])
 
 
+@pytest.mark.parametrize("n,E,top,offset", [(1, 1, 1, 0), (1, 64, 32, 0), (4, 5, 8, 0), (16, 2, 2, 0), (32, 70, 1, 0), (11, 5, 3, 0), (5, 6, 6, 1), (33, 40, 1, 0),
+                                            (31, 2, 1, 0), (6, 200, 5, 0)])
+def test_experts_of_few_choices(n, E, top, offset):
+    """Around 32 choices in all, up to which no kernel puts them in order: an expert of more rows than a tile, ids that are no expert's, repeated ones, an
+    input whose rows do not begin at 16 bytes; a call in a graph, replayed with other choices."""
+    W, F = 256, 136
+    layer, (gate, up, down) = _experts(E, W, F)
+    x = _rand(n, n, W + offset, dtype=BF)[:, offset:]
+    g = torch.Generator().manual_seed(n)
+    choice, weights = torch.randint(0, E, (n, top), generator=g, dtype=torch.int32).cuda(), torch.rand(top, n, generator=g).cuda()
+    scratch, out = layer.scratch(n, top), torch.empty(n, W, device="cuda")
+    layer.forward(x, choice, weights, out, scratch)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        layer.forward(x, choice, weights, out, scratch)
+    for other in (choice.clone(), torch.zeros_like(choice), torch.full_like(choice, -1), torch.where(choice % 2 == 0, choice.flip(0), E + 3)):
+        choice.copy_(other)
+        out.fill_(float("nan"))
+        graph.replay()
+        want, bound = plain.experts(x.to(F64), choice, weights, gate, up, down)
+        assert ((out.to(F64) - want).abs() <= bound + HALF_STEP[F32] * (want.abs() + bound)).all()
+
+
 def test_experts_of_a_token_do_not_depend_on_the_step():
     """Alone, in a few and in many, whoever else chose the same experts; the same twice over the same scratch."""
     layer, _ = _experts(8, 384, 264)
