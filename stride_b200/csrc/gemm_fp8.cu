@@ -1233,7 +1233,8 @@ gemm_fp8_token_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_co
 constexpr int kOrderThreads = 1024, kHeld = 16;
 __global__ void __launch_bounds__(kOrderThreads) expert_order_kernel(const int32_t* choice, int n, int top, int E, int tile,
                                                                      int32_t* order, int32_t* place, int32_t* list) {
-  __shared__ int count[kMaxExperts], next[kMaxExperts], tile_at[kMaxExperts];
+  __shared__ int count[kMaxExperts], next[kMaxExperts], tile_at[kMaxExperts], rows;
+  __shared__ __align__(4) uint16_t sorted[kHeld * kOrderThreads];      // the tokens of held choices by row (stored to memory one by one they took 6 us)
   sb::grid_launch_dependents();
   for (int e = threadIdx.x; e < E; e += blockDim.x) count[e] = 0;
   __syncthreads();
@@ -1242,14 +1243,20 @@ __global__ void __launch_bounds__(kOrderThreads) expert_order_kernel(const int32
   uint32_t held[kHeld];
 #pragma unroll
   for (int j = 0; j < kHeld; ++j) held[j] = t + j * kOrderThreads < pairs ? static_cast<uint32_t>(choice[t + j * kOrderThreads]) : 0xFFFFFFFFu;
+  int rank[kHeld];                       // a held choice's place among its expert's
 #pragma unroll
-  for (int j = 0; j < kHeld; ++j)
-    if (held[j] < static_cast<uint32_t>(E)) atomicAdd(&count[held[j]], 1);
-  for (int i = t + kHeld * kOrderThreads; i < pairs; i += kOrderThreads) {
-    const uint32_t e = static_cast<uint32_t>(choice[i]);
-    if (e < static_cast<uint32_t>(E)) atomicAdd(&count[e], 1);
-  }
+  for (int j = 0; j < kHeld; ++j) rank[j] = held[j] < static_cast<uint32_t>(E) ? atomicAdd(&count[held[j]], 1) : 0;
   __syncthreads();
+  int* held_of = reinterpret_cast<int*>(sorted);         // (of more choices than those: how many of an expert's are held)
+  if (pairs > kHeld * kOrderThreads) {
+    for (int e = t; e < E; e += kOrderThreads) held_of[e] = count[e];
+    __syncthreads();
+    for (int i = t + kHeld * kOrderThreads; i < pairs; i += kOrderThreads) {
+      const uint32_t e = static_cast<uint32_t>(choice[i]);
+      if (e < static_cast<uint32_t>(E)) atomicAdd(&count[e], 1);
+    }
+    __syncthreads();
+  }
   if (threadIdx.x < 32) {
     const int lane = threadIdx.x;
     int rows_before = 0, tiles_before = 0;
@@ -1263,7 +1270,7 @@ __global__ void __launch_bounds__(kOrderThreads) expert_order_kernel(const int32
       if (e < E) next[e] = rows_before + cs - c, tile_at[e] = tiles_before + ts - ct;
       rows_before += __shfl_sync(0xffffffffu, cs, 31), tiles_before += __shfl_sync(0xffffffffu, ts, 31);
     }
-    if (lane == 0) list[0] = tiles_before, list[1] = rows_before;
+    if (lane == 0) list[0] = tiles_before, list[1] = rows = rows_before;
   }
   __syncthreads();
   for (int e = threadIdx.x; e < E; e += blockDim.x) {
@@ -1271,19 +1278,29 @@ __global__ void __launch_bounds__(kOrderThreads) expert_order_kernel(const int32
     int32_t* to = list + 2 + 3 * static_cast<int64_t>(tile_at[e]);
     for (int r = first; r < end; r += tile, to += 3) to[0] = e, to[1] = r, to[2] = end;
   }
-  __syncthreads();
-  auto put = [&](int i, uint32_t e) {
-    int at = -1;
-    if (e < static_cast<uint32_t>(E)) {
-      at = atomicAdd(&next[e], 1);
-      order[at] = i / top;
-    }
-    place[i] = at;
-  };
 #pragma unroll
-  for (int j = 0; j < kHeld; ++j)
-    if (t + j * kOrderThreads < pairs) put(t + j * kOrderThreads, held[j]);
-  for (int i = t + kHeld * kOrderThreads; i < pairs; i += kOrderThreads) put(i, static_cast<uint32_t>(choice[i]));
+  for (int j = 0; j < kHeld; ++j) {
+    const int i = t + j * kOrderThreads;
+    if (i >= pairs) break;
+    const bool there = held[j] < static_cast<uint32_t>(E);
+    const int at = there ? next[held[j]] + rank[j] : -1;
+    if (there && pairs <= kHeld * kOrderThreads) sorted[at] = static_cast<uint16_t>(i / top);
+    else if (there) order[at] = i / top;
+    place[i] = at;
+  }
+  __syncthreads();
+  if (pairs <= kHeld * kOrderThreads) {
+    for (int i = t; i < rows; i += kOrderThreads) order[i] = sorted[i];
+    return;
+  }
+  for (int e = t; e < E; e += kOrderThreads) next[e] += held_of[e];
+  __syncthreads();
+  for (int i = t + kHeld * kOrderThreads; i < pairs; i += kOrderThreads) {
+    const uint32_t e = static_cast<uint32_t>(choice[i]);
+    const int at = e < static_cast<uint32_t>(E) ? atomicAdd(&next[e], 1) : -1;
+    if (at >= 0) order[at] = i / top;
+    place[i] = at;
+  }
 }
 
 // out[t] = the sum over the token's choices, in their order, of weight times result: parts [rows][ldp], rows 16-byte aligned, by `place` [n][top] (-1:

@@ -392,7 +392,8 @@ def _choices(seed, n, E, top, missing=0.0):
 
 
 EXPERTS = [(1, 4, 2, 128, 128, 0.0), (1, 64, 6, 256, 200, 0.0), (3, 8, 3, 300, 100, 0.3), (32, 8, 2, 512, 384, 0.0), (64, 3, 3, 200, 70, 0.2),
-           (257, 16, 4, 256, 520, 0.1), (1000, 4, 1, 384, 256, 0.5), (500, 40, 6, 640, 260, 0.0)]
+           (257, 16, 4, 256, 520, 0.1), (1000, 4, 1, 384, 256, 0.5), (500, 40, 6, 640, 260, 0.0),
+           (3000, 16, 6, 128, 128, 0.1)]
 
 
 @pytest.mark.parametrize("n,E,top,W,F,missing", EXPERTS)
