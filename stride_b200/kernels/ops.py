@@ -17,7 +17,7 @@ from .build import library
 F32, BF16 = 0, 1
 _DTYPE_CODE = {torch.float32: F32, torch.bfloat16: BF16}
 
-_configured: set = set()
+_configured: dict = {}          # (library, function) -> (library, function) with its argument types set
 
 
 def dtype_code(dtype: torch.dtype) -> int:
@@ -28,13 +28,14 @@ def dtype_code(dtype: torch.dtype) -> int:
 
 
 def _fn(lib_name: str, fn_name: str, argtypes):
-    lib = library(lib_name)
-    fn = getattr(lib, fn_name)
-    if (lib_name, fn_name) not in _configured:
+    entry = _configured.get((lib_name, fn_name))
+    if entry is None:
+        lib = library(lib_name)
+        fn = getattr(lib, fn_name)
         fn.argtypes = argtypes
         fn.restype = c_int
-        _configured.add((lib_name, fn_name))
-    return lib, fn
+        entry = _configured[lib_name, fn_name] = lib, fn
+    return entry
 
 
 launches = 0    # kernels launched through this module since import (bench.py reports the difference)
@@ -58,12 +59,13 @@ def _ptr(t) -> int:
 
 
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)      # (there are CUDA tensors by now: nothing is left to initialise)
 
 
 def _stream() -> int:
     """The current torch stream's handle (kernels are launched on it, so they order with torch's own work)."""
     if _raw_stream is not None:
-        return _raw_stream(torch.cuda.current_device())
+        return _raw_stream(_device())
     return torch.cuda.current_stream().cuda_stream
 
 
@@ -841,6 +843,7 @@ class Fp8Linear:
 
 
 ROUTER_SCORES = {"sigmoid": 0, "softmax": 1}
+_FLOAT, _INT = torch.float32, torch.int32
 
 
 def route_experts(logits: torch.Tensor, choice: torch.Tensor, weights: torch.Tensor, score: str = "sigmoid", bias=None, groups: int = 1,
@@ -850,12 +853,14 @@ def route_experts(logits: torch.Tensor, choice: torch.Tensor, weights: torch.Ten
     s + bias; weight s (divided by (the chosen s' sum + 1e-20) if `renormalise`) times `scale`.
     choice [n, top] int32, weights [top, n] float32. An expert with a logit or a bias of -infinity or NaN is never chosen; a place that nothing is
     left for gets -1 and weight 0."""
-    _cuda(logits, bias, choice, weights)
-    if score not in ROUTER_SCORES:
+    if not (logits.is_cuda and choice.is_cuda and weights.is_cuda and (bias is None or bias.is_cuda)):
+        _cuda(logits, bias, choice, weights)
+    code = ROUTER_SCORES.get(score)
+    if code is None:
         raise ValueError(f"route_experts: unknown score '{score}' (known: {', '.join(ROUTER_SCORES)})")
-    (n, E), (rows, top), f32 = logits.shape, choice.shape, torch.float32
+    (n, E), (rows, top), f32 = logits.shape, choice.shape, _FLOAT
     (ldz, step_z), (ldw, step_w) = logits.stride(), weights.stride()
-    if logits.dtype != f32 or weights.dtype != f32 or choice.dtype != torch.int32 or (bias is not None and bias.dtype != f32):
+    if logits.dtype is not f32 or weights.dtype is not f32 or choice.dtype is not _INT or (bias is not None and bias.dtype is not f32):
         raise TypeError("route_experts takes float32 logits, bias and weights and an int32 choice")
     if rows != n or weights.shape != (top, n) or not choice.is_contiguous() or (n > 1 and step_w != 1) or (E > 1 and step_z != 1) \
             or (bias is not None and (bias.shape != (E,) or not bias.is_contiguous())):
@@ -863,7 +868,7 @@ def route_experts(logits: torch.Tensor, choice: torch.Tensor, weights: torch.Ten
                          + (f", bias {tuple(bias.shape)}" if bias is not None else ""))
     lib, fn = _fn("router", "sb_route_experts", [c_char_p, c_void_p])
     call = _ROUTE_CALL.pack(logits.data_ptr(), ldz if n > 1 else max(ldz, E), 0 if bias is None else bias.data_ptr(), choice.data_ptr(), weights.data_ptr(),
-                            ldw if top > 1 else max(ldw, n), n, E, top, ROUTER_SCORES[score], groups, top_groups, group_best, int(renormalise), scale)
+                            ldw if top > 1 else max(ldw, n), n, E, top, code, groups, top_groups, group_best, 1 if renormalise else 0, scale)
     _check(lib, fn(call, _stream()))
 
 
