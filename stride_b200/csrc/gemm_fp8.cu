@@ -130,7 +130,7 @@ struct Fp8Params {
   int half_rows;
   int scale_rows;            // blocks of rows of one expert's scales
   int ranges, range_blocks;  // K ranges and blocks of columns in each
-  int split;                 // the ranges run on CTAs of their own
+  int split;                 // the ranges of a CTA, if they run on CTAs of their own; else 0
   int stages;
   int tiles_m, tiles_n, vec_out;      // (kernels that walk tiles; vec_out: the result takes 16-byte stores)
   const int32_t* tiles;      // experts: the list of `expert_order_kernel`; else null
@@ -982,17 +982,19 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
 
 // The same for more tokens than a few and fewer than many, with tokens as the product's rows too (with weight rows as the product's rows [6144, 4096] of
 // 128 tokens took 20.4 us, so 13.9): up to 128 tokens by 128
-// weight rows, or 64 gate rows and their 64 up rows. SPLIT: the K ranges are the CTAs of a cluster. Warp 0 loads, warp 1 issues the
+// weight rows, or 64 gate rows and their 64 up rows. SPLIT: the K ranges are shared out among the
+// CTAs of a cluster, one or two each (0: one CTA has them all). Warp 0 loads, warp 1 issues the
 // products, warp 2 multiplies the scales, sixteen warps are the epilogue, a token a lane and 32 columns each; those without tokens pass over.
 constexpr int kTokenThreads = 640, kTokenRows = 128, kTokenSlots = 4;
 constexpr int kRowPitch = 132;                   // floats from a token's sums to the next one's: 16-byte pieces of eight tokens meet in no bank
 constexpr int kTokenStage = 2 * kStageA, kTokenStages = 6;
 
-template <int EPI, class OUT, bool SPLIT>
+template <int EPI, class OUT, int SPLIT>
 __global__ void __launch_bounds__(kTokenThreads, 1)
 gemm_fp8_token_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const Fp8Params p) {
+  constexpr int kStages = SPLIT == 2 ? kTokenStages - 2 : kTokenStages;         // (two make room for the first range's sums)
   extern __shared__ __align__(1024) uint8_t smem_raw[];
-  __shared__ __align__(8) uint64_t full_bar[kTokenStages], empty_bar[kTokenStages];
+  __shared__ __align__(8) uint64_t full_bar[kStages], empty_bar[kStages];
   __shared__ __align__(8) uint64_t accum_full[kTokenSlots], accum_empty[kTokenSlots];
   __shared__ __align__(8) uint64_t factor_full[kBatches], factor_empty[kBatches];
   __shared__ float factor[kBatches][kBatch][EPI == kGated ? 2 : 1][kTokenRows];
@@ -1002,8 +1004,8 @@ gemm_fp8_token_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_co
   const uint32_t smem0 = (smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* smem0_p = smem_raw + (smem0 - smem_u32(smem_raw));
   const int tile_m = blockIdx.x;
-  const int b0 = SPLIT ? blockIdx.z * p.range_blocks : 0;
-  const int iters = (SPLIT ? min(p.blocks, b0 + p.range_blocks) : p.blocks) - b0;
+  const int b0 = SPLIT ? blockIdx.z * SPLIT * p.range_blocks : 0;
+  const int iters = (SPLIT ? min(p.blocks, b0 + SPLIT * p.range_blocks) : p.blocks) - b0;
 
   if (warp == 1) tmem_alloc(smem_u32(&tmem_base_s), 512);
   __syncthreads();
@@ -1013,7 +1015,7 @@ gemm_fp8_token_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_co
   if (threadIdx.x == 0) {
     prefetch_tensormap(&map_w);
     prefetch_tensormap(&map_x);
-    for (int s = 0; s < kTokenStages; ++s) mbar_init(smem_u32(&full_bar[s]), 1), mbar_init(smem_u32(&empty_bar[s]), 1);
+    for (int s = 0; s < kStages; ++s) mbar_init(smem_u32(&full_bar[s]), 1), mbar_init(smem_u32(&empty_bar[s]), 1);
     for (int s = 0; s < kTokenSlots; ++s) mbar_init(smem_u32(&accum_full[s]), 1), mbar_init(smem_u32(&accum_empty[s]), 4 * quarters);
     for (int s = 0; s < kBatches; ++s) mbar_init(smem_u32(&factor_full[s]), 32), mbar_init(smem_u32(&factor_empty[s]), 4 * quarters);
     mbar_init_fence();
@@ -1023,6 +1025,7 @@ gemm_fp8_token_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_co
   fence_after_sync();
   const uint32_t tmem_base = tmem_base_s;
   float* sums = reinterpret_cast<float*>(smem0_p);
+  constexpr int kFirstSums = SPLIT == 2 ? kStages * kTokenStage / 4 : 0;         // SPLIT 2: where the first range's are, the second's are `sums`
 
   if (warp == 0) {
     const int row_w = tile_m * (EPI == kGated ? 64 : kBlock);
@@ -1034,18 +1037,18 @@ gemm_fp8_token_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_co
     };
     auto load_x = [&](int i, int st) { issue_load<false>(smem0 + st * kTokenStage, &map_x, smem_u32(&full_bar[st]), (b0 + i) * kBlock, n0); };
     // (the weights are nobody's result: the first ring of them is under way before the kernels in front have ended)
-    const int ahead = min(iters, kTokenStages);
+    const int ahead = min(iters, kStages);
     for (int i = 0; i < ahead; ++i) load_w(i, i);
     sb::grid_dependency_wait();
     for (int i = 0; i < ahead; ++i) load_x(i, i);
-    int st = ahead == kTokenStages ? 0 : ahead;
+    int st = ahead == kStages ? 0 : ahead;
     uint32_t par = 0;
     for (int i = ahead; i < iters; ++i) {
       mbar_wait(smem_u32(&empty_bar[st]), par, p.status, 61);
       __syncwarp();
       load_w(i, st);
       load_x(i, st);
-      if (++st == kTokenStages) st = 0, par ^= 1;
+      if (++st == kStages) st = 0, par ^= 1;
     }
   } else if (warp == 1) {
     const uint32_t idesc = instr_desc_e4m3(kBlock);
@@ -1064,7 +1067,7 @@ gemm_fp8_token_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_co
       issue_products<false>(tmem_base + slot * kBlock, da, da + (kStageA >> 4), idesc);
       issue_signal<false>(smem_u32(&empty_bar[st]));
       issue_signal<false>(smem_u32(&accum_full[slot]));
-      if (++st == kTokenStages) st = 0, par ^= 1;
+      if (++st == kStages) st = 0, par ^= 1;
       if (++slot == kTokenSlots) slot = 0, slot_par ^= 1;
       ready = mbar_over(smem_u32(&accum_empty[slot]), slot_par) && mbar_over(smem_u32(&full_bar[st]), par);
     }
@@ -1147,12 +1150,18 @@ gemm_fp8_token_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_co
 #pragma unroll
         for (int c = 0; c < 32; ++c) total[c] += acc[c], acc[c] = 0.0f;
       }
+      if (SPLIT == 2 && i + 1 == min(p.range_blocks, iters)) {
+        float* to = sums + kFirstSums + token * kRowPitch + part * 32;
+#pragma unroll
+        for (int c = 0; c < 32; c += 4)
+          *reinterpret_cast<float4*>(to + c) = make_float4(acc[c], acc[c + 1], acc[c + 2], acc[c + 3]), acc[c] = acc[c + 1] = acc[c + 2] = acc[c + 3] = 0.0f;
+      }
     }
     // the sums to shared memory, a row a token: every load has arrived and every product that reads the ring is done
+    float* to = sums + token * kRowPitch + part * 32;
     const float* done = SPLIT ? acc : total;
 #pragma unroll
-    for (int c = 0; c < 32; c += 4)
-      *reinterpret_cast<float4*>(sums + token * kRowPitch + part * 32 + c) = make_float4(done[c], done[c + 1], done[c + 2], done[c + 3]);
+    for (int c = 0; c < 32; c += 4) *reinterpret_cast<float4*>(to + c) = make_float4(done[c], done[c + 1], done[c + 2], done[c + 3]);
   }
   __syncwarp();
   if (SPLIT) sb::cluster_sync();
@@ -1160,16 +1169,17 @@ gemm_fp8_token_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_co
   if (warp >= 4 && *reinterpret_cast<volatile int*>(p.status) == 0) {      // (a wait that gave up has left no sums)
     sb::grid_dependency_wait();
     const int rank = SPLIT ? static_cast<int>(sb::cluster_rank()) : 0, ranges = SPLIT ? p.ranges : 1;
+    const int ctas = SPLIT ? gridDim.z : 1;
     constexpr int kPer = EPI == kGated ? 2 : 4;                  // features of a lane
     const int m = tile_m * (EPI == kGated ? 64 : kBlock) + lane * kPer, M = EPI == kGated ? p.half_rows : p.M;
-    for (int t = rank + ranges * (warp - 4); t < count; t += ranges * 16) {
+    for (int t = rank + ctas * (warp - 4); t < count; t += ctas * 16) {
       float v[kPer], u[EPI == kGated ? 2 : 1];
       const uint32_t here = smem0 + (t * kRowPitch + lane * kPer) * 4;
       for (int r = 0; r < ranges; ++r) {
         float a[kPer], b[2] = {0.0f, 0.0f};
         if (SPLIT) {
           uint32_t peer;
-          asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(peer) : "r"(here), "r"(r));
+          asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(peer) : "r"(here + (SPLIT == 2 && (r & 1) == 0 ? 4 * kFirstSums : 0)), "r"(SPLIT == 2 ? r >> 1 : r));
 #pragma unroll
           for (int i = 0; i < kPer; i += 2) {
             const float2 x = sb::cluster_load_float2(peer + 4 * i);
@@ -1437,20 +1447,21 @@ int launch_token(const void* w, int64_t rows_w, int64_t ldw, const void* q, int6
     return sb::fail("gemm_fp8: no tensor map for a weight of %lld x %d (stride %lld)", (long long)rows_w, p.K, (long long)ldw);
   const int piece = (EPI == kGated ? 2 : 4) * static_cast<int>(sizeof(OUT));
   p.vec_out = p.ldo * sizeof(OUT) % piece == 0 && (reinterpret_cast<uintptr_t>(p.out) & (piece - 1)) == 0;
-  const size_t smem = static_cast<size_t>(kTokenStages) * kTokenStage + 1024;
-  const bool split = p.split != 0;
-  const dim3 grid(tiles_m, tiles_n, split ? p.ranges : 1);
-  static sb::DeviceOnce once[2];
+  const size_t smem = static_cast<size_t>(kTokenStages) * kTokenStage + (p.split == 2 ? kTokenRows * kRowPitch * 4 - 2 * kTokenStage : 0) + 1024;
+  const int ctas = p.split ? (p.ranges + p.split - 1) / p.split : 1;
+  const dim3 grid(tiles_m, tiles_n, ctas);
+  static sb::DeviceOnce once[3];
   auto run = [&](auto kernel, sb::DeviceOnce& first) {
     if (first.needed()) {
       if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)) != cudaSuccess) return sb::check_launch("gemm_fp8");
       first.done();
     }
-    if (split) sb::launch_pdl_cluster(kernel, grid, dim3(kTokenThreads), smem, st, dim3(1, 1, p.ranges), map_w, map_x, p);
+    if (p.split) sb::launch_pdl_cluster(kernel, grid, dim3(kTokenThreads), smem, st, dim3(1, 1, ctas), map_w, map_x, p);
     else sb::launch_pdl(kernel, grid, dim3(kTokenThreads), smem, st, map_w, map_x, p);
     return sb::check_launch("gemm_fp8");
   };
-  return split ? run(gemm_fp8_token_kernel<EPI, OUT, true>, once[0]) : run(gemm_fp8_token_kernel<EPI, OUT, false>, once[1]);
+  if (p.split == 2) return run(gemm_fp8_token_kernel<EPI, OUT, 2>, once[2]);
+  return p.split ? run(gemm_fp8_token_kernel<EPI, OUT, 1>, once[0]) : run(gemm_fp8_token_kernel<EPI, OUT, 0>, once[1]);
 }
 
 template <int EPI, bool WIDE, class OUT, bool GROUPED, bool PAIR>
@@ -1516,11 +1527,13 @@ int launch_quantize(const void* x, int xdtype, int64_t ldx, const int32_t* place
   return vec ? run(quantize_kernel<bf16, true>, static_cast<const bf16*>(x)) : run(quantize_kernel<bf16, false>, static_cast<const bf16*>(x));
 }
 
-// Tokens of a tile of the product; sets whether its K ranges run on CTAs of their own. Up to 128 tokens they do, more are for pairs of CTAs (gated
-// with ranges, whose sums and totals would not fit a pair's registers: for single ones), unless a weight of several ranges has so few tiles that
-// most pairs had none: then whichever takes fewer rounds of the SMs, a block of columns costing a pair some 0.43 us and a CTA of a
-// cluster 0.6, a round's beginning and end 5 and 3.5 ([4096, 14336] of 256 tokens: 49.7 us on pairs, 39.0 on clusters; [4096, 4096] 18.8 and 24.1;
-// [6144, 4096] of 333 32.8 and 26.1).
+// Tokens of a tile of the product; sets `split`, the K ranges of a CTA where they run on CTAs of their own (0: they do not). Up to 128 tokens they do,
+// one each. More are for pairs of CTAs (gated with ranges, whose sums and totals would not fit a pair's registers: for single ones), unless a weight
+// of several ranges has so few tiles that a cluster's CTAs, with one or two ranges each, are done sooner: in microseconds, a block of columns costs
+// a pair some 0.38, a single CTA 0.42, a cluster's CTA 0.34; a pass of pairs begins and ends in 4, a round of single CTAs in 2.3, of clusters in 4.8
+// gated, else in 6.6, with two ranges 7.5 (the first 6 of a further round). 256 tokens, [4096, 14336]: 49.7 us on pairs, 38.5 with a range each in
+// two rounds, 31.9 with two each; [4096, 4096] 23.9, 24.1, 16.7; [2048, 4096] gated 19.6 on single ones, 11.4 with a range each; [2500, 2056] 13.0 on
+// pairs, 14.2 with two each; 333 tokens, [6144, 4096]: 32.8 on pairs, 26.1 with a range each.
 //
 // More than 32 tokens of a weight with more tiles than SMs: walked too if the wide tiles then take half the rounds (a round of those takes half as
 // long again). 64 tokens, [20000, 2048]: 19.8 and 15.6 us, [28000, 4096]: 31.2 and 26.6; [14000, 8192], one round either way: 27.1 and 39.6.
@@ -1535,14 +1548,19 @@ int token_tile(Fp8Params& p, int epilogue) {
     if (p.ranges == 1 && (tiles + sms - 1) / sms >= 2 * ((wide + sms - 1) / sms)) return kPairTokens;
     return p.n <= 64 ? 64 : kTokenRows;
   }
-  if (p.split && !gated) {
-    const long long tiles = (p.M + kBlock - 1) / kBlock;
+  if (p.ranges > 1) {
+    const long long tiles = gated ? (p.half_rows + 63) / 64 : (p.M + kBlock - 1) / kBlock, of_tokens = (p.n + kTokenRows - 1) / kTokenRows;
     const long long pair_rounds = (tiles * ((p.n + kPairTokens - 1) / kPairTokens) + sms / 2 - 1) / (sms / 2);
-    const long long split_rounds = (tiles * ((p.n + kTokenRows - 1) / kTokenRows) * p.ranges + sms - 1) / sms;
-    if (split_rounds * (60 * p.range_blocks + 350) < pair_rounds * 43 * p.blocks + 500) return kTokenRows;
+    auto rounds = [&](int ctas) { return (tiles * of_tokens * ctas + sms - 1) / sms; };
+    long long best = gated ? rounds(1) * (42 * p.blocks + 230) : pair_rounds * 38 * p.blocks + 400;
+    p.split = 0;
+    for (int each = 1; each <= 2 && each < p.ranges; ++each) {
+      const long long c = rounds((p.ranges + each - 1) / each) * (34 * each * p.range_blocks + (gated ? 480 : 600)) + (gated ? 0 : each == 1 ? 60 : 150);
+      if (c < best) best = c, p.split = each;
+    }
+    if (gated || p.split != 0) return kTokenRows;
   }
-  p.split = 0;
-  return gated && p.ranges > 1 ? kTokenRows : kPairTokens;
+  return kPairTokens;
 }
 
 // The input as it is, for the forms that quantise it themselves: they copy 16 bytes at a time.

@@ -90,7 +90,7 @@ def test_quantised_rows_at_the_ends_of_the_range(dtype):
 
 
 SIZES = [(1, 1, 1), (1, 128, 128), (2, 130, 100), (16, 2048, 2048), (17, 500, 1000), (40, 128, 4096), (64, 1000, 900), (65, 300, 2056), (129, 256, 640),
-         (333, 2500, 2056), (1000, 640, 384), (300, 12000, 256), (3000, 1300, 384), (200, 1000, 4096), (50, 20000, 256), (120, 19000, 130)]
+         (333, 2500, 2056), (1000, 640, 384), (300, 12000, 256), (3000, 1300, 384), (200, 1000, 4096), (50, 20000, 256), (120, 19000, 130), (600, 1001, 4090)]
 
 
 @pytest.mark.parametrize("n,M,K", SIZES)
@@ -105,7 +105,7 @@ def test_product(n, M, K, x_dtype, out_dtype):
     assert ((out.to(F64) - want).abs() <= bound + HALF_STEP[out_dtype] * (want.abs() + bound)).all()
 
 
-@pytest.mark.parametrize("n,I,K", [(1, 1, 16), (1, 64, 128), (3, 100, 300), (8, 8192, 2048), (31, 65, 2048), (64, 1000, 520), (200, 200, 700), (333, 1408, 2056)])
+@pytest.mark.parametrize("n,I,K", [(1, 1, 16), (1, 64, 128), (3, 100, 300), (8, 8192, 2048), (31, 65, 2048), (64, 1000, 520), (200, 200, 700), (333, 1408, 2056), (150, 200, 1100), (300, 1400, 2048)])
 @pytest.mark.parametrize("out_dtype", [BF, F32])
 def test_gated_product(n, I, K, out_dtype):
     """Gate and up matrices of any height, also where the up rows' scales do not begin at a multiple of 128."""
@@ -158,6 +158,28 @@ def test_a_tokens_bits_do_not_depend_on_the_step(M, K):
         part = torch.full((n, M), float("nan"), device="cuda")
         layer.forward(x[first:first + n], part, workspace=_workspace(300))
         assert torch.equal(part, whole[first:first + n]), (first, n)
+
+
+@pytest.mark.parametrize("n,M,K,gated", [(600, 1001, 4090, False), (256, 4096, 1100, False), (300, 2816, 2048, True), (150, 400, 1100, True), (520, 1400, 4096, True)])
+def test_bits_of_many_tokens_whose_ranges_are_shared_out(n, M, K, gated):
+    """Weights of three and four ranges of K, a CTA of a cluster with one or two of them: the bits of a few tokens, where every range has a CTA; stored, gated
+    and added to a residual."""
+    from stride_b200.kernels import ops
+    from stride_b200.kernels.linear import Fp8Weight, Linear
+    x, W = _rand(M, n, K, dtype=BF), M // 2 if gated else M
+    weight = Fp8Weight.stack([_weight(K, W, K), _weight(K + 1, W, K)]) if gated else _weight(K, M, K)
+    layer, ws = Linear(weight, BF), _workspace(n)
+    run = (lambda x, out: layer.forward_swiglu(x, out, None, workspace=ws)) if gated else (lambda x, out: layer.forward(x, out, workspace=ws))
+    whole, part = torch.full((n, W), float("nan"), device="cuda"), torch.full((40, W), float("nan"), device="cuda")
+    run(x, whole)
+    for first in (0, 90, n - 40):
+        run(x[first:first + 40], part)
+        assert torch.equal(part, whole[first:first + 40]), first
+    if not gated:
+        h = _rand(3, n, M)
+        added = h.clone()
+        ops.gemm_fp8(*_quantize(x), weight, added, ops.ADD)
+        assert torch.equal(added, whole + h)
 
 
 @pytest.mark.parametrize("n", [1, 9, 16, 30, 50, 100, 300])
