@@ -152,7 +152,11 @@ __device__ __forceinline__ uint32_t keep_groups(const Routing& r, int lane, cons
   a = __shfl_sync(0xffffffffu, a, (lane << shift) & 31), b = __shfl_sync(0xffffffffu, b, (lane << shift) & 31);      // lane g: group g's
   if (lane >= r.groups) a = b = -INFINITY;
   __syncwarp();
-  const T mine = r.group_best > 1 && b > static_cast<T>(-INFINITY) ? a + b : a;
+  T mine = a;
+  if (r.group_best > 1 && b > static_cast<T>(-INFINITY)) {
+    mine = a + b;
+    if (sizeof(T) == 4) mine = fmax(mine, static_cast<T>(-FLT_MAX));      // (a sum beyond the floats is no empty group: those alone are -infinity)
+  }
   int before = 0;                              // groups that come before this lane's
 #pragma unroll 4
   for (int g = 0; g < r.groups; ++g) {

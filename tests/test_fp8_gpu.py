@@ -541,3 +541,22 @@ def test_router_and_experts_together():
         want, bound = plain.experts(x.to(F64), choice, want_weights.cuda(), gate, up, down)
         bound = bound + 2.0 ** -20 * want.abs().amax()
         assert ((out.to(F64) - want).abs() <= bound + 2.0 ** -8 * (want.abs() + bound)).all()
+
+
+@pytest.mark.parametrize("E,groups", [(8, 4), (12, 4), (64, 4), (160, 5), (256, 8)])
+@pytest.mark.parametrize("score", ["sigmoid", "softmax"])
+def test_groups_whose_best_two_sum_beyond_the_floats(E, groups, score):
+    """Experts pushed down by biases of the lowest float, or up by the largest: groups judged by sums that 32 bits do not hold, beside groups in which
+    every expert is switched off."""
+    low, size = torch.finfo(F32).min, E // groups
+    z = _rand(E, 5, E)
+    for biases in ([None, low, None, None], [None, low, None, -3.0e38], [-3.2e38, low, None, -3.0e38], [0.0, None, -low, 3.0e38], [low, -low, low, low]):
+        bias = torch.full((E,), float("-inf"), device="cuda")
+        for g, value in enumerate(biases):
+            if value is not None:
+                bias[g * size:(g + 1) * size] = value
+        for top_groups in (1, 2):
+            kw = {"groups": groups, "top_groups": top_groups, "group_best": 2}
+            choice, _ = _route(z, 2, bias, score=score, **kw)
+            want, _ = plain.route(z.cpu(), 2, score, bias.cpu(), **kw)
+            assert torch.equal(choice, want), (biases, top_groups)
