@@ -20,6 +20,21 @@ class ConfigError(ValueError):
     """A config.json key is missing or has a value this engine does not support."""
 
 
+# The one form of `quantization_config` that describes stored matrices which the kernels take as they are.
+_QUANTISATION = {"quant_method": "fp8", "weight_block_size": [128, 128], "activation_scheme": "dynamic", "fmt": "e4m3"}
+
+
+def other_quantisation(config: dict) -> Optional[str]:
+    """Why matrices in 8 bits beside this config.json are not weights with a scale per block of 128 x 128; None where its `quantization_config` says
+    that they are, or is absent."""
+    given = config.get("quantization_config")
+    if given is not None:
+        for key, only in _QUANTISATION.items():
+            if not isinstance(given, dict) or given.get(key, only if key == "fmt" else None) != only:
+                return f"config.json: quantization_config needs '{key}' = {only!r} (weights in 8 bits with a scale per block of 128 x 128)"
+    return None
+
+
 @dataclass(frozen=True)
 class RopeScaling:
     rope_type: str = "default"           # "default" | "llama3"
@@ -74,12 +89,9 @@ class LlamaConfig:
         for key in ("attention_bias", "mlp_bias"):
             if j.get(key):
                 raise ConfigError(f"config.json: '{key}' = true is not supported (the decoder has no bias terms)")
-        quantised = j.get("quantization_config")
-        if quantised is not None:
-            known = {"quant_method": "fp8", "weight_block_size": [128, 128], "activation_scheme": "dynamic", "fmt": "e4m3"}
-            for key, only in known.items():
-                if not isinstance(quantised, dict) or quantised.get(key, only if key == "fmt" else None) != only:
-                    raise ConfigError(f"config.json: quantization_config needs '{key}' = {only!r} (weights in 8 bits with a scale per block of 128 x 128)")
+        other = other_quantisation(j)
+        if other is not None:
+            raise ConfigError(other)
         act = j.get("hidden_act", "silu")
         if act != "silu":
             raise ConfigError(f"config.json: hidden_act '{act}' is not supported (only 'silu')")

@@ -44,4 +44,10 @@ def llama_model_spec(cfg: LlamaConfig) -> ModelSpec:
         max_positions=cfg.max_position_embeddings, eos_token_ids=cfg.eos_token_ids)
 
 
-register_architecture(Architecture("LlamaForCausalLM", LlamaConfig.from_dict, llama_model_spec), "llama")
+def _parse_config(config: dict) -> LlamaConfig:
+    """A `quantization_config` of any kind may stand beside plain matrices (it describes a cache, or what a conversion left behind): what it says counts
+    once a matrix in 8 bits is met (`weights.loader`)."""
+    return LlamaConfig.from_dict({key: value for key, value in config.items() if key != "quantization_config"})
+
+
+register_architecture(Architecture("LlamaForCausalLM", _parse_config, llama_model_spec), "llama")

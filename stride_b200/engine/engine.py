@@ -125,9 +125,9 @@ class Engine:
             self._status_device = ops.shared_status_word(libraries | {"sampling"})
         plan = self.model.tensor_plan()
         if tensors is None:
-            tensors = load_weights(model_dir, plan, self.device)
+            tensors = load_weights(model_dir, plan, self.device, config)
         else:
-            check_plan(with_scales(plan, {n: t.dtype for n, t in tensors.items()}), {n: tuple(t.shape) for n, t in tensors.items()}, "the given tensors")
+            check_plan(with_scales(plan, {n: t.dtype for n, t in tensors.items()}, config), {n: tuple(t.shape) for n, t in tensors.items()}, "the given tensors")
             tensors = join_scales({n: t.to(self.device) for n, t in tensors.items()})
         if self._status_device is not None and any(isinstance(t, Fp8Weight) for t in tensors.values()):
             ops.shared_status_word({"gemm_fp8"})

@@ -16,6 +16,7 @@ from pathlib import Path
 
 import torch
 
+from ..config.llama import ConfigError, other_quantisation
 from ..kernels.linear import FP8_SCALES, Fp8Weight, fp8_scales_shape
 from .safetensors_io import SafetensorsFile
 
@@ -45,12 +46,16 @@ def check_plan(plan: dict, available: dict, source: str) -> None:
     raise WeightsError("\n".join(lines), missing, unexpected, wrong)
 
 
-def with_scales(plan: dict, dtypes: dict) -> dict:
-    """`plan` with a scale tensor beside every matrix that is stored in 8 bits. `dtypes`: name -> dtype of the stored tensors."""
+def with_scales(plan: dict, dtypes: dict, config: dict | None = None) -> dict:
+    """`plan` with a scale tensor beside every matrix that is stored in 8 bits. `dtypes`: name -> dtype of the stored tensors; `config`: the
+    config.json beside them, whose `quantization_config` then has to be of this form."""
     out = {}
     for name, want in plan.items():
         out[name] = want
         if dtypes.get(name) == torch.float8_e4m3fn:
+            other = other_quantisation(config or {})
+            if other is not None:
+                raise ConfigError(f"{name} is stored in 8 bits; {other}")
             if not want.fp8:
                 raise WeightsError(f"{name} is stored in 8 bits, which its layer does not take", wrong_shape=())
             out[name + FP8_SCALES] = type(want)(fp8_scales_shape(*want.shape))
@@ -114,12 +119,13 @@ def tensor_shapes(model_dir) -> dict:
             f.close()
 
 
-def load_weights(model_dir, plan: dict, device) -> dict:
-    """Read the model folder's safetensors (one file or shards), check them against `plan`, return name -> device tensor."""
+def load_weights(model_dir, plan: dict, device, config: dict | None = None) -> dict:
+    """Read the model folder's safetensors (one file or shards), check them against `plan` (and 8-bit matrices against the `config` beside them),
+    return name -> device tensor."""
     where = _open_files(model_dir)
     try:
         dtypes = {n: f.dtype(n) for n, f in where.items()}
-        check_plan(with_scales(plan, dtypes), {n: f.shape(n) for n, f in where.items()}, str(Path(model_dir)))
+        check_plan(with_scales(plan, dtypes, config), {n: f.shape(n) for n, f in where.items()}, str(Path(model_dir)))
         out = {}
         for name, want in plan.items():
             if name not in where:

@@ -17,6 +17,7 @@ from pathlib import Path
 import torch
 
 from ..config import resolve_architecture
+from ..config.llama import other_quantisation
 from ..kernels.linear import FP8_SCALES, Fp8Weight
 from ..parts import BuildEnv, DecoderModel
 from .safetensors_io import write_safetensors
@@ -37,13 +38,13 @@ def model_plan(config: dict) -> dict:
 def random_tensors(config: dict, seed: int, device="cpu", dtype=torch.bfloat16, std: float = 0.02,
                    gain_std: float = 0.1, include_optional: bool | None = None) -> dict:
     """name -> tensor for every tensor of the plan. Optional tensors (an untied head) are made when
-    `include_optional`, which defaults to config['tie_word_embeddings'] being false. With a
-    `quantization_config`, matrices that may be stored in 8 bits are, rounded from those values, each beside its scales."""
+    `include_optional`, which defaults to config['tie_word_embeddings'] being false. With a `quantization_config` of 8 bits and
+    blocks of 128 x 128, matrices that may be stored so are, rounded from those values, each beside its scales."""
     plan = model_plan(config)
     if include_optional is None:
         include_optional = config.get("tie_word_embeddings") is False
     device = torch.device(device)
-    quantised = config.get("quantization_config") is not None
+    quantised = config.get("quantization_config") is not None and other_quantisation(config) is None
     out = {}
     for name, want in plan.items():
         if want.optional and not include_optional:

@@ -191,3 +191,33 @@ def test_scored_experts_take_8_bit_matrices_in_the_bfloat16_engine():
     tensors = {n: torch.zeros(p.shape, dtype=torch.bfloat16) for n, p in part.tensor_plan().items()}
     with pytest.raises(TypeError, match="8 bits"):
         part.bind(tensors)
+
+
+OTHER = {"quant_method": "fp8", "weight_block_size": [64, 128], "activation_scheme": "dynamic"}
+
+
+@pytest.mark.parametrize("given", [OTHER, {"quant_method": "awq", "bits": 4}, {"kv_cache_scheme": {"num_bits": 8}}, "none"])
+def test_a_quantisation_of_another_kind_counts_only_where_matrices_are_in_8_bits(tmp_path, given):
+    """Plain matrices load whatever the key says, and random ones are written plain; 8-bit ones beside it are refused by name."""
+    from stride_b200.config import ConfigError, resolve_architecture
+    from stride_b200.weights.loader import load_weights
+    from stride_b200.weights.random_init import model_plan, random_tensors, write_random_model
+    from stride_b200.weights.safetensors_io import write_safetensors
+    config = {**CONFIG, "quantization_config": given}
+    assert resolve_architecture(config).parse_config(config).hidden_size == CONFIG["hidden_size"]
+    folder = write_random_model(tmp_path / "m", config, 3)
+    plan = model_plan(config)
+    loaded = load_weights(folder, plan, "cpu", config)
+    assert all(isinstance(t, torch.Tensor) and t.dtype == torch.bfloat16 for t in loaded.values())
+    write_safetensors(folder / "model.safetensors", random_tensors(CONFIG, 3))
+    with pytest.raises(ConfigError, match="is stored in 8 bits; .*quantization_config needs"):
+        load_weights(folder, plan, "cpu", config)
+    assert load_weights(folder, plan, "cpu", CONFIG)
+
+
+def test_random_weights_of_other_designs_go_by_the_form_too():
+    from stride_b200.weights.random_init import random_tensors
+    from keralorn_cases import KERALORN_P
+    plain_names = set(random_tensors(KERALORN_P, 1))
+    assert set(random_tensors({**KERALORN_P, "quantization_config": OTHER}, 1)) == plain_names
+    assert set(random_tensors({**KERALORN_P, "quantization_config": CONFIG["quantization_config"]}, 1)) >= plain_names
