@@ -53,6 +53,8 @@ class Fp8Weight:
         rows = halves * -(-(M // halves) // ops.FP8_BLOCK)
         if scales.dim() != 2 or tuple(scales.shape) != (rows, -(-K // ops.FP8_BLOCK)) or scales.dtype != torch.float32:
             raise ValueError(f"the scales of a {M} x {K} weight are float32 [{rows}, {-(-K // ops.FP8_BLOCK)}], not {scales.dtype} {list(scales.shape)}")
+        if scales.device != q.device:
+            raise ValueError(f"an 8-bit weight on {q.device} has its scales there too, not on {scales.device}")
         self.shape = (M, K)
         self.stride = -(-K // 16) * 16
         if q.stride(0) == self.stride and (K == 1 or q.stride(1) == 1) and q.data_ptr() % 16 == 0 and self.stride == K:
@@ -125,6 +127,8 @@ class Fp8Experts:
         shapes = {w.shape for w in gate_up}, {w.shape for w in down}
         if len(gate_up) != 2 * len(down) or not down or len(shapes[0]) != 1 or len(shapes[1]) != 1 or down[0].shape != gate_up[0].shape[::-1]:
             raise ValueError("experts have a gate and an up matrix [inner, width] and a down matrix [width, inner] each")
+        if len({w.device for w in gate_up + down}) != 1:
+            raise ValueError("the experts' matrices are all on one device")
         self.experts = len(down)
         self.inner, self.width = gate_up[0].shape
         self.gate_up = torch.cat([w.q.view(torch.uint8) for w in gate_up]).view(torch.float8_e4m3fn)
@@ -134,6 +138,7 @@ class Fp8Experts:
         self._layout = ops._Fp8ExpertsLayout(self.gate_up.data_ptr(), self.gate_up.stride(0), self.gate_up_scales.data_ptr(), self.down.data_ptr(),
                                              self.down.stride(0), self.down_scales.data_ptr(), self.experts, self.width, self.inner)
         self.address = ctypes.addressof(self._layout)
+        self.at = self.down.get_device()          # -1: not on a CUDA device
 
     def weight_bytes(self) -> int:
         """Of one expert."""

@@ -731,6 +731,18 @@ FP8_BLOCK = 128
 _EPILOGUES_FP8 = {STORE: 0, ADD: 1, SWIGLU: 2, GEGLU_TANH: 2, CLAMPED_GLU: 2}
 
 
+def _refuse_devices(what: str, *tensors) -> None:
+    """Raises: the tensors are not all on the current CUDA device, where the kernel would be launched (it would read addresses of another)."""
+    _cuda(*tensors)
+    raise ValueError(f"{what}: tensors on {', '.join(sorted({str(t.device) for t in tensors if t is not None}))}, the current device is cuda:{_device()}")
+
+
+def _check_devices(what: str, *tensors) -> None:
+    at = tensors[0].get_device()
+    if at < 0 or any(t.get_device() != at for t in tensors) or _device() != at:
+        _refuse_devices(what, *tensors)
+
+
 def _check_fp8_rows(what: str, q: torch.Tensor, scales: torch.Tensor, n: int, K: int) -> None:
     if q.dtype != torch.float8_e4m3fn or scales.dtype != torch.float32:
         raise TypeError(f"{what}: quantised rows are float8_e4m3fn with float32 scales")
@@ -749,7 +761,7 @@ def quantize_fp8(x: torch.Tensor, q: torch.Tensor, scales: torch.Tensor) -> None
     """q[i, j] = e4m3(x[i, j] / s), s = scales[j // 128, i] = 2^e the smallest power of two (e >= -100) with max |x| of the row's block of 128
     columns / s <= 448. x [n, K] float32 or bfloat16; q [n, K or more columns] float8_e4m3fn with rows 16-byte aligned; scales float32
     [ceil(K / 128), n or more]. A block that holds an infinity or a NaN gets the scale NaN."""
-    _cuda(x, q, scales)
+    _check_devices("quantize_fp8", x, q, scales)
     n, K = x.shape
     _check_fp8_rows("quantize_fp8", q, scales, n, K)
     if x.stride(1) != 1 and K > 1:
@@ -783,7 +795,7 @@ def gemm_fp8(q: torch.Tensor, scales: torch.Tensor, weight, out: torch.Tensor, e
     STORE: out float32 or bfloat16 [n, M]. ADD: out float32 += result. SWIGLU, GEGLU_TANH, CLAMPED_GLU: weight stacked from gate and up rows,
     out float32 or bfloat16 [n, M / 2] (`gemm_tc`). out overlaps no input. The weight may be read while this module's kernels in front still run:
     it is not what one of them writes."""
-    _cuda(q, scales, weight.q, out)
+    _check_devices("gemm_fp8", q, scales, weight.q, out)
     n, K = q.shape[0], weight.shape[1]
     _check_fp8_rows("gemm_fp8", q, scales, n, K)
     M, code, half = _fp8_product(weight, out, epilogue, n)
@@ -812,7 +824,9 @@ class Fp8Linear:
     overlap x. Calls that share buffers run on one stream."""
 
     def __init__(self, weight, q: torch.Tensor, scales: torch.Tensor):
-        _cuda(q, scales, weight.q)
+        self._at = q.get_device()
+        if self._at < 0 or scales.get_device() != self._at or weight.q.get_device() != self._at:
+            _refuse_devices("linear_fp8", q, scales, weight.q)
         self.M, self.K = weight.shape
         _check_fp8_rows("linear_fp8", q, scales, q.shape[0], self.K)
         self.rows, self.halves, self.in_blocks = min(q.shape[0], scales.shape[1]), weight.halves, weight.in_blocks
@@ -824,8 +838,9 @@ class Fp8Linear:
         self._lib, self._fn = _fn("gemm_fp8", "sb_linear_fp8", [c_char_p, c_void_p])
 
     def __call__(self, x: torch.Tensor, out: torch.Tensor, epilogue: int = STORE, constants=(0.0, 0.0)) -> None:
-        if not (x.is_cuda and out.is_cuda):
-            _cuda(x, out)
+        at = self._at
+        if x.get_device() != at or out.get_device() != at or _device() != at:
+            _refuse_devices("linear_fp8", x, out, self._keep[1])
         gated = epilogue >= SWIGLU
         (n, K), (rows, M) = x.shape, out.shape
         ldx, step_x = x.stride()
@@ -853,8 +868,9 @@ def route_experts(logits: torch.Tensor, choice: torch.Tensor, weights: torch.Ten
     s + bias; weight s (divided by (the chosen s' sum + 1e-20) if `renormalise`) times `scale`.
     choice [n, top] int32, weights [top, n] float32. An expert with a logit or a bias of -infinity or NaN is never chosen; a place that nothing is
     left for gets -1 and weight 0."""
-    if not (logits.is_cuda and choice.is_cuda and weights.is_cuda and (bias is None or bias.is_cuda)):
-        _cuda(logits, bias, choice, weights)
+    at = logits.get_device()
+    if at < 0 or choice.get_device() != at or weights.get_device() != at or (bias is not None and bias.get_device() != at) or _device() != at:
+        _refuse_devices("route_experts", logits, bias, choice, weights)
     code = ROUTER_SCORES.get(score)
     if code is None:
         raise ValueError(f"route_experts: unknown score '{score}' (known: {', '.join(ROUTER_SCORES)})")
@@ -883,7 +899,10 @@ def experts_fp8(x: torch.Tensor, choice: torch.Tensor, weights: torch.Tensor, ex
     """out[t] = sum over k of weights[k, t] * down_e (silu(gate_e x_t) * (up_e x_t)), e = choice[t, k], in the order of the choices; an id that is no
     expert's has no term. x [n, width] float32 or bfloat16, choice [n, top] int32, weights [top, n] float32, `experts` an `Fp8Experts`, out float32 or
     bfloat16 [n, width], scratch uint8 of `experts_fp8_scratch` bytes. Inputs of both projections are quantised as `quantize_fp8` does."""
-    _cuda(x, choice, weights, out, scratch)
+    at = experts.at
+    if at < 0 or x.get_device() != at or choice.get_device() != at or weights.get_device() != at or out.get_device() != at or scratch.get_device() != at \
+            or _device() != at:
+        _refuse_devices("experts_fp8", x, choice, weights, out, scratch, experts.down)
     (n, W), (rows, top) = x.shape, choice.shape
     (ldx, step_x), (ldo, step_o) = x.stride(), out.stride()
     if choice.dtype != torch.int32 or weights.dtype != torch.float32 or scratch.dtype != torch.uint8:

@@ -221,3 +221,56 @@ def test_random_weights_of_other_designs_go_by_the_form_too():
     plain_names = set(random_tensors(KERALORN_P, 1))
     assert set(random_tensors({**KERALORN_P, "quantization_config": OTHER}, 1)) == plain_names
     assert set(random_tensors({**KERALORN_P, "quantization_config": CONFIG["quantization_config"]}, 1)) >= plain_names
+
+
+def test_weights_on_several_devices_are_refused():
+    """(The kernels get addresses: one of another device's memory, or of the host's, must not reach them.)"""
+    from stride_b200.kernels.linear import Fp8Experts, Fp8Weight
+    w = _weight(128, 64)
+    with pytest.raises(ValueError, match="has its scales there too"):
+        Fp8Weight(w.q, w.scales.to("meta"))
+    elsewhere = Fp8Weight(torch.empty(64, 128, dtype=torch.float8_e4m3fn, device="meta"), torch.empty(1, 1, device="meta"))
+    with pytest.raises(ValueError, match="all on one device"):
+        Fp8Experts([w, w], [elsewhere])
+
+
+def test_calls_with_tensors_beside_the_current_device_are_refused(monkeypatch):
+    """Tensors of two devices, or of one that is not the current: refused before anything is launched (devices made up on the host)."""
+    from types import SimpleNamespace
+    from stride_b200.kernels import ops
+
+    class On(torch.Tensor):
+        """A host tensor that says it lies on a CUDA device."""
+        at = 0
+        is_cuda = True
+        device = property(lambda self: torch.device("cuda", self.at))
+
+        def get_device(self):
+            return self.at
+
+    def on(at, *shape, dtype=torch.float32):
+        t = torch.zeros(*shape).to(dtype).as_subclass(On)
+        t.at = at
+        return t
+
+    monkeypatch.setattr(ops, "_fn", lambda *a: (None, lambda *args: pytest.fail("launched")))
+    monkeypatch.setattr(ops, "_device", lambda: 0)
+    for where in ([1] * 6, [0, 1, 0, 0, 0, 0], [0, 0, 1, 0, 0, 0], [0, 0, 0, 1, 0, 0], [0, 0, 0, 0, 1, 0], [0, 0, 0, 0, 0, 1]):
+        a, b, c, d, e, f = where
+        weight = SimpleNamespace(q=on(c, 128, 16, dtype=torch.float8_e4m3fn), scales=on(c, 1, 1), shape=(128, 16), stride=16, halves=1, in_blocks=True)
+        q, scales = on(a, 2, 16, dtype=torch.float8_e4m3fn), on(b, 1, 2)
+        if 1 in where[:3]:
+            with pytest.raises(ValueError, match="quantize_fp8: tensors on .*the current device is cuda:0"):
+                ops.quantize_fp8(on(c, 2, 16), q, scales)
+        if 1 in where[:4]:
+            with pytest.raises(ValueError, match="gemm_fp8: tensors on"):
+                ops.gemm_fp8(q, scales, weight, on(d, 2, 128))
+            with pytest.raises(ValueError, match="linear_fp8: tensors on"):
+                ops.Fp8Linear(weight, q, scales)(on(d, 2, 16), on(a, 2, 128))
+            with pytest.raises(ValueError, match="linear_fp8: tensors on"):
+                ops.Fp8Linear(weight, q, scales)(on(a, 2, 16), on(d, 2, 128))
+            with pytest.raises(ValueError, match="route_experts: tensors on"):
+                ops.route_experts(on(a, 2, 4), on(b, 2, 1, dtype=torch.int32), on(c, 1, 2), bias=on(d, 4))
+        layer = SimpleNamespace(at=a, down=on(a, 16, 16), width=16, address=0)
+        with pytest.raises(ValueError, match="experts_fp8: tensors on"):
+            ops.experts_fp8(on(b, 2, 16), on(c, 2, 1, dtype=torch.int32), on(d, 1, 2), layer, on(e, 2, 16), on(f, 64, dtype=torch.uint8))
