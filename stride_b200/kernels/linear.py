@@ -127,6 +127,8 @@ class Fp8Experts:
         shapes = {w.shape for w in gate_up}, {w.shape for w in down}
         if len(gate_up) != 2 * len(down) or not down or len(shapes[0]) != 1 or len(shapes[1]) != 1 or down[0].shape != gate_up[0].shape[::-1]:
             raise ValueError("experts have a gate and an up matrix [inner, width] and a down matrix [width, inner] each")
+        if not all(w.in_blocks for w in gate_up + down):
+            raise ValueError("an expert's matrices are plain ones: blocks of scales that begin anew in the middle of one are not laid out so")
         if len({w.device for w in gate_up + down}) != 1:
             raise ValueError("the experts' matrices are all on one device")
         self.experts = len(down)

@@ -274,3 +274,18 @@ def test_calls_with_tensors_beside_the_current_device_are_refused(monkeypatch):
         layer = SimpleNamespace(at=a, down=on(a, 16, 16), width=16, address=0)
         with pytest.raises(ValueError, match="experts_fp8: tensors on"):
             ops.experts_fp8(on(b, 2, 16), on(c, 2, 1, dtype=torch.int32), on(d, 1, 2), layer, on(e, 2, 16), on(f, 64, dtype=torch.uint8))
+
+
+def test_experts_of_stacked_matrices():
+    """A stacked matrix whose second half's scales begin beside a multiple of 128 rows has more blocks of scales than an expert's is read with."""
+    from stride_b200.kernels.linear import Fp8Experts, Fp8Weight
+    stacked, down = Fp8Weight.stack([_weight(100, 64, 1), _weight(100, 64, 2)]), _weight(64, 200)
+    assert stacked.shape == (200, 64) and stacked.scales.shape[0] == 2
+    narrow = Fp8Weight.stack([_weight(40, 64, 1), _weight(40, 64, 2)])          # (two blocks of scales where 80 rows have one)
+    with pytest.raises(ValueError, match="plain ones"):
+        Fp8Experts([narrow, narrow], [_weight(64, 80)])
+    with pytest.raises(ValueError, match="plain ones"):
+        Fp8Experts([stacked, stacked], [down])
+    whole = Fp8Weight.stack([_weight(128, 64, 1), _weight(128, 64, 2)])
+    layer = Fp8Experts([whole, whole], [_weight(64, 256)])
+    assert layer.gate_up_scales.shape[0] == 4 and layer.inner == 256
