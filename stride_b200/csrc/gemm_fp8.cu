@@ -1664,6 +1664,15 @@ ExpertScratch expert_scratch(int64_t n, int64_t top, int64_t E, int64_t W, int64
 }  // namespace
 
 SB_EXPORT void sb_gemm_fp8_use_status_word(int* device_word) { status_word_given() = device_word; }
+// 0 if every wait of these kernels completed, else where one gave up; resets it. Until then the clustered and the token form store nothing.
+SB_EXPORT int sb_gemm_fp8_status() {
+  int* status = status_word();
+  if (!status) return -1;
+  int host = 0;
+  if (cudaMemcpy(&host, status, sizeof(int), cudaMemcpyDeviceToHost) != cudaSuccess) return -2;
+  if (host != 0) cudaMemset(status, 0, sizeof(int));
+  return host;
+}
 
 // x [n][ldx] float32 (0) or bfloat16 (1) -> q [n][ldq] e4m3, scales [ceil(K / 128)][lds] float32.
 SB_EXPORT int sb_quantize_fp8(const void* x, int xdtype, int64_t ldx, void* q, int64_t ldq, float* scales, int64_t lds, int n, int K, void* stream) {

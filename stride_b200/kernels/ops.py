@@ -770,6 +770,14 @@ def quantize_fp8(x: torch.Tensor, q: torch.Tensor, scales: torch.Tensor) -> None
     _check(lib, fn(_ptr(x), dtype_code(x.dtype), _row_stride(x), _ptr(q), _row_stride(q), _ptr(scales), _row_stride(scales), n, K, _stream()))
 
 
+def gemm_fp8_status() -> int:
+    """0 if every wait inside the kernels of 8-bit products and experts completed since the last call; synchronises. Anything else: results since then
+    are missing (a wait that gave up stores nothing). Inside an engine the sampler reports it; a caller of the products alone asks here."""
+    lib = library("gemm_fp8")
+    lib.sb_gemm_fp8_status.restype = c_int
+    return lib.sb_gemm_fp8_status()
+
+
 def check_fp8_epilogue(weight, gated: bool) -> None:
     """Whether a product with the 8-bit weight (its `halves` and `in_blocks`) can be gated, or plain."""
     if gated and weight.halves != 2:

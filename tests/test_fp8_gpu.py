@@ -560,3 +560,22 @@ def test_groups_whose_best_two_sum_beyond_the_floats(E, groups, score):
             choice, _ = _route(z, 2, bias, score=score, **kw)
             want, _ = plain.route(z.cpu(), 2, score, bias.cpu(), **kw)
             assert torch.equal(choice, want), (biases, top_groups)
+
+
+@pytest.mark.parametrize("n", [1, 40, 100])
+def test_a_lost_signal_can_be_read_and_the_products_run_again(n):
+    """A caller without an engine: the word into which a wait that gave up reports (written by the host here) is read, and reset with that."""
+    from stride_b200.kernels import ops
+    from stride_b200.kernels.linear import Linear
+    layer, x, work = Linear(_weight(1, 256, 2048), BF), _rand(2, n, 2048, dtype=BF), _workspace(n)
+    want, out = torch.empty(n, 256, device="cuda"), torch.zeros(n, 256, device="cuda")
+    layer.forward(x, want, workspace=work)
+    assert ops.gemm_fp8_status() == 0
+    ops.shared_status_word({"gemm_fp8"}).fill_(45)
+    layer.forward(x, out, workspace=work)
+    torch.cuda.synchronize()
+    assert (out == 0).all()
+    assert ops.gemm_fp8_status() == 45
+    assert ops.gemm_fp8_status() == 0
+    layer.forward(x, out, workspace=work)
+    assert torch.equal(out, want)
