@@ -229,6 +229,19 @@ __device__ __forceinline__ bool mbar_over(uint32_t bar, uint32_t parity) {
       : "memory");
   return ok != 0;
 }
+// `mbar_wait` by a warp that leaves it as a whole, as loads from tensor memory need it: its lanes go on once all have seen the phase end. (A
+// wait of each lane's own and a `__syncwarp` behind it: 4,096 tokens through 28,672 gate and up rows 558 to 566 us in a recorded graph, so 546 to 551.)
+__device__ __forceinline__ bool mbar_wait_warp(uint32_t bar, uint32_t parity, int* status, int code) {
+  long long began = 0;
+  for (int spins = 1; !__all_sync(0xffffffffu, mbar_try_wait(bar, parity)); ++spins) {
+    if ((spins & 255) != 0) continue;
+    if (began == 0) began = clock64();
+    const bool late = clock64() - began > kWaitCycles;
+    if (late) atomicCAS(status, 0, code);
+    if (__any_sync(0xffffffffu, late || *reinterpret_cast<volatile int*>(status) != 0)) return false;
+  }
+  return true;
+}
 // Waits for this warp's loads from tensor memory; what they brought passes through, so that no use of it can be moved in front of the wait.
 __device__ __forceinline__ void tmem_arrived16(uint32_t* r) {
   asm volatile("tcgen05.wait::ld.sync.aligned;"
@@ -901,8 +914,12 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
       for (int i = 0, in_batch = 0; i < blocks; ++i) {
         if (in_batch == 0) ok = mbar_wait(smem_u32(&factor_full[batch]), batch_par, p.status, 56) && ok;
         const float f0 = factor[batch][in_batch][0][quarter * 32 + lane], f1 = factor[batch][in_batch][WIDE ? 1 : 0][quarter * 32 + lane];
-        if (WIDE || !__all_sync(0xffffffffu, ready)) ok = mbar_wait(smem_u32(&accum_full[slot]), slot_par, p.status, 55) && ok;
-        if (!WIDE) __syncwarp();
+        if (WIDE) {
+          ok = mbar_wait_warp(smem_u32(&accum_full[slot]), slot_par, p.status, 55) && ok;
+        } else {
+          if (!__all_sync(0xffffffffu, ready)) ok = mbar_wait(smem_u32(&accum_full[slot]), slot_par, p.status, 55) && ok;
+          __syncwarp();
+        }
         fence_after_sync();
         const uint32_t from = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + slot * S::kColumns + part * 32;
         uint32_t v[16];

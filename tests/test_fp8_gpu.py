@@ -579,3 +579,23 @@ def test_a_lost_signal_can_be_read_and_the_products_run_again(n):
     assert ops.gemm_fp8_status() == 0
     layer.forward(x, out, workspace=work)
     assert torch.equal(out, want)
+
+
+@pytest.mark.parametrize("n,M,K", [(1100, 12000, 1300), (300, 20000, 2048)])
+@pytest.mark.parametrize("gated", [False, True])
+def test_wide_tiles_walked_in_several_rounds(n, M, K, gated):
+    """CTAs and pairs that walk tiles of 256 weight rows, with waits for accumulators that are never there yet: the same bits every time, and a few
+    tokens' in a step of their own."""
+    from stride_b200.kernels.linear import Fp8Weight, Linear
+    layer = Linear(Fp8Weight.stack([_weight(1, M // 2, K), _weight(2, M // 2, K)]) if gated else _weight(1, M, K), BF)
+    x, work = _rand(3, n, K, dtype=BF), _workspace(n)
+    call = (lambda x, out: layer.forward_swiglu(x, out, None, workspace=work)) if gated else (lambda x, out: layer.forward(x, out, workspace=work))
+    want = torch.empty(n, M // 2 if gated else M, device="cuda")
+    call(x, want)
+    few = torch.empty(9, want.shape[1], device="cuda")
+    call(x[n - 9:], few)
+    assert torch.equal(few, want[n - 9:])
+    for _ in range(10):
+        out = torch.full_like(want, float("nan"))
+        call(x, out)
+        assert torch.equal(out, want)
