@@ -1650,13 +1650,13 @@ int check_product(const char* who, const void* w, int64_t ldw, int out_dtype, in
 // CTAs that walk tiles, which pays from nine or so on average if there are many pairs in all (64 experts of 2,048 x 1,408, six a token: 100 tokens
 // 131 us in tiles of 16, 123 walked, 150 tokens 157 and 127; 20 tokens, two of four experts of 1,024 x 512: 24.3 and 28.2). Tiles of 256 on pairs
 // of CTAs were no faster even with 1,000 rows an expert (82.6 us, 80.4 walked by single ones).
-int expert_tile(int pairs, int E) {
-  const int mean = (pairs + E - 1) / E;
-  return mean <= 8 || (mean <= 16 && pairs <= 256) ? 16 : kTokenRows;
-}
+int64_t most_in_tiles_of_16(int64_t E) { return std::max<int64_t>(8 * E, std::min<int64_t>(16 * E, 256)); }
+int expert_tile(int pairs, int E) { return pairs <= most_in_tiles_of_16(E) ? 16 : kTokenRows; }
 int most_tiles(int pairs, int E, int tile) { return std::min(pairs, pairs / tile + std::min(pairs, E)); }
 
-// Where an expert call's intermediate results lie in its scratch buffer, every one 256-byte aligned.
+// Where an expert call's intermediate results lie in its scratch buffer, every one 256-byte aligned. z is for the products on tiles of 16 rows (the others
+// quantise it as they make it), so for as many choices as those have at most: of 8,192 tokens, eight of 256 experts of 7,168 x 2,048, 16 MB and not 512. With more
+// tokens every part is as large or larger: a buffer for some serves fewer.
 struct ExpertScratch {
   int64_t order, place, list, xq, xs, z, zq, zs, parts, bytes, ldx, ldz, ldp;
 };
@@ -1672,7 +1672,7 @@ ExpertScratch expert_scratch(int64_t n, int64_t top, int64_t E, int64_t W, int64
   s.ldx = (W + 15) / 16 * 16, s.ldz = (F + 15) / 16 * 16, s.ldp = (W + 3) / 4 * 4;
   s.order = take(4 * pairs), s.place = take(4 * pairs), s.list = take(4 * (2 + 3 * pairs));
   s.xq = take(pairs * s.ldx), s.xs = take(4 * pairs * ((W + kBlock - 1) / kBlock));
-  s.z = take(4 * pairs * s.ldz), s.zq = take(pairs * s.ldz), s.zs = take(4 * pairs * ((F + kBlock - 1) / kBlock));
+  s.z = take(4 * std::min(pairs, most_in_tiles_of_16(E)) * s.ldz), s.zq = take(pairs * s.ldz), s.zs = take(4 * pairs * ((F + kBlock - 1) / kBlock));
   s.parts = take(4 * pairs * s.ldp);
   s.bytes = at;
   return s;

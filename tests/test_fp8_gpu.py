@@ -599,3 +599,37 @@ def test_wide_tiles_walked_in_several_rounds(n, M, K, gated):
         out = torch.full_like(want, float("nan"))
         call(x, out)
         assert torch.equal(out, want)
+
+
+@pytest.mark.parametrize("E,top", [(8, 4), (2, 2), (40, 8), (16, 8)])
+def test_experts_keep_within_their_scratch(E, top):
+    """Around the number of choices from which tiles of rows are walked (a mean of eight, or of sixteen and 256 in all), with scratch of just the bytes
+    that are asked for and a border behind it; a buffer for more tokens serves fewer."""
+    W, F = 256, 136
+    layer, (gate, up, down) = _experts(E, W, F)
+    border = max(8 * E, min(16 * E, 256)) // top
+    sizes = [layer.scratch(n, top).numel() for n in range(0, 2 * border + 40)]
+    assert sizes == sorted(sizes)
+    for n in (1, border - 1, border, border + 1, border + 33):
+        choice, weights = _choices(n, n, E, top)
+        for offset in (0, 1):                      # (rows off 16-byte borders: quantised by a kernel of its own in either form)
+            rows = _rand(n, n, W + offset, dtype=BF)[:, offset:]
+            whole = torch.full((layer.scratch(n, top).numel() + 4096,), 0xA5, dtype=torch.uint8, device="cuda")
+            out = torch.empty(n, W, device="cuda")
+            layer.forward(rows, choice, weights, out, whole[:-4096])
+            assert (whole[-4096:] == 0xA5).all()
+            want, bound = plain.experts(rows.to(F64), choice, weights, gate, up, down)
+            assert ((out.to(F64) - want).abs() <= bound + HALF_STEP[F32] * (want.abs() + bound)).all()
+            large = torch.empty(sizes[-1], dtype=torch.uint8, device="cuda")
+            again = torch.empty(n, W, device="cuda")
+            layer.forward(rows, choice, weights, again, large)
+            assert torch.equal(again, out)
+
+
+def test_scratch_of_many_tokens_has_no_room_for_what_few_need():
+    """32-bit gated products are kept for few choices only: a long step's scratch is what its 8-bit rows, their scales and the results take."""
+    from stride_b200.kernels import ops
+    n, top, E, W, F = 8192, 8, 256, 7168, 2048
+    pairs = n * top
+    used = pairs * (W + 4 * (W // 128) + F + 4 * (F // 128) + 4 * W + 4 * 5)
+    assert ops.experts_fp8_scratch(n, top, E, W, F) <= used + 2 * 8 * E * 4 * F + 4096
