@@ -14,8 +14,8 @@
 // PFLOP/s at best; without it, as a trial, 348), the weights' bytes the small ones.
 //
 // K is cut into ranges, a function of the weight's shape alone (`fp8_ranges`): few weight tiles leave SMs without work. The sum of a range
-// starts from zero, the ranges are added in ascending order. With few tokens the ranges are the CTAs of a cluster, which add up through
-// distributed shared memory; with many one CTA walks them all. So a token's bits depend neither on the step it is part of nor on the tile,
+// starts from zero, the ranges are added in ascending order. With few tokens, and with more where that takes fewer rounds, the ranges are shared out
+// among the CTAs of a cluster, which add up through distributed shared memory; else one CTA walks them all. So a token's bits depend neither on the step it is part of nor on the tile,
 // nor on which of the forms made them:
 //   `gemm_fp8_kernel`        up to 64 tokens: 128 weight rows by 16, 32 or 64 tokens; of 16 it may quantise its input itself
 //   `gemm_fp8_token_kernel`  up to 128, and more where that takes fewer rounds: tokens are the product's rows
@@ -337,7 +337,8 @@ struct FewChoices {
 template <int BN>
 struct Shape {
   static constexpr int kEpilogueWarps = BN >= 64 ? 16 : BN >= 32 ? 8 : 4;
-  static constexpr int kColumns = BN * 4 / kEpilogueWarps;             // columns of a thread's row of the tile
+  static constexpr int kColumns = 16;                                  // columns of a thread's row of the tile
+  static_assert(kColumns * kEpilogueWarps == 4 * BN, "four warps see all 128 rows");
   static constexpr int threads(bool quant) { return 128 + 32 * kEpilogueWarps + (quant ? 192 : 0); }
   static constexpr int kSlots = BN <= 32 ? 8 : 4;                      // accumulators under way
   static constexpr int kStage = kStageA + BN * 128;
@@ -345,17 +346,18 @@ struct Shape {
   static constexpr int kCtas = BN <= 32 ? 2 : 1;                       // of an SM: with few tokens one fills its ring while the other drains
 };
 
-// blockIdx = (weight tile, token tile, K range: the rank in the cluster when SPLIT). Warp 0 loads, warp 1 issues the products, warps 2 and 3
-// multiply the scales, the others are the epilogue: four of them see all 128 rows, with eight each half takes half of the columns. QUANT (few
-// tokens): the input comes as it is, and four warps quantise it, the same arithmetic as `quantize_kernel`, straight into the ring's stages. A
-// block is one warp's, so that eight (of float32, where two CTAs share an SM's memory, four) are on their way at a time; all warps on one block at a time took 1.2 us for it. A lane
-// copies the columns that it reads. A warp meets a stage's barrier only now and then, and could take one phase for the one two further on:
-// it looks there only once its accumulator, of which there are eight, is free, and with it the last but one block of that stage.
-constexpr int kQuantWarps = 8;
+// blockIdx = (weight tile, token tile, K range: the rank in the cluster when SPLIT; else there is one range). Warp 0 loads, warp 1 issues the
+// products, warps 2 and 3 multiply the scales, the others are the epilogue: four of them see all 128 rows, of 16 tokens. QUANT (tiles of 16 tokens): the
+// input comes as it is, and eight warps quantise it, the same arithmetic as `quantize_kernel`, straight into the ring's stages. A block is one
+// warp's, so that eight (of float32, where two CTAs share an SM's memory, four, of as many warps) are on their way at a time; all warps on one block at a
+// time took 1.2 us for it. A lane copies the columns that it reads. A warp meets a stage's barrier only now and then, and could take one phase for the
+// one two further on: it looks there only once its accumulator, of which there are eight, is free, and with it the last but one block of that stage.
+constexpr int kQuantWarps = 8, kQuantRows = 16;
 template <int EPI, int BN, class OUT, bool GROUPED, bool SPLIT, bool QUANT>
-__global__ void __launch_bounds__(Shape<BN>::threads(QUANT), QUANT && BN > 16 ? 1 : Shape<BN>::kCtas)
+__global__ void __launch_bounds__(Shape<BN>::threads(QUANT), Shape<BN>::kCtas)
 gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const Fp8Params p) {
   using S = Shape<BN>;
+  static_assert(!QUANT || BN == kQuantRows, "two lanes a row of the input");
   constexpr int kScaleWarps = QUANT ? kQuantWarps : 2, kFirst = 2 + kScaleWarps;        // the epilogue's first warp
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   __shared__ __align__(8) uint64_t full_bar[kMaxStages], empty_bar[kMaxStages];
@@ -448,14 +450,14 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
       ready = mbar_over(smem_u32(&slot_empty[slot]), slot_par) && mbar_over(smem_u32(&full_bar[st]), par);
     }
   } else if (warp < kFirst) {
-    // the scales' products, two columns a thread; four blocks are read ahead of their turn
-    constexpr int kAhead = 4, kPer = (BN + 63) / 64;
+    // the scales' products, a column a thread; four blocks are read ahead of their turn
+    constexpr int kAhead = 4;
     const int t = threadIdx.x - 64;
     const float* ws0 = p.w_scales + static_cast<int64_t>(expert * p.scale_rows + (EPI == kGated ? tile_m / 2 : tile_m)) * p.blocks + b0;
     const float* ws1 = EPI == kGated ? ws0 + static_cast<int64_t>(p.scale_rows / 2) * p.blocks : ws0;
     if (!GROUPED) sb::grid_dependency_wait();
     if constexpr (QUANT) {
-      constexpr int kPerRow = 32 / BN, kColumns = 128 / kPerRow;            // lanes of a row of the tile, columns of a lane
+      constexpr int kPerRow = 2, kColumns = 128 / kPerRow;            // lanes of a row of the tile, columns of a lane
       const int r = lane / kPerRow, part = lane % kPerRow, first = warp - 2, warps = p.quant_warps, size = p.x_f32 ? 4 : 2,
                 pieces = kColumns * size / 16;
       const bool live = n0 + r < end;
@@ -495,7 +497,7 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
             for (int k = 0; k < 4; ++k) amax = max(amax, max((w[k] << 16) & 0x7FFFFFFFu, w[k] & 0x7FFF0000u));
           }
         }
-        if (kPerRow == 2) amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+        amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
         const bool finite = amax < 0x7F800000u;
         const int e = finite ? scale_exponent(amax) : 0, st = i % p.stages, slot = i % S::kSlots;
         const float inverse = power_of_two(-e), scale = finite ? power_of_two(e) : __uint_as_float(0x7FC00000u);
@@ -535,15 +537,11 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
         if (lane == 0) mbar_arrive(smem_u32(&scale_full[slot]));
       }
     } else {
-    float xs[kAhead][kPer], w0[kAhead], w1[kAhead];
+    float xs[kAhead], w0[kAhead], w1[kAhead];
     auto fetch = [&](int i, int a) {
       if (i >= iters) return;
       w0[a] = __ldg(ws0 + i), w1[a] = EPI == kGated ? __ldg(ws1 + i) : 0.0f;
-#pragma unroll
-      for (int k = 0; k < kPer; ++k) {
-        const int c = t + 64 * k;
-        xs[a][k] = c < BN && n0 + c < end ? p.x_scales[static_cast<int64_t>(b0 + i) * p.ldxs + n0 + c] : 0.0f;
-      }
+      xs[a] = t < BN && n0 + t < end ? p.x_scales[static_cast<int64_t>(b0 + i) * p.ldxs + n0 + t] : 0.0f;
     };
 #pragma unroll
     for (int a = 0; a < kAhead; ++a) fetch(a, a);
@@ -555,13 +553,9 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
         const int i = i0 + a;
         if (i >= iters) break;
         mbar_wait(smem_u32(&slot_empty[slot]), slot_par, p.status, 44);
-#pragma unroll
-        for (int k = 0; k < kPer; ++k) {
-          const int c = t + 64 * k;
-          if (c < BN) {
-            factor[slot][0][c] = xs[a][k] * w0[a];
-            if (EPI == kGated) factor[slot][1][c] = xs[a][k] * w1[a];
-          }
+        if (t < BN) {
+          factor[slot][0][t] = xs[a] * w0[a];
+          if (EPI == kGated) factor[slot][1][t] = xs[a] * w1[a];
         }
         mbar_arrive(smem_u32(&scale_full[slot]));
         fetch(i + kAhead, a);
@@ -571,16 +565,12 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
     }
   } else {
     const int quarter = warp & 3, half = (warp - kFirst) >> 2, row = quarter * 32 + lane;
-    constexpr int C = S::kColumns, kChunk = C < 32 ? C : 32;
-    float acc[C], total[SPLIT ? 1 : C];
+    constexpr int C = S::kColumns;
+    float acc[C];
 #pragma unroll
     for (int c = 0; c < C; ++c) acc[c] = 0.0f;
-    if (!SPLIT) {
-#pragma unroll
-      for (int c = 0; c < C; ++c) total[c] = -0.0f;          // (the first range is added to nothing: -0 + v = v, signs of zeros too)
-    }
     bool ok = true;
-    int slot = 0, left = p.range_blocks;
+    int slot = 0;
     uint32_t slot_par = 0;
     bool ready = false;
     for (int i = 0; i < iters; ++i) {
@@ -592,29 +582,21 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
       fence_after_sync();
       const uint32_t from = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + slot * BN + half * C;
       const float* f = factor[slot][EPI == kGated && quarter >= 2 ? 1 : 0] + half * C;
-#pragma unroll
-      for (int c0 = 0; c0 < C; c0 += kChunk) {
-        uint32_t v[kChunk];
-        if (kChunk == 32) tmem_load32_nowait(from + c0, v), tmem_arrived32(v);
-        else tmem_load16_nowait(from + c0, v), tmem_arrived16(v);
-        add_scaled<kChunk>(acc + c0, v, f + c0);
-      }
+      uint32_t v[C];
+      tmem_load16_nowait(from, v);
+      tmem_arrived16(v);
+      add_scaled<C>(acc, v, f);
       fence_before_sync();
       __syncwarp();
       if (lane == 0) mbar_arrive(smem_u32(&slot_empty[slot]));
       if (++slot == S::kSlots) slot = 0, slot_par ^= 1;
       ready = mbar_over(smem_u32(&accum_full[slot]), slot_par) && mbar_over(smem_u32(&scale_full[slot]), slot_par);
-      if (!SPLIT && (--left == 0 || i + 1 == iters)) {
-        left = p.range_blocks;
-#pragma unroll
-        for (int c = 0; c < C; ++c) total[c] += acc[c], acc[c] = 0.0f;
-      }
     }
     // the tile's sums to shared memory, [token][row]: every load has arrived and every product that reads the ring is done
     float* tile = reinterpret_cast<float*>(smem0_p);
     if (ok) {
 #pragma unroll
-      for (int c = 0; c < C; ++c) tile[(half * C + c) * kBlock + row] = SPLIT ? acc[c] : total[c];
+      for (int c = 0; c < C; ++c) tile[(half * C + c) * kBlock + row] = acc[c];
     }
     if (!ok) tile = nullptr;
     asm volatile("bar.sync 1, %0;" ::"r"(32 * S::kEpilogueWarps) : "memory");
@@ -1424,10 +1406,9 @@ int fp8_ranges(int tiles, int blocks) {
   return (blocks + (blocks + s - 1) / s - 1) / ((blocks + s - 1) / s);        // (no empty range)
 }
 
-// Up to this many rows of a tile the product can quantise its input itself. Of a dense product it does where a CTA has few blocks of columns: that
+// Up to `kQuantRows` rows of a tile the product can quantise its input itself. Of a dense product it does where a CTA has up to this many blocks: that
 // saves a launch, but a block takes longer (2,048 x 2,048 of one token 7.7 us with a launch, 4.6 without; 16,384 x 2,048, 16 blocks a CTA, of eight
 // 10.1 and 12.1). The experts' two inputs would need two launches.
-constexpr int kQuantRows = 16;
 constexpr int kQuantBlocks = 6;
 
 template <int EPI, int BN, class OUT, bool GROUPED>
