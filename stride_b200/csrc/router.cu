@@ -410,7 +410,10 @@ __device__ __forceinline__ void route_row(const Routing& r, int row, int lane, c
     kept_e = lane < min(count, r.top) ? e : -1;
   }
   float kept_s = 0.0f, sum = 0.0f;
-  if (kept_e >= 0) kept_s = r.softmax ? held_scores[kept_e] : 1.0f / (1.0f + expf(-fminf(held_scores[kept_e], FLT_MAX)));
+  if (kept_e >= 0) {
+    kept_s = held_scores[kept_e];
+    if (!r.softmax) kept_s = kept_s < -80.0f ? expf(kept_s) : 1.0f / (1.0f + expf(-fminf(kept_s, FLT_MAX)));      // (e^88 and more would leave nothing of it)
+  }
   if (r.renormalise) sum = warp_sum(kept_s);
   if (r.renormalise && kept_e >= 0 && sum < 0x1p-50f) sure = false;      // (scores below the smallest floats count where all are)
   sure = __all_sync(0xffffffffu, sure);

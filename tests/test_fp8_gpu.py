@@ -633,3 +633,20 @@ def test_scratch_of_many_tokens_has_no_room_for_what_few_need():
     pairs = n * top
     used = pairs * (W + 4 * (W // 128) + F + 4 * (F // 128) + 4 * W + 4 * 5)
     assert ops.experts_fp8_scratch(n, top, E, W, F) <= used + 2 * 8 * E * 4 * F + 4096
+
+
+@pytest.mark.parametrize("E", [8, 40, 256])
+def test_weights_below_the_smallest_normal_float(E):
+    """Sigmoids of far negative logits, taken as they are: within the exponential's two units and the type's smallest step of e^z."""
+    z = torch.linspace(-106.0, -70.0, E, device="cuda")[None].repeat(3, 1)
+    z[1] = -95.0
+    z[2, : E // 2] = float("-inf")
+    choice, weights = _route(z, 4, renormalise=False, scale=0.5)
+    want, want_weights = plain.route(z.cpu(), 4, "sigmoid", renormalise=False, scale=0.5)
+    assert torch.equal(choice, want)
+    # (s is off by 2 units of 2^-23 and a rounding to the smallest step, 2^-149; times the scale, rounded to that step again)
+    assert ((weights.to(F64) - want_weights).abs() <= 2.0 ** -21 * want_weights + 2.0 ** -149).all()
+    choice, weights = _route(z, 4, renormalise=True)
+    assert _close(weights, plain.route(z.cpu(), 4, "sigmoid")[1])
+    z = torch.full((1, E), -95.0, device="cuda")
+    assert (_route(z, 2, renormalise=False)[1] > 0).all()
