@@ -31,7 +31,8 @@ def model_plan(config: dict) -> dict:
     """The tensor plan (name -> TensorPlan) of the architecture that `config` names."""
     arch = resolve_architecture(config)
     spec = arch.model_spec(arch.parse_config(config))
-    env = BuildEnv(device=torch.device("cpu"), compute_dtype=torch.float32, max_tokens=1, max_positions=2)
+    # (the serving precision: some parts run in no other)
+    env = BuildEnv(device=torch.device("cpu"), compute_dtype=torch.bfloat16, max_tokens=1, max_positions=2)
     return DecoderModel(spec, env).tensor_plan()
 
 

@@ -289,3 +289,14 @@ def test_experts_of_stacked_matrices():
     whole = Fp8Weight.stack([_weight(128, 64, 1), _weight(128, 64, 2)])
     layer = Fp8Experts([whole, whole], [_weight(64, 256)])
     assert layer.gate_up_scales.shape[0] == 4 and layer.inner == 256
+
+
+def test_random_weights_of_a_model_with_scored_experts():
+    """A part that runs in the bfloat16 engine alone has a plan, and random weights, like any other."""
+    from stride_b200.weights.random_init import model_plan, random_tensors
+    from test_scored_experts_gpu import CONFIG as SCORED, architecture
+    with architecture():
+        plan, tensors = model_plan(SCORED), random_tensors(SCORED, 3)
+    name = "model.layers.1.mlp.experts.15.down_proj.weight"
+    assert plan[name].fp8 and tensors[name].dtype == torch.float8_e4m3fn and tensors[name + "_scale_inv"].shape == (2, 2)
+    assert not plan["model.layers.1.mlp.gate.weight"].fp8
