@@ -50,7 +50,7 @@ __device__ __forceinline__ T warp_sum(T v) {
 }
 // e^(z - top): the difference with what its rounding dropped, so that far logits keep their relative accuracy too.
 __device__ __forceinline__ float exp_difference(float z, float top) {
-  const float d = z - top, back = d + top, dropped = (z - back) + (top - (back - d));
+  const float d = z - top, back = d + top, dropped = (z - back) + ((back - d) - top);
   return fabsf(dropped) < 1.0f ? expf(d) * (1.0f + dropped) : expf(d);
 }
 

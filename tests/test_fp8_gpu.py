@@ -650,3 +650,19 @@ def test_weights_below_the_smallest_normal_float(E):
     assert _close(weights, plain.route(z.cpu(), 4, "sigmoid")[1])
     z = torch.full((1, E), -95.0, device="cuda")
     assert (_route(z, 2, renormalise=False)[1] > 0).all()
+
+
+@pytest.mark.parametrize("E", [7, 32, 90, 256])
+@pytest.mark.parametrize("renormalise", [False, True])
+def test_softmax_weights_far_below_the_largest(E, renormalise):
+    """Logits whose distance from the largest is no float: its rounding is made good again, so that a far weight is as exact as a near one."""
+    n, top, per = 64, min(E, 6), 1 if E <= 32 else 4 if E <= 128 else 8
+    z = _rand(E, n, E, std=2.0)
+    z[:, :top] -= torch.rand(n, top, generator=torch.Generator("cuda").manual_seed(E), device="cuda") * 70.0 + 8.0
+    bias = torch.zeros(E, device="cuda")
+    bias[:top] = 4.0
+    choice, weights = _route(z, top, bias, score="softmax", renormalise=renormalise)
+    want, want_weights = plain.route(z.cpu(), top, "softmax", bias.cpu(), renormalise=renormalise)
+    assert torch.equal(choice, want)
+    # two units of the exponential and two roundings around it, above and below the line; up to 8 + per additions; two divisions, the scale
+    assert ((weights.to(F64) - want_weights).abs() <= (2 * 6 + 8 + per + 3) * 2.0 ** -24 * want_weights + 2.0 ** -149).all()
