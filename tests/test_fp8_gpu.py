@@ -666,3 +666,15 @@ def test_softmax_weights_far_below_the_largest(E, renormalise):
     assert torch.equal(choice, want)
     # two units of the exponential and two roundings around it, above and below the line; up to 8 + per additions; two divisions, the scale
     assert ((weights.to(F64) - want_weights).abs() <= (2 * 6 + 8 + per + 3) * 2.0 ** -24 * want_weights + 2.0 ** -149).all()
+
+
+@pytest.mark.parametrize("n,E,top", [(2100, 256, 8), (5000, 256, 8), (300, 1024, 8), (1200, 1024, 32)])
+def test_many_experts_of_many_choices(n, E, top):
+    """Hundreds of experts, few rows each and many, beyond the choices that are put in order from registers."""
+    layer, (gate, up, down) = _experts(E, 144, 72)
+    x = _rand(n, n, 144, dtype=BF)
+    choice, weights = _choices(n, n, E, top, 0.02)
+    out = torch.empty(n, 144, device="cuda")
+    layer.forward(x, choice, weights, out, layer.scratch(n, top))
+    want, bound = plain.experts(x.to(F64), choice, weights, gate, up, down)
+    assert ((out.to(F64) - want).abs() <= bound + HALF_STEP[F32] * (want.abs() + bound)).all()
