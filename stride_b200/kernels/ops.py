@@ -69,6 +69,9 @@ def _stream() -> int:
     return torch.cuda.current_stream().cuda_stream
 
 
+_stream_of = _raw_stream or (lambda device: torch.cuda.current_stream(device).cuda_stream)      # of a device that is known to be the current one
+
+
 def embed(tokens: torch.Tensor, table: torch.Tensor, out: torch.Tensor, slots=None, sampled=None, copy=None, scale: float = 1.0) -> None:
     """out[i, :] = float32(table[tokens[i], :]) * scale; a token of -1 means sampled[slots[i]] (the request's last sampled token).
     `copy` (float32, the shape of out) receives the same rows."""
@@ -861,8 +864,7 @@ class Fp8Linear:
             ldx, ldo = max(ldx, K), max(ldo, M)          # (of a single row the stride says nothing)
         call = _LINEAR_CALL.pack(self._address, x.data_ptr(), ldx, out.data_ptr(), ldo, dtype_code(x.dtype), dtype_code(out.dtype), n,
                                  epilogue if epilogue < SWIGLU else 2, epilogue - SWIGLU if gated else 0, *constants)
-        rc = self._fn(call, _stream())
-        _check(self._lib, rc)
+        _check(self._lib, self._fn(call, _stream_of(at)))
 
 
 ROUTER_SCORES = {"sigmoid": 0, "softmax": 1}
@@ -893,7 +895,7 @@ def route_experts(logits: torch.Tensor, choice: torch.Tensor, weights: torch.Ten
     lib, fn = _fn("router", "sb_route_experts", [c_char_p, c_void_p])
     call = _ROUTE_CALL.pack(logits.data_ptr(), ldz if n > 1 else max(ldz, E), 0 if bias is None else bias.data_ptr(), choice.data_ptr(), weights.data_ptr(),
                             ldw if top > 1 else max(ldw, n), n, E, top, code, groups, top_groups, group_best, 1 if renormalise else 0, scale)
-    _check(lib, fn(call, _stream()))
+    _check(lib, fn(call, _stream_of(at)))
 
 
 def experts_fp8_scratch(n: int, top: int, experts: int, width: int, inner: int) -> int:
@@ -924,7 +926,7 @@ def experts_fp8(x: torch.Tensor, choice: torch.Tensor, weights: torch.Tensor, ex
     lib, fn = _fn("gemm_fp8", "sb_experts_fp8", [c_char_p, c_void_p])
     call = _EXPERTS_CALL.pack(experts.address, x.data_ptr(), ldx, choice.data_ptr(), weights.data_ptr(), out.data_ptr(), ldo, scratch.data_ptr(),
                               scratch.numel(), dtype_code(x.dtype), dtype_code(out.dtype), n, top)
-    _check(lib, fn(call, _stream()))
+    _check(lib, fn(call, _stream_of(at)))
 
 
 class _Fp8ExpertsLayout(ctypes.Structure):
