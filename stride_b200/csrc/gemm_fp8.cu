@@ -9,14 +9,16 @@
 // The product: y[t, m] = sum over blocks b of columns of s[t, b] w_s[m / 128, b] (sum of q w over the block). The inner sum runs on the tensor cores
 // (tcgen05.mma kind::f8f6f4, float32 accumulators): every block of 128 columns, one row of the 128-byte swizzle, is a fresh accumulator in
 // tensor memory, of which there is a ring; the epilogue's warps take it from there and add it, times its two scales, to the tile's sum in
-// registers, one fused multiply-add an element, in 32 bits. That addition is what bounds large products (one multiply-add an element and
-// block beside 128 products on the tensor cores: 4,096 tokens through 28,672 gate and up rows of 4,096 470 to 530 us, with the clock, 2.0
-// PFLOP/s at best; without it, as a trial, 348), the weights' bytes the small ones.
+// registers, one fused multiply-add an element, in 32 bits. That addition is what bounds large products beside the power limit (one multiply-add an
+// element and block beside 128 products on the tensor cores: 4,096 tokens through 28,672 gate and up rows of 4,096 take 470 us in a burst of
+// 20 calls, 2.05 PFLOP/s, and 510 to 560 in a long run of them, at the clock that the limit leaves; a trial without the additions 393 and 440), the
+// weights' bytes the small ones. Times here are of the kernels in a row, in a recorded graph or a burst; a call among others from Python adds up to
+// 3 us to short ones.
 //
 // K is cut into ranges, a function of the weight's shape alone (`fp8_ranges`): few weight tiles leave SMs without work. The sum of a range
 // starts from zero, the ranges are added in ascending order. With few tokens, and with more where that takes fewer rounds, the ranges are shared out
-// among the CTAs of a cluster, which add up through distributed shared memory; else one CTA walks them all. So a token's bits depend neither on the step it is part of nor on the tile,
-// nor on which of the forms made them:
+// among the CTAs of a cluster, which add up through distributed shared memory; else one CTA walks them all. So a token's bits depend neither on the
+// step it is part of nor on the tile, nor on which of the forms made them:
 //   `gemm_fp8_kernel`        up to 64 tokens: 128 weight rows by 16, 32 or 64 tokens; of 16 it may quantise its input itself
 //   `gemm_fp8_token_kernel`  up to 128, and more where that takes fewer rounds: tokens are the product's rows
 //   `gemm_fp8_pair_kernel`   many, and the experts': tokens are the product's rows, CTAs or pairs of CTAs walk the tiles
@@ -162,9 +164,9 @@ __device__ __forceinline__ uint32_t instr_desc_e4m3(int n) {      // D float32, 
   return (1u << 4) | (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(kBlock >> 4) << 24);
 }
 // One block of 128 columns: four products of 32 columns (32 bytes of both operands' rows each) into a fresh accumulator, by one thread of a warp
-// that is here as a whole, as it is for the signals behind them. Descriptors and addresses are then
-// values of the warp, not of a thread: issued from a branch of one thread, a block took 850 cycles of moving them instead of 250 (a pair's
-// tensor cores need 512 for 256 columns).
+// that is here as a whole, as it is for the signals behind them. Descriptors and addresses are then values of the warp, not of a thread: issued
+// from a branch of one thread, moving them takes longer than the tensor cores do (4,096 tokens through 28,672 gate and up rows 545 us, so 470; 64 tokens
+// through [4096, 14336] 19.7, so 16.4).
 template <bool PAIR>
 __device__ __forceinline__ void issue_products(uint32_t tmem_d, uint64_t da, uint64_t db, uint32_t idesc) {
 #define SB_PRODUCT(GROUP, STEP, ACCUMULATE)                                                                                                  \
@@ -293,7 +295,7 @@ __device__ __forceinline__ float cluster_load_float(uint32_t addr) {
 }
 
 // Up to 32 choices of experts: a lane each, and every warp knows all about them without a kernel that puts them in order (one token's six through
-// experts of 2,048 x 1,408: 22.7 us with it, 20.4 without). Rows in the order of the experts, an expert's in the choices' order.
+// experts of 2,048 x 1,408: 22.7 us with it, 20.4 without, 20.0 by now). Rows in the order of the experts, an expert's in the choices' order.
 constexpr int kMaxExperts = 1024;
 constexpr int kFewChoices = 32;
 struct FewChoices {
@@ -664,10 +666,11 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
 // A block's product is issued as two chains, each with half of both CTAs' weight rows (of a gated product: a feature's gate row and its up row
 // in the same chain) and accumulators of its own, and the epilogue's warps as two sets, one a chain: a set's way from one accumulator to the
 // next (signals, first loads) then falls into the other's additions. Each chain has a warp that issues it: one for both took longer than the
-// tensor cores (574 us, with a warp each 524, at the time).
+// tensor cores (574 us, with a warp each 524, when that was measured).
 //
 // PAIR false (experts, whose rows rarely fill 256, and dense products that need fewer rounds so): one CTA with the pair's weight rows and 128
-// tokens, 48 KB a block for the same 512 cycles (2,000 tokens through 64 experts, six each: 280 us on pairs, 238 so). The weight rows lie in
+// tokens, 48 KB a block for the same 512 cycles (2,000 tokens through 64 experts, six each: 280 us on pairs, 238 so, in bursts;
+// in a long run of calls 265 to 277 so). The weight rows lie in
 // shared memory as the pair's CTAs would have them, 64 of the first chain's each, then the second's.
 constexpr int kPairTokens = 256;
 constexpr int kPairThreads = 640;                // a warp that loads, two that issue the products, one for the scales, sixteen of the epilogue

@@ -790,7 +790,7 @@ def check_fp8_epilogue(weight, gated: bool) -> None:
 
 
 def _fp8_product(weight, out: torch.Tensor, epilogue: int, n: int):
-    """(weight's address, stride, scales, out's address, dtype, stride, M, epilogue code, half rows, gate) of a product, checked."""
+    """(weight rows, epilogue code, half rows) of a product, checked."""
     M = weight.shape[0]
     code = _EPILOGUES_FP8[epilogue]
     half = M // 2 if code == 2 else 0
@@ -908,7 +908,8 @@ def experts_fp8_scratch(n: int, top: int, experts: int, width: int, inner: int) 
 def experts_fp8(x: torch.Tensor, choice: torch.Tensor, weights: torch.Tensor, experts, out: torch.Tensor, scratch: torch.Tensor) -> None:
     """out[t] = sum over k of weights[k, t] * down_e (silu(gate_e x_t) * (up_e x_t)), e = choice[t, k], in the order of the choices; an id that is no
     expert's has no term. x [n, width] float32 or bfloat16, choice [n, top] int32, weights [top, n] float32, `experts` an `Fp8Experts`, out float32 or
-    bfloat16 [n, width], scratch uint8 of `experts_fp8_scratch` bytes. Inputs of both projections are quantised as `quantize_fp8` does."""
+    bfloat16 [n, width], scratch uint8 of `experts_fp8_scratch` bytes for as many tokens or more. Inputs of both projections are quantised as
+    `quantize_fp8` does. Calls that share scratch run on one stream."""
     at = experts.at
     if at < 0 or x.get_device() != at or choice.get_device() != at or weights.get_device() != at or out.get_device() != at or scratch.get_device() != at \
             or _device() != at:
